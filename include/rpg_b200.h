@@ -205,6 +205,94 @@ RPGB_API int32_t rpgb_sample_noalloc(const float* logits_dev, int32_t n, const r
 /* u = H(seed, counter) in [0, 1) (DevCounterUniform, src/sampler_gpu.cu:364). */
 RPGB_API float rpgb_counter_uniform(uint64_t seed, uint64_t counter);
 
+/* ------------------------------------------------------------------ paged key-value cache
+ *
+ * Operators for hosts that hold many conversations in one pool of pages (no
+ * counterpart in the reference, whose cache is one conversation's).  The
+ * caller owns all memory: per layer a pool of pages for k and one for v, and
+ * per batch a page table.  Position p of conversation s lives in pool page
+ * pages[s * stride + p / page_size] at offset p % page_size.  All pointers in
+ * these structs except the structs themselves are device pointers; the calls
+ * run on `stream` of the current device, return without waiting, allocate
+ * nothing and can be captured in a CUDA graph.
+ *
+ * A page id outside [0, n_pages), a position past the table and a
+ * conversation outside [0, n_seq) are never followed: append then writes
+ * nothing and gives NaN in q_out, gather and attend give NaN, for the rows
+ * concerned.  A row with position < 0 is padding: zeros, nothing written. */
+
+/* Element types of activations and caches. */
+#define RPGB_F32 0
+#define RPGB_F16 1
+#define RPGB_BF16 2
+#define RPGB_KV_F16 0 /* f16 values */
+#define RPGB_KV_Q8 1  /* int8 codes c standing for c * d */
+#define RPGB_KV_Q4 2  /* 4-bit codes c standing for (c - 8) * d; the even value of a byte in its low half */
+
+/* Pages of one layer.  head_dim is 64 or 128, page_size a power of two from
+ * 16 to 4096.  Strides are in bytes: [page][kv head][position] of codes
+ * (multiples of 16, at least a row: 2, 1 or 1/2 byte per value).  Quantised
+ * caches have a scale d (f16) for every 64 values of a row, dense
+ * [position][head_dim / 64] inside a head's page, with strides of their own.
+ * k and v share the strides; k, v and the scales are 16-byte aligned. */
+typedef struct rpgb_kv_pages {
+  int32_t type, head_dim, n_kv, page_size, n_pages, reserved;
+  void *k, *v, *k_scale, *v_scale;
+  int64_t page_stride, head_stride, pos_stride;
+  int64_t scale_page_stride, scale_head_stride;
+} rpgb_kv_pages;
+
+/* Page table of n_seq conversations (int32 [n_seq][stride], max_pages used). */
+typedef struct rpgb_kv_table {
+  const int32_t* pages;
+  int64_t stride;
+  int32_t n_seq, max_pages;
+} rpgb_kv_table;
+
+/* Per-head RMSNorm weights (f32 [head_dim], NULL = no norm) and the rotation
+ * table (f32 [rope_positions][head_dim]: the cosines of the head_dim / 2
+ * angles, then the sines; NULL = no rotation). */
+typedef struct rpgb_kv_rotary {
+  const float* rope;
+  const float *q_norm, *k_norm;
+  int32_t rope_positions;
+  float eps;
+} rpgb_kv_rotary;
+
+/* Writes n_tok new rows.  qkv_dev: rows q | k | v of n_heads, n_kv and n_kv
+ * heads.  The q and k heads are normalised and rotated for position
+ * pos_dev[t] (value j of a head pairs with j + head_dim / 2); k and v go to
+ * that position of conversation seq_dev[t] (seq_dev NULL: row t belongs to
+ * conversation t), q to q_out_dev in the rows' type (NULL: not wanted; it may
+ * be the q part of qkv_dev itself).  A quantised cache rounds to the nearest
+ * code of d = f16(max |x| / 127 or / 7); magnitudes past 127 or 7 times 65504
+ * saturate, a group that holds a NaN reads back as NaN.  Rows must not name
+ * the same position twice.  rotary NULL: k and q go through as they are. */
+RPGB_API int32_t rpgb_kv_append(const rpgb_kv_pages* kv, const rpgb_kv_table* table, const rpgb_kv_rotary* rotary,
+                                int32_t type, const void* qkv_dev, int64_t qkv_stride, int32_t n_heads,
+                                const int32_t* seq_dev, const int32_t* pos_dev, int64_t n_tok, void* q_out_dev,
+                                int64_t q_stride, void* stream);
+
+/* Reads rows back: k_out_dev[t] and v_out_dev[t] (rows of n_kv heads, either
+ * may be NULL) = position pos_dev[t] of conversation seq_dev[t], rounded once
+ * to `type`. */
+RPGB_API int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type,
+                                const int32_t* seq_dev, const int32_t* pos_dev, int64_t n_tok, void* k_out_dev,
+                                void* v_out_dev, int64_t out_stride, void* stream);
+
+/* Attention of one new token per conversation: row s of out_dev =
+ * softmax(scale q K^T) V per head over positions [starts_dev[s], lens_dev[s])
+ * of conversation s (starts_dev NULL: from 0; pages wholly before the start
+ * are not looked at).  An empty range gives zeros.  n_heads is any multiple
+ * of n_kv; q head h reads KV head h / (n_heads / n_kv).  The sums are in f32.
+ * workspace_dev: rpgb_kv_attend_workspace bytes, 256-byte aligned, zeroed
+ * once before its first use; calls that may overlap need one each. */
+RPGB_API int64_t rpgb_kv_attend_workspace(int32_t n_seq, int32_t n_heads, int32_t n_kv, int32_t head_dim);
+RPGB_API int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type, const void* q_dev,
+                                int64_t q_stride, int32_t n_heads, const int32_t* lens_dev, const int32_t* starts_dev,
+                                float scale, void* out_dev, int64_t out_stride, void* workspace_dev,
+                                int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ text layer
  *
  * The host text layer rpg_engine_generate runs, without a GPU: the same token

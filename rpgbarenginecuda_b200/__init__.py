@@ -15,15 +15,23 @@ import ctypes
 
 import numpy as np
 
-from ._lib import EngineError, SampleOptions, check, load_engine  # noqa: F401
+from ._lib import (EngineError, KvPagesDesc, KvRotaryDesc, KvTableDesc, SampleOptions, check,  # noqa: F401
+                   load_engine)
 
 __all__ = ["Model", "Session", "Matrix", "SampleOptions", "EngineError", "TpGroup", "shard_plan", "sample",
-           "counter_uniform", "launch_count", "library_path", "GGML_Q4_K", "GGML_Q5_K", "GGML_Q6_K", "GGML_Q8_0"]
+           "counter_uniform", "launch_count", "library_path", "GGML_Q4_K", "GGML_Q5_K", "GGML_Q6_K", "GGML_Q8_0",
+           "PagedKv", "PageTable", "Rotary", "attend_workspace", "rope_table", "F32", "F16", "BF16", "KV_F16", "KV_Q8",
+           "KV_Q4", "KV_GROUP"]
 
 GGML_Q8_0 = 8
 GGML_Q4_K = 12
 GGML_Q5_K = 13
 GGML_Q6_K = 14
+
+# element types of activations, storage types of paged caches (include/rpg_b200.h)
+F32, F16, BF16 = 0, 1, 2
+KV_F16, KV_Q8, KV_Q4 = 0, 1, 2
+KV_GROUP = 64  # values of a quantised cache row that share a scale
 
 
 def library_path() -> str:
@@ -240,6 +248,90 @@ def sample(logits_ptr: int, n: int, opts: SampleOptions, seed: int, counter: int
     lib = load_engine()
     check(lib.rpgb_sample(logits_ptr, n, ctypes.byref(opts), seed, counter, probs_ptr, tok_ptr, stream or None),
           "sample")
+
+
+class PageTable:
+    """Page table of a batch: int32 [n_seq][stride] on the device, `max_pages` entries of a row used."""
+
+    def __init__(self, pages_ptr: int, n_seq: int, max_pages: int, stride: int = 0):
+        self.desc = KvTableDesc(pages_ptr, stride or max_pages, n_seq, max_pages)
+        self._ref = ctypes.addressof(self.desc)
+
+
+class Rotary:
+    """Rotation table ([rope_positions][head_dim] f32, as `rope_table` makes it) and per-head norm weights; a
+    pointer of 0 leaves its step out."""
+
+    def __init__(self, rope_ptr: int = 0, rope_positions: int = 0, q_norm_ptr: int = 0, k_norm_ptr: int = 0,
+                 eps: float = 1e-6):
+        self.desc = KvRotaryDesc(rope_ptr or None, q_norm_ptr or None, k_norm_ptr or None, rope_positions, eps)
+        self._ref = ctypes.addressof(self.desc)
+
+
+class PagedKv:
+    """Key-value pages of one layer in device memory that the caller owns (rpgb_kv_pages).
+
+    k and v are pools [n_pages][n_kv][page_size][row] (f16 values, int8 codes
+    or 4-bit codes), the scales of a quantised cache [n_pages][n_kv]
+    [page_size][head_dim / 64] f16; other layouts through the byte strides.
+    All calls take device pointers, run on `stream` (0: the legacy stream) of
+    the current device and return without waiting."""
+
+    def __init__(self, kv_type: int, head_dim: int, n_kv: int, page_size: int, n_pages: int, k_ptr: int, v_ptr: int,
+                 k_scale_ptr: int = 0, v_scale_ptr: int = 0, page_stride: int = 0, head_stride: int = 0,
+                 pos_stride: int = 0, scale_page_stride: int = 0, scale_head_stride: int = 0):
+        self._lib = load_engine()
+        self.head_dim, self.n_kv = head_dim, n_kv
+        row = {KV_F16: 2 * head_dim, KV_Q8: head_dim, KV_Q4: head_dim // 2}.get(kv_type, 0)
+        pos_stride = pos_stride or row
+        head_stride = head_stride or page_size * pos_stride
+        scale_head_stride = scale_head_stride or page_size * (head_dim // KV_GROUP) * 2
+        self.desc = KvPagesDesc(kv_type, head_dim, n_kv, page_size, n_pages, 0, k_ptr or None, v_ptr or None,
+                                k_scale_ptr or None, v_scale_ptr or None, page_stride or n_kv * head_stride, head_stride,
+                                pos_stride, scale_page_stride or n_kv * scale_head_stride, scale_head_stride)
+        self._ref = ctypes.addressof(self.desc)
+
+    def append(self, table: PageTable, rotary: Rotary | None, dtype: int, qkv_ptr: int, n_heads: int, pos_ptr: int,
+               n_tok: int, q_out_ptr: int = 0, seq_ptr: int = 0, qkv_stride: int = 0, q_stride: int = 0,
+               stream: int = 0):
+        """Norm, rotation and (quantised) write of n_tok q|k|v rows (rpgb_kv_append)."""
+        if self._lib.rpgb_kv_append(self._ref, table._ref, rotary._ref if rotary is not None else None, dtype, qkv_ptr,
+                                    qkv_stride or (n_heads + 2 * self.n_kv) * self.head_dim, n_heads, seq_ptr or None,
+                                    pos_ptr, n_tok, q_out_ptr or None, q_stride or n_heads * self.head_dim,
+                                    stream or None) < 0:
+            check(-1, "kv_append")
+
+    def gather(self, table: PageTable, dtype: int, pos_ptr: int, n_tok: int, k_out_ptr: int = 0, v_out_ptr: int = 0,
+               seq_ptr: int = 0, out_stride: int = 0, stream: int = 0):
+        """Stored rows back as `dtype` (rpgb_kv_gather)."""
+        if self._lib.rpgb_kv_gather(self._ref, table._ref, dtype, seq_ptr or None, pos_ptr, n_tok, k_out_ptr or None,
+                                    v_out_ptr or None, out_stride or self.n_kv * self.head_dim, stream or None) < 0:
+            check(-1, "kv_gather")
+
+    def attend(self, table: PageTable, dtype: int, q_ptr: int, n_heads: int, lens_ptr: int, scale: float, out_ptr: int,
+               workspace_ptr: int, workspace_bytes: int, starts_ptr: int = 0, q_stride: int = 0, out_stride: int = 0,
+               stream: int = 0):
+        """Attention of one new token per conversation (rpgb_kv_attend)."""
+        row = n_heads * self.head_dim
+        if self._lib.rpgb_kv_attend(self._ref, table._ref, dtype, q_ptr, q_stride or row, n_heads, lens_ptr,
+                                    starts_ptr or None, scale, out_ptr, out_stride or row, workspace_ptr,
+                                    workspace_bytes, stream or None) < 0:
+            check(-1, "kv_attend")
+
+
+def attend_workspace(n_seq: int, n_heads: int, n_kv: int, head_dim: int) -> int:
+    """Bytes of the workspace `PagedKv.attend` needs (zeroed once by the caller)."""
+    n = int(load_engine().rpgb_kv_attend_workspace(n_seq, n_heads, n_kv, head_dim))
+    if n < 0:
+        check(-1, "kv_attend_workspace")
+    return n
+
+
+def rope_table(n_pos: int, head_dim: int = 128, theta: float = 1e6) -> np.ndarray:
+    """f32 [n_pos][head_dim]: cos then sin of pos * theta^(-2 i / head_dim), angles in 64 bits (as the engine's own)."""
+    inv = 1.0 / np.power(float(theta), np.arange(0, head_dim, 2, dtype=np.float64) / head_dim)
+    ang = np.arange(n_pos, dtype=np.float64)[:, None] * inv
+    return np.concatenate([np.cos(ang), np.sin(ang)], 1).astype(np.float32)
 
 
 def launch_count() -> int:

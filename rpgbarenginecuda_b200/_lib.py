@@ -29,6 +29,26 @@ class SampleOptions(ctypes.Structure):
         super().__init__(temperature, top_k, top_p)
 
 
+class KvPagesDesc(ctypes.Structure):
+    """rpgb_kv_pages (include/rpg_b200.h)."""
+
+    _fields_ = [(n, c_i32) for n in ("type", "head_dim", "n_kv", "page_size", "n_pages", "reserved")] + \
+        [(n, c_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+        [(n, c_i64) for n in ("page_stride", "head_stride", "pos_stride", "scale_page_stride", "scale_head_stride")]
+
+
+class KvTableDesc(ctypes.Structure):
+    """rpgb_kv_table."""
+
+    _fields_ = [("pages", c_p), ("stride", c_i64), ("n_seq", c_i32), ("max_pages", c_i32)]
+
+
+class KvRotaryDesc(ctypes.Structure):
+    """rpgb_kv_rotary."""
+
+    _fields_ = [("rope", c_p), ("q_norm", c_p), ("k_norm", c_p), ("rope_positions", c_i32), ("eps", c_f32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "rpgb_version": (ctypes.c_char_p, []),
@@ -62,6 +82,10 @@ _SIGS = {
     "rpgb_sample": (c_i32, [c_p, c_i32, ctypes.POINTER(SampleOptions), c_u64, c_u64, c_p, c_p, c_p]),
     "rpgb_sample_noalloc": (c_i32, [c_p, c_i32, ctypes.POINTER(SampleOptions), c_u64, c_u64, c_p, c_p]),
     "rpgb_counter_uniform": (c_f32, [c_u64, c_u64]),
+    "rpgb_kv_append": (c_i32, [c_p, c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_i64, c_p, c_i64, c_p]),
+    "rpgb_kv_gather": (c_i32, [c_p, c_p, c_i32, c_p, c_p, c_i64, c_p, c_p, c_i64, c_p]),
+    "rpgb_kv_attend_workspace": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "rpgb_kv_attend": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_f32, c_p, c_i64, c_p, c_i64, c_p]),
     "rpgb_text_open": (c_p, [ctypes.c_char_p]),
     "rpgb_text_close": (None, [c_p]),
     "rpgb_text_encode": (c_i64, [c_p, ctypes.c_char_p, c_i64, c_i32, c_p, c_i64]),
