@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t MaxAbs4(const float (&x)[4]) {
 template <KvType KIND>
 __device__ __forceinline__ __half GroupScale(uint32_t max_bits) {
   const float m = __uint_as_float(max_bits);
-  return __float2half_rn(max_bits > 0x7F800000u ? m : fminf(m / MostCode<KIND>(), 65504.f));
+  return __float2half_rn(max_bits > 0x7F800000u ? m : fminf(m * (1.f / MostCode<KIND>()), 65504.f));
 }
 
 // Codes of four consecutive values x, nearest with ties to even.  A scale that
@@ -53,9 +53,40 @@ __device__ __forceinline__ void StoreCodes(char* row, int i, const float (&x)[4]
   }
 }
 
+// 1 / sqrt(mean x^2 + eps) of a head, in f32.  The squares and sums round one
+// by one (no fused multiply-add) in a fixed tree: the halves' lanes, then
+// lanes 8, 4, 2 and 1 apart.
+template <int D>
+__device__ __forceinline__ float InvRms(const float (&a)[4], const float (&b)[4], float eps) {
+  float t[4], s;
+  if (D == 128) {  // runs of four values first
+    float u = __fmul_rn(a[0], a[0]), v = __fmul_rn(b[0], b[0]);
+#pragma unroll
+    for (int e = 1; e < 4; ++e) {
+      u = __fadd_rn(u, __fmul_rn(a[e], a[e]));
+      v = __fadd_rn(v, __fmul_rn(b[e], b[e]));
+    }
+    s = __fadd_rn(u, v);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xFFFFFFFFu, s, o));
+  } else {  // the lanes first, then the values of a lane
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e] = __fadd_rn(__fmul_rn(a[e], a[e]), __fmul_rn(b[e], b[e]));
+#pragma unroll
+      for (int o = D / 16; o > 0; o >>= 1) t[e] = __fadd_rn(t[e], __shfl_xor_sync(0xFFFFFFFFu, t[e], o));
+    }
+    s = __fadd_rn(__fadd_rn(t[0], t[2]), __fadd_rn(t[1], t[3]));
+  }
+  return rsqrtf(__fadd_rn(__fmul_rn(s, 1.0f / D), eps));
+}
+
 // One row t, one head per D / 8 lanes.  Lane i holds values 4 i .. 4 i + 3 of
 // the first half (a) and of the second (b), so a rotation pair (j, j + D / 2)
-// sits in one lane and a scale group of 64 values in the same lanes.
+// sits in one lane and a scale group of 64 values in the same lanes.  Norm and
+// rotation round every product and sum on its own, so a value that falls near
+// a rounding boundary of the cache gets the code of the formulas evaluated
+// step by step in f32.
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams p) {
   constexpr int L = D / 8;
@@ -80,20 +111,15 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
     kvd::Load4(x + D / 2 + 4 * i, b);
   }
   const float* w = kind == kQ ? p.q_norm : (kind == kK ? p.k_norm : nullptr);
-  float ss = 0.f;  // in f32: eight terms a lane, then a tree over the lanes
-#pragma unroll
-  for (int e = 0; e < 4; ++e) ss += a[e] * a[e] + b[e] * b[e];
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+  const float r = InvRms<D>(a, b, p.eps);  // every lane takes part, whatever its head
   if (w != nullptr) {
-    const float r = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
     float wa[4], wb[4];
     kvd::Load4(w + 4 * i, wa);
     kvd::Load4(w + D / 2 + 4 * i, wb);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      a[e] = a[e] * r * wa[e];
-      b[e] = b[e] * r * wb[e];
+      a[e] = __fmul_rn(__fmul_rn(a[e], r), wa[e]);
+      b[e] = __fmul_rn(__fmul_rn(b[e], r), wb[e]);
     }
   }
   if (kind != kV && p.rope != nullptr && ok) {
@@ -104,12 +130,12 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x = a[e], y = b[e];
-      a[e] = x * c[e] - y * s[e];
-      b[e] = y * c[e] + x * s[e];
+      a[e] = __fsub_rn(__fmul_rn(x, c[e]), __fmul_rn(y, s[e]));
+      b[e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(x, s[e]));
     }
   }
   uint32_t ma = 0, mb = 0;
-  if (KIND != KvType::kF16) {  // every lane takes part, whatever its head
+  if (KIND != KvType::kF16) {
     ma = MaxAbs4(a);
     mb = MaxAbs4(b);
     if (D == kKvGroup) ma = mb = max(ma, mb);

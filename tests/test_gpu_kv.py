@@ -446,7 +446,7 @@ def test_append_codes_are_exact_without_norm_and_rotation(kind):
         rows = x[:, lo:lo + 256].cpu().numpy().reshape(64, 2, 2, 64)
         m = np.abs(rows).max(-1)  # NaN where there is one
         with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
-            d16 = np.where(np.isnan(m), m, np.minimum(m / most, np.float32(65504))).astype(np.float16)
+            d16 = np.where(np.isnan(m), m, np.minimum(m * (np.float32(1) / most), np.float32(65504))).astype(np.float16)
             d = d16.astype(np.float32)[..., None]
             c = np.where(d > 0, np.clip(np.rint(rows / np.where(d > 0, d, 1)), -most, most), 0)
         got_d = pool.scale[name][page, :2][torch.arange(64), :, at].cpu().numpy()
