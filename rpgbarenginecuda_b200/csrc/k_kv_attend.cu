@@ -741,80 +741,124 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
       __syncthreads();
       const bool whole = seg == 0 && use.tile + 1 == use.span.tiles;
-      const long long item0 = at - use.tile;  // the item's first tile
+      const int64_t out = use.seq * p.out_stride + col;
       const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
-      char* records = static_cast<char*>(p.workspace) +
-                      (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256;
-      constexpr int kRecord = kKvMaxQueries * (D + 2);
-      float* rec = reinterpret_cast<float*>(records) +
-                   static_cast<int64_t>(2 * blockIdx.x + (item0 >= first ? 1 : 0)) * kRecord;
-      const int64_t out = use.seq * p.out_stride + col;
-      auto put = [&](int64_t i, float v, float sum) {
-        v = sum != 0.f ? v / sum : 0.f;  // nothing in range: zero
-        if (past) v = kvd::Nan();
-        switch (p.type) {
-          case ElemType::kF32: static_cast<float*>(p.out)[out + i] = v; break;
-          case ElemType::kF16: static_cast<__half*>(p.out)[out + i] = __float2half_rn(v); break;
-          case ElemType::kBF16: static_cast<__nv_bfloat16*>(p.out)[out + i] = __float2bfloat16_rn(v); break;
-        }
-      };
-      for (int i = tid; i < queries * D; i += kThreads) {
+      // The warps' shares joined: value i of the item's queries, its sum, its maximum.
+      auto join = [&](int i, float& sum, float& top) {
         const int q = i / D;
-        float top = -INFINITY;
+        top = s_m[0][q];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][q]);
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][q]);
         const float ref = top == -INFINITY ? 0.f : top;
-        float v = 0.f, sum = 0.f;
+        float v = 0.f;
+        sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float f = Exp2(s_m[w][q] - ref);
           v += f * comb[w * (C::COMB / 4) + i];
           sum += f * s_l[w][q];
         }
-        if (whole) {
-          put(i, v, sum);
-        } else {
-          rec[i] = v;
-          if (i % D == 0) {
-            rec[kKvMaxQueries * D + q] = top;
-            rec[kKvMaxQueries * D + kKvMaxQueries + q] = sum;
-          }
-        }
-      }
+        return v;
+      };
+      bool finish = whole;
       if (!whole) {
-        // blocks that hold a part of the item: those of its first and last
-        // tile and all between
-        const long long item1 = item0 + use.span.tiles - 1;
+        // This block's record: one for an item that began in an earlier block,
+        // one for an item that begins here.  Blocks b0 .. b1 hold the parts.
+        const long long item0 = at - use.tile, item1 = item0 + use.span.tiles - 1;
         const int b0 = static_cast<int>(((item0 + 1) * blocks - 1) / total);
         const int b1 = static_cast<int>(((item1 + 1) * blocks - 1) / total);
+        constexpr int kRecord = kKvMaxQueries * (D + 2);
+        float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
+                                                  (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256);
+        auto record = [&](int b) { return records + (2 * b + (b == b0 ? 1 : 0)) * kRecord; };
         unsigned* count = static_cast<unsigned*>(p.workspace) + static_cast<int64_t>(use.seq) * items + use.item;
+        float* rec = record(blockIdx.x);
+        for (int i = tid; i < queries * D; i += kThreads) {
+          float sum, top;
+          rec[i] = join(i, sum, top);
+          if (i % D == 0) {
+            rec[kKvMaxQueries * D + i / D] = top;
+            rec[kKvMaxQueries * (D + 1) + i / D] = sum;
+          }
+        }
         __threadfence();
         __syncthreads();
         if (tid == 0) s_last = atomicAdd(count, 1u) == static_cast<unsigned>(b1 - b0);
         __syncthreads();
-        if (s_last) {
+        finish = s_last != 0;
+        if (finish) {
+          // The last block joins all records: warp w adds up records b0 + w,
+          // b0 + w + 4, ... under the maximum of all, in that order.
           __threadfence();
-          const float* base = reinterpret_cast<const float*>(records);
-          auto record = [&](int b) {
-            const long long begin = total * b / blocks;
-            return base + static_cast<int64_t>(2 * b + (item0 >= begin ? 1 : 0)) * kRecord;
-          };
-          for (int i = tid; i < queries * D; i += kThreads) {
-            const int q = i / D;
-            float top = -INFINITY;
-            for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(record(b) + kKvMaxQueries * D + q));
-            const float ref = top == -INFINITY ? 0.f : top;
-            float v = 0.f, sum = 0.f;
-            for (int b = b0; b <= b1; ++b) {
-              const float* r = record(b);
-              const float f = Exp2(__ldcg(r + kKvMaxQueries * D + q) - ref);
-              v += f * __ldcg(r + i);
-              sum += f * __ldcg(r + kKvMaxQueries * D + kKvMaxQueries + q);
-            }
-            put(i, v, sum);
-          }
           if (tid == 0) *count = 0;
+          constexpr int kVec = C::QUERIES * D / 128;  // float4 of a lane
+          float top[C::QUERIES], sum[C::QUERIES];
+          float4 v[kVec];
+#pragma unroll
+          for (int q = 0; q < C::QUERIES; ++q) {
+            top[q] = -INFINITY;
+            sum[q] = 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int b = b0 + lane; b <= b1; b += 32) {
+            const float* r = record(b) + kKvMaxQueries * D;
+#pragma unroll
+            for (int q = 0; q < C::QUERIES; ++q) {
+              if (q < queries) top[q] = fmaxf(top[q], __ldcg(r + q));
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < C::QUERIES; ++q) top[q] = dev::WarpMax(top[q]);
+#pragma unroll 2
+          for (int b = b0 + warp; b <= b1; b += kWarps) {
+            const float* r = record(b);
+            float f[C::QUERIES];
+#pragma unroll
+            for (int q = 0; q < C::QUERIES; ++q) {
+              f[q] = 0.f;
+              if (q < queries) {
+                f[q] = Exp2(__ldcg(r + kKvMaxQueries * D + q) - (top[q] == -INFINITY ? 0.f : top[q]));
+                sum[q] += f[q] * __ldcg(r + kKvMaxQueries * (D + 1) + q);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+              const int q = k * 128 / D + (D == 128 ? 0 : lane >> 4);
+              if (q < queries) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(r) + 32 * k + lane);
+                const float fq = D == 128 ? f[k % C::QUERIES] : (lane >= 16 ? f[(2 * k + 1) % C::QUERIES] : f[(2 * k) % C::QUERIES]);
+                v[k].x += fq * x.x;
+                v[k].y += fq * x.y;
+                v[k].z += fq * x.z;
+                v[k].w += fq * x.w;
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) reinterpret_cast<float4*>(mineq)[32 * k + lane] = v[k];
+          if (lane == 0) {
+#pragma unroll
+            for (int q = 0; q < C::QUERIES; ++q) {
+              s_m[warp][q] = top[q];
+              s_l[warp][q] = sum[q];
+            }
+          }
+          __syncthreads();
+        }
+      }
+      if (finish) {
+        for (int i = tid; i < queries * D; i += kThreads) {
+          float sum, top;
+          float v = join(i, sum, top);
+          v = sum != 0.f ? v / sum : 0.f;  // nothing in range: zero
+          if (past) v = kvd::Nan();
+          switch (p.type) {
+            case ElemType::kF32: static_cast<float*>(p.out)[out + i] = v; break;
+            case ElemType::kF16: static_cast<__half*>(p.out)[out + i] = __float2half_rn(v); break;
+            case ElemType::kBF16: static_cast<__nv_bfloat16*>(p.out)[out + i] = __float2bfloat16_rn(v); break;
+          }
         }
       }
       __syncthreads();  // the next item writes the join area again
