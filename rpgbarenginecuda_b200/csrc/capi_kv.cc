@@ -41,7 +41,8 @@ KvPages Pages(const rpgb_kv_pages* d) {
   p.head_stride = d->head_stride;
   p.pos_stride = d->pos_stride;
   for (const int64_t s : {p.page_stride, p.head_stride, p.pos_stride}) {
-    RPGB_CHECK(s >= row && s % 16 == 0, "kv: stride %lld; a multiple of 16 bytes of at least a row (%lld) is needed",
+    RPGB_CHECK(s >= row && s % 16 == 0 && s <= kKvMaxStride,
+               "kv: stride %lld; a multiple of 16 bytes of at least a row (%lld) is needed",
                static_cast<long long>(s), static_cast<long long>(row));
   }
   if (p.type != KvType::kF16) {
@@ -54,7 +55,7 @@ KvPages Pages(const rpgb_kv_pages* d) {
     p.scale_page_stride = d->scale_page_stride;
     p.scale_head_stride = d->scale_head_stride;
     for (const int64_t s : {p.scale_page_stride, p.scale_head_stride}) {
-      RPGB_CHECK(s >= page && s % 16 == 0,
+      RPGB_CHECK(s >= page && s % 16 == 0 && s <= kKvMaxStride,
                  "kv: scale stride %lld; a multiple of 16 bytes of at least a page's scales (%lld) is needed",
                  static_cast<long long>(s), static_cast<long long>(page));
     }

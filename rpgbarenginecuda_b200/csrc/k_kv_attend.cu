@@ -64,35 +64,44 @@ struct Cfg {
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;  // 16-byte chunks of a row
-  static constexpr int SC = QUANT ? R * NG * 2 : 0;
-  static constexpr int SLOT = R * ROW + SC;
-  static constexpr int RING = DEPTH * 2 * SLOT;  // per warp: K and V
+  static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
+  static constexpr int KSLOT = R * ROW + 2 * SC;     // K codes, K scales, V scales
+  static constexpr int VSLOT = R * ROW;
+  static constexpr int RING = DEPTH * (KSLOT + VSLOT);  // per warp
+  static_assert(KSLOT % 128 == 0 && VSLOT % 128 == 0, "tiles are 128-byte lines");
   static constexpr int COMB = QUERIES * D * 4;   // per warp
   static constexpr int SMEM = kWarps * (RING + COMB);
   static constexpr int BLOCKS = PACK || D == 64 ? 3 : 2;  // resident per SM: what registers and shared memory allow
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte lines.  The
-// chunk's place in its line is permuted by the row so that the lanes of one
-// load (8 rows of one chunk for ldmatrix; see LoadK / LoadV for the codes)
-// touch different banks.
+// chunk's place in its line is permuted (an exclusive or with bits of the row)
+// so that the lanes of one load (8 rows of one chunk for ldmatrix; see KRows
+// and VFragments for the codes) touch different banks.
 template <typename C, bool V>
-__device__ __forceinline__ int ChunkAt(int r, int c) {
-  int key;
-  if (C::KIND == KvType::kF16) {
-    key = r & 7;
-  } else if (C::KIND == KvType::kQ8) {
-    key = V ? ((r >> 1) & 3) << 1 : (C::D == 128 ? (r & 1) << 2 : 0);
-  } else {
-    key = V ? (C::D == 128 ? ((r >> 1) & 3) << 1 : ((r >> 2) & 1) << 1) : (C::D == 128 ? ((r >> 1) & 1) << 1 : 0);
-  }
+__host__ __device__ constexpr int ChunkAt(int r, int c) {
+  const int key = C::KIND == KvType::kF16  ? r & 7
+                  : C::KIND == KvType::kQ8 ? (V ? ((r >> 1) & 3) << 1 : (C::D == 128 ? (r & 1) << 2 : 0))
+                  : V                      ? (C::D == 128 ? ((r >> 1) & 3) << 1 : ((r >> 2) & 1) << 1)
+                                           : (C::D == 128 ? ((r >> 1) & 1) << 1 : 0);
   const int q = r * C::CPR + c;
   return (q >> 3) * 128 + (((q & 7) ^ key) << 4);
+}
+// The address dr rows and dc chunks from `base`, the address of (r, c): where
+// r and dr, c and dc share no bits the permutation is linear, so this is one
+// exclusive or with a constant at most.
+template <typename C, bool V>
+__device__ __forceinline__ uint32_t Moved(uint32_t base, int dr, int dc) {
+  const int x = ChunkAt<C, V>(dr, dc);
+  return (base ^ (x & 127)) + (x & ~127);
 }
 
 // ------------------------------------------------------------------ instructions
 
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src, bool read) {
+__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void CopyAsync16OrZero(uint32_t dst, const void* src, bool read) {
   const int n = read ? 16 : 0;  // the rest is filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -122,6 +131,12 @@ __device__ __forceinline__ void Mma(float (&d)[4], const uint32_t (&a)[4], uint3
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same with nothing to add to.
+__device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t Lds32(uint32_t a) {
   uint32_t x;
@@ -180,81 +195,122 @@ __device__ __forceinline__ Span SpanOf(const KvAttendParams& p, int seq) {
   s.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(p.lens + seq), 0)), cap));
   s.start = p.starts != nullptr ? max(__ldg(p.starts + seq), 0) : 0;
   if (s.start >= s.len) s.start = s.len = 0;
-  s.base = s.start & ~15;  // a 16-position unit lies in one page
+  s.base = s.start & ~(C::R - 1);  // a step lies in one page, or its halves in two of 16
   s.tiles = max(1, (s.len - s.base + C::TILE - 1) / C::TILE);  // an empty item still writes its zeros
   return s;
 }
 
-// A place in the sequence of tiles: conversation, item of it (KV head and
-// query chunk), tile of the item.
+// A place in the sequence of tiles: conversation, KV head, query chunk, tile.
 template <typename C>
 struct Cursor {
-  int seq, item, tile;
+  int seq, head, chunk, tile;
   Span span;
-  __device__ __forceinline__ void Next(const KvAttendParams& p, int items) {
+  __device__ __forceinline__ void Next(const KvAttendParams& p, int chunks) {
     if (++tile < span.tiles) return;
     tile = 0;
-    if (++item < items) return;
-    item = 0;
+    if (++chunk < chunks) return;
+    chunk = 0;
+    if (++head < p.kv.n_kv) return;
+    head = 0;
     if (++seq < p.table.n_seq) span = SpanOf<C>(p, seq);
   }
 };
 
-// One step of a warp: R positions, their memory, what of them is in range.
+// One step of a warp: R positions, what of them is in range, and where the
+// 16-row halves lie (offsets in units of 16 bytes).
 struct Step {
-  int lo, hi;                // rows [lo, hi) are in range
-  int64_t off[2], soff[2];   // code and scale offsets of the 16-row halves
-  bool have[2];              // the half has rows in range, and a page
-  uint32_t bad;              // bit h: half h has rows in range but no page
+  int lo, hi;            // rows [lo, hi) are in range
+  uint64_t off[2], soff[2];
+  bool have[2];          // the half has rows in range, and a page
+  uint32_t bad;          // bit h: half h has rows in range but no page
 };
 template <typename C>
-__device__ __forceinline__ Step StepAt(const KvAttendParams& p, const Cursor<C>& c, int warp, int chunks, bool more) {
+__device__ __forceinline__ Step StepAt(const KvAttendParams& p, const Cursor<C>& c, int warp, bool more) {
   Step s;
   const int pos = c.span.base + c.tile * C::TILE + warp * C::R;
   s.lo = c.span.start - pos;
   s.hi = more ? c.span.len - pos : 0;
   s.bad = 0;
-  const int head = c.item / chunks;
-  const int mask = (1 << p.kv.page_log2) - 1;
+  const uint32_t mask = (1u << p.kv.page_log2) - 1;
+  s.off[0] = s.off[1] = s.soff[0] = s.soff[1] = 0;
+  s.have[0] = s.have[1] = false;
+  // (positions lie inside the table and the conversation exists: SpanOf)
+  const int32_t* pages = p.table.pages + c.seq * p.table.stride;
+  const uint64_t head = static_cast<uint32_t>(c.head);
+  const bool two = C::MT == 2 && p.kv.page_log2 == 4;  // the halves lie in two pages
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    s.off[h] = s.soff[h] = 0;
-    s.have[h] = false;
-    if (h < C::MT && s.hi > 16 * h && s.lo < 16 * h + 16) {
-      const int at = pos + 16 * h;
-      const int page = kvd::PageOf(p.table, p.kv.n_pages, c.seq, at >> p.kv.page_log2);
-      if (page >= 0) {
-        s.have[h] = true;
-        s.off[h] = kvd::CodeOffset(p.kv, page, head, at & mask);
-        if (C::QUANT) s.soff[h] = kvd::ScaleOffset(p.kv, page, head, at & mask);
-      } else {
-        s.bad |= 1u << h;
+  for (int h = 0; h < C::MT; ++h) {
+    const bool in = s.hi > 16 * h && s.lo < 16 * h + 16;
+    if (h == 0 || two) {
+      if (in || (h == 0 && !two && s.hi > 0 && s.lo < C::R)) {
+        const int at = pos + 16 * h;
+        const int page = __ldg(pages + (at >> p.kv.page_log2));
+        s.have[h] = static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
+        const uint32_t id = s.have[h] ? page : 0, row = at & mask;
+        s.off[h] = static_cast<uint64_t>(id) * p.page16 + head * p.head16 + static_cast<uint64_t>(row) * p.pos16;
+        if (C::QUANT) s.soff[h] = static_cast<uint64_t>(id) * p.spage16 + head * p.shead16 + row * C::NG / 8;
       }
+    } else {
+      s.have[1] = s.have[0];
+      s.off[1] = s.off[0] + 16ull * p.pos16;
+      if (C::QUANT) s.soff[1] = s.soff[0] + 2 * C::NG;
     }
+    s.bad |= in && !s.have[h] ? 1u << h : 0u;
   }
   return s;
 }
+
+// Copies a step's K codes (and all its scales) or V codes into a slot; rows
+// out of range become zeros.  `lane_off`: the lane's part of a source offset,
+// `row_step`: bytes from one copy instruction's rows to the next's.
 template <typename C, bool V>
-__device__ __forceinline__ void Issue(const KvAttendParams& p, const Step& s, uint32_t slot, int lane) {
+__device__ __forceinline__ void Issue(const KvAttendParams& p, const Step& s, uint32_t slot, int lane,
+                                      int64_t lane_off) {
+  constexpr int kRows = 32 / C::CPR;             // rows of a copy instruction: all in one half
+  constexpr int kPerHalf = 16 / kRows;
   const char* plane = V ? p.kv.v : p.kv.k;
-  if (s.have[0] || s.have[1]) {
+  const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
+  const int64_t row_step = static_cast<int64_t>(kRows) * p.kv.pos_stride;
+  const bool all = s.have[0] && (C::MT == 1 || s.have[1]) && s.lo <= 0 && s.hi >= C::R;
+  if (all && p.kv.pos_stride == C::ROW) {  // dense rows: constant steps
 #pragma unroll
-    for (int j = 0; j < C::R * C::CPR / 32; ++j) {
-      constexpr int kRows = 32 / C::CPR;  // rows of one copy instruction: all in one half
-      const int r = lane / C::CPR + kRows * j, c = lane % C::CPR;
-      const int h = kRows * j / 16;
-      const bool read = s.have[h] && r >= s.lo && r < s.hi;
-      const char* src = plane + s.off[h] + (r & 15) * p.kv.pos_stride + c * 16;
-      CopyAsync16(slot + ChunkAt<C, V>(r, c), read ? src : plane, read);
+    for (int h = 0; h < C::MT; ++h) {
+      const char* src = plane + (s.off[h] << 4) + lane * 16;
+#pragma unroll
+      for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
     }
-    if (C::QUANT) {  // a half's scales are dense: 16 rows of 2 NG bytes
-      constexpr int kPer = 16 * C::NG * 2 / 16;
-      if (lane < C::MT * kPer) {
-        const char* sp = V ? p.kv.v_scale : p.kv.k_scale;
-        const bool second = lane >= kPer, read = second ? s.have[1] : s.have[0];
-        CopyAsync16(slot + C::R * C::ROW + lane * 16,
-                    read ? sp + (second ? s.soff[1] : s.soff[0]) + (lane % kPer) * 16 : sp, read);
+  } else if (all) {
+#pragma unroll
+    for (int h = 0; h < C::MT; ++h) {
+      const char* src = plane + (s.off[h] << 4) + lane_off;
+#pragma unroll
+      for (int j = 0; j < kPerHalf; ++j) {
+        CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src);
+        src += row_step;
       }
+    }
+  } else if (s.have[0] || s.have[1]) {
+#pragma unroll
+    for (int h = 0; h < C::MT; ++h) {
+      const char* src = plane + (s.off[h] << 4) + lane_off;
+#pragma unroll
+      for (int j = 0; j < kPerHalf; ++j) {
+        const int r = lane / C::CPR + kRows * (h * kPerHalf + j);
+        const bool read = s.have[h] && r >= s.lo && r < s.hi;
+        CopyAsync16OrZero(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), read ? src : plane, read);
+        src += row_step;
+      }
+    }
+  }
+  if (C::QUANT && !V && (s.have[0] || s.have[1])) {
+    constexpr int kPer = 16 * C::NG * 2 / 16;  // a half's scales are dense: 16 rows of 2 NG bytes
+    if (lane < 2 * C::MT * kPer) {
+      const bool of_v = lane >= C::MT * kPer;
+      const int i = lane % (C::MT * kPer);
+      const char* sp = of_v ? p.kv.v_scale : p.kv.k_scale;
+      const bool second = i >= kPer, read = second ? s.have[1] : s.have[0];
+      CopyAsync16OrZero(slot + C::R * C::ROW + lane * 16,
+                        read ? sp + ((second ? s.soff[1] : s.soff[0]) << 4) + (i % kPer) * 16 : sp, read);
     }
   }
   CopyCommit();
@@ -268,19 +324,23 @@ __device__ __forceinline__ void Issue(const KvAttendParams& p, const Step& s, ui
 template <typename C>
 struct KRows {
   uint4 w[2];  // q8: 16 codes of rows g and g + 8; q4: .x, .y
-  __device__ __forceinline__ void Load(uint32_t tile, int mt, int gp, int lane) {
-    const int g = lane >> 2, t = lane & 3;
+  // `base`: LaneOffset from the slot
+  __device__ __forceinline__ void Load(uint32_t base, int mt, int gp) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = 16 * mt + 8 * i + g;
       if (C::KIND == KvType::kQ8) {
-        w[i] = Lds128(tile + ChunkAt<C, false>(r, 4 * gp + t));
+        w[i] = Lds128(Moved<C, false>(base, 16 * mt + 8 * i, 4 * gp));
       } else {
-        const uint2 x = Lds64(tile + ChunkAt<C, false>(r, 2 * gp + (t >> 1)) + (t & 1) * 8);
+        const uint2 x = Lds64(Moved<C, false>(base, 16 * mt + 8 * i, 2 * gp));
         w[i].x = x.x;
         w[i].y = x.y;
       }
     }
+  }
+  static __device__ __forceinline__ int LaneOffset(int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    if (C::KIND == KvType::kF16) return ChunkAt<C, false>(lane & 15, lane >> 4);  // for ldmatrix
+    return C::KIND == KvType::kQ8 ? ChunkAt<C, false>(g, t) : ChunkAt<C, false>(g, t >> 1) + (t & 1) * 8;
   }
   __device__ __forceinline__ void Fragment(uint32_t (&a)[4], int j) const {
 #pragma unroll
@@ -302,18 +362,24 @@ struct KRows {
 // tiles (rows = values).  Lane g takes values 8 g .. 8 g + 7 of the group:
 // row g of tile i is value 8 g + i, row g + 8 value 8 g + 4 + i.
 template <typename C>
-__device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t tile, int kt, int gp, int lane) {
+__device__ __forceinline__ int VLaneOffset(int lane) {
   const int g = lane >> 2, t = lane & 3;
+  if (C::KIND == KvType::kF16) return ChunkAt<C, true>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);  // for ldmatrix
+  return C::KIND == KvType::kQ8 ? ChunkAt<C, true>(2 * t, g >> 1) + (g & 1) * 8
+                                : ChunkAt<C, true>(2 * t, g >> 2) + (g & 3) * 4;
+}
+template <typename C>
+__device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t base, int kt, int gp) {
   uint32_t lo[4], hi[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int r = 16 * kt + 2 * t + (j & 1) + 8 * (j >> 1);
+    const int r = 16 * kt + (j & 1) + 8 * (j >> 1);  // from row 2 t
     if (C::KIND == KvType::kQ8) {
-      const uint2 x = Lds64(tile + ChunkAt<C, true>(r, 4 * gp + (g >> 1)) + (g & 1) * 8);
+      const uint2 x = Lds64(Moved<C, true>(base, r, 4 * gp));
       lo[j] = x.x;
       hi[j] = x.y;
     } else {
-      lo[j] = Lds32(tile + ChunkAt<C, true>(r, 2 * gp + (g >> 2)) + (g & 3) * 4);
+      lo[j] = Lds32(Moved<C, true>(base, r, 2 * gp));
     }
   }
 #pragma unroll
@@ -375,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   constexpr int D = C::D;
   extern __shared__ __align__(128) char smem[];
   __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-  __shared__ long long s_sum[kWarps + 1], s_begin;
+  __shared__ long long s_sum[kWarps], s_begin;
   __shared__ int s_seq, s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.kv.n_kv;
@@ -407,7 +473,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   }
   const long long blocks = min(static_cast<long long>(gridDim.x), total);
   if (blockIdx.x >= blocks) return;
-  const long long first = total * blockIdx.x / blocks, last = total * (blockIdx.x + 1) / blocks;
+  const long long first = total * blockIdx.x / blocks;
+  int left = static_cast<int>(total * (blockIdx.x + 1) / blocks - first);  // tiles to do
   if (first >= upto - mine && first < upto) {
     long long at = upto - mine;
     int s = tid * run;
@@ -423,45 +490,55 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   Cursor<C> use;
   use.seq = s_seq;
   use.span = SpanOf<C>(p, use.seq);
-  use.item = static_cast<int>((first - s_begin) / use.span.tiles);
-  use.tile = static_cast<int>((first - s_begin) % use.span.tiles);
+  {
+    const long long in = first - s_begin;  // inside the conversation
+    const int item = static_cast<int>(in / use.span.tiles);
+    use.head = item / chunks;
+    use.chunk = item % chunks;
+    use.tile = static_cast<int>(in % use.span.tiles);
+  }
   Cursor<C> fill = use;
 
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
   float* comb = reinterpret_cast<float*>(smem + kWarps * C::RING);
+  float* mineq = comb + warp * (C::COMB / 4);
+  const int64_t lane_off = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
+  const uint32_t k_lane = KRows<C>::LaneOffset(lane), v_lane = VLaneOffset<C>(lane);
   uint32_t bad = 0;  // two bits per step in flight
-  long long to_fill = last - first;
+  int to_fill = left;
 #pragma unroll
   for (int d = 0; d < C::DEPTH; ++d) {
-    const Step s = StepAt<C>(p, fill, warp, chunks, to_fill > 0);
-    Issue<C, false>(p, s, ring + (2 * d) * C::SLOT, lane);
-    Issue<C, true>(p, s, ring + (2 * d + 1) * C::SLOT, lane);
+    const Step s = StepAt<C>(p, fill, warp, to_fill > 0);
+    const uint32_t slot = ring + d * (C::KSLOT + C::VSLOT);
+    Issue<C, false>(p, s, slot, lane, lane_off);
+    Issue<C, true>(p, s, slot + C::KSLOT, lane, lane_off);
     bad = bad << 2 | s.bad;
-    if (--to_fill > 0) fill.Next(p, items);
+    if (--to_fill > 0) fill.Next(p, chunks);
   }
 
   uint32_t qh[C::KS][2], ql[C::PACK ? 1 : C::KS][2];
   const bool two_terms = p.type == ElemType::kF32;
-  float cs[2];                 // from products of the f16 terms to scores in log2 units
-  float m[2], l[2];            // of columns 2 t and 2 t + 1
+  float cs[2];            // from products of the f16 terms to scores in log2 units
+  float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
+  float l[2];             // sum of this lane's weights
   float acc[D / 16][4];
-  int nu = 0;                  // biased exponent of the power of two over the V scales seen
-  int seg = 0;                 // first tile of the item in this block
+  int nu = 0;             // biased exponent of the power of two over the V scales seen
+  int queries = 0, seg = 0;  // of the item; its first tile in this block
   bool fresh = true;
-  int slot = 0;
+  long long at = first;
+  uint32_t kslot = ring;
 
-  for (long long at = first; at < last; ++at) {
-    Step next = StepAt<C>(p, fill, warp, chunks, to_fill > 0);
-    const int chunk = use.item % chunks;
-    const int queries = min(per_chunk, group - chunk * per_chunk);
-    const int64_t col = (static_cast<int64_t>(use.item / chunks) * group + chunk * per_chunk) * D;
+  for (;;) {
+    const Step next = StepAt<C>(p, fill, warp, to_fill > 0);
     if (fresh) {
       fresh = false;
       seg = use.tile;
+      queries = min(per_chunk, group - use.chunk * per_chunk);
       const int qi = C::PACK ? g & 3 : g;
       float x[C::KS][2][2] = {};
       if (qi < queries) {
-        const int64_t o = use.seq * p.q_stride + col + qi * D;
+        const int64_t o = use.seq * p.q_stride +
+                          (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk + qi) * D;
         switch (p.type) {
           case ElemType::kF32: ReadQ<C>(x, static_cast<const float*>(p.q) + o, t); break;
           case ElemType::kF16: ReadQ<C>(x, static_cast<const __half*>(p.q) + o, t); break;
@@ -475,10 +552,13 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[ks][e >> 1][e & 1]));
       }
       top = LaneQuadMax(top);
-      // 2^-e of the largest value's exponent (kept in f32's normal range)
+      // 2^-e of the largest value's exponent (kept in f32's normal range); the
+      // sign of the scale goes with it, so that cs is positive and the largest
+      // product has the largest score (a scale of zero clears q instead)
       const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
-      const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-      const float up = __uint_as_float(static_cast<uint32_t>(e) << 23) * (p.scale * kLog2e);
+      const float mag = fabsf(p.scale) * kLog2e;
+      const float down = p.scale == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23), p.scale);
+      const float up = p.scale == 0.f ? 1.f : fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * mag, 1e-37f);
 #pragma unroll
       for (int ks = 0; ks < C::KS; ++ks) {
 #pragma unroll
@@ -498,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         cs[c] = __shfl_sync(0xFFFFFFFFu, up, 4 * (C::PACK ? (2 * t + c) & 3 : 2 * t + c));
-        m[c] = -INFINITY;
+        m[c] = ref[c] = -INFINITY;
         l[c] = 0.f;
       }
 #pragma unroll
@@ -513,45 +593,52 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     const int lo = use.span.start - pos, hi = use.span.len - pos;
     const bool work = lo < C::R && hi > 0;
     const uint32_t bad_now = (bad >> (2 * (C::DEPTH - 1))) & 3u;
-    const uint32_t kslot = ring + (2 * slot) * C::SLOT, vslot = kslot + C::SLOT;
+    const bool edge = lo > 0 || hi < C::R || bad_now != 0;
+    const uint32_t vslot = kslot + C::KSLOT;
 
-    // ---- scores
+    // ---- scores (and the V scales)
     CopyWait<2 * C::DEPTH - 1>();
     __syncwarp();
     float s[C::MT][4];
+    uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
     if (work) {
+      const uint32_t kbase = kslot + k_lane, sbase = kslot + C::R * C::ROW + g * (2 * C::NG);
 #pragma unroll
       for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[mt][c] = 0.f;
         if (!C::QUANT) {
 #pragma unroll
           for (int ks = 0; ks < C::KS; ++ks) {
             uint32_t a[4];
-            LdMatrix(a, kslot + ChunkAt<C, false>(16 * mt + (lane & 15), 2 * ks + (lane >> 4)));
-            Mma(s[mt], a, qh[ks][0], qh[ks][1]);
+            LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
+            ks == 0 ? MmaFirst(s[mt], a, qh[ks][0], qh[ks][1]) : Mma(s[mt], a, qh[ks][0], qh[ks][1]);
             if (!C::PACK && two_terms) Mma(s[mt], a, ql[C::PACK ? 0 : ks][0], ql[C::PACK ? 0 : ks][1]);
           }
         } else {
+          float2 d[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a = sbase + (16 * mt + 8 * i) * (2 * C::NG);
+            const uint32_t k = C::NG == 2 ? Lds32(a) : Lds16(a);
+            vsc[mt][i] = C::NG == 2 ? Lds32(a + C::SC) : Lds16(a + C::SC);
+            d[i] = __half22float2(BitsHalf(k));
+          }
 #pragma unroll
           for (int gp = 0; gp < C::NG; ++gp) {
             KRows<C> rows;
-            rows.Load(kslot, mt, gp, lane);
-            float part[4] = {};
+            rows.Load(kbase, mt, gp);
+            float part[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int ks = 4 * gp + j;
               uint32_t a[4];
               rows.Fragment(a, j);
-              Mma(part, a, qh[ks][0], qh[ks][1]);
+              j == 0 ? MmaFirst(part, a, qh[ks][0], qh[ks][1]) : Mma(part, a, qh[ks][0], qh[ks][1]);
               if (!C::PACK && two_terms) Mma(part, a, ql[C::PACK ? 0 : ks][0], ql[C::PACK ? 0 : ks][1]);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(
-                  Lds16(kslot + C::R * C::ROW + ((16 * mt + 8 * i + g) * C::NG + gp) * 2))));
-              s[mt][2 * i] += part[2 * i] * d;
-              s[mt][2 * i + 1] += part[2 * i + 1] * d;
+            for (int c = 0; c < 4; ++c) {
+              const float f = gp == 0 ? d[c >> 1].x : d[c >> 1].y;
+              s[mt][c] = gp == 0 ? part[c] * f : fmaf(part[c], f, s[mt][c]);
             }
           }
         }
@@ -562,46 +649,61 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     __syncwarp();
-    Issue<C, false>(p, next, kslot, lane);
+    Issue<C, false>(p, next, kslot, lane, lane_off);
 
-    // ---- weights
+    // ---- weights: 2^(score - ref) with ref a power of two over the largest,
+    // so that a weight times its V scale is at most 2^14 and small ones stay
+    // normal f16 numbers
     float alpha[2] = {1.f, 1.f};
     if (work) {
-      float mx[2] = {-INFINITY, -INFINITY};
-      const bool edge = lo > 0 || hi < C::R || bad_now != 0;
-#pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v = s[mt][c] * cs[c & 1];
-          if (edge) {
-            const int r = 16 * mt + 8 * (c >> 1) + g;
-            if ((bad_now >> mt) & 1) v = kvd::Nan();
-            if (r < lo || r >= hi) v = -INFINITY;
-          }
-          s[mt][c] = v;
-          mx[c & 1] = fmaxf(mx[c & 1], v);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], o));
-        const float mn = fmaxf(m[c], mx[c]);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        alpha[c] = Exp2(m[c] - ref);
-        m[c] = mn;
-        float sum = 0.f;
+      if (edge) {
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float w = Exp2(s[mt][2 * i + c] - ref);
-            s[mt][2 * i + c] = w;
-            sum += w;
+            const int r = 16 * mt + 8 * i + g;
+            if ((bad_now >> mt) & 1) s[mt][2 * i] = s[mt][2 * i + 1] = kvd::Nan();
+            if (r < lo || r >= hi) {
+              s[mt][2 * i] = s[mt][2 * i + 1] = -INFINITY;
+              vsc[mt][i] = 0;  // a scale out of range may be anything
+            }
           }
         }
-        l[c] = l[c] * alpha[c] + sum;
+      }
+      if (C::QUANT) {
+        __half2 top = BitsHalf(0);
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top = __hmax2(top, __habs2(BitsHalf(vsc[mt][i])));
+        }
+        const uint32_t u = HalfBits(top);
+        const uint32_t f16 = __reduce_max_sync(0xFFFFFFFFu, max(u & 0xFFFFu, u >> 16));
+        const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(f16)));
+        nu = max(nu, min(static_cast<int>(__float_as_uint(d) >> 23), 127 + 16) + 1);
+      }
+      const float shift = C::QUANT ? static_cast<float>(nu - 127 - kWeightBits) : -static_cast<float>(kWeightBits);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = fmaxf(s[0][c], s[0][2 + c]);
+#pragma unroll
+        for (int mt = 1; mt < C::MT; ++mt) top = fmaxf(top, fmaxf(s[mt][c], s[mt][2 + c]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        m[c] = fmaxf(m[c], top * cs[c]);
+        const float now = (m[c] == -INFINITY ? 0.f : m[c]) + shift;
+        alpha[c] = Exp2(ref[c] - now);
+        ref[c] = m[c] == -INFINITY ? -INFINITY : now;
+        l[c] *= alpha[c];
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float w = Exp2(fmaf(s[mt][2 * i + c], cs[c], -now));
+            s[mt][2 * i + c] = w;
+            l[c] += w;
+          }
+        }
       }
     }
 
@@ -609,46 +711,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     CopyWait<2 * C::DEPTH - 1>();
     __syncwarp();
     if (work) {
-      float ws[C::MT][2][C::NG];  // weight factors of the lane's rows
-      if (!C::QUANT) {
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) ws[mt][0][0] = ws[mt][1][0] = static_cast<float>(1 << kWeightBits);
-      } else {
-        uint32_t top = 0;
-        const bool edge = lo > 0 || hi < C::R;
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = 16 * mt + 8 * i + g;
-#pragma unroll
-            for (int gp = 0; gp < C::NG; ++gp) {
-              uint32_t d = Lds16(vslot + C::R * C::ROW + (r * C::NG + gp) * 2);
-              if (edge && (r < lo || r >= hi)) d = 0;  // a scale out of range may be anything
-              top = max(top, d & 0x7FFFu);
-              ws[mt][i][gp] = __half2float(__ushort_as_half(static_cast<unsigned short>(d)));
-            }
-          }
-        }
-        top = __reduce_max_sync(0xFFFFFFFFu, top);
-        const int e = min(static_cast<int>(__float_as_uint(__half2float(
-                              __ushort_as_half(static_cast<unsigned short>(top)))) >> 23), 127 + 16) + 1;
-        if (e > nu) {
-          const float f = __uint_as_float(static_cast<uint32_t>(127 + nu - e) << 23);
-          alpha[0] *= f;
-          alpha[1] *= f;
-          nu = e;
-        }
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + kWeightBits + 127 - nu) << 23);
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int gp = 0; gp < C::NG; ++gp) ws[mt][i][gp] *= up;
-          }
-        }
-      }
+      const uint32_t vbase = vslot + v_lane;
+      const float of_rest = t >= 2 ? 1.f : 0.f, of_lead = t >= 2 ? -1.f : 1.f;  // which term this lane's columns take
 #pragma unroll
       for (int gp = 0; gp < C::NG; ++gp) {
         uint32_t b[C::MT][2][C::PACK ? 1 : 2];
@@ -656,72 +720,71 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float u = s[mt][2 * i] * ws[mt][i][gp], v = s[mt][2 * i + 1] * ws[mt][i][gp];
-            const uint32_t h = PackHalf(u, v);
-            const float2 f = __half22float2(BitsHalf(h));
-            const uint32_t r = PackHalf(u - f.x, v - f.y);
+            float u = s[mt][2 * i], v = s[mt][2 * i + 1];
+            if (C::QUANT) {
+              const float2 d = __half22float2(BitsHalf(vsc[mt][i]));
+              u *= gp == 0 ? d.x : d.y;
+              v *= gp == 0 ? d.x : d.y;
+            }
+            // the first term is the leading 11 bits, the second the rest
+            const float uh = __uint_as_float(__float_as_uint(u) & 0xFFFFE000u);
+            const float vh = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
             if (C::PACK) {
-              b[mt][i][0] = Transposed(t >= 2 ? r : h);
+              b[mt][i][0] = Transposed(PackHalf(fmaf(u, of_rest, uh * of_lead), fmaf(v, of_rest, vh * of_lead)));
             } else {
-              b[mt][i][0] = Transposed(h);
-              b[mt][i][C::PACK ? 0 : 1] = Transposed(r);
+              b[mt][i][0] = Transposed(PackHalf(uh, vh));
+              b[mt][i][C::PACK ? 0 : 1] = Transposed(PackHalf(u - uh, v - vh));
             }
           }
         }
-        constexpr int kTiles = C::QUANT ? 4 : D / 16;
         if (C::QUANT) {
-          float part[4][4] = {};
+          float part[4][4];
 #pragma unroll
           for (int kt = 0; kt < C::MT; ++kt) {
             uint32_t a[4][4];
-            VFragments<C>(a, vslot, kt, gp, lane);
+            VFragments<C>(a, vbase, kt, gp);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-#pragma unroll
-              for (int n = 0; n < (C::PACK ? 1 : 2); ++n) Mma(part[i], a[i], b[kt][0][n], b[kt][1][n]);
+              kt == 0 ? MmaFirst(part[i], a[i], b[kt][0][0], b[kt][1][0]) : Mma(part[i], a[i], b[kt][0][0], b[kt][1][0]);
+              if (!C::PACK) Mma(part[i], a[i], b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
             }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              acc[4 * gp + i][c] = acc[4 * gp + i][c] * alpha[c & 1] + part[i][c];
-            }
+            for (int c = 0; c < 4; ++c) acc[4 * gp + i][c] = fmaf(acc[4 * gp + i][c], alpha[c & 1], part[i][c]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            float part[4] = {};
+          for (int i = 0; i < D / 16; ++i) {
+            float part[4];
 #pragma unroll
             for (int kt = 0; kt < C::MT; ++kt) {
               uint32_t a[4];
-              LdMatrixT(a, vslot + ChunkAt<C, true>(16 * kt + (lane & 7) + ((lane >> 4) << 3),
-                                                    2 * i + ((lane >> 3) & 1)));
-#pragma unroll
-              for (int n = 0; n < (C::PACK ? 1 : 2); ++n) Mma(part, a, b[kt][0][n], b[kt][1][n]);
+              LdMatrixT(a, Moved<C, true>(vbase, 16 * kt, 2 * i));
+              kt == 0 ? MmaFirst(part, a, b[kt][0][0], b[kt][1][0]) : Mma(part, a, b[kt][0][0], b[kt][1][0]);
+              if (!C::PACK) Mma(part, a, b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][c] = acc[i][c] * alpha[c & 1] + part[c];
+            for (int c = 0; c < 4; ++c) acc[i][c] = fmaf(acc[i][c], alpha[c & 1], part[c]);
           }
         }
       }
     }
     __syncwarp();
-    Issue<C, true>(p, next, vslot, lane);
+    Issue<C, true>(p, next, vslot, lane, lane_off);
     bad = bad << 2 | next.bad;
-    if (--to_fill > 0) fill.Next(p, items);
-    slot = slot + 1 == C::DEPTH ? 0 : slot + 1;
+    if (--to_fill > 0) fill.Next(p, chunks);
+    kslot = kslot + C::KSLOT + C::VSLOT == ring + C::RING ? ring : kslot + C::KSLOT + C::VSLOT;
 
     // ---- the end of the item, or of this block's share of it
-    if (use.tile + 1 == use.span.tiles || at + 1 == last) {
+    if (use.tile + 1 == use.span.tiles || left == 1) {
       fresh = true;
-      const float down = C::QUANT ? __uint_as_float(static_cast<uint32_t>(nu - kWeightBits) << 23) : 1.f / (1 << kWeightBits);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], o);
       }
-      float* mineq = comb + warp * (C::COMB / 4);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
@@ -729,19 +792,19 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           float v = acc[i][c];
           if (C::PACK) v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
           const int value = C::QUANT ? 64 * (i >> 2) + 8 * g + 4 * (c >> 1) + (i & 3) : 16 * i + 8 * (c >> 1) + g;
-          if (!C::PACK || t < 2) mineq[(2 * t + (c & 1)) * D + value] = v * down;
+          if (!C::PACK || t < 2) mineq[(2 * t + (c & 1)) * D + value] = v;
         }
       }
       if (g == 0 && (!C::PACK || t < 2)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          s_m[warp][2 * t + c] = m[c];
+          s_m[warp][2 * t + c] = ref[c];
           s_l[warp][2 * t + c] = l[c];
         }
       }
       __syncthreads();
       const bool whole = seg == 0 && use.tile + 1 == use.span.tiles;
-      const int64_t out = use.seq * p.out_stride + col;
+      const int64_t out = use.seq * p.out_stride + (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
       const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
       // The warps' shares joined: value i of the item's queries, its sum, its maximum.
@@ -772,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
                                                   (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256);
         auto record = [&](int b) { return records + (2 * b + (b == b0 ? 1 : 0)) * kRecord; };
-        unsigned* count = static_cast<unsigned*>(p.workspace) + static_cast<int64_t>(use.seq) * items + use.item;
+        unsigned* count = static_cast<unsigned*>(p.workspace) + (static_cast<int64_t>(use.seq) * p.kv.n_kv + use.head) * chunks + use.chunk;
         float* rec = record(blockIdx.x);
         for (int i = tid; i < queries * D; i += kThreads) {
           float sum, top;
@@ -863,7 +926,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
       __syncthreads();  // the next item writes the join area again
     }
-    use.Next(p, items);
+    if (--left == 0) break;
+    ++at;
+    use.Next(p, chunks);
   }
   CopyWait<0>();
 }
@@ -889,7 +954,13 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
   const int64_t tiles = ((cap + 15) / C::TILE + 1) * p.kv.n_kv * chunks;
   if (tiles < grid && tiles * p.table.n_seq < grid) grid = static_cast<int>(tiles * p.table.n_seq);
-  KvAttendKernel<C><<<grid, kThreads, C::SMEM, s>>>(p);
+  KvAttendParams a = p;
+  a.page16 = static_cast<uint32_t>(p.kv.page_stride / 16);
+  a.head16 = static_cast<uint32_t>(p.kv.head_stride / 16);
+  a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);
+  a.spage16 = static_cast<uint32_t>(p.kv.scale_page_stride / 16);
+  a.shead16 = static_cast<uint32_t>(p.kv.scale_head_stride / 16);
+  KvAttendKernel<C><<<grid, kThreads, C::SMEM, s>>>(a);
 }
 
 template <int D, KvType KIND>
