@@ -101,10 +101,6 @@ __device__ __forceinline__ uint32_t Moved(uint32_t base, int dr, int dc) {
 __device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void CopyAsync16OrZero(uint32_t dst, const void* src, bool read) {
-  const int n = read ? 16 : 0;  // the rest is filled with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void CopyWait() {
@@ -158,6 +154,9 @@ __device__ __forceinline__ uint4 Lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
   return x;
 }
+__device__ __forceinline__ void Sts128Zero(uint32_t a) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
+}
 __device__ __forceinline__ float Exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -173,13 +172,22 @@ __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return HalfBi
 __device__ __forceinline__ uint32_t SubHalf(uint32_t x, uint32_t bias) {
   return HalfBits(__hsub2(BitsHalf(x), BitsHalf(bias)));
 }
+// The 0x6400 pair comes from a kernel argument: as a constant beside the mask
+// it would take a second instruction, since one may hold a single literal.
 constexpr uint32_t kMagic = 0x64006400u;
-constexpr uint32_t kMagicByte = 0x64u;
 constexpr uint32_t kBias8 = 0x64806480u;  // 1024 + 128
 constexpr uint32_t kBias4 = 0x64086408u;  // 1024 + 8
-__device__ __forceinline__ uint32_t Low4(uint32_t w) { return SubHalf((w & 0x000F000Fu) | kMagic, kBias4); }
-__device__ __forceinline__ uint32_t High4(uint32_t w) {  // (1024 + 16 u) / 16 - 72 = u - 8
-  return HalfBits(__hfma2(BitsHalf((w & 0x00F000F0u) | kMagic), BitsHalf(0x2C002C00u), BitsHalf(0xD480D480u)));
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t MaskOr(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));  // (w & MASK) | magic
+  return r;
+}
+__device__ __forceinline__ uint32_t Low4(uint32_t w, uint32_t magic) {
+  return SubHalf(MaskOr<0x000F000Fu>(w, magic), kBias4);
+}
+__device__ __forceinline__ uint32_t High4(uint32_t w, uint32_t magic) {  // (1024 + 16 u) / 16 - 72 = u - 8
+  return HalfBits(__hfma2(BitsHalf(MaskOr<0x00F000F0u>(w, magic)), BitsHalf(0x2C002C00u), BitsHalf(0xD480D480u)));
 }
 
 // ------------------------------------------------------------------ work
@@ -205,8 +213,9 @@ template <typename C>
 struct Cursor {
   int seq, head, chunk, tile;
   Span span;
-  __device__ __forceinline__ void Next(const KvAttendParams& p, int chunks) {
-    if (++tile < span.tiles) return;
+  __device__ __forceinline__ void Next(const KvAttendParams& p, int chunks, int n = 1) {
+    tile += n;
+    if (tile < span.tiles) return;
     tile = 0;
     if (++chunk < chunks) return;
     chunk = 0;
@@ -216,105 +225,100 @@ struct Cursor {
   }
 };
 
-// One step of a warp: R positions, what of them is in range, and where the
-// 16-row halves lie (offsets in units of 16 bytes).
-struct Step {
-  int lo, hi;            // rows [lo, hi) are in range
-  uint64_t off[2], soff[2];
-  bool have[2];          // the half has rows in range, and a page
-  uint32_t bad;          // bit h: half h has rows in range but no page
+// The copying side of a warp.  The places of the next few steps are worked
+// out together, one 16-row half per lane, and left in shared memory; the page
+// ids they need are requested one such batch earlier.
+struct Place {
+  int64_t code, scale;  // byte offsets of the half in the planes
 };
 template <typename C>
-__device__ __forceinline__ Step StepAt(const KvAttendParams& p, const Cursor<C>& c, int warp, bool more) {
-  Step s;
-  const int pos = c.span.base + c.tile * C::TILE + warp * C::R;
-  s.lo = c.span.start - pos;
-  s.hi = more ? c.span.len - pos : 0;
-  s.bad = 0;
-  const uint32_t mask = (1u << p.kv.page_log2) - 1;
-  s.off[0] = s.off[1] = s.soff[0] = s.soff[1] = 0;
-  s.have[0] = s.have[1] = false;
-  // (positions lie inside the table and the conversation exists: SpanOf)
-  const int32_t* pages = p.table.pages + c.seq * p.table.stride;
-  const uint64_t head = static_cast<uint32_t>(c.head);
-  const bool two = C::MT == 2 && p.kv.page_log2 == 4;  // the halves lie in two pages
-#pragma unroll
-  for (int h = 0; h < C::MT; ++h) {
-    const bool in = s.hi > 16 * h && s.lo < 16 * h + 16;
-    if (h == 0 || two) {
-      if (in || (h == 0 && !two && s.hi > 0 && s.lo < C::R)) {
-        const int at = pos + 16 * h;
-        const int page = __ldg(pages + (at >> p.kv.page_log2));
-        s.have[h] = static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
-        const uint32_t id = s.have[h] ? page : 0, row = at & mask;
-        s.off[h] = static_cast<uint64_t>(id) * p.page16 + head * p.head16 + static_cast<uint64_t>(row) * p.pos16;
-        if (C::QUANT) s.soff[h] = static_cast<uint64_t>(id) * p.spage16 + head * p.shead16 + row * C::NG / 8;
-      }
-    } else {
-      s.have[1] = s.have[0];
-      s.off[1] = s.off[0] + 16ull * p.pos16;
-      if (C::QUANT) s.soff[1] = s.soff[0] + 2 * C::NG;
-    }
-    s.bad |= in && !s.have[h] ? 1u << h : 0u;
-  }
-  return s;
-}
+struct Filler {
+  static constexpr int kHalves = 8, kSteps = kHalves / C::MT;
+  Cursor<C> at;        // the first step after the batch
+  int left;            // steps not yet put in a batch
+  int count = 0;       // steps of the batch not yet issued
+  int next = 0;        // first half of the next of them
+  uint32_t have = 0;   // bit per half of the batch, the next step's lowest: it has rows in range and a page
+  uint32_t bad = 0;    // as `have`: it has rows in range but no page
+  int page = 0;        // this lane's half of the next batch
+  const char *k, *v, *scale;  // this lane's part of a copy's source, without the place
+  Place* places;
 
-// Copies a step's K codes (and all its scales) or V codes into a slot; rows
-// out of range become zeros.  `lane_off`: the lane's part of a source offset,
-// `row_step`: bytes from one copy instruction's rows to the next's.
-template <typename C, bool V>
-__device__ __forceinline__ void Issue(const KvAttendParams& p, const Step& s, uint32_t slot, int lane,
-                                      int64_t lane_off) {
-  constexpr int kRows = 32 / C::CPR;             // rows of a copy instruction: all in one half
-  constexpr int kPerHalf = 16 / kRows;
-  const char* plane = V ? p.kv.v : p.kv.k;
-  const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
-  const int64_t row_step = static_cast<int64_t>(kRows) * p.kv.pos_stride;
-  const bool all = s.have[0] && (C::MT == 1 || s.have[1]) && s.lo <= 0 && s.hi >= C::R;
-  if (all && p.kv.pos_stride == C::ROW) {  // dense rows: constant steps
-#pragma unroll
-    for (int h = 0; h < C::MT; ++h) {
-      const char* src = plane + (s.off[h] << 4) + lane * 16;
-#pragma unroll
-      for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
-    }
-  } else if (all) {
-#pragma unroll
-    for (int h = 0; h < C::MT; ++h) {
-      const char* src = plane + (s.off[h] << 4) + lane_off;
-#pragma unroll
-      for (int j = 0; j < kPerHalf; ++j) {
-        CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src);
-        src += row_step;
-      }
-    }
-  } else if (s.have[0] || s.have[1]) {
-#pragma unroll
-    for (int h = 0; h < C::MT; ++h) {
-      const char* src = plane + (s.off[h] << 4) + lane_off;
-#pragma unroll
-      for (int j = 0; j < kPerHalf; ++j) {
-        const int r = lane / C::CPR + kRows * (h * kPerHalf + j);
-        const bool read = s.have[h] && r >= s.lo && r < s.hi;
-        CopyAsync16OrZero(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), read ? src : plane, read);
-        src += row_step;
-      }
+  __device__ __forceinline__ int Pos(int warp, int lane) const {
+    return at.span.base + (at.tile + lane / C::MT) * C::TILE + warp * C::R + (lane % C::MT) * 16;
+  }
+  __device__ __forceinline__ bool InRange(int pos, int lane) const {
+    return lane < kHalves && lane / C::MT < min(left, at.span.tiles - at.tile) && pos + 16 > at.span.start &&
+           pos < at.span.len;
+  }
+  __device__ __forceinline__ void Request(const KvAttendParams& p, int warp, int lane) {
+    const int pos = Pos(warp, lane);
+    // (positions in range lie inside the table: SpanOf)
+    if (left > 0 && InRange(pos, lane)) {
+      page = __ldg(p.table.pages + at.seq * p.table.stride + (pos >> p.kv.page_log2));
     }
   }
-  if (C::QUANT && !V && (s.have[0] || s.have[1])) {
-    constexpr int kPer = 16 * C::NG * 2 / 16;  // a half's scales are dense: 16 rows of 2 NG bytes
-    if (lane < 2 * C::MT * kPer) {
-      const bool of_v = lane >= C::MT * kPer;
-      const int i = lane % (C::MT * kPer);
-      const char* sp = of_v ? p.kv.v_scale : p.kv.k_scale;
-      const bool second = i >= kPer, read = second ? s.have[1] : s.have[0];
-      CopyAsync16OrZero(slot + C::R * C::ROW + lane * 16,
-                        read ? sp + ((second ? s.soff[1] : s.soff[0]) << 4) + (i % kPer) * 16 : sp, read);
+  __device__ __forceinline__ void Batch(const KvAttendParams& p, int warp, int lane, int chunks) {
+    const int pos = Pos(warp, lane);
+    const bool in = InRange(pos, lane);
+    const bool ok = in && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
+    const int row = pos & ((1 << p.kv.page_log2) - 1);
+    __syncwarp();  // the last batch has been read
+    if (lane < kHalves) {
+      Place q;
+      q.code = page * p.kv.page_stride + at.head * p.kv.head_stride + row * p.kv.pos_stride;
+      q.scale = page * p.kv.scale_page_stride + at.head * p.kv.scale_head_stride + row * (2 * C::NG);
+      places[lane] = q;
     }
+    have = __ballot_sync(0xFFFFFFFFu, ok);
+    bad = __ballot_sync(0xFFFFFFFFu, in && !ok);
+    count = min(kSteps, min(left, at.span.tiles - at.tile));
+    left -= count;
+    next = 0;
+    if (left > 0) at.Next(p, chunks, count);
+    Request(p, warp, lane);
   }
-  CopyCommit();
-}
+
+  // Copies the next step's K codes (and all its scales) or V codes into a
+  // slot.  Halves that are out of range or have no page are left as they are.
+  template <bool V>
+  __device__ __forceinline__ void Issue(const KvAttendParams& p, uint32_t slot, int lane) {
+    if (count > 0) {
+      constexpr int kRows = 32 / C::CPR, kPerHalf = 16 / kRows;  // rows of a copy instruction: all in one half
+      const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
+      const Place* q = places + next;
+#pragma unroll
+      for (int h = 0; h < C::MT; ++h) {
+        if ((have >> h) & 1) {
+          const char* src = (V ? v : k) + q[h].code;
+          if (p.kv.pos_stride == C::ROW) {  // dense rows: constant steps
+#pragma unroll
+            for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPerHalf; ++j) {
+              CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + j * kRows * p.kv.pos_stride);
+            }
+          }
+        }
+      }
+      if (C::QUANT && !V) {
+        constexpr int kPer = 2 * C::NG;  // a half's scales are dense: 16 rows of 2 NG bytes, in 16-byte pieces
+        const int h = lane / kPer % C::MT;
+        if (lane < 2 * C::MT * kPer && ((have >> h) & 1)) {
+          CopyAsync16(slot + C::R * C::ROW + lane * 16, scale + q[h].scale);
+        }
+      }
+    }
+    CopyCommit();
+  }
+  __device__ __forceinline__ void Pop() {
+    --count;
+    next += C::MT;
+    have >>= C::MT;
+    bad >>= C::MT;
+  }
+};
 
 // ------------------------------------------------------------------ operands
 
@@ -342,17 +346,17 @@ struct KRows {
     if (C::KIND == KvType::kF16) return ChunkAt<C, false>(lane & 15, lane >> 4);  // for ldmatrix
     return C::KIND == KvType::kQ8 ? ChunkAt<C, false>(g, t) : ChunkAt<C, false>(g, t >> 1) + (t & 1) * 8;
   }
-  __device__ __forceinline__ void Fragment(uint32_t (&a)[4], int j) const {
+  __device__ __forceinline__ void Fragment(uint32_t (&a)[4], int j, uint32_t magic) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (C::KIND == KvType::kQ8) {
         const uint32_t u = (j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w) ^ 0x80808080u;
-        a[i] = SubHalf(__byte_perm(u, kMagicByte, 0x4140), kBias8);
-        a[2 + i] = SubHalf(__byte_perm(u, kMagicByte, 0x4342), kBias8);
+        a[i] = SubHalf(__byte_perm(u, magic, 0x5150), kBias8);
+        a[2 + i] = SubHalf(__byte_perm(u, magic, 0x5352), kBias8);
       } else {
         const uint32_t u = (j < 2 ? w[i].x : w[i].y) >> ((j & 1) * 8);
-        a[i] = Low4(u);
-        a[2 + i] = High4(u);
+        a[i] = Low4(u, magic);
+        a[2 + i] = High4(u, magic);
       }
     }
   }
@@ -369,7 +373,7 @@ __device__ __forceinline__ int VLaneOffset(int lane) {
                                 : ChunkAt<C, true>(2 * t, g >> 2) + (g & 3) * 4;
 }
 template <typename C>
-__device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t base, int kt, int gp) {
+__device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t base, int kt, int gp, uint32_t magic) {
   uint32_t lo[4], hi[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -389,19 +393,19 @@ __device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t base, i
       for (int m = 0; m < 2; ++m) {
         const uint32_t w0 = m ? hi[2 * k] : lo[2 * k], w1 = m ? hi[2 * k + 1] : lo[2 * k + 1];
         const uint32_t x = __byte_perm(w0, w1, 0x5140) ^ 0x80808080u, y = __byte_perm(w0, w1, 0x7362) ^ 0x80808080u;
-        a[0][2 * k + m] = SubHalf(__byte_perm(x, kMagicByte, 0x4140), kBias8);
-        a[1][2 * k + m] = SubHalf(__byte_perm(x, kMagicByte, 0x4342), kBias8);
-        a[2][2 * k + m] = SubHalf(__byte_perm(y, kMagicByte, 0x4140), kBias8);
-        a[3][2 * k + m] = SubHalf(__byte_perm(y, kMagicByte, 0x4342), kBias8);
+        a[0][2 * k + m] = SubHalf(__byte_perm(x, magic, 0x5150), kBias8);
+        a[1][2 * k + m] = SubHalf(__byte_perm(x, magic, 0x5352), kBias8);
+        a[2][2 * k + m] = SubHalf(__byte_perm(y, magic, 0x5150), kBias8);
+        a[3][2 * k + m] = SubHalf(__byte_perm(y, magic, 0x5352), kBias8);
       }
     } else {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const uint32_t x = __byte_perm(lo[2 * k], lo[2 * k + 1], m ? 0x7632 : 0x5410), y = x >> 8;
-        a[0][2 * k + m] = Low4(x);
-        a[1][2 * k + m] = High4(x);
-        a[2][2 * k + m] = Low4(y);
-        a[3][2 * k + m] = High4(y);
+        a[0][2 * k + m] = Low4(x, magic);
+        a[1][2 * k + m] = High4(x, magic);
+        a[2][2 * k + m] = Low4(y, magic);
+        a[3][2 * k + m] = High4(y, magic);
       }
     }
   }
@@ -443,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   __shared__ float s_m[kWarps][8], s_l[kWarps][8];
   __shared__ long long s_sum[kWarps], s_begin;
   __shared__ int s_seq, s_last;
+  __shared__ __align__(16) Place s_places[kWarps][Filler<C>::kHalves];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.kv.n_kv;
   const int chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
@@ -497,26 +502,37 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     use.chunk = item % chunks;
     use.tile = static_cast<int>(in % use.span.tiles);
   }
-  Cursor<C> fill = use;
 
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
   float* comb = reinterpret_cast<float*>(smem + kWarps * C::RING);
   float* mineq = comb + warp * (C::COMB / 4);
-  const int64_t lane_off = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
   const uint32_t k_lane = KRows<C>::LaneOffset(lane), v_lane = VLaneOffset<C>(lane);
+  Filler<C> fill;
+  fill.at = use;
+  fill.left = left;
+  fill.places = s_places[warp];
+  {
+    const int64_t part = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
+    fill.k = p.kv.k + part;
+    fill.v = p.kv.v + part;
+    constexpr int kPer = 2 * C::NG;
+    fill.scale = (lane < C::MT * kPer ? p.kv.k_scale : p.kv.v_scale) + lane % kPer * 16;
+  }
   uint32_t bad = 0;  // two bits per step in flight
-  int to_fill = left;
-#pragma unroll
+  fill.Request(p, warp, lane);
+#pragma unroll 1
   for (int d = 0; d < C::DEPTH; ++d) {
-    const Step s = StepAt<C>(p, fill, warp, to_fill > 0);
+    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
+    __syncwarp();
     const uint32_t slot = ring + d * (C::KSLOT + C::VSLOT);
-    Issue<C, false>(p, s, slot, lane, lane_off);
-    Issue<C, true>(p, s, slot + C::KSLOT, lane, lane_off);
-    bad = bad << 2 | s.bad;
-    if (--to_fill > 0) fill.Next(p, chunks);
+    fill.template Issue<false>(p, slot, lane);
+    fill.template Issue<true>(p, slot + C::KSLOT, lane);
+    bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
+    if (fill.count > 0) fill.Pop();
   }
 
   uint32_t qh[C::KS][2], ql[C::PACK ? 1 : C::KS][2];
+  const uint32_t magic = p.magic;
   const bool two_terms = p.type == ElemType::kF32;
   float cs[2];            // from products of the f16 terms to scores in log2 units
   float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
@@ -529,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   uint32_t kslot = ring;
 
   for (;;) {
-    const Step next = StepAt<C>(p, fill, warp, to_fill > 0);
+    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
     if (fresh) {
       fresh = false;
       seg = use.tile;
@@ -631,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
             for (int j = 0; j < 4; ++j) {
               const int ks = 4 * gp + j;
               uint32_t a[4];
-              rows.Fragment(a, j);
+              rows.Fragment(a, j, magic);
               j == 0 ? MmaFirst(part, a, qh[ks][0], qh[ks][1]) : Mma(part, a, qh[ks][0], qh[ks][1]);
               if (!C::PACK && two_terms) Mma(part, a, ql[C::PACK ? 0 : ks][0], ql[C::PACK ? 0 : ks][1]);
             }
@@ -649,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     __syncwarp();
-    Issue<C, false>(p, next, kslot, lane, lane_off);
+    fill.template Issue<false>(p, kslot, lane);
 
     // ---- weights: 2^(score - ref) with ref a power of two over the largest,
     // so that a weight times its V scale is at most 2^14 and small ones stay
@@ -657,6 +673,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     float alpha[2] = {1.f, 1.f};
     if (work) {
       if (edge) {
+        asm volatile("" ::: "memory");  // a branch, not predicates: few steps come here
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
@@ -711,6 +728,14 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     CopyWait<2 * C::DEPTH - 1>();
     __syncwarp();
     if (work) {
+      if (!C::QUANT && edge) {  // what lies out of range may be anything, NaN too: zeros
+#pragma unroll 1
+        for (int i = lane; i < C::R * C::CPR; i += 32) {
+          const int r = i / C::CPR;
+          if (r < lo || r >= hi) Sts128Zero(vslot + ChunkAt<C, true>(r, i % C::CPR));
+        }
+        __syncwarp();
+      }
       const uint32_t vbase = vslot + v_lane;
       const float of_rest = t >= 2 ? 1.f : 0.f, of_lead = t >= 2 ? -1.f : 1.f;  // which term this lane's columns take
 #pragma unroll
@@ -742,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
           for (int kt = 0; kt < C::MT; ++kt) {
             uint32_t a[4][4];
-            VFragments<C>(a, vbase, kt, gp);
+            VFragments<C>(a, vbase, kt, gp, magic);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               kt == 0 ? MmaFirst(part[i], a[i], b[kt][0][0], b[kt][1][0]) : Mma(part[i], a[i], b[kt][0][0], b[kt][1][0]);
@@ -772,9 +797,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     __syncwarp();
-    Issue<C, true>(p, next, vslot, lane, lane_off);
-    bad = bad << 2 | next.bad;
-    if (--to_fill > 0) fill.Next(p, chunks);
+    fill.template Issue<true>(p, vslot, lane);
+    bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
+    if (fill.count > 0) fill.Pop();
     kslot = kslot + C::KSLOT + C::VSLOT == ring + C::RING ? ring : kslot + C::KSLOT + C::VSLOT;
 
     // ---- the end of the item, or of this block's share of it
@@ -955,11 +980,7 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   const int64_t tiles = ((cap + 15) / C::TILE + 1) * p.kv.n_kv * chunks;
   if (tiles < grid && tiles * p.table.n_seq < grid) grid = static_cast<int>(tiles * p.table.n_seq);
   KvAttendParams a = p;
-  a.page16 = static_cast<uint32_t>(p.kv.page_stride / 16);
-  a.head16 = static_cast<uint32_t>(p.kv.head_stride / 16);
-  a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);
-  a.spage16 = static_cast<uint32_t>(p.kv.scale_page_stride / 16);
-  a.shead16 = static_cast<uint32_t>(p.kv.scale_head_stride / 16);
+  a.magic = kMagic;
   KvAttendKernel<C><<<grid, kThreads, C::SMEM, s>>>(a);
 }
 
