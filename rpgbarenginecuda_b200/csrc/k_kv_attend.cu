@@ -70,7 +70,8 @@ struct Cfg {
   static constexpr int RING = DEPTH * (KSLOT + VSLOT);  // per warp
   static_assert(KSLOT % 128 == 0 && VSLOT % 128 == 0, "tiles are 128-byte lines");
   static constexpr int COMB = QUERIES * D * 4;   // per warp
-  static constexpr int SMEM = kWarps * (RING + COMB);
+  static constexpr int JOIN = kWarps * COMB > QUERIES * kKvMaxBlocks * 4 ? kWarps * COMB : QUERIES * kKvMaxBlocks * 4;
+  static constexpr int SMEM = kWarps * RING + JOIN;
   static constexpr int BLOCKS = PACK || D == 64 ? 3 : 2;  // resident per SM: what registers and shared memory allow
 };
 
@@ -154,6 +155,14 @@ __device__ __forceinline__ uint4 Lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
   return x;
 }
+__device__ __forceinline__ uint64_t Lds64u(uint32_t a) {
+  uint64_t x;
+  asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x) : "r"(a) : "memory");
+  return x;
+}
+__device__ __forceinline__ void Sts64(uint32_t a, uint64_t x) {
+  asm volatile("st.shared.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory");
+}
 __device__ __forceinline__ void Sts128Zero(uint32_t a) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
 }
@@ -229,7 +238,7 @@ struct Cursor {
 // out together, one 16-row half per lane, and left in shared memory; the page
 // ids they need are requested one such batch earlier.
 struct Place {
-  int64_t code, scale;  // byte offsets of the half in the planes
+  uint64_t code, scale;  // byte offsets of the half in the planes
 };
 template <typename C>
 struct Filler {
@@ -242,7 +251,7 @@ struct Filler {
   uint32_t bad = 0;    // as `have`: it has rows in range but no page
   int page = 0;        // this lane's half of the next batch
   const char *k, *v, *scale;  // this lane's part of a copy's source, without the place
-  Place* places;
+  uint32_t places;  // shared-memory address
 
   __device__ __forceinline__ int Pos(int warp, int lane) const {
     return at.span.base + (at.tile + lane / C::MT) * C::TILE + warp * C::R + (lane % C::MT) * 16;
@@ -265,10 +274,10 @@ struct Filler {
     const int row = pos & ((1 << p.kv.page_log2) - 1);
     __syncwarp();  // the last batch has been read
     if (lane < kHalves) {
-      Place q;
-      q.code = page * p.kv.page_stride + at.head * p.kv.head_stride + row * p.kv.pos_stride;
-      q.scale = page * p.kv.scale_page_stride + at.head * p.kv.scale_head_stride + row * (2 * C::NG);
-      places[lane] = q;
+      const uint64_t id = static_cast<uint32_t>(page), head = static_cast<uint32_t>(at.head);
+      const uint64_t code = id * p.page16 + head * p.head16 + static_cast<uint64_t>(static_cast<uint32_t>(row)) * p.pos16;
+      Sts64(places + lane * 16, code << 4);
+      if (C::QUANT) Sts64(places + lane * 16 + 8, ((id * p.spage16 + head * p.shead16) << 4) + row * (2 * C::NG));
     }
     have = __ballot_sync(0xFFFFFFFFu, ok);
     bad = __ballot_sync(0xFFFFFFFFu, in && !ok);
@@ -286,12 +295,12 @@ struct Filler {
     if (count > 0) {
       constexpr int kRows = 32 / C::CPR, kPerHalf = 16 / kRows;  // rows of a copy instruction: all in one half
       const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
-      const Place* q = places + next;
+      const uint32_t q = places + next * 16;
 #pragma unroll
       for (int h = 0; h < C::MT; ++h) {
         if ((have >> h) & 1) {
-          const char* src = (V ? v : k) + q[h].code;
-          if (p.kv.pos_stride == C::ROW) {  // dense rows: constant steps
+          const char* src = (V ? v : k) + Lds64u(q + 16 * h);
+          if (p.pos16 == C::ROW / 16) {  // dense rows: constant steps
 #pragma unroll
             for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
           } else {
@@ -306,7 +315,7 @@ struct Filler {
         constexpr int kPer = 2 * C::NG;  // a half's scales are dense: 16 rows of 2 NG bytes, in 16-byte pieces
         const int h = lane / kPer % C::MT;
         if (lane < 2 * C::MT * kPer && ((have >> h) & 1)) {
-          CopyAsync16(slot + C::R * C::ROW + lane * 16, scale + q[h].scale);
+          CopyAsync16(slot + C::R * C::ROW + lane * 16, scale + Lds64u(q + 16 * h + 8));
         }
       }
     }
@@ -319,6 +328,19 @@ struct Filler {
     bad >>= C::MT;
   }
 };
+
+// Block b of n takes tiles [total b / n, total (b + 1) / n); ShareOf is the
+// block that has tile x.  Few tiles need no 64-bit division.
+__device__ __forceinline__ long long ShareBegin(long long total, int b, int n) {
+  if (total < (1 << 22)) return static_cast<uint32_t>(total) * static_cast<uint32_t>(b) / static_cast<uint32_t>(n);
+  return total * b / n;
+}
+__device__ __forceinline__ int ShareOf(long long x, long long total, int n) {
+  if (total < (1 << 22)) {
+    return (static_cast<uint32_t>(x + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint32_t>(total);
+  }
+  return static_cast<int>(((x + 1) * n - 1) / total);
+}
 
 // ------------------------------------------------------------------ operands
 
@@ -423,12 +445,30 @@ __device__ __forceinline__ constexpr int ValueOf(int ks, int b, int e, int t) {
 
 template <typename C, typename T>
 __device__ __forceinline__ void ReadQ(float (&x)[C::KS][2][2], const T* row, int t) {
+  if (!C::QUANT) {  // pairs
 #pragma unroll
-  for (int ks = 0; ks < C::KS; ++ks) {
+    for (int ks = 0; ks < C::KS; ++ks) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b) {
+        const kvd::Pack<T, 2> r = *reinterpret_cast<const kvd::Pack<T, 2>*>(row + ValueOf<C>(ks, b, 0, t));
+        x[ks][b][0] = kvd::ToFloat(r.v[0]);
+        x[ks][b][1] = kvd::ToFloat(r.v[1]);
+      }
+    }
+  } else {  // runs of 16
 #pragma unroll
-      for (int e = 0; e < 2; ++e) x[ks][b][e] = kvd::ToFloat(row[ValueOf<C>(ks, b, e, t)]);
+    for (int gp = 0; gp < C::NG; ++gp) {
+      float y[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kvd::Load4(row + 64 * gp + 16 * t + 4 * j, y[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = ValueOf<C>(j, e >> 1, e & 1, 0);  // of the run
+          x[4 * gp + j][e >> 1][e & 1] = y[i >> 2][i & 3];
+        }
+      }
     }
   }
 }
@@ -476,10 +516,10 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     if (w == warp) upto += total;
     total += s_sum[w];
   }
-  const long long blocks = min(static_cast<long long>(gridDim.x), total);
-  if (blockIdx.x >= blocks) return;
-  const long long first = total * blockIdx.x / blocks;
-  int left = static_cast<int>(total * (blockIdx.x + 1) / blocks - first);  // tiles to do
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  if (static_cast<int>(blockIdx.x) >= blocks) return;
+  const long long first = ShareBegin(total, blockIdx.x, blocks);
+  int left = static_cast<int>(ShareBegin(total, blockIdx.x + 1, blocks) - first);  // tiles to do
   if (first >= upto - mine && first < upto) {
     long long at = upto - mine;
     int s = tid * run;
@@ -497,10 +537,11 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   use.span = SpanOf<C>(p, use.seq);
   {
     const long long in = first - s_begin;  // inside the conversation
-    const int item = static_cast<int>(in / use.span.tiles);
-    use.head = item / chunks;
-    use.chunk = item % chunks;
-    use.tile = static_cast<int>(in % use.span.tiles);
+    const long long item = in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(use.span.tiles)
+                                            : in / use.span.tiles;
+    use.tile = static_cast<int>(in - item * use.span.tiles);
+    use.head = static_cast<int>(item) / chunks;
+    use.chunk = static_cast<int>(item) % chunks;
   }
 
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
@@ -510,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   Filler<C> fill;
   fill.at = use;
   fill.left = left;
-  fill.places = s_places[warp];
+  fill.places = dev::SmemAddr(s_places[warp]);
   {
     const int64_t part = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
     fill.k = p.kv.k + part;
@@ -520,47 +561,47 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   }
   uint32_t bad = 0;  // two bits per step in flight
   fill.Request(p, warp, lane);
-#pragma unroll 1
-  for (int d = 0; d < C::DEPTH; ++d) {
-    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
-    __syncwarp();
-    const uint32_t slot = ring + d * (C::KSLOT + C::VSLOT);
-    fill.template Issue<false>(p, slot, lane);
-    fill.template Issue<true>(p, slot + C::KSLOT, lane);
-    bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
-    if (fill.count > 0) fill.Pop();
-  }
 
-  uint32_t qh[C::KS][2], ql[C::PACK ? 1 : C::KS][2];
+  uint32_t kslot = ring;
   const uint32_t magic = p.magic;
   const bool two_terms = p.type == ElemType::kF32;
-  float cs[2];            // from products of the f16 terms to scores in log2 units
-  float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
-  float l[2];             // sum of this lane's weights
-  float acc[D / 16][4];
-  int nu = 0;             // biased exponent of the power of two over the V scales seen
-  int queries = 0, seg = 0;  // of the item; its first tile in this block
-  bool fresh = true;
-  long long at = first;
-  uint32_t kslot = ring;
-
-  for (;;) {
-    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
-    if (fresh) {
-      fresh = false;
-      seg = use.tile;
-      queries = min(per_chunk, group - use.chunk * per_chunk);
+  long long item0 = first - use.tile;  // the item's first tile
+  for (bool begin = true;; begin = false) {
+    // ---- an item: its queries, as B fragments
+    const int queries = min(per_chunk, group - use.chunk * per_chunk);
+    const int64_t col = (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
+    const int seg = use.tile;
+    float x[C::KS][2][2] = {};
+    {
       const int qi = C::PACK ? g & 3 : g;
-      float x[C::KS][2][2] = {};
       if (qi < queries) {
-        const int64_t o = use.seq * p.q_stride +
-                          (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk + qi) * D;
+        const int64_t o = use.seq * p.q_stride + col + qi * D;
         switch (p.type) {
           case ElemType::kF32: ReadQ<C>(x, static_cast<const float*>(p.q) + o, t); break;
           case ElemType::kF16: ReadQ<C>(x, static_cast<const __half*>(p.q) + o, t); break;
           case ElemType::kBF16: ReadQ<C>(x, static_cast<const __nv_bfloat16*>(p.q) + o, t); break;
         }
       }
+    }
+    if (begin) {  // the first steps' copies, while the queries are on their way
+#pragma unroll 1
+      for (int d = 0; d < C::DEPTH; ++d) {
+        if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
+        __syncwarp();
+        const uint32_t slot = ring + d * (C::KSLOT + C::VSLOT);
+        fill.template Issue<false>(p, slot, lane);
+        fill.template Issue<true>(p, slot + C::KSLOT, lane);
+        bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
+        if (fill.count > 0) fill.Pop();
+      }
+    }
+    uint32_t qh[C::KS][2], ql[C::PACK ? 1 : C::KS][2];
+    float cs[2];            // from products of the f16 terms to scores in log2 units
+    float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
+    float l[2];             // sum of this lane's weights
+    float acc[D / 16][4];
+    int nu = 127 - 25;      // biased exponent of the power of two over the V scales seen
+    {
       float top = 0.f;
 #pragma unroll
       for (int ks = 0; ks < C::KS; ++ks) {
@@ -602,9 +643,11 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
       }
-      nu = 127 - 25;
     }
 
+    // ---- its tiles
+    for (;;) {
+    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
     const int pos = use.span.base + use.tile * C::TILE + warp * C::R;
     const int lo = use.span.start - pos, hi = use.span.len - pos;
     const bool work = lo < C::R && hi > 0;
@@ -802,9 +845,13 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     if (fill.count > 0) fill.Pop();
     kslot = kslot + C::KSLOT + C::VSLOT == ring + C::RING ? ring : kslot + C::KSLOT + C::VSLOT;
 
+    --left;
+    if (left == 0 || use.tile + 1 == use.span.tiles) break;
+    ++use.tile;
+    }
+
     // ---- the end of the item, or of this block's share of it
-    if (use.tile + 1 == use.span.tiles || left == 1) {
-      fresh = true;
+    {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -829,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
       __syncthreads();
       const bool whole = seg == 0 && use.tile + 1 == use.span.tiles;
-      const int64_t out = use.seq * p.out_stride + (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
+      const int64_t out = use.seq * p.out_stride + col;
       const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
       // The warps' shares joined: value i of the item's queries, its sum, its maximum.
@@ -853,9 +900,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       if (!whole) {
         // This block's record: one for an item that began in an earlier block,
         // one for an item that begins here.  Blocks b0 .. b1 hold the parts.
-        const long long item0 = at - use.tile, item1 = item0 + use.span.tiles - 1;
-        const int b0 = static_cast<int>(((item0 + 1) * blocks - 1) / total);
-        const int b1 = static_cast<int>(((item1 + 1) * blocks - 1) / total);
+        const int b0 = ShareOf(item0, total, blocks), b1 = ShareOf(item0 + use.span.tiles - 1, total, blocks);
         constexpr int kRecord = kKvMaxQueries * (D + 2);
         float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
                                                   (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256);
@@ -876,63 +921,64 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         __syncthreads();
         finish = s_last != 0;
         if (finish) {
-          // The last block joins all records: warp w adds up records b0 + w,
-          // b0 + w + 4, ... under the maximum of all, in that order.
+          // The last block joins all records under the maximum of all.  First
+          // the records' factors, a query per warp and a record per lane, into
+          // the join area; then warp w adds up records b0 + w, b0 + w + 4, ...
+          // in that order, a few of them in flight.
           __threadfence();
           if (tid == 0) *count = 0;
-          constexpr int kVec = C::QUERIES * D / 128;  // float4 of a lane
-          float top[C::QUERIES], sum[C::QUERIES];
+          float* factor = comb;  // [query][record]
+          for (int q = warp; q < queries; q += kWarps) {
+            float top = -INFINITY, sum = 0.f;
+            for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, __ldcg(record(b) + kKvMaxQueries * D + q));
+            top = dev::WarpMax(top);
+            for (int b = b0 + lane; b <= b1; b += 32) {
+              const float* r = record(b) + kKvMaxQueries * D + q;
+              const float f = Exp2(__ldcg(r) - (top == -INFINITY ? 0.f : top));
+              factor[q * kKvMaxBlocks + b - b0] = f;
+              sum += f * __ldcg(r + kKvMaxQueries);
+            }
+            sum = dev::WarpSum(sum);
+            if (lane < kWarps) {
+              s_m[lane][q] = top;
+              s_l[lane][q] = lane == 0 ? sum : 0.f;
+            }
+          }
+          __syncthreads();
+          constexpr int kVec = C::QUERIES * D / 128, kFlight = 8 / kVec;  // float4 of a lane; records in flight
           float4 v[kVec];
 #pragma unroll
-          for (int q = 0; q < C::QUERIES; ++q) {
-            top[q] = -INFINITY;
-            sum[q] = 0.f;
-          }
-#pragma unroll
           for (int k = 0; k < kVec; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int b = b0 + lane; b <= b1; b += 32) {
-            const float* r = record(b) + kKvMaxQueries * D;
+          for (int b = b0 + warp; b <= b1; b += kWarps * kFlight) {
+            float4 r[kFlight][kVec];
 #pragma unroll
-            for (int q = 0; q < C::QUERIES; ++q) {
-              if (q < queries) top[q] = fmaxf(top[q], __ldcg(r + q));
-            }
-          }
+            for (int n = 0; n < kFlight; ++n) {
 #pragma unroll
-          for (int q = 0; q < C::QUERIES; ++q) top[q] = dev::WarpMax(top[q]);
-#pragma unroll 2
-          for (int b = b0 + warp; b <= b1; b += kWarps) {
-            const float* r = record(b);
-            float f[C::QUERIES];
-#pragma unroll
-            for (int q = 0; q < C::QUERIES; ++q) {
-              f[q] = 0.f;
-              if (q < queries) {
-                f[q] = Exp2(__ldcg(r + kKvMaxQueries * D + q) - (top[q] == -INFINITY ? 0.f : top[q]));
-                sum[q] += f[q] * __ldcg(r + kKvMaxQueries * (D + 1) + q);
+              for (int k = 0; k < kVec; ++k) {
+                const int q = D == 128 ? k : 2 * k + (lane >> 4);
+                if (b + n * kWarps <= b1 && q < queries) {
+                  r[n][k] = __ldcg(reinterpret_cast<const float4*>(record(b + n * kWarps)) + 32 * k + lane);
+                }
               }
             }
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) {
-              const int q = k * 128 / D + (D == 128 ? 0 : lane >> 4);
-              if (q < queries) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(r) + 32 * k + lane);
-                const float fq = D == 128 ? f[k % C::QUERIES] : (lane >= 16 ? f[(2 * k + 1) % C::QUERIES] : f[(2 * k) % C::QUERIES]);
-                v[k].x += fq * x.x;
-                v[k].y += fq * x.y;
-                v[k].z += fq * x.z;
-                v[k].w += fq * x.w;
+            for (int n = 0; n < kFlight; ++n) {
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) {
+                const int q = D == 128 ? k : 2 * k + (lane >> 4);
+                if (b + n * kWarps <= b1 && q < queries) {
+                  const float f = factor[q * kKvMaxBlocks + b - b0 + n * kWarps];
+                  v[k].x += f * r[n][k].x;
+                  v[k].y += f * r[n][k].y;
+                  v[k].z += f * r[n][k].z;
+                  v[k].w += f * r[n][k].w;
+                }
               }
             }
           }
+          __syncthreads();  // the factors have been read
 #pragma unroll
           for (int k = 0; k < kVec; ++k) reinterpret_cast<float4*>(mineq)[32 * k + lane] = v[k];
-          if (lane == 0) {
-#pragma unroll
-            for (int q = 0; q < C::QUERIES; ++q) {
-              s_m[warp][q] = top[q];
-              s_l[warp][q] = sum[q];
-            }
-          }
           __syncthreads();
         }
       }
@@ -951,8 +997,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
       __syncthreads();  // the next item writes the join area again
     }
-    if (--left == 0) break;
-    ++at;
+    if (left == 0) break;
+    item0 += use.span.tiles;
     use.Next(p, chunks);
   }
   CopyWait<0>();
@@ -981,6 +1027,11 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   if (tiles < grid && tiles * p.table.n_seq < grid) grid = static_cast<int>(tiles * p.table.n_seq);
   KvAttendParams a = p;
   a.magic = kMagic;
+  a.page16 = static_cast<uint32_t>(p.kv.page_stride / 16);
+  a.head16 = static_cast<uint32_t>(p.kv.head_stride / 16);
+  a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);
+  a.spage16 = static_cast<uint32_t>(p.kv.scale_page_stride / 16);
+  a.shead16 = static_cast<uint32_t>(p.kv.scale_head_stride / 16);
   KvAttendKernel<C><<<grid, kThreads, C::SMEM, s>>>(a);
 }
 

@@ -20,7 +20,7 @@ constexpr int kKvGroup = 64;         // values that share a scale
 constexpr int kKvMinPage = 16;       // a page holds whole 16-position units
 constexpr int kKvMaxPage = 4096;
 constexpr int kKvMaxQueries = 8;     // query heads of a KV head that one attend pass takes
-constexpr int64_t kKvMaxStride = int64_t{1} << 38;  // bytes; more than any GPU holds
+constexpr int64_t kKvMaxStride = int64_t{1} << 35;  // bytes; a sixteenth of it fits 32 bits
 constexpr int kKvMaxBlocks = 512;    // bound of the attend grid (sizes the workspace)
 
 struct KvPages {
@@ -88,7 +88,9 @@ struct KvAttendParams {
   void* out = nullptr;
   int64_t out_stride = 0;  // elements
   void* workspace = nullptr;
-  uint32_t magic = 0;  // a constant of the kernel, filled in by LaunchKvAttend
+  // filled in by LaunchKvAttend: a constant of the kernel, and the strides of
+  // kv in units of 16 bytes
+  uint32_t magic = 0, page16 = 0, head16 = 0, pos16 = 0, spage16 = 0, shead16 = 0;
 };
 // Workspace bytes of LaunchKvAttend (its first bytes are counters that start
 // at zero and are zero again after every call).
