@@ -58,7 +58,7 @@ struct Cfg {
   static constexpr int QUERIES = PACK ? 4 : 8;
   static constexpr int R = QUANT || D == 64 ? 32 : 16;  // positions of a warp's step
   static constexpr int TILE = kWarps * R;
-  static constexpr int DEPTH = KIND == KvType::kQ4 ? 3 : 2;
+  static constexpr int DEPTH = 1;
   static constexpr int MT = R / 16;     // 16-position tiles of a step
   static constexpr int KS = D / 16;     // 16-value slices of a head
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
@@ -71,7 +71,11 @@ struct Cfg {
   static_assert(KSLOT % 128 == 0 && VSLOT % 128 == 0, "tiles are 128-byte lines");
   static constexpr int COMB = QUERIES * D * 4;   // per warp
   static constexpr int JOIN = kWarps * COMB > QUERIES * kKvMaxBlocks * 4 ? kWarps * COMB : QUERIES * kKvMaxBlocks * 4;
-  static constexpr int SMEM = kWarps * RING + JOIN;
+  // q as B fragments: f16 terms, or up to three digit tiles of 8-bit integers
+  static constexpr int QTILES = QUANT ? (PACK ? 2 : 3) : (PACK ? 1 : 2);
+  static constexpr int QWORDS = QUANT ? 4 * NG : 2 * KS;  // of a lane and tile
+  static constexpr int QBYTES = QTILES * QWORDS * 128;
+  static constexpr int SMEM = kWarps * RING + JOIN + QBYTES;
   static constexpr int BLOCKS = PACK || D == 64 ? 3 : 2;  // resident per SM: what registers and shared memory allow
 };
 
@@ -135,6 +139,32 @@ __device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], 
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
+// Products of integer codes (signed bytes, or 4-bit ones as unsigned bytes)
+// and signed digits; 32 values of a row at a time.
+template <bool UNSIGNED>
+__device__ __forceinline__ void MmaInt(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (UNSIGNED) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+template <bool UNSIGNED>
+__device__ __forceinline__ void MmaIntFirst(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c) {
+  if (UNSIGNED) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
+  } else {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
+  }
+}
 __device__ __forceinline__ uint32_t Lds32(uint32_t a) {
   uint32_t x;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(a) : "memory");
@@ -154,6 +184,9 @@ __device__ __forceinline__ uint4 Lds128(uint32_t a) {
   uint4 x;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
   return x;
+}
+__device__ __forceinline__ void Sts32(uint32_t a, uint32_t x) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
 }
 __device__ __forceinline__ uint64_t Lds64u(uint32_t a) {
   uint64_t x;
@@ -186,6 +219,9 @@ __device__ __forceinline__ uint32_t SubHalf(uint32_t x, uint32_t bias) {
 constexpr uint32_t kMagic = 0x64006400u;
 constexpr uint32_t kBias8 = 0x64806480u;  // 1024 + 128
 constexpr uint32_t kBias4 = 0x64086408u;  // 1024 + 8
+// An integer sum that starts at the bits of 1.5 2^23 is that float plus the sum.
+constexpr int kIntStart = 0x4B400000;
+constexpr float kIntBias = 12582912.f;
 template <uint32_t MASK>
 __device__ __forceinline__ uint32_t MaskOr(uint32_t w, uint32_t magic) {
   uint32_t r;
@@ -344,45 +380,37 @@ __device__ __forceinline__ int ShareOf(long long x, long long total, int n) {
 
 // ------------------------------------------------------------------ operands
 
-// K of 16 positions, 16-value slice ks, as the A fragment (rows = positions).
-// Code tiles: lane t of a row takes 16 consecutive values of a 64-value group
-// (they are a slice's columns in that order; LoadQ takes q the same way).
+// Where a lane's part of a K tile lies: for ldmatrix, or 16 consecutive values
+// (lane t's run) of row g.
 template <typename C>
-struct KRows {
-  uint4 w[2];  // q8: 16 codes of rows g and g + 8; q4: .x, .y
-  // `base`: LaneOffset from the slot
-  __device__ __forceinline__ void Load(uint32_t base, int mt, int gp) {
+__device__ __forceinline__ int KLaneOffset(int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  if (C::KIND == KvType::kF16) return ChunkAt<C, false>(lane & 15, lane >> 4);
+  return C::KIND == KvType::kQ8 ? ChunkAt<C, false>(g, t) : ChunkAt<C, false>(g, t >> 1) + (t & 1) * 8;
+}
+// K codes of 16 positions (rows g, g + 8 of tile mt) and a 64-value group as A
+// fragments of two 32-value slices.  The columns of a slice are the lanes'
+// runs, 8 values of each: q8 codes as they are, 4-bit codes spread to bytes,
+// the even values of the 8, then the odd ones (LaneDigits takes q the same way).
+template <typename C>
+__device__ __forceinline__ void KFragments(uint32_t (&a)[2][4], uint32_t base, int mt, int gp) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (C::KIND == KvType::kQ8) {
-        w[i] = Lds128(Moved<C, false>(base, 16 * mt + 8 * i, 4 * gp));
-      } else {
-        const uint2 x = Lds64(Moved<C, false>(base, 16 * mt + 8 * i, 2 * gp));
-        w[i].x = x.x;
-        w[i].y = x.y;
-      }
+  for (int i = 0; i < 2; ++i) {
+    if (C::KIND == KvType::kQ8) {
+      const uint4 x = Lds128(Moved<C, false>(base, 16 * mt + 8 * i, 4 * gp));
+      a[0][i] = x.x;
+      a[0][2 + i] = x.y;
+      a[1][i] = x.z;
+      a[1][2 + i] = x.w;
+    } else {
+      const uint2 x = Lds64(Moved<C, false>(base, 16 * mt + 8 * i, 2 * gp));
+      a[0][i] = x.x & 0x0F0F0F0Fu;
+      a[0][2 + i] = (x.x >> 4) & 0x0F0F0F0Fu;
+      a[1][i] = x.y & 0x0F0F0F0Fu;
+      a[1][2 + i] = (x.y >> 4) & 0x0F0F0F0Fu;
     }
   }
-  static __device__ __forceinline__ int LaneOffset(int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    if (C::KIND == KvType::kF16) return ChunkAt<C, false>(lane & 15, lane >> 4);  // for ldmatrix
-    return C::KIND == KvType::kQ8 ? ChunkAt<C, false>(g, t) : ChunkAt<C, false>(g, t >> 1) + (t & 1) * 8;
-  }
-  __device__ __forceinline__ void Fragment(uint32_t (&a)[4], int j, uint32_t magic) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (C::KIND == KvType::kQ8) {
-        const uint32_t u = (j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w) ^ 0x80808080u;
-        a[i] = SubHalf(__byte_perm(u, magic, 0x5150), kBias8);
-        a[2 + i] = SubHalf(__byte_perm(u, magic, 0x5352), kBias8);
-      } else {
-        const uint32_t u = (j < 2 ? w[i].x : w[i].y) >> ((j & 1) * 8);
-        a[i] = Low4(u, magic);
-        a[2 + i] = High4(u, magic);
-      }
-    }
-  }
-};
+}
 
 // V^T of a 64-value group and 16 positions as A fragments of four 16-row
 // tiles (rows = values).  Lane g takes values 8 g .. 8 g + 7 of the group:
@@ -433,49 +461,116 @@ __device__ __forceinline__ void VFragments(uint32_t (&a)[4][4], uint32_t base, i
   }
 }
 
-// Value of a head that column pair b (0, 1), element e of lane t's B fragment
-// of slice ks stands for: the order LdMatrix or KRows gives K in.
-template <typename C>
-__device__ __forceinline__ constexpr int ValueOf(int ks, int b, int e, int t) {
-  return C::KIND == KvType::kF16 ? 16 * ks + 8 * b + 2 * t + e
-         : C::KIND == KvType::kQ8
-             ? 64 * (ks >> 2) + 16 * t + 4 * (ks & 3) + 2 * b + e
-             : 64 * (ks >> 2) + 16 * t + 8 * ((ks & 3) >> 1) + 2 * (ks & 1) + b + 4 * e;
-}
-
+// A lane's values of a q row: f16 caches take pairs 16 ks + 8 b + 2 t (value
+// 4 ks + 2 b + e of x), quantised ones the run 16 t of every 64 values.
 template <typename C, typename T>
-__device__ __forceinline__ void ReadQ(float (&x)[C::KS][2][2], const T* row, int t) {
-  if (!C::QUANT) {  // pairs
+__device__ __forceinline__ void ReadQ(float (&x)[C::D / 4], const T* row, int t) {
+  if (!C::QUANT) {
 #pragma unroll
-    for (int ks = 0; ks < C::KS; ++ks) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const kvd::Pack<T, 2> r = *reinterpret_cast<const kvd::Pack<T, 2>*>(row + ValueOf<C>(ks, b, 0, t));
-        x[ks][b][0] = kvd::ToFloat(r.v[0]);
-        x[ks][b][1] = kvd::ToFloat(r.v[1]);
-      }
+    for (int i = 0; i < C::D / 8; ++i) {
+      const kvd::Pack<T, 2> r = *reinterpret_cast<const kvd::Pack<T, 2>*>(row + 8 * i + 2 * t);
+      x[2 * i] = kvd::ToFloat(r.v[0]);
+      x[2 * i + 1] = kvd::ToFloat(r.v[1]);
     }
-  } else {  // runs of 16
+  } else {
 #pragma unroll
-    for (int gp = 0; gp < C::NG; ++gp) {
-      float y[4][4];
+    for (int i = 0; i < C::D / 16; ++i) {
+      float y[4];
+      kvd::Load4(row + 64 * (i >> 2) + 16 * t + 4 * (i & 3), y);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kvd::Load4(row + 64 * gp + 16 * t + 4 * j, y[j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = ValueOf<C>(j, e >> 1, e & 1, 0);  // of the run
-          x[4 * gp + j][e >> 1][e & 1] = y[i >> 2][i & 3];
-        }
-      }
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
     }
   }
 }
 
-__device__ __forceinline__ float LaneQuadMax(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+// The lanes' q rows (lane g: column g's query) as B fragments in shared
+// memory: word i of tile n, lane at base + ((n * QWORDS + i) / 4 * 32 + lane) *
+// 16 + i % 4 * 4, written by warp i % kWarps.  Returns what turns a product
+// back into a score in log2 units (the scale's magnitude included; its sign
+// goes into the fragments, so that the largest product is the largest score).
+//
+// f16 cache: q times a power of two that brings its largest value into
+// [1, 2), as two f16 terms (the second is zero for a 16-bit q).  Quantised
+// cache: q / largest as a 24-bit integer in three signed base-256 digits.
+template <typename C>
+__device__ __forceinline__ float WriteQ(uint32_t base, const float (&x)[C::D / 4], float scale, bool f32, int warp,
+                                        int lane, float (&bias)[C::NG][C::QTILES]) {
+  const int g = lane >> 2;
+  uint32_t top_bits = 0;
+#pragma unroll
+  for (int i = 0; i < C::D / 4; ++i) top_bits = max(top_bits, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  top_bits = max(top_bits, __shfl_xor_sync(0xFFFFFFFFu, top_bits, 1));
+  top_bits = max(top_bits, __shfl_xor_sync(0xFFFFFFFFu, top_bits, 2));
+  const float sign = scale < 0.f ? -1.f : (scale > 0.f ? 1.f : 0.f), mag = fabsf(scale) * kLog2e;
+  // positive, so that scores of -infinity stay; with a NaN or an infinity in q no score means anything
+  auto back = [&](float f) { return top_bits >= 0x7F800000u ? kvd::Nan() : fmaxf(f, 1e-30f); };
+  auto put = [&](int n, int i, uint32_t w) {
+    const int k = n * C::QWORDS + i;
+    if (i % kWarps == warp) Sts32(base + ((k >> 2) * 32 + lane) * 16 + (k & 3) * 4, w);
+  };
+  if (!C::QUANT) {
+    const int e = min(max(static_cast<int>(top_bits >> 23), 1), 253);  // kept in f32's normal range
+    const float down = sign * __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < C::QWORDS; ++i) {
+      const float u = x[2 * i] * down, v = x[2 * i + 1] * down;
+      const uint32_t h = PackHalf(u, v);
+      const float2 f = __half22float2(BitsHalf(h));
+      const uint32_t r = PackHalf(u - f.x, v - f.y);
+      if (C::PACK) {
+        put(0, i, f32 && g >= 4 ? r : h);
+      } else {
+        put(0, i, h);
+        put(C::QTILES - 1, i, r);
+      }
+    }
+    return back(__uint_as_float(static_cast<uint32_t>(e) << 23) * mag);
+  }
+  constexpr float most = 8355700.f;  // 127 in every digit, less room for the product's rounding
+  const float top = fmaxf(__uint_as_float(top_bits), 1e-30f);
+  const float to_int = sign * (most / top);
+  int sum[C::NG][C::QTILES] = {};
+#pragma unroll
+  for (int i = 0; i < C::QWORDS; ++i) {  // word i: values 4 (i & 1) .. of the run's 8-value half, i / 4 the group
+    uint32_t digit[3] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int first = 16 * (i >> 2) + 8 * ((i >> 1) & 1);
+      const int v = first + (C::KIND == KvType::kQ8 ? 4 * (i & 1) + e : 2 * e + (i & 1));
+      int q = __float2int_rn(x[v] * to_int);
+#pragma unroll
+      for (int d = 0; d < 3; ++d) {
+        const int b = static_cast<int8_t>(q);
+        digit[d] |= static_cast<uint32_t>(b & 255) << (8 * e);
+        q = (q - b) >> 8;
+      }
+    }
+    uint32_t w[3];
+    if (C::PACK) {
+      w[0] = g < 4 ? digit[2] : digit[1];
+      w[1] = g < 4 ? digit[0] : 0;
+    } else {
+      w[0] = digit[2];
+      w[1] = digit[1];
+      w[2] = digit[0];
+    }
+#pragma unroll
+    for (int n = 0; n < C::QTILES; ++n) {
+      put(n, i, w[n]);
+      sum[i >> 2][n] = __dp4a(static_cast<int>(w[n]), 0x01010101, sum[i >> 2][n]);
+    }
+  }
+#pragma unroll
+  for (int gp = 0; gp < C::NG; ++gp) {
+#pragma unroll
+    for (int n = 0; n < C::QTILES; ++n) {
+      int v = sum[gp][n];
+      v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+      v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+      bias[gp][n] = kIntBias + (C::KIND == KvType::kQ4 ? 8.f * static_cast<float>(v) : 0.f);
+    }
+  }
+  return back(top / most * 65536.f * mag);  // the highest digit counts 65536
 }
 
 // ------------------------------------------------------------------ kernel
@@ -487,6 +582,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   __shared__ float s_m[kWarps][8], s_l[kWarps][8];
   __shared__ long long s_sum[kWarps], s_begin;
   __shared__ int s_seq, s_last;
+  __shared__ __align__(8) float s_bias[C::NG][3][8];
   __shared__ __align__(16) Place s_places[kWarps][Filler<C>::kHalves];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.kv.n_kv;
@@ -547,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
   float* comb = reinterpret_cast<float*>(smem + kWarps * C::RING);
   float* mineq = comb + warp * (C::COMB / 4);
-  const uint32_t k_lane = KRows<C>::LaneOffset(lane), v_lane = VLaneOffset<C>(lane);
+  const uint32_t q_smem = dev::SmemAddr(smem) + kWarps * C::RING + C::JOIN;
+  const uint32_t k_lane = KLaneOffset<C>(lane), v_lane = VLaneOffset<C>(lane);
   Filler<C> fill;
   fill.at = use;
   fill.left = left;
@@ -571,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     const int queries = min(per_chunk, group - use.chunk * per_chunk);
     const int64_t col = (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
     const int seg = use.tile;
-    float x[C::KS][2][2] = {};
+    float x[D / 4] = {};
     {
       const int qi = C::PACK ? g & 3 : g;
       if (qi < queries) {
@@ -595,46 +692,26 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         if (fill.count > 0) fill.Pop();
       }
     }
-    uint32_t qh[C::KS][2], ql[C::PACK ? 1 : C::KS][2];
-    float cs[2];            // from products of the f16 terms to scores in log2 units
+    float cs[2];            // from products to scores in log2 units
     float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
     float l[2];             // sum of this lane's weights
     float acc[D / 16][4];
     int nu = 127 - 25;      // biased exponent of the power of two over the V scales seen
     {
-      float top = 0.f;
+      float bias[C::NG][C::QTILES];
+      const float up = WriteQ<C>(q_smem, x, p.scale, two_terms, warp, lane, bias);
+      if (C::QUANT && warp == 0 && t == 0) {
 #pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) {
+        for (int gp = 0; gp < C::NG; ++gp) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[ks][e >> 1][e & 1]));
-      }
-      top = LaneQuadMax(top);
-      // 2^-e of the largest value's exponent (kept in f32's normal range); the
-      // sign of the scale goes with it, so that cs is positive and the largest
-      // product has the largest score (a scale of zero clears q instead)
-      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
-      const float mag = fabsf(p.scale) * kLog2e;
-      const float down = p.scale == 0.f ? 0.f : copysignf(__uint_as_float(static_cast<uint32_t>(254 - e) << 23), p.scale);
-      const float up = p.scale == 0.f ? 1.f : fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * mag, 1e-37f);
-#pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float u = x[ks][b][0] * down, v = x[ks][b][1] * down;
-          const uint32_t h = PackHalf(u, v);
-          const float2 f = __half22float2(BitsHalf(h));
-          const uint32_t lo = PackHalf(u - f.x, v - f.y);
-          if (C::PACK) {
-            qh[ks][b] = two_terms && g >= 4 ? lo : h;
-          } else {
-            qh[ks][b] = h;
-            ql[ks][b] = lo;
-          }
+          for (int n = 0; n < C::QTILES; ++n) s_bias[gp][n][g] = bias[gp][n];
         }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         cs[c] = __shfl_sync(0xFFFFFFFFu, up, 4 * (C::PACK ? (2 * t + c) & 3 : 2 * t + c));
+        // (lanes that join the digits from the lower one have 256 times the product)
+        if (C::QUANT && C::PACK && t >= 2) cs[c] *= 1.f / 256;
         m[c] = ref[c] = -INFINITY;
         l[c] = 0.f;
       }
@@ -644,6 +721,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
       }
     }
+    __syncthreads();
 
     // ---- its tiles
     for (;;) {
@@ -662,46 +740,86 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
     if (work) {
       const uint32_t kbase = kslot + k_lane, sbase = kslot + C::R * C::ROW + g * (2 * C::NG);
+      const uint32_t qbase = q_smem + lane * 16;
+      if (!C::QUANT) {
 #pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
-        if (!C::QUANT) {
+        for (int k4 = 0; k4 < C::QWORDS / 4; ++k4) {
+          const uint4 q = Lds128(qbase + k4 * 512);
+          uint4 r = q;
+          if (!C::PACK && two_terms) r = Lds128(qbase + (C::QWORDS / 4 + k4) * 512);
 #pragma unroll
-          for (int ks = 0; ks < C::KS; ++ks) {
-            uint32_t a[4];
-            LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
-            ks == 0 ? MmaFirst(s[mt], a, qh[ks][0], qh[ks][1]) : Mma(s[mt], a, qh[ks][0], qh[ks][1]);
-            if (!C::PACK && two_terms) Mma(s[mt], a, ql[C::PACK ? 0 : ks][0], ql[C::PACK ? 0 : ks][1]);
+          for (int j = 0; j < 2; ++j) {
+            const int ks = 2 * k4 + j;
+#pragma unroll
+            for (int mt = 0; mt < C::MT; ++mt) {
+              uint32_t a[4];
+              LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
+              ks == 0 ? MmaFirst(s[mt], a, q.x, q.y) : Mma(s[mt], a, j == 0 ? q.x : q.z, j == 0 ? q.y : q.w);
+              if (!C::PACK && two_terms) Mma(s[mt], a, j == 0 ? r.x : r.z, j == 0 ? r.y : r.w);
+            }
           }
-        } else {
-          float2 d[2];
+        }
+      } else {
+        constexpr bool kU = C::KIND == KvType::kQ4;
+        float2 d[C::MT][2];
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t a = sbase + (16 * mt + 8 * i) * (2 * C::NG);
             const uint32_t k = C::NG == 2 ? Lds32(a) : Lds16(a);
             vsc[mt][i] = C::NG == 2 ? Lds32(a + C::SC) : Lds16(a + C::SC);
-            d[i] = __half22float2(BitsHalf(k));
+            d[mt][i] = __half22float2(BitsHalf(k));
+          }
+        }
+#pragma unroll
+        for (int gp = 0; gp < C::NG; ++gp) {
+          const uint4 q0 = Lds128(qbase + gp * 512);
+          const uint4 q1 = Lds128(qbase + (C::NG + gp) * 512);
+          const uint4 q2 = C::PACK ? q1 : Lds128(qbase + (2 * C::NG + gp) * 512);
+          float2 b0 = make_float2(kIntBias, kIntBias), b1 = b0, b2 = b0;
+          if (kU) {
+            b0 = *reinterpret_cast<const float2*>(&s_bias[gp][0][2 * t]);
+            b1 = *reinterpret_cast<const float2*>(&s_bias[gp][1][2 * t]);
+            b2 = *reinterpret_cast<const float2*>(&s_bias[gp][C::QTILES - 1][2 * t]);
           }
 #pragma unroll
-          for (int gp = 0; gp < C::NG; ++gp) {
-            KRows<C> rows;
-            rows.Load(kbase, mt, gp);
-            float part[4];
+          for (int mt = 0; mt < C::MT; ++mt) {
+            uint32_t a[2][4];
+            KFragments<C>(a, kbase, mt, gp);
+            auto product = [&](const uint4& q, const float2& b, float (&v)[4]) {
+              int n[4];
+              MmaIntFirst<kU>(n, a[0], q.x, q.y, kIntStart);
+              MmaInt<kU>(n, a[1], q.z, q.w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int ks = 4 * gp + j;
-              uint32_t a[4];
-              rows.Fragment(a, j, magic);
-              j == 0 ? MmaFirst(part, a, qh[ks][0], qh[ks][1]) : Mma(part, a, qh[ks][0], qh[ks][1]);
-              if (!C::PACK && two_terms) Mma(part, a, ql[C::PACK ? 0 : ks][0], ql[C::PACK ? 0 : ks][1]);
+              for (int c = 0; c < 4; ++c) v[c] = __int_as_float(n[c]) - ((c & 1) ? b.y : b.x);
+            };
+            float v[4], r[4];
+            product(q0, b0, v);
+            product(q1, b1, r);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = fmaf(r[c], C::PACK ? 1.f / 65536 : 1.f / 256, v[c]);
+            if (!C::PACK) {
+              product(q2, b2, r);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) v[c] = fmaf(r[c], 1.f / 65536, v[c]);
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float f = gp == 0 ? d[c >> 1].x : d[c >> 1].y;
-              s[mt][c] = gp == 0 ? part[c] * f : fmaf(part[c], f, s[mt][c]);
+              const float f = gp == 0 ? d[mt][c >> 1].x : d[mt][c >> 1].y;
+              s[mt][c] = gp == 0 ? v[c] * f : fmaf(v[c], f, s[mt][c]);
             }
           }
         }
-        if (C::PACK && two_terms) {
+      }
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt) {
+        if (C::PACK && C::QUANT) {  // lanes t < 2 hold the first digit, the others the second
+          const float f = t < 2 ? 1.f / 256 : 256.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[mt][c] = fmaf(__shfl_xor_sync(0xFFFFFFFFu, s[mt][c], 2), f, s[mt][c]);
+        }
+        if (C::PACK && !C::QUANT && two_terms) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) s[mt][c] += __shfl_xor_sync(0xFFFFFFFFu, s[mt][c], 2);
         }
