@@ -58,7 +58,6 @@ struct Cfg {
   static constexpr int QUERIES = PACK ? 4 : 8;
   static constexpr int R = QUANT || D == 64 ? 32 : 16;  // positions of a warp's step
   static constexpr int TILE = kWarps * R;
-  static constexpr int DEPTH = 1;
   static constexpr int MT = R / 16;     // 16-position tiles of a step
   static constexpr int KS = D / 16;     // 16-value slices of a head
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
@@ -67,7 +66,7 @@ struct Cfg {
   static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
   static constexpr int KSLOT = R * ROW + 2 * SC;     // K codes, K scales, V scales
   static constexpr int VSLOT = R * ROW;
-  static constexpr int RING = DEPTH * (KSLOT + VSLOT);  // per warp
+  static constexpr int RING = KSLOT + VSLOT;  // per warp
   static_assert(KSLOT % 128 == 0 && VSLOT % 128 == 0, "tiles are 128-byte lines");
   static constexpr int COMB = QUERIES * D * 4;   // per warp
   static constexpr int JOIN = kWarps * COMB > QUERIES * kKvMaxBlocks * 4 ? kWarps * COMB : QUERIES * kKvMaxBlocks * 4;
@@ -193,6 +192,11 @@ __device__ __forceinline__ uint64_t Lds64u(uint32_t a) {
   asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x) : "r"(a) : "memory");
   return x;
 }
+__device__ __forceinline__ ulonglong2 Lds64x2(uint32_t a) {
+  ulonglong2 x;
+  asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(x.x), "=l"(x.y) : "r"(a) : "memory");
+  return x;
+}
 __device__ __forceinline__ void Sts64(uint32_t a, uint64_t x) {
   asm volatile("st.shared.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory");
 }
@@ -270,31 +274,30 @@ struct Cursor {
   }
 };
 
-// The copying side of a warp.  The places of the next few steps are worked
-// out together, one 16-row half per lane, and left in shared memory; the page
-// ids they need are requested one such batch earlier.
-struct Place {
-  uint64_t code, scale;  // byte offsets of the half in the planes
+// The copying side of a warp.  The places of the next steps are worked out
+// together, one 16-row half per lane, and left in shared memory; the page ids
+// they need are requested one such batch earlier.
+struct Places {
+  uint64_t code[32], scale[32];  // byte offsets of the halves in the planes
 };
 template <typename C>
 struct Filler {
-  static constexpr int kHalves = 8, kSteps = kHalves / C::MT;
+  static constexpr int kSteps = 32 / C::MT;
+  static constexpr uint32_t kStep = (1u << C::MT) - 1;  // the halves of a step
   Cursor<C> at;        // the first step after the batch
   int left;            // steps not yet put in a batch
   int count = 0;       // steps of the batch not yet issued
-  int next = 0;        // first half of the next of them
   uint32_t have = 0;   // bit per half of the batch, the next step's lowest: it has rows in range and a page
   uint32_t bad = 0;    // as `have`: it has rows in range but no page
   int page = 0;        // this lane's half of the next batch
-  const char *k, *v, *scale;  // this lane's part of a copy's source, without the place
-  uint32_t places;  // shared-memory address
+  uint32_t place;      // shared-memory address of the next step's first code offset
+  uint32_t places;
 
   __device__ __forceinline__ int Pos(int warp, int lane) const {
     return at.span.base + (at.tile + lane / C::MT) * C::TILE + warp * C::R + (lane % C::MT) * 16;
   }
   __device__ __forceinline__ bool InRange(int pos, int lane) const {
-    return lane < kHalves && lane / C::MT < min(left, at.span.tiles - at.tile) && pos + 16 > at.span.start &&
-           pos < at.span.len;
+    return lane / C::MT < min(left, at.span.tiles - at.tile) && pos + 16 > at.span.start && pos < at.span.len;
   }
   __device__ __forceinline__ void Request(const KvAttendParams& p, int warp, int lane) {
     const int pos = Pos(warp, lane);
@@ -307,61 +310,69 @@ struct Filler {
     const int pos = Pos(warp, lane);
     const bool in = InRange(pos, lane);
     const bool ok = in && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
-    const int row = pos & ((1 << p.kv.page_log2) - 1);
+    const uint32_t row = pos & ((1 << p.kv.page_log2) - 1);
     __syncwarp();  // the last batch has been read
-    if (lane < kHalves) {
-      const uint64_t id = static_cast<uint32_t>(page), head = static_cast<uint32_t>(at.head);
-      const uint64_t code = id * p.page16 + head * p.head16 + static_cast<uint64_t>(static_cast<uint32_t>(row)) * p.pos16;
-      Sts64(places + lane * 16, code << 4);
-      if (C::QUANT) Sts64(places + lane * 16 + 8, ((id * p.spage16 + head * p.shead16) << 4) + row * (2 * C::NG));
-    }
+    const uint64_t id = static_cast<uint32_t>(page), head = static_cast<uint32_t>(at.head);
+    Sts64(places + lane * 8, (id * p.page16 + head * p.head16 + static_cast<uint64_t>(row) * p.pos16) << 4);
+    if (C::QUANT) Sts64(places + 256 + lane * 8, ((id * p.spage16 + head * p.shead16) << 4) + row * (2 * C::NG));
     have = __ballot_sync(0xFFFFFFFFu, ok);
     bad = __ballot_sync(0xFFFFFFFFu, in && !ok);
     count = min(kSteps, min(left, at.span.tiles - at.tile));
     left -= count;
-    next = 0;
+    place = places;
     if (left > 0) at.Next(p, chunks, count);
     Request(p, warp, lane);
+    __syncwarp();
   }
 
   // Copies the next step's K codes (and all its scales) or V codes into a
   // slot.  Halves that are out of range or have no page are left as they are.
+  // `lane_off` is the lane's part of a source offset.
   template <bool V>
-  __device__ __forceinline__ void Issue(const KvAttendParams& p, uint32_t slot, int lane) {
-    if (count > 0) {
-      constexpr int kRows = 32 / C::CPR, kPerHalf = 16 / kRows;  // rows of a copy instruction: all in one half
-      const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
-      const uint32_t q = places + next * 16;
+  __device__ __forceinline__ void Issue(const KvAttendParams& p, uint32_t slot, int lane, int64_t lane_off) {
+    constexpr int kRows = 32 / C::CPR, kPerHalf = 16 / kRows;  // rows of a copy instruction: all in one half
+    const uint32_t dst = slot + ChunkAt<C, V>(lane / C::CPR, lane % C::CPR);
+    const char* plane = (V ? p.kv.v : p.kv.k) + lane_off;
+    if ((have & kStep) == kStep && p.pos16 == C::ROW / 16) {  // the usual case: all of it, dense rows
+      ulonglong2 off;
+      if (C::MT == 2) {
+        off = Lds64x2(place);
+      } else {
+        off.x = off.y = Lds64u(place);
+      }
 #pragma unroll
       for (int h = 0; h < C::MT; ++h) {
-        if ((have >> h) & 1) {
-          const char* src = (V ? v : k) + Lds64u(q + 16 * h);
-          if (p.pos16 == C::ROW / 16) {  // dense rows: constant steps
+        const char* src = plane + (h == 0 ? off.x : off.y);
 #pragma unroll
-            for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
-          } else {
-#pragma unroll
-            for (int j = 0; j < kPerHalf; ++j) {
-              CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + j * kRows * p.kv.pos_stride);
-            }
-          }
-        }
+        for (int j = 0; j < kPerHalf; ++j) CopyAsync16(Moved<C, V>(dst, kRows * (h * kPerHalf + j), 0), src + 512 * j);
       }
-      if (C::QUANT && !V) {
-        constexpr int kPer = 2 * C::NG;  // a half's scales are dense: 16 rows of 2 NG bytes, in 16-byte pieces
-        const int h = lane / kPer % C::MT;
-        if (lane < 2 * C::MT * kPer && ((have >> h) & 1)) {
-          CopyAsync16(slot + C::R * C::ROW + lane * 16, scale + Lds64u(q + 16 * h + 8));
-        }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < C::MT * kPerHalf; ++i) {
+        const int h = i / kPerHalf;
+        if (!((have >> h) & 1)) continue;
+        CopyAsync16(slot + ChunkAt<C, V>(lane / C::CPR + kRows * i, lane % C::CPR),
+                    plane + Lds64u(place + 8 * h) + (i % kPerHalf) * kRows * p.kv.pos_stride);
+      }
+    }
+    if (C::QUANT && !V) {
+      constexpr int kPer = 2 * C::NG;  // a half's scales are dense: 16 rows of 2 NG bytes, in 16-byte pieces
+      const int h = lane / kPer % C::MT;
+      if (lane < 2 * C::MT * kPer && ((have >> h) & 1)) {
+        const char* sp = (lane < C::MT * kPer ? p.kv.k_scale : p.kv.v_scale) + lane % kPer * 16;
+        CopyAsync16(slot + C::R * C::ROW + lane * 16, sp + Lds64u(place + 256 + 8 * h));
       }
     }
     CopyCommit();
   }
-  __device__ __forceinline__ void Pop() {
+  // After both: on to the next step.  Returns the step's `bad`.
+  __device__ __forceinline__ uint32_t Pop() {
+    const uint32_t b = bad & kStep;
     --count;
-    next += C::MT;
+    place += 8 * C::MT;
     have >>= C::MT;
     bad >>= C::MT;
+    return b;
   }
 };
 
@@ -583,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   __shared__ long long s_sum[kWarps], s_begin;
   __shared__ int s_seq, s_last;
   __shared__ __align__(8) float s_bias[C::NG][3][8];
-  __shared__ __align__(16) Place s_places[kWarps][Filler<C>::kHalves];
+  __shared__ __align__(16) Places s_places[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.kv.n_kv;
   const int chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
@@ -648,18 +659,12 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   Filler<C> fill;
   fill.at = use;
   fill.left = left;
-  fill.places = dev::SmemAddr(s_places[warp]);
-  {
-    const int64_t part = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
-    fill.k = p.kv.k + part;
-    fill.v = p.kv.v + part;
-    constexpr int kPer = 2 * C::NG;
-    fill.scale = (lane < C::MT * kPer ? p.kv.k_scale : p.kv.v_scale) + lane % kPer * 16;
-  }
-  uint32_t bad = 0;  // two bits per step in flight
+  fill.places = fill.place = dev::SmemAddr(&s_places[warp]);
+  const int64_t lane_off = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
   fill.Request(p, warp, lane);
 
-  uint32_t kslot = ring;
+  const uint32_t kslot = ring, vslot = ring + C::KSLOT;
+  uint32_t bad_now = 0;  // the step's halves that have rows in range but no page
   const uint32_t magic = p.magic;
   const bool two_terms = p.type == ElemType::kF32;
   long long item0 = first - use.tile;  // the item's first tile
@@ -681,16 +686,10 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     if (begin) {  // the first steps' copies, while the queries are on their way
-#pragma unroll 1
-      for (int d = 0; d < C::DEPTH; ++d) {
-        if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
-        __syncwarp();
-        const uint32_t slot = ring + d * (C::KSLOT + C::VSLOT);
-        fill.template Issue<false>(p, slot, lane);
-        fill.template Issue<true>(p, slot + C::KSLOT, lane);
-        bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
-        if (fill.count > 0) fill.Pop();
-      }
+      fill.Batch(p, warp, lane, chunks);
+      fill.template Issue<false>(p, kslot, lane, lane_off);
+      fill.template Issue<true>(p, vslot, lane, lane_off);
+      bad_now = fill.Pop();
     }
     float cs[2];            // from products to scores in log2 units
     float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
@@ -725,16 +724,13 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 
     // ---- its tiles
     for (;;) {
-    if (fill.count == 0 && fill.left > 0) fill.Batch(p, warp, lane, chunks);
     const int pos = use.span.base + use.tile * C::TILE + warp * C::R;
     const int lo = use.span.start - pos, hi = use.span.len - pos;
     const bool work = lo < C::R && hi > 0;
-    const uint32_t bad_now = (bad >> (2 * (C::DEPTH - 1))) & 3u;
     const bool edge = lo > 0 || hi < C::R || bad_now != 0;
-    const uint32_t vslot = kslot + C::KSLOT;
 
     // ---- scores (and the V scales)
-    CopyWait<2 * C::DEPTH - 1>();
+    CopyWait<1>();
     __syncwarp();
     float s[C::MT][4];
     uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
@@ -826,7 +822,16 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     __syncwarp();
-    fill.template Issue<false>(p, kslot, lane);
+    if (fill.count == 0) {
+      if (fill.left > 0) {
+        fill.Batch(p, warp, lane, chunks);
+      } else {
+        fill.have = 0;  // no more steps
+      }
+    }
+    fill.template Issue<false>(p, kslot, lane, lane_off);
+    CopyWait<1>();  // V
+    __syncwarp();
 
     // ---- weights: 2^(score - ref) with ref a power of two over the largest,
     // so that a weight times its V scale is at most 2^14 and small ones stay
@@ -886,8 +891,6 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     }
 
     // ---- values
-    CopyWait<2 * C::DEPTH - 1>();
-    __syncwarp();
     if (work) {
       if (!C::QUANT && edge) {  // what lies out of range may be anything, NaN too: zeros
 #pragma unroll 1
@@ -958,11 +961,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       }
     }
     __syncwarp();
-    fill.template Issue<true>(p, vslot, lane);
-    bad = bad << 2 | (fill.count > 0 ? fill.bad & ((1u << C::MT) - 1) : 0u);
-    if (fill.count > 0) fill.Pop();
-    kslot = kslot + C::KSLOT + C::VSLOT == ring + C::RING ? ring : kslot + C::KSLOT + C::VSLOT;
-
+    fill.template Issue<true>(p, vslot, lane, lane_off);
+    bad_now = fill.Pop();
     --left;
     if (left == 0 || use.tile + 1 == use.span.tiles) break;
     ++use.tile;
