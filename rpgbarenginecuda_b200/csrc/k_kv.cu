@@ -1,6 +1,7 @@
 // k_kv.cu -- writing a paged key-value cache and reading it back.
 #include "common.h"
 #include "kv_dev.cuh"
+#include "launch.h"
 
 namespace rpgb {
 namespace {
@@ -90,6 +91,8 @@ __device__ __forceinline__ float InvRms(const float (&a)[4], const float (&b)[4]
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams p) {
   constexpr int L = D / 8;
+  dev::GridLaunchDependents();
+  dev::GridWait();  // (launched before the stream's previous kernel has finished)
   const int64_t t = blockIdx.x;
   const int hq = p.q_out != nullptr ? p.n_heads : 0;
   const int head = blockIdx.y * (kThreads / L) + threadIdx.x / L;  // the q heads that are wanted, k heads, v heads
@@ -179,6 +182,8 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(kThreads) KvGatherKernel(const KvGatherParams p) {
   constexpr int L = D / 8;
+  dev::GridLaunchDependents();
+  dev::GridWait();
   const int64_t t = blockIdx.x;
   const int head = blockIdx.y * (kThreads / L) + threadIdx.x / L;  // k heads, then v heads
   const int i = (threadIdx.x % L) * 8;
@@ -240,7 +245,7 @@ struct Append {
     constexpr int kHeads = kThreads / (D / 8);
     const int heads = (p.q_out != nullptr ? p.n_heads : 0) + 2 * p.kv.n_kv;
     const dim3 grid(static_cast<unsigned>(p.n_tok), (heads + kHeads - 1) / kHeads);
-    KvAppendKernel<D, KIND, T><<<grid, kThreads, 0, s>>>(p);
+    LaunchKernelArgs(reinterpret_cast<const void*>(KvAppendKernel<D, KIND, T>), grid, dim3(kThreads), 0, s, true, p);
   }
 };
 template <int D, KvType KIND, typename T>
@@ -248,7 +253,7 @@ struct Gather {
   static void Run(const KvGatherParams& p, cudaStream_t s) {
     constexpr int kHeads = kThreads / (D / 8);
     const dim3 grid(static_cast<unsigned>(p.n_tok), (2 * p.kv.n_kv + kHeads - 1) / kHeads);
-    KvGatherKernel<D, KIND, T><<<grid, kThreads, 0, s>>>(p);
+    LaunchKernelArgs(reinterpret_cast<const void*>(KvGatherKernel<D, KIND, T>), grid, dim3(kThreads), 0, s, true, p);
   }
 };
 

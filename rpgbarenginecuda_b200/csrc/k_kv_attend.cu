@@ -40,6 +40,7 @@
 
 #include "common.h"
 #include "kv_dev.cuh"
+#include "launch.h"
 
 namespace rpgb {
 namespace {
@@ -63,6 +64,7 @@ struct Cfg {
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;  // 16-byte chunks of a row
+  static constexpr int BORDER = QUANT ? 1 : 2;  // the end of an item costs a block about as much as so many tiles
   static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
   static constexpr int KSLOT = R * ROW + 2 * SC;     // K codes, K scales, V scales
   static constexpr int VSLOT = R * ROW;
@@ -318,7 +320,7 @@ struct Filler {
     have = __ballot_sync(0xFFFFFFFFu, ok);
     bad = __ballot_sync(0xFFFFFFFFu, in && !ok);
     count = min(kSteps, min(left, at.span.tiles - at.tile));
-    left -= count;
+    left -= count + (at.tile + count == at.span.tiles ? C::BORDER : 0);
     place = places;
     if (left > 0) at.Next(p, chunks, count);
     Request(p, warp, lane);
@@ -543,19 +545,19 @@ __device__ __forceinline__ float WriteQ(uint32_t base, const float (&x)[C::D / 4
   int sum[C::NG][C::QTILES] = {};
 #pragma unroll
   for (int i = 0; i < C::QWORDS; ++i) {  // word i: values 4 (i & 1) .. of the run's 8-value half, i / 4 the group
-    uint32_t digit[3] = {};
+    uint32_t u[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int first = 16 * (i >> 2) + 8 * ((i >> 1) & 1);
       const int v = first + (C::KIND == KvType::kQ8 ? 4 * (i & 1) + e : 2 * e + (i & 1));
-      int q = __float2int_rn(x[v] * to_int);
-#pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        const int b = static_cast<int8_t>(q);
-        digit[d] |= static_cast<uint32_t>(b & 255) << (8 * e);
-        q = (q - b) >> 8;
-      }
+      // with 128 added to every digit the digits are the bytes, each plus 128
+      u[e] = static_cast<uint32_t>(__float2int_rn(x[v] * to_int) + 0x808080);
     }
+    const uint32_t p01 = __byte_perm(u[0], u[1], 0x5140), p23 = __byte_perm(u[2], u[3], 0x5140);
+    uint32_t digit[3] = {__byte_perm(p01, p23, 0x5410), __byte_perm(p01, p23, 0x7632),
+                         __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410)};
+#pragma unroll
+    for (int d = 0; d < 3; ++d) digit[d] ^= 0x80808080u;
     uint32_t w[3];
     if (C::PACK) {
       w[0] = g < 4 ? digit[2] : digit[1];
@@ -586,6 +588,13 @@ __device__ __forceinline__ float WriteQ(uint32_t base, const float (&x)[C::D / 4
 
 // ------------------------------------------------------------------ kernel
 
+__device__ __forceinline__ void AddScaled(float4& v, float f, const float4& x) {
+  v.x += f * x.x;
+  v.y += f * x.y;
+  v.z += f * x.z;
+  v.w += f * x.w;
+}
+
 template <typename C>
 __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAttendParams p) {
   constexpr int D = C::D;
@@ -601,13 +610,15 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   const int per_chunk = (group + chunks - 1) / chunks;
   const int items = p.kv.n_kv * chunks;
 
-  // This block's share of the tiles: prefix sums of the conversations' tiles,
-  // a run of conversations per thread.
+  dev::GridLaunchDependents();
+  dev::GridWait();  // (launched before the stream's previous kernel has finished)
+  // This block's share of the tiles: prefix sums of the conversations' tiles
+  // (and their items' borders), a run of conversations per thread.
   const int run = (p.table.n_seq + kThreads - 1) / kThreads;
   long long mine = 0;
   for (int i = 0; i < run; ++i) {
     const int s = tid * run + i;
-    if (s < p.table.n_seq) mine += static_cast<long long>(SpanOf<C>(p, s).tiles) * items;
+    if (s < p.table.n_seq) mine += static_cast<long long>(SpanOf<C>(p, s).tiles + C::BORDER) * items;
   }
   long long upto = mine;
 #pragma unroll
@@ -631,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     long long at = upto - mine;
     int s = tid * run;
     for (;; ++s) {
-      const long long n = static_cast<long long>(SpanOf<C>(p, s).tiles) * items;
+      const long long n = static_cast<long long>(SpanOf<C>(p, s).tiles + C::BORDER) * items;
       if (first < at + n) break;
       at += n;
     }
@@ -640,15 +651,24 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   }
   __syncthreads();
   Cursor<C> use;
+  long long item0;  // the item's first tile
   use.seq = s_seq;
   use.span = SpanOf<C>(p, use.seq);
   {
     const long long in = first - s_begin;  // inside the conversation
-    const long long item = in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(use.span.tiles)
-                                            : in / use.span.tiles;
-    use.tile = static_cast<int>(in - item * use.span.tiles);
+    const int n = use.span.tiles + C::BORDER;
+    const long long item = in < (1ll << 31) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(n) : in / n;
+    use.tile = static_cast<int>(in - item * n);
     use.head = static_cast<int>(item) / chunks;
     use.chunk = static_cast<int>(item) % chunks;
+    item0 = first - use.tile;
+    if (use.tile >= use.span.tiles) {  // the share begins in an item's border
+      left -= n - use.tile;
+      if (left <= 0) return;
+      item0 += n;
+      use.tile = use.span.tiles;
+      use.Next(p, chunks, 0);
+    }
   }
 
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
@@ -667,7 +687,6 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   uint32_t bad_now = 0;  // the step's halves that have rows in range but no page
   const uint32_t magic = p.magic;
   const bool two_terms = p.type == ElemType::kF32;
-  long long item0 = first - use.tile;  // the item's first tile
   for (bool begin = true;; begin = false) {
     // ---- an item: its queries, as B fragments
     const int queries = min(per_chunk, group - use.chunk * per_chunk);
@@ -964,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     fill.template Issue<true>(p, vslot, lane, lane_off);
     bad_now = fill.Pop();
     --left;
-    if (left == 0 || use.tile + 1 == use.span.tiles) break;
+    if (left <= 0 || use.tile + 1 == use.span.tiles) break;
     ++use.tile;
     }
 
@@ -997,23 +1016,34 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       const int64_t out = use.seq * p.out_stride + col;
       const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
-      // The warps' shares joined: value i of the item's queries, its sum, its maximum.
+      // The warps' shares joined: values 4 i .. 4 i + 3 of the item's queries.
       auto join = [&](int i, float& sum, float& top) {
-        const int q = i / D;
+        const int q = 4 * i / D;
         top = s_m[0][q];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][q]);
         const float ref = top == -INFINITY ? 0.f : top;
-        float v = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float f = Exp2(s_m[w][q] - ref);
-          v += f * comb[w * (C::COMB / 4) + i];
-          sum += f * s_l[w][q];
+          AddScaled(v, Exp2(s_m[w][q] - ref), reinterpret_cast<const float4*>(comb + w * (C::COMB / 4))[i]);
+          sum += Exp2(s_m[w][q] - ref) * s_l[w][q];
         }
         return v;
       };
+      auto put = [&](int i, const float4& v, float sum) {
+        const float f = sum != 0.f ? 1.f / sum : 0.f;  // nothing in range: zero
+        float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = past ? kvd::Nan() : y[e];
+        switch (p.type) {
+          case ElemType::kF32: kvd::Store4(static_cast<float*>(p.out) + out + 4 * i, y); break;
+          case ElemType::kF16: kvd::Store4(static_cast<__half*>(p.out) + out + 4 * i, y); break;
+          case ElemType::kBF16: kvd::Store4(static_cast<__nv_bfloat16*>(p.out) + out + 4 * i, y); break;
+        }
+      };
+      const int vecs = queries * D / 4;
       bool finish = whole;
       if (!whole) {
         // This block's record: one for an item that began in an earlier block,
@@ -1025,26 +1055,62 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         auto record = [&](int b) { return records + (2 * b + (b == b0 ? 1 : 0)) * kRecord; };
         unsigned* count = static_cast<unsigned*>(p.workspace) + (static_cast<int64_t>(use.seq) * p.kv.n_kv + use.head) * chunks + use.chunk;
         float* rec = record(blockIdx.x);
-        for (int i = tid; i < queries * D; i += kThreads) {
+        for (int i = tid; i < vecs; i += kThreads) {
           float sum, top;
-          rec[i] = join(i, sum, top);
-          if (i % D == 0) {
-            rec[kKvMaxQueries * D + i / D] = top;
-            rec[kKvMaxQueries * (D + 1) + i / D] = sum;
+          reinterpret_cast<float4*>(rec)[i] = join(i, sum, top);
+          if (i % (D / 4) == 0) {
+            rec[kKvMaxQueries * D + i / (D / 4)] = top;
+            rec[kKvMaxQueries * (D + 1) + i / (D / 4)] = sum;
           }
         }
-        __threadfence();
         __syncthreads();
-        if (tid == 0) s_last = atomicAdd(count, 1u) == static_cast<unsigned>(b1 - b0);
+        if (tid == 0) {
+          __threadfence();  // the whole block's record, after the barrier
+          s_last = atomicAdd(count, 1u) == static_cast<unsigned>(b1 - b0);
+          __threadfence();
+        }
         __syncthreads();
         finish = s_last != 0;
+        if (finish && tid == 0) *count = 0;
+        constexpr int kFew = 4;
+        if (finish && b1 - b0 < kFew) {
+          // Few records: every thread reads what it needs of all of them at once.
+          finish = false;
+          for (int i = tid; i < vecs; i += kThreads) {
+            const int q = 4 * i / D;
+            float top = -INFINITY, m_[kFew], l_[kFew];
+            float4 v[kFew];
+#pragma unroll
+            for (int n = 0; n < kFew; ++n) {
+              m_[n] = -INFINITY;
+              l_[n] = 0.f;
+              v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (b0 + n <= b1) {
+                const float* r = record(b0 + n);
+                m_[n] = __ldcg(r + kKvMaxQueries * D + q);
+                l_[n] = __ldcg(r + kKvMaxQueries * (D + 1) + q);
+                v[n] = __ldcg(reinterpret_cast<const float4*>(r) + i);
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < kFew; ++n) top = fmaxf(top, m_[n]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 sumv = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < kFew; ++n) {
+              const float f = Exp2(m_[n] - ref);
+              AddScaled(sumv, f, v[n]);
+              sum += f * l_[n];
+            }
+            put(i, sumv, sum);
+          }
+        }
         if (finish) {
           // The last block joins all records under the maximum of all.  First
           // the records' factors, a query per warp and a record per lane, into
           // the join area; then warp w adds up records b0 + w, b0 + w + 4, ...
           // in that order, a few of them in flight.
-          __threadfence();
-          if (tid == 0) *count = 0;
           float* factor = comb;  // [query][record]
           for (int q = warp; q < queries; q += kWarps) {
             float top = -INFINITY, sum = 0.f;
@@ -1086,10 +1152,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
                 const int q = D == 128 ? k : 2 * k + (lane >> 4);
                 if (b + n * kWarps <= b1 && q < queries) {
                   const float f = factor[q * kKvMaxBlocks + b - b0 + n * kWarps];
-                  v[k].x += f * r[n][k].x;
-                  v[k].y += f * r[n][k].y;
-                  v[k].z += f * r[n][k].z;
-                  v[k].w += f * r[n][k].w;
+                  AddScaled(v[k], f, r[n][k]);
                 }
               }
             }
@@ -1101,22 +1164,17 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         }
       }
       if (finish) {
-        for (int i = tid; i < queries * D; i += kThreads) {
+        for (int i = tid; i < vecs; i += kThreads) {
           float sum, top;
-          float v = join(i, sum, top);
-          v = sum != 0.f ? v / sum : 0.f;  // nothing in range: zero
-          if (past) v = kvd::Nan();
-          switch (p.type) {
-            case ElemType::kF32: static_cast<float*>(p.out)[out + i] = v; break;
-            case ElemType::kF16: static_cast<__half*>(p.out)[out + i] = __float2half_rn(v); break;
-            case ElemType::kBF16: static_cast<__nv_bfloat16*>(p.out)[out + i] = __float2bfloat16_rn(v); break;
-          }
+          const float4 v = join(i, sum, top);
+          put(i, v, sum);
         }
       }
       __syncthreads();  // the next item writes the join area again
     }
-    if (left == 0) break;
-    item0 += use.span.tiles;
+    left -= C::BORDER;  // (a share that ends inside the item ends all the same)
+    if (left <= 0) break;
+    item0 += use.span.tiles + C::BORDER;
     use.Next(p, chunks);
   }
   CopyWait<0>();
@@ -1141,7 +1199,7 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   }
   // no more blocks than tiles there can be
   const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
-  const int64_t tiles = ((cap + 15) / C::TILE + 1) * p.kv.n_kv * chunks;
+  const int64_t tiles = ((cap + 15) / C::TILE + 1 + C::BORDER) * p.kv.n_kv * chunks;
   if (tiles < grid && tiles * p.table.n_seq < grid) grid = static_cast<int>(tiles * p.table.n_seq);
   KvAttendParams a = p;
   a.magic = kMagic;
@@ -1150,7 +1208,7 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);
   a.spage16 = static_cast<uint32_t>(p.kv.scale_page_stride / 16);
   a.shead16 = static_cast<uint32_t>(p.kv.scale_head_stride / 16);
-  KvAttendKernel<C><<<grid, kThreads, C::SMEM, s>>>(a);
+  LaunchKernelArgs(reinterpret_cast<const void*>(KvAttendKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, a);
 }
 
 template <int D, KvType KIND>
