@@ -1,4 +1,6 @@
 // k_kv.cu -- writing a paged key-value cache and reading it back.
+#include <atomic>
+
 #include "common.h"
 #include "kv_dev.cuh"
 #include "launch.h"
@@ -21,10 +23,10 @@ __device__ __forceinline__ uint32_t LanesMax(uint32_t v) {
   for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
   return v;
 }
-__device__ __forceinline__ uint32_t MaxAbs4(const float (&x)[4]) {
+__device__ __forceinline__ uint32_t MaxAbs8(const float (&x)[8]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
   return m;
 }
 // The scale of a group from the bits of its largest magnitude: rounded to f16
@@ -36,182 +38,242 @@ __device__ __forceinline__ __half GroupScale(uint32_t max_bits) {
   return __float2half_rn(max_bits > 0x7F800000u ? m : fminf(m * (1.f / MostCode<KIND>()), 65504.f));
 }
 
-// Codes of four consecutive values x, nearest with ties to even.  A scale that
-// was rounded down (far down where it is subnormal) needs the clamp.
+// x / d rounded to the nearest integer, ties to even, as the IEEE quotient
+// gives it: the product with 1 / d is off by less than 1e-4 for quotients to
+// 127, so only a product that close to a tie needs the division.
+__device__ __forceinline__ float RoundedQuotient(float x, float d, float inv) {
+  const float y = x * inv;
+  float c = rintf(y);
+  if (fabsf(fabsf(y - c) - 0.5f) < 1e-4f) c = rintf(x / d);
+  return c;
+}
+
+// Codes of eight consecutive values.  A scale that was rounded down (far down
+// where it is subnormal) needs the clamp.
 template <KvType KIND>
-__device__ __forceinline__ void StoreCodes(char* row, int i, const float (&x)[4], float d) {
-  uint32_t w = 0;
+__device__ __forceinline__ void StoreCodes(char* row, int i, const float (&x)[8], float d) {
+  constexpr float kMost = MostCode<KIND>();
+  // (a subnormal scale has an infinite reciprocal only below 2^-128: f16 scales are at least 2^-24)
+  const float inv = d > 0.f ? 1.f / d : 0.f;
+  uint32_t w[2] = {};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float c = d > 0.f ? fminf(fmaxf(rintf(x[e] / d), -MostCode<KIND>()), MostCode<KIND>()) : 0.f;
+  for (int e = 0; e < 8; ++e) {
+    const float c = d > 0.f ? fminf(fmaxf(RoundedQuotient(x[e], d, inv), -kMost), kMost) : 0.f;
     const int q = static_cast<int>(c);
-    w |= KIND == KvType::kQ8 ? static_cast<uint32_t>(q & 255) << (8 * e) : static_cast<uint32_t>(q + 8) << (4 * e);
+    if (KIND == KvType::kQ8) {
+      w[e >> 2] |= static_cast<uint32_t>(q & 255) << (8 * (e & 3));
+    } else {
+      w[0] |= static_cast<uint32_t>(q + 8) << (4 * e);
+    }
   }
   if (KIND == KvType::kQ8) {
-    *reinterpret_cast<uint32_t*>(row + i) = w;
+    *reinterpret_cast<uint2*>(row + i) = make_uint2(w[0], w[1]);
   } else {
-    *reinterpret_cast<uint16_t*>(row + i / 2) = static_cast<uint16_t>(w);
+    *reinterpret_cast<uint32_t*>(row + i / 2) = w[0];
   }
 }
 
 // 1 / sqrt(mean x^2 + eps) of a head, in f32.  The squares and sums round one
-// by one (no fused multiply-add) in a fixed tree: the halves' lanes, then
-// lanes 8, 4, 2 and 1 apart.
+// by one (no fused multiply-add) in a fixed tree.
 template <int D>
-__device__ __forceinline__ float InvRms(const float (&a)[4], const float (&b)[4], float eps) {
-  float t[4], s;
-  if (D == 128) {  // runs of four values first
-    float u = __fmul_rn(a[0], a[0]), v = __fmul_rn(b[0], b[0]);
+__device__ __forceinline__ float InvRms(const float (&a)[8], const float (&b)[8], float eps) {
+  float s;
+  if (D == 128) {  // runs of four values, then runs 64, 32, 16, 8 and 4 values apart
+    float u[2];
 #pragma unroll
-    for (int e = 1; e < 4; ++e) {
-      u = __fadd_rn(u, __fmul_rn(a[e], a[e]));
-      v = __fadd_rn(v, __fmul_rn(b[e], b[e]));
+    for (int h = 0; h < 2; ++h) {
+      float p = __fmul_rn(a[4 * h], a[4 * h]), q = __fmul_rn(b[4 * h], b[4 * h]);
+#pragma unroll
+      for (int e = 4 * h + 1; e < 4 * h + 4; ++e) {
+        p = __fadd_rn(p, __fmul_rn(a[e], a[e]));
+        q = __fadd_rn(q, __fmul_rn(b[e], b[e]));
+      }
+      u[h] = __fadd_rn(p, q);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) u[h] = __fadd_rn(u[h], __shfl_xor_sync(0xFFFFFFFFu, u[h], o));
     }
-    s = __fadd_rn(u, v);
+    s = __fadd_rn(u[0], u[1]);
+  } else {  // values 32, 16, 8, 4, 2 and 1 apart
+    float t[8];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xFFFFFFFFu, s, o));
-  } else {  // the lanes first, then the values of a lane
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
       t[e] = __fadd_rn(__fmul_rn(a[e], a[e]), __fmul_rn(b[e], b[e]));
 #pragma unroll
-      for (int o = D / 16; o > 0; o >>= 1) t[e] = __fadd_rn(t[e], __shfl_xor_sync(0xFFFFFFFFu, t[e], o));
+      for (int o = 2; o > 0; o >>= 1) t[e] = __fadd_rn(t[e], __shfl_xor_sync(0xFFFFFFFFu, t[e], o));
     }
-    s = __fadd_rn(__fadd_rn(t[0], t[2]), __fadd_rn(t[1], t[3]));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+      for (int e = 0; e < o; ++e) t[e] = __fadd_rn(t[e], t[e + o]);
+    }
+    s = t[0];
   }
   return rsqrtf(__fadd_rn(__fmul_rn(s, 1.0f / D), eps));
 }
 
-// One row t, one head per D / 8 lanes.  Lane i holds values 4 i .. 4 i + 3 of
-// the first half (a) and of the second (b), so a rotation pair (j, j + D / 2)
-// sits in one lane and a scale group of 64 values in the same lanes.  Norm and
-// rotation round every product and sum on its own, so a value that falls near
-// a rounding boundary of the cache gets the code of the formulas evaluated
-// step by step in f32.
+// One row t per block (and a part of its heads when the rows are few), one
+// head per D / 16 lanes at a time.  Lane i holds values 8 i .. 8 i + 7 of the
+// first half (a) and of the second (b), so a rotation pair (j, j + D / 2) sits
+// in one lane and a scale group of 64 values in the same lanes; the rotation
+// stays in registers for all heads.  Norm and rotation round every product and
+// sum on its own, so a value that falls near a rounding boundary of the cache
+// gets the code of the formulas evaluated step by step in f32.
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams p) {
-  constexpr int L = D / 8;
+  constexpr int L = D / 16, kHeads = kThreads / L;
   dev::GridLaunchDependents();
   dev::GridWait();  // (launched before the stream's previous kernel has finished)
   const int64_t t = blockIdx.x;
   const int hq = p.q_out != nullptr ? p.n_heads : 0;
-  const int head = blockIdx.y * (kThreads / L) + threadIdx.x / L;  // the q heads that are wanted, k heads, v heads
+  const int heads = hq + 2 * p.kv.n_kv;  // the q heads that are wanted, k heads, v heads
   const int i = threadIdx.x % L;
-  const bool live = head < hq + 2 * p.kv.n_kv;
   const int pos = p.pos[t];
   const int seq = p.seq != nullptr ? p.seq[t] : static_cast<int>(t);
   const int page = pos < 0 ? -1 : kvd::PageOf(p.table, p.kv.n_pages, seq, pos >> p.kv.page_log2);
   const bool ok = page >= 0 && (p.rope == nullptr || pos < p.rope_positions);
-  enum { kQ, kK, kV };
-  const int kind = head < hq ? kQ : (head < hq + p.kv.n_kv ? kK : kV);
-  const int h = kind == kQ ? head : (kind == kK ? head - hq : head - hq - p.kv.n_kv);
-  const int col = (kind == kQ ? h : p.n_heads + (kind == kV ? p.kv.n_kv : 0) + h) * D;
-
-  float a[4] = {}, b[4] = {};
-  if (live && ok) {
-    const T* x = static_cast<const T*>(p.qkv) + t * p.qkv_stride + col;
-    kvd::Load4(x + 4 * i, a);
-    kvd::Load4(x + D / 2 + 4 * i, b);
-  }
-  const float* w = kind == kQ ? p.q_norm : (kind == kK ? p.k_norm : nullptr);
-  const float r = InvRms<D>(a, b, p.eps);  // every lane takes part, whatever its head
-  if (w != nullptr) {
-    float wa[4], wb[4];
-    kvd::Load4(w + 4 * i, wa);
-    kvd::Load4(w + D / 2 + 4 * i, wb);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = __fmul_rn(__fmul_rn(a[e], r), wa[e]);
-      b[e] = __fmul_rn(__fmul_rn(b[e], r), wb[e]);
-    }
-  }
-  if (kind != kV && p.rope != nullptr && ok) {
-    const float* rr = p.rope + static_cast<int64_t>(pos) * D;
-    float c[4], s[4];
-    kvd::Load4(rr + 4 * i, c);
-    kvd::Load4(rr + D / 2 + 4 * i, s);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = a[e], y = b[e];
-      a[e] = __fsub_rn(__fmul_rn(x, c[e]), __fmul_rn(y, s[e]));
-      b[e] = __fadd_rn(__fmul_rn(y, c[e]), __fmul_rn(x, s[e]));
-    }
-  }
-  uint32_t ma = 0, mb = 0;
-  if (KIND != KvType::kF16) {
-    ma = MaxAbs4(a);
-    mb = MaxAbs4(b);
-    if (D == kKvGroup) ma = mb = max(ma, mb);
-    ma = LanesMax<L>(ma);
-    mb = D == kKvGroup ? ma : LanesMax<L>(mb);
-  }
-  if (!live) return;
-  if (kind == kQ) {
-    if (!ok) {  // padding rows are zero, rows without a place NaN
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[e] = b[e] = pos < 0 ? 0.f : kvd::Nan();
-    }
-    T* q = static_cast<T*>(p.q_out) + t * p.q_stride + static_cast<int64_t>(h) * D;
-    kvd::Store4(q + 4 * i, a);
-    kvd::Store4(q + D / 2 + 4 * i, b);
-    return;
-  }
-  if (!ok) return;
   const int at = pos & ((1 << p.kv.page_log2) - 1);
-  char* row = (kind == kK ? p.kv.k : p.kv.v) + kvd::CodeOffset(p.kv, page, h, at);
-  if (KIND == KvType::kF16) {
-    kvd::Store4(reinterpret_cast<__half*>(row) + 4 * i, a);
-    kvd::Store4(reinterpret_cast<__half*>(row) + D / 2 + 4 * i, b);
-    return;
+  const bool turn = p.rope != nullptr && ok;
+  float cs[8], sn[8];
+  if (turn) {
+    const float* rr = p.rope + static_cast<int64_t>(pos) * D;
+    kvd::Load8(rr + 8 * i, cs);
+    kvd::Load8(rr + D / 2 + 8 * i, sn);
   }
-  __half* sc = reinterpret_cast<__half*>((kind == kK ? p.kv.k_scale : p.kv.v_scale) +
-                                         kvd::ScaleOffset(p.kv, page, h, at));
-  const __half da = GroupScale<KIND>(ma), db = GroupScale<KIND>(mb);
-  if (i == 0) {
-    if (D == kKvGroup) {
-      *sc = da;
-    } else {
-      *reinterpret_cast<__half2*>(sc) = __halves2half2(da, db);
+  enum { kQ, kK, kV };
+  // (every lane of a warp goes round as often: the shuffles need them all)
+  for (int head0 = blockIdx.y * kHeads; head0 < heads; head0 += gridDim.y * kHeads) {
+    const int head = head0 + threadIdx.x / L;
+    const bool live = head < heads;
+    const int kind = head < hq ? kQ : (head < hq + p.kv.n_kv ? kK : kV);
+    const int h = kind == kQ ? head : (kind == kK ? head - hq : head - hq - p.kv.n_kv);
+    const int col = (kind == kQ ? h : p.n_heads + (kind == kV ? p.kv.n_kv : 0) + h) * D;
+    float a[8] = {}, b[8] = {};
+    if (live && ok) {
+      const T* x = static_cast<const T*>(p.qkv) + t * p.qkv_stride + col;
+      kvd::Load8(x + 8 * i, a);
+      kvd::Load8(x + D / 2 + 8 * i, b);
     }
+    const float* w = kind == kQ ? p.q_norm : (kind == kK ? p.k_norm : nullptr);
+    const float r = InvRms<D>(a, b, p.eps);
+    if (w != nullptr) {
+      float wa[8], wb[8];
+      kvd::Load8(w + 8 * i, wa);
+      kvd::Load8(w + D / 2 + 8 * i, wb);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[e] = __fmul_rn(__fmul_rn(a[e], r), wa[e]);
+        b[e] = __fmul_rn(__fmul_rn(b[e], r), wb[e]);
+      }
+    }
+    if (kind != kV && turn) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = a[e], y = b[e];
+        a[e] = __fsub_rn(__fmul_rn(x, cs[e]), __fmul_rn(y, sn[e]));
+        b[e] = __fadd_rn(__fmul_rn(y, cs[e]), __fmul_rn(x, sn[e]));
+      }
+    }
+    uint32_t ma = 0, mb = 0;
+    if (KIND != KvType::kF16) {
+      ma = MaxAbs8(a);
+      mb = MaxAbs8(b);
+      if (D == kKvGroup) ma = mb = max(ma, mb);
+      ma = LanesMax<L>(ma);
+      mb = D == kKvGroup ? ma : LanesMax<L>(mb);
+    }
+    if (!live) continue;
+    if (kind == kQ) {
+      if (!ok) {  // padding rows are zero, rows without a place NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = b[e] = pos < 0 ? 0.f : kvd::Nan();
+      }
+      T* q = static_cast<T*>(p.q_out) + t * p.q_stride + static_cast<int64_t>(h) * D;
+      kvd::Store8(q + 8 * i, a);
+      kvd::Store8(q + D / 2 + 8 * i, b);
+      continue;
+    }
+    if (!ok) continue;
+    char* row = (kind == kK ? p.kv.k : p.kv.v) + kvd::CodeOffset(p.kv, page, h, at);
+    if (KIND == KvType::kF16) {
+      kvd::Store8(reinterpret_cast<__half*>(row) + 8 * i, a);
+      kvd::Store8(reinterpret_cast<__half*>(row) + D / 2 + 8 * i, b);
+      continue;
+    }
+    __half* sc = reinterpret_cast<__half*>((kind == kK ? p.kv.k_scale : p.kv.v_scale) +
+                                           kvd::ScaleOffset(p.kv, page, h, at));
+    const __half da = GroupScale<KIND>(ma), db = GroupScale<KIND>(mb);
+    if (i == 0) {
+      if (D == kKvGroup) {
+        *sc = da;
+      } else {
+        *reinterpret_cast<__half2*>(sc) = __halves2half2(da, db);
+      }
+    }
+    StoreCodes<KIND>(row, 8 * i, a, __half2float(da));
+    StoreCodes<KIND>(row, D / 2 + 8 * i, b, __half2float(db));
   }
-  StoreCodes<KIND>(row, 4 * i, a, __half2float(da));
-  StoreCodes<KIND>(row, D / 2 + 4 * i, b, __half2float(db));
 }
 
-// One row t; eight consecutive values of one head's k or v row per thread.
+// Sixteen consecutive values of one head's k or v row per thread and row; the
+// block's threads cover (values of a head) x (k heads, then v heads) x (rows),
+// and each takes kRows rows of every blockDim.z at once, so that their chains
+// of loads (position, page, codes) run side by side.
+constexpr int kRows = 4;
 template <int D, KvType KIND, typename T>
-__global__ void __launch_bounds__(kThreads) KvGatherKernel(const KvGatherParams p) {
-  constexpr int L = D / 8;
+__global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
   dev::GridLaunchDependents();
   dev::GridWait();
-  const int64_t t = blockIdx.x;
-  const int head = blockIdx.y * (kThreads / L) + threadIdx.x / L;  // k heads, then v heads
-  const int i = (threadIdx.x % L) * 8;
+  const int i = threadIdx.x * 16;
+  const int head = blockIdx.y * blockDim.y + threadIdx.y;
   if (head >= 2 * p.kv.n_kv) return;
   const bool is_k = head < p.kv.n_kv;
   const int h = is_k ? head : head - p.kv.n_kv;
   T* out = static_cast<T*>(is_k ? p.k_out : p.v_out);
   if (out == nullptr) return;
-  out += t * p.out_stride + static_cast<int64_t>(h) * D + i;
-  const int pos = p.pos[t];
-  const int seq = p.seq != nullptr ? p.seq[t] : static_cast<int>(t);
-  const int page = pos < 0 ? -1 : kvd::PageOf(p.table, p.kv.n_pages, seq, pos >> p.kv.page_log2);
-  const int at = pos & ((1 << p.kv.page_log2) - 1);
-  float x[2][4];
-  if (page < 0) {
+  const char* plane = is_k ? p.kv.k : p.kv.v;
+  const char* scales = is_k ? p.kv.k_scale : p.kv.v_scale;
+  int64_t t[kRows];
+  int pos[kRows], page[kRows];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = pos < 0 ? 0.f : kvd::Nan();
-  } else {
-    const char* row = (is_k ? p.kv.k : p.kv.v) + kvd::CodeOffset(p.kv, page, h, at);
-    const __half* sc = nullptr;
-    if (KIND != KvType::kF16) {
-      sc = reinterpret_cast<const __half*>((is_k ? p.kv.k_scale : p.kv.v_scale) + kvd::ScaleOffset(p.kv, page, h, at));
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = kvd::Value<KIND>(row, sc, i + e);
+  for (int r = 0; r < kRows; ++r) {
+    t[r] = (static_cast<int64_t>(blockIdx.x) * kRows + r) * blockDim.z + threadIdx.z;
+    pos[r] = -1;
+    page[r] = -1;
+    if (t[r] < p.n_tok) pos[r] = __ldg(p.pos + t[r]);
   }
-  kvd::Store4(out, x[0]);
-  kvd::Store4(out + 4, x[1]);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (pos[r] >= 0) {
+      const int seq = p.seq != nullptr ? __ldg(p.seq + t[r]) : static_cast<int>(t[r]);
+      page[r] = kvd::PageOf(p.table, p.kv.n_pages, seq, pos[r] >> p.kv.page_log2);
+    }
+  }
+  kvd::Codes16<KIND> codes[kRows];
+  __half d[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (page[r] >= 0) {
+      const int at = pos[r] & ((1 << p.kv.page_log2) - 1);
+      codes[r].Load(plane + kvd::CodeOffset(p.kv, page[r], h, at), i);
+      if (KIND != KvType::kF16) {
+        d[r] = *reinterpret_cast<const __half*>(scales + kvd::ScaleOffset(p.kv, page[r], h, at) + i / kKvGroup * 2);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (t[r] >= p.n_tok) continue;
+    T* row = out + t[r] * p.out_stride + static_cast<int64_t>(h) * D + i;
+    if (page[r] >= 0) {
+      codes[r].Store(row, d[r]);
+    } else {  // padding rows are zero, rows without a place NaN
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = pos[r] < 0 ? 0.f : kvd::Nan();
+      kvd::Store8(row, x);
+      kvd::Store8(row + 8, x);
+    }
+  }
 }
 
 template <template <int, KvType, typename> class F, typename P>
@@ -239,21 +301,40 @@ void Dispatch(const P& p, cudaStream_t s) {
   }
 }
 
+int NumSms() {
+  static std::atomic<int> sms[64];
+  int dev = 0, n = 0;
+  RPGB_CUDA(cudaGetDevice(&dev));
+  RPGB_CHECK(dev < 64, "kv: device %d", dev);
+  n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    RPGB_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <int D, KvType KIND, typename T>
 struct Append {
   static void Run(const KvAppendParams& p, cudaStream_t s) {
-    constexpr int kHeads = kThreads / (D / 8);
+    constexpr int kHeads = kThreads / (D / 16);
     const int heads = (p.q_out != nullptr ? p.n_heads : 0) + 2 * p.kv.n_kv;
-    const dim3 grid(static_cast<unsigned>(p.n_tok), (heads + kHeads - 1) / kHeads);
+    // few rows: their heads go to blocks of their own (latency); many: a block keeps its row's rotation
+    const int parts = (heads + kHeads - 1) / kHeads;
+    const dim3 grid(static_cast<unsigned>(p.n_tok), p.n_tok * parts <= 4 * NumSms() ? parts : 1);
     LaunchKernelArgs(reinterpret_cast<const void*>(KvAppendKernel<D, KIND, T>), grid, dim3(kThreads), 0, s, true, p);
   }
 };
 template <int D, KvType KIND, typename T>
 struct Gather {
   static void Run(const KvGatherParams& p, cudaStream_t s) {
-    constexpr int kHeads = kThreads / (D / 8);
-    const dim3 grid(static_cast<unsigned>(p.n_tok), (2 * p.kv.n_kv + kHeads - 1) / kHeads);
-    LaunchKernelArgs(reinterpret_cast<const void*>(KvGatherKernel<D, KIND, T>), grid, dim3(kThreads), 0, s, true, p);
+    constexpr int L = D / 16;
+    const int heads = 2 * p.kv.n_kv, y = heads < 256 / L ? heads : 256 / L;
+    // few rows: a block takes kRows at most; many: as many as fit its threads
+    const int64_t fit = 256 / (L * y), z = p.n_tok < 2 * NumSms() ? 1 : fit;
+    const dim3 block(L, y, static_cast<unsigned>(z));
+    const dim3 grid(static_cast<unsigned>((p.n_tok + kRows * z - 1) / (kRows * z)), (heads + y - 1) / y);
+    LaunchKernelArgs(reinterpret_cast<const void*>(KvGatherKernel<D, KIND, T>), grid, block, 0, s, true, p);
   }
 };
 

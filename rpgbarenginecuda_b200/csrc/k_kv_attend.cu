@@ -210,8 +210,8 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t HalfBits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 BitsHalf(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+using kvd::BitsHalf;
+using kvd::HalfBits;
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return HalfBits(__floats2half2_rn(lo, hi)); }
 
 // 1024 + u as f16 is 0x6400 | u for u < 1024, so a code in the low bits of

@@ -60,16 +60,94 @@ __device__ __forceinline__ void Store4(T* p, const float (&x)[4]) {
   for (int i = 0; i < 4; ++i) r.v[i] = FromFloat<T>(x[i]);
   *reinterpret_cast<Pack<T, 4>*>(p) = r;
 }
-
-// Value `i` of a cache row (codes at `row`, its scales at `sc`).
-template <KvType KIND>
-__device__ __forceinline__ float Value(const char* row, const __half* sc, int i) {
-  if (KIND == KvType::kF16) return __half2float(reinterpret_cast<const __half*>(row)[i]);
-  const float d = __half2float(sc[i / kKvGroup]);
-  if (KIND == KvType::kQ8) return static_cast<float>(reinterpret_cast<const int8_t*>(row)[i]) * d;
-  const int b = reinterpret_cast<const uint8_t*>(row)[i >> 1];
-  return static_cast<float>(((i & 1) ? (b >> 4) : (b & 15)) - 8) * d;
+// Eight values, 16 bytes at a time.
+template <typename T>
+__device__ __forceinline__ void Load8(const T* p, float (&x)[8]) {
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 8; j += N) {
+    const Pack<T, N> r = *reinterpret_cast<const Pack<T, N>*>(p + j);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[j + i] = ToFloat(r.v[i]);
+  }
 }
+template <typename T>
+__device__ __forceinline__ void Store8(T* p, const float (&x)[8]) {
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 8; j += N) {
+    Pack<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = FromFloat<T>(x[j + i]);
+    *reinterpret_cast<Pack<T, N>*>(p + j) = r;
+  }
+}
+
+__device__ __forceinline__ uint32_t HalfBits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 BitsHalf(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// Sixteen consecutive values of a cache row.  1024 + u as f16 is 0x6400 | u
+// for u < 1024, so codes become exact f16 integers by one subtraction (or one
+// multiply-add for a code four bits up).  An integer of 8 bits times an f16
+// scale is exact in f32, so one f16 product rounds as the f32 product rounded
+// to f16 does.
+template <KvType KIND>
+struct Codes16 {
+  static constexpr int kWords = KIND == KvType::kF16 ? 8 : (KIND == KvType::kQ8 ? 4 : 2);
+  uint32_t w[kWords];
+  __device__ __forceinline__ void Load(const char* row, int i) {
+    if (KIND == KvType::kQ4) {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + i / 2);
+      w[0] = x.x;
+      w[1] = x.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kWords / 4; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + i * (KIND == KvType::kF16 ? 2 : 1) + 16 * j);
+        w[4 * j] = x.x;
+        w[4 * j + 1] = x.y;
+        w[4 * j + 2] = x.z;
+        w[4 * j + 3] = x.w;
+      }
+    }
+  }
+  // Values 2 j, 2 j + 1 before the scale.
+  __device__ __forceinline__ __half2 Pair(int j) const {
+    if (KIND == KvType::kF16) return BitsHalf(w[j]);
+    if (KIND == KvType::kQ8) {
+      const uint32_t u = w[j >> 1] ^ 0x80808080u;
+      return __hsub2(BitsHalf(__byte_perm(u, 0x64646464u, (j & 1) ? 0x4342 : 0x4140)), BitsHalf(0x64806480u));
+    }
+    const uint32_t b = w[j >> 2] >> (8 * (j & 3));  // two codes: the low four bits, then the high four
+    return __hsub2(BitsHalf((b & 15u) | ((b & 0xF0u) << 12) | 0x64006400u), BitsHalf(0x64086408u));
+  }
+  template <typename T>
+  __device__ __forceinline__ void Store(T* out, __half d) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (KIND == KvType::kF16 && sizeof(T) == 2 && !IsBf16(out)) {
+        *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      } else if (sizeof(T) == 2 && !IsBf16(out)) {
+        uint32_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = HalfBits(__hmul2(Pair(4 * k + j), __half2half2(d)));
+        *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+      } else {
+        const float f = KIND == KvType::kF16 ? 1.f : __half2float(d);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = __half22float2(Pair(4 * k + j));
+          y[2 * j] = KIND == KvType::kF16 ? x.x : x.x * f;
+          y[2 * j + 1] = KIND == KvType::kF16 ? x.y : x.y * f;
+        }
+        Store8(out + 8 * k, y);
+      }
+    }
+  }
+  static __device__ __forceinline__ bool IsBf16(const __nv_bfloat16*) { return true; }
+  static __device__ __forceinline__ bool IsBf16(const void*) { return false; }
+};
 
 }  // namespace kvd
 }  // namespace rpgb
