@@ -127,31 +127,42 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
   const int hq = p.q_out != nullptr ? p.n_heads : 0;
   const int heads = hq + 2 * p.kv.n_kv;  // the q heads that are wanted, k heads, v heads
   const int i = threadIdx.x % L;
+  const int skip = p.n_heads - hq;
+  // the heads of a row follow one another: head x (of those wanted) is its head x, past the q heads that are not
+  const T* x0 = static_cast<const T*>(p.qkv) + t * p.qkv_stride + static_cast<int64_t>(skip) * D + 8 * i;
+  int head = blockIdx.y * kHeads + threadIdx.x / L;
+  kvd::Raw8<T> xa, xb;  // of the next head, requested one round ahead
+  if (head < heads) {
+    xa.Load(x0 + head * D);
+    xb.Load(x0 + head * D + D / 2);
+  }
   const int pos = p.pos[t];
   const int seq = p.seq != nullptr ? p.seq[t] : static_cast<int>(t);
-  const int page = pos < 0 ? -1 : kvd::PageOf(p.table, p.kv.n_pages, seq, pos >> p.kv.page_log2);
-  const bool ok = page >= 0 && (p.rope == nullptr || pos < p.rope_positions);
-  const int at = pos & ((1 << p.kv.page_log2) - 1);
-  const bool turn = p.rope != nullptr && ok;
+  const bool turn = p.rope != nullptr && pos >= 0 && pos < p.rope_positions;
   float cs[8], sn[8];
   if (turn) {
     const float* rr = p.rope + static_cast<int64_t>(pos) * D;
     kvd::Load8(rr + 8 * i, cs);
     kvd::Load8(rr + D / 2 + 8 * i, sn);
   }
+  const int page = pos < 0 ? -1 : kvd::PageOf(p.table, p.kv.n_pages, seq, pos >> p.kv.page_log2);
+  const bool ok = page >= 0 && (p.rope == nullptr || turn);
+  const int at = pos & ((1 << p.kv.page_log2) - 1);
   enum { kQ, kK, kV };
   // (every lane of a warp goes round as often: the shuffles need them all)
-  for (int head0 = blockIdx.y * kHeads; head0 < heads; head0 += gridDim.y * kHeads) {
-    const int head = head0 + threadIdx.x / L;
+  for (int head0 = blockIdx.y * kHeads; head0 < heads; head0 += gridDim.y * kHeads, head += gridDim.y * kHeads) {
     const bool live = head < heads;
     const int kind = head < hq ? kQ : (head < hq + p.kv.n_kv ? kK : kV);
     const int h = kind == kQ ? head : (kind == kK ? head - hq : head - hq - p.kv.n_kv);
-    const int col = (kind == kQ ? h : p.n_heads + (kind == kV ? p.kv.n_kv : 0) + h) * D;
     float a[8] = {}, b[8] = {};
-    if (live && ok) {
-      const T* x = static_cast<const T*>(p.qkv) + t * p.qkv_stride + col;
-      kvd::Load8(x + 8 * i, a);
-      kvd::Load8(x + D / 2 + 8 * i, b);
+    if (live) {
+      xa.Floats(a);
+      xb.Floats(b);
+      const int next = head + gridDim.y * kHeads;
+      if (next < heads) {
+        xa.Load(x0 + next * D);
+        xb.Load(x0 + next * D + D / 2);
+      }
     }
     const float* w = kind == kQ ? p.q_norm : (kind == kK ? p.k_norm : nullptr);
     const float r = InvRms<D>(a, b, p.eps);
@@ -232,6 +243,7 @@ __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
   if (out == nullptr) return;
   const char* plane = is_k ? p.kv.k : p.kv.v;
   const char* scales = is_k ? p.kv.k_scale : p.kv.v_scale;
+  const bool wide = (reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(p.out_stride * sizeof(T))) % 32 == 0;
   int64_t t[kRows];
   int pos[kRows], page[kRows];
 #pragma unroll
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
     if (t[r] >= p.n_tok) continue;
     T* row = out + t[r] * p.out_stride + static_cast<int64_t>(h) * D + i;
     if (page[r] >= 0) {
-      codes[r].Store(row, d[r]);
+      codes[r].Store(row, d[r], wide);
     } else {  // padding rows are zero, rows without a place NaN
       float x[8];
 #pragma unroll

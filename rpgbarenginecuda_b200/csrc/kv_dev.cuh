@@ -83,6 +83,32 @@ __device__ __forceinline__ void Store8(T* p, const float (&x)[8]) {
   }
 }
 
+// Eight values as they are in memory, to be converted later.
+template <typename T>
+struct Raw8 {
+  static constexpr int N = sizeof(T) / 2;
+  uint4 w[N];
+  __device__ __forceinline__ void Load(const T* p) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
+  __device__ __forceinline__ void Floats(float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const Pack<T, 8 / N> r = *reinterpret_cast<const Pack<T, 8 / N>*>(&w[j]);
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) x[j * (8 / N) + i] = ToFloat(r.v[i]);
+    }
+  }
+};
+
+// 32 bytes, a whole sector, in one store.
+__device__ __forceinline__ void Store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t HalfBits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 BitsHalf(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
@@ -121,27 +147,42 @@ struct Codes16 {
     const uint32_t b = w[j >> 2] >> (8 * (j & 3));  // two codes: the low four bits, then the high four
     return __hsub2(BitsHalf((b & 15u) | ((b & 0xF0u) << 12) | 0x64006400u), BitsHalf(0x64086408u));
   }
+  // `wide`: out is a multiple of 32 bytes.
   template <typename T>
-  __device__ __forceinline__ void Store(T* out, __half d) const {
+  __device__ __forceinline__ void Store(T* out, __half d, bool wide) const {
+    constexpr int N = 8 * sizeof(T);  // bytes of half the values
+    uint32_t y[4 * sizeof(T)];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (KIND == KvType::kF16 && sizeof(T) == 2 && !IsBf16(out)) {
-        *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-      } else if (sizeof(T) == 2 && !IsBf16(out)) {
-        uint32_t y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = HalfBits(__hmul2(Pair(4 * k + j), __half2half2(d)));
-        *reinterpret_cast<uint4*>(out + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+    for (int j = 0; j < 8; ++j) {
+      if (sizeof(T) == 2 && !IsBf16(out)) {
+        y[j] = KIND == KvType::kF16 ? HalfBits(Pair(j)) : HalfBits(__hmul2(Pair(j), __half2half2(d)));
       } else {
-        const float f = KIND == KvType::kF16 ? 1.f : __half2float(d);
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 x = __half22float2(Pair(4 * k + j));
-          y[2 * j] = KIND == KvType::kF16 ? x.x : x.x * f;
-          y[2 * j + 1] = KIND == KvType::kF16 ? x.y : x.y * f;
+        float2 x = __half22float2(Pair(j));
+        if (KIND != KvType::kF16) {
+          x.x *= __half2float(d);
+          x.y *= __half2float(d);
         }
-        Store8(out + 8 * k, y);
+        if (sizeof(T) == 2) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(x.x, x.y);
+          y[j] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          y[2 * j % (4 * sizeof(T))] = __float_as_uint(x.x);
+          y[(2 * j + 1) % (4 * sizeof(T))] = __float_as_uint(x.y);
+        }
+      }
+    }
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < 2 * N / 32; ++k) {
+        uint32_t z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = y[8 * k + j];
+        Store32(reinterpret_cast<char*>(out) + 32 * k, z);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2 * N / 16; ++k) {
+        reinterpret_cast<uint4*>(out)[k] = make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
       }
     }
   }
