@@ -38,38 +38,46 @@ __device__ __forceinline__ __half GroupScale(uint32_t max_bits) {
   return __float2half_rn(max_bits > 0x7F800000u ? m : fminf(m * (1.f / MostCode<KIND>()), 65504.f));
 }
 
-// x / d rounded to the nearest integer, ties to even, as the IEEE quotient
-// gives it: the product with 1 / d is off by less than 1e-4 for quotients to
-// 127, so only a product that close to a tie needs the division.
-__device__ __forceinline__ float RoundedQuotient(float x, float d, float inv) {
-  const float y = x * inv;
-  float c = rintf(y);
-  if (fabsf(fabsf(y - c) - 0.5f) < 1e-4f) c = rintf(x / d);
-  return c;
-}
-
-// Codes of eight consecutive values.  A scale that was rounded down (far down
-// where it is subnormal) needs the clamp.
+// Codes of eight consecutive values: the IEEE quotient x / d rounded to the
+// nearest integer, ties to even.  The product with 1 / d is off the quotient
+// by less than 1e-4 (quotients are at most 127.1), so its rounding is the same
+// unless it is that close to a tie; the low bits of 1.5 2^23 + y are y rounded.
+// A scale that was rounded far down (it is subnormal) or is the largest can
+// leave quotients past the largest code; those take the slow way too.
 template <KvType KIND>
 __device__ __forceinline__ void StoreCodes(char* row, int i, const float (&x)[8], float d) {
   constexpr float kMost = MostCode<KIND>();
-  // (a subnormal scale has an infinite reciprocal only below 2^-128: f16 scales are at least 2^-24)
-  const float inv = d > 0.f ? 1.f / d : 0.f;
-  uint32_t w[2] = {};
+  constexpr float kRound = 12582912.f;
+  constexpr float kZero = KIND == KvType::kQ8 ? 0.f : 8.f;  // the code that stands for zero
+  uint32_t c[8];
+  const float inv = 1.f / d;
+  float off = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float c = d > 0.f ? fminf(fmaxf(RoundedQuotient(x[e], d, inv), -kMost), kMost) : 0.f;
-    const int q = static_cast<int>(c);
-    if (KIND == KvType::kQ8) {
-      w[e >> 2] |= static_cast<uint32_t>(q & 255) << (8 * (e & 3));
-    } else {
-      w[0] |= static_cast<uint32_t>(q + 8) << (4 * e);
+    const float y = x[e] * inv;
+    const float z = y + (kRound + kZero);
+    off = fmaxf(off, fabsf(y - (z - (kRound + kZero))));
+    c[e] = __float_as_uint(z);
+  }
+  if (!(off < 0.4999f && d >= 6.2e-5f && d < 65504.f)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = d > 0.f ? fminf(fmaxf(rintf(x[e] / d), -kMost), kMost) : 0.f;
+      c[e] = static_cast<uint32_t>(static_cast<int>(q + kZero));
     }
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    w[k] = __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040),
+                       0x5410);
   }
   if (KIND == KvType::kQ8) {
     *reinterpret_cast<uint2*>(row + i) = make_uint2(w[0], w[1]);
   } else {
-    *reinterpret_cast<uint32_t*>(row + i / 2) = w[0];
+    w[0] &= 0x0F0F0F0Fu;
+    w[1] &= 0x0F0F0F0Fu;
+    *reinterpret_cast<uint32_t*>(row + i / 2) = __byte_perm(w[0] | w[0] >> 4, w[1] | w[1] >> 4, 0x6420);
   }
 }
 
@@ -165,7 +173,8 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
       }
     }
     const float* w = kind == kQ ? p.q_norm : (kind == kK ? p.k_norm : nullptr);
-    const float r = InvRms<D>(a, b, p.eps);
+    // (a warp has heads of one kind, or of several: the shuffles need all its lanes)
+    const float r = __any_sync(0xFFFFFFFFu, w != nullptr) ? InvRms<D>(a, b, p.eps) : 1.f;
     if (w != nullptr) {
       float wa[8], wb[8];
       kvd::Load8(w + 8 * i, wa);
@@ -185,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
       }
     }
     uint32_t ma = 0, mb = 0;
-    if (KIND != KvType::kF16) {
+    if (KIND != KvType::kF16 && __any_sync(0xFFFFFFFFu, kind != kQ)) {
       ma = MaxAbs8(a);
       mb = MaxAbs8(b);
       if (D == kKvGroup) ma = mb = max(ma, mb);
@@ -277,7 +286,7 @@ __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
     if (t[r] >= p.n_tok) continue;
     T* row = out + t[r] * p.out_stride + static_cast<int64_t>(h) * D + i;
     if (page[r] >= 0) {
-      codes[r].Store(row, d[r], wide);
+      codes[r].Store(row, d[r], wide, p.magic);
     } else {  // padding rows are zero, rows without a place NaN
       float x[8];
 #pragma unroll
@@ -359,7 +368,9 @@ void LaunchKvAppend(const KvAppendParams& p, cudaStream_t s) {
 }
 
 void LaunchKvGather(const KvGatherParams& p, cudaStream_t s) {
-  Dispatch<Gather>(p, s);
+  KvGatherParams a = p;
+  a.magic = kvd::kMagic;
+  Dispatch<Gather>(a, s);
   RPGB_CUDA(cudaGetLastError());
   CountLaunches(1);
 }

@@ -214,32 +214,13 @@ using kvd::BitsHalf;
 using kvd::HalfBits;
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return HalfBits(__floats2half2_rn(lo, hi)); }
 
-// 1024 + u as f16 is 0x6400 | u for u < 1024, so a code in the low bits of
-// 0x6400 becomes the integer it stands for by one exact subtraction (or, four
-// bits up, one exact multiply-add).
-__device__ __forceinline__ uint32_t SubHalf(uint32_t x, uint32_t bias) {
-  return HalfBits(__hsub2(BitsHalf(x), BitsHalf(bias)));
-}
-// The 0x6400 pair comes from a kernel argument: as a constant beside the mask
-// it would take a second instruction, since one may hold a single literal.
-constexpr uint32_t kMagic = 0x64006400u;
-constexpr uint32_t kBias8 = 0x64806480u;  // 1024 + 128
-constexpr uint32_t kBias4 = 0x64086408u;  // 1024 + 8
+using kvd::High4;
+using kvd::kBias8;
+using kvd::Low4;
+using kvd::SubHalf;
 // An integer sum that starts at the bits of 1.5 2^23 is that float plus the sum.
 constexpr int kIntStart = 0x4B400000;
 constexpr float kIntBias = 12582912.f;
-template <uint32_t MASK>
-__device__ __forceinline__ uint32_t MaskOr(uint32_t w, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));  // (w & MASK) | magic
-  return r;
-}
-__device__ __forceinline__ uint32_t Low4(uint32_t w, uint32_t magic) {
-  return SubHalf(MaskOr<0x000F000Fu>(w, magic), kBias4);
-}
-__device__ __forceinline__ uint32_t High4(uint32_t w, uint32_t magic) {  // (1024 + 16 u) / 16 - 72 = u - 8
-  return HalfBits(__hfma2(BitsHalf(MaskOr<0x00F000F0u>(w, magic)), BitsHalf(0x2C002C00u), BitsHalf(0xD480D480u)));
-}
 
 // ------------------------------------------------------------------ work
 
@@ -1202,7 +1183,7 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   const int64_t tiles = ((cap + 15) / C::TILE + 1 + C::BORDER) * p.kv.n_kv * chunks;
   if (tiles < grid && tiles * p.table.n_seq < grid) grid = static_cast<int>(tiles * p.table.n_seq);
   KvAttendParams a = p;
-  a.magic = kMagic;
+  a.magic = kvd::kMagic;
   a.page16 = static_cast<uint32_t>(p.kv.page_stride / 16);
   a.head16 = static_cast<uint32_t>(p.kv.head_stride / 16);
   a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);

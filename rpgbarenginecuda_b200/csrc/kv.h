@@ -72,6 +72,7 @@ struct KvGatherParams {
   int64_t n_tok = 0;
   void *k_out = nullptr, *v_out = nullptr;  // either may be null
   int64_t out_stride = 0;                   // elements
+  uint32_t magic = 0;  // a constant of the kernel, filled in by LaunchKvGather
 };
 void LaunchKvGather(const KvGatherParams& p, cudaStream_t s);
 

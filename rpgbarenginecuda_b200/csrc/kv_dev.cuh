@@ -112,11 +112,36 @@ __device__ __forceinline__ void Store32(void* p, const uint32_t (&w)[8]) {
 __device__ __forceinline__ uint32_t HalfBits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 BitsHalf(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// Sixteen consecutive values of a cache row.  1024 + u as f16 is 0x6400 | u
-// for u < 1024, so codes become exact f16 integers by one subtraction (or one
-// multiply-add for a code four bits up).  An integer of 8 bits times an f16
-// scale is exact in f32, so one f16 product rounds as the f32 product rounded
-// to f16 does.
+// 1024 + u as f16 is 0x6400 | u for u < 1024, so a code in the low bits of
+// 0x6400 becomes the integer it stands for by one exact subtraction (or, four
+// bits up, one exact multiply-add).
+__device__ __forceinline__ uint32_t SubHalf(uint32_t x, uint32_t bias) {
+  return HalfBits(__hsub2(BitsHalf(x), BitsHalf(bias)));
+}
+// The 0x6400 pair comes to the kernels as an argument: as a constant beside
+// the mask it would take a second instruction, since one may hold a single
+// literal.
+constexpr uint32_t kMagic = 0x64006400u;
+constexpr uint32_t kBias8 = 0x64806480u;  // 1024 + 128
+constexpr uint32_t kBias4 = 0x64086408u;  // 1024 + 8
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t MaskOr(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));  // (w & MASK) | magic
+  return r;
+}
+// The 4-bit codes 0 and 4 (1 and 5) of a word as integers.
+__device__ __forceinline__ uint32_t Low4(uint32_t w, uint32_t magic) {
+  return SubHalf(MaskOr<0x000F000Fu>(w, magic), kBias4);
+}
+__device__ __forceinline__ uint32_t High4(uint32_t w, uint32_t magic) {  // (1024 + 16 u) / 16 - 72 = u - 8
+  return HalfBits(
+      __hfma2(BitsHalf(MaskOr<0x00F000F0u>(w, magic)), BitsHalf(0x2C002C00u), BitsHalf(0xD480D480u)));
+}
+
+// Sixteen consecutive values of a cache row.  An integer of 8 bits times an
+// f16 scale is exact in f32, so one f16 product rounds as the f32 product
+// rounded to f16 does.
 template <KvType KIND>
 struct Codes16 {
   static constexpr int kWords = KIND == KvType::kF16 ? 8 : (KIND == KvType::kQ8 ? 4 : 2);
@@ -137,27 +162,42 @@ struct Codes16 {
       }
     }
   }
-  // Values 2 j, 2 j + 1 before the scale.
-  __device__ __forceinline__ __half2 Pair(int j) const {
-    if (KIND == KvType::kF16) return BitsHalf(w[j]);
-    if (KIND == KvType::kQ8) {
-      const uint32_t u = w[j >> 1] ^ 0x80808080u;
-      return __hsub2(BitsHalf(__byte_perm(u, 0x64646464u, (j & 1) ? 0x4342 : 0x4140)), BitsHalf(0x64806480u));
+  // The values before the scale, in pairs.
+  __device__ __forceinline__ void Pairs(uint32_t (&y)[8], uint32_t magic) const {
+    if (KIND == KvType::kF16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = w[j % kWords];
+    } else if (KIND == KvType::kQ8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = w[j % kWords] ^ 0x80808080u;
+        y[2 * j] = SubHalf(__byte_perm(u, magic, 0x5150), kBias8);
+        y[2 * j + 1] = SubHalf(__byte_perm(u, magic, 0x5352), kBias8);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t a = Low4(w[j], magic), b = High4(w[j], magic);            // codes 0, 4; 1, 5
+        const uint32_t c = Low4(w[j] >> 8, magic), d = High4(w[j] >> 8, magic);  // codes 2, 6; 3, 7
+        y[4 * j] = __byte_perm(a, b, 0x5410);
+        y[4 * j + 1] = __byte_perm(c, d, 0x5410);
+        y[4 * j + 2] = __byte_perm(a, b, 0x7632);
+        y[4 * j + 3] = __byte_perm(c, d, 0x7632);
+      }
     }
-    const uint32_t b = w[j >> 2] >> (8 * (j & 3));  // two codes: the low four bits, then the high four
-    return __hsub2(BitsHalf((b & 15u) | ((b & 0xF0u) << 12) | 0x64006400u), BitsHalf(0x64086408u));
   }
   // `wide`: out is a multiple of 32 bytes.
   template <typename T>
-  __device__ __forceinline__ void Store(T* out, __half d, bool wide) const {
+  __device__ __forceinline__ void Store(T* out, __half d, bool wide, uint32_t magic) const {
     constexpr int N = 8 * sizeof(T);  // bytes of half the values
-    uint32_t y[4 * sizeof(T)];
+    uint32_t y[4 * sizeof(T)], h[8];
+    Pairs(h, magic);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (sizeof(T) == 2 && !IsBf16(out)) {
-        y[j] = KIND == KvType::kF16 ? HalfBits(Pair(j)) : HalfBits(__hmul2(Pair(j), __half2half2(d)));
+        y[j] = KIND == KvType::kF16 ? h[j] : HalfBits(__hmul2(BitsHalf(h[j]), __half2half2(d)));
       } else {
-        float2 x = __half22float2(Pair(j));
+        float2 x = __half22float2(BitsHalf(h[j]));
         if (KIND != KvType::kF16) {
           x.x *= __half2float(d);
           x.y *= __half2float(d);
