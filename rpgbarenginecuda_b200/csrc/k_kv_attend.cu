@@ -267,7 +267,7 @@ template <typename C>
 struct Filler {
   static constexpr int kSteps = 32 / C::MT;
   static constexpr uint32_t kStep = (1u << C::MT) - 1;  // the halves of a step
-  Cursor<C> at;        // the first step after the batch
+  Cursor<C>* at;       // the first step after the batch; in shared memory, to leave the registers to the math
   int left;            // steps not yet put in a batch
   int count = 0;       // steps of the batch not yet issued
   uint32_t have = 0;   // bit per half of the batch, the next step's lowest: it has rows in range and a page
@@ -276,35 +276,39 @@ struct Filler {
   uint32_t place;      // shared-memory address of the next step's first code offset
   uint32_t places;
 
-  __device__ __forceinline__ int Pos(int warp, int lane) const {
-    return at.span.base + (at.tile + lane / C::MT) * C::TILE + warp * C::R + (lane % C::MT) * 16;
+  static __device__ __forceinline__ int Pos(const Cursor<C>& c, int warp, int lane) {
+    return c.span.base + (c.tile + lane / C::MT) * C::TILE + warp * C::R + (lane % C::MT) * 16;
   }
-  __device__ __forceinline__ bool InRange(int pos, int lane) const {
-    return lane / C::MT < min(left, at.span.tiles - at.tile) && pos + 16 > at.span.start && pos < at.span.len;
+  __device__ __forceinline__ bool InRange(const Cursor<C>& c, int pos, int lane) const {
+    return lane / C::MT < min(left, c.span.tiles - c.tile) && pos + 16 > c.span.start && pos < c.span.len;
   }
-  __device__ __forceinline__ void Request(const KvAttendParams& p, int warp, int lane) {
-    const int pos = Pos(warp, lane);
+  __device__ __forceinline__ void Request(const KvAttendParams& p, const Cursor<C>& c, int warp, int lane) {
+    const int pos = Pos(c, warp, lane);
     // (positions in range lie inside the table: SpanOf)
-    if (left > 0 && InRange(pos, lane)) {
-      page = __ldg(p.table.pages + at.seq * p.table.stride + (pos >> p.kv.page_log2));
+    if (left > 0 && InRange(c, pos, lane)) {
+      page = __ldg(p.table.pages + c.seq * p.table.stride + (pos >> p.kv.page_log2));
     }
   }
   __device__ __forceinline__ void Batch(const KvAttendParams& p, int warp, int lane, int chunks) {
-    const int pos = Pos(warp, lane);
-    const bool in = InRange(pos, lane);
+    __syncwarp();  // the last batch has been read
+    Cursor<C> c = *at;
+    const int pos = Pos(c, warp, lane);
+    const bool in = InRange(c, pos, lane);
     const bool ok = in && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
     const uint32_t row = pos & ((1 << p.kv.page_log2) - 1);
-    __syncwarp();  // the last batch has been read
-    const uint64_t id = static_cast<uint32_t>(page), head = static_cast<uint32_t>(at.head);
+    const uint64_t id = static_cast<uint32_t>(page), head = static_cast<uint32_t>(c.head);
     Sts64(places + lane * 8, (id * p.page16 + head * p.head16 + static_cast<uint64_t>(row) * p.pos16) << 4);
     if (C::QUANT) Sts64(places + 256 + lane * 8, ((id * p.spage16 + head * p.shead16) << 4) + row * (2 * C::NG));
     have = __ballot_sync(0xFFFFFFFFu, ok);
     bad = __ballot_sync(0xFFFFFFFFu, in && !ok);
-    count = min(kSteps, min(left, at.span.tiles - at.tile));
-    left -= count + (at.tile + count == at.span.tiles ? C::BORDER : 0);
+    count = min(kSteps, min(left, c.span.tiles - c.tile));
+    left -= count + (c.tile + count == c.span.tiles ? C::BORDER : 0);
     place = places;
-    if (left > 0) at.Next(p, chunks, count);
-    Request(p, warp, lane);
+    if (left > 0) {
+      c.Next(p, chunks, count);
+      Request(p, c, warp, lane);
+      if (lane == 0) *at = c;
+    }
     __syncwarp();
   }
 
@@ -581,8 +585,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   constexpr int D = C::D;
   extern __shared__ __align__(128) char smem[];
   __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-  __shared__ long long s_sum[kWarps], s_begin;
+  __shared__ long long s_sum[kWarps], s_begin, s_item0[kWarps];
   __shared__ int s_seq, s_last;
+  __shared__ Cursor<C> s_use[kWarps], s_fill[kWarps];
   __shared__ __align__(8) float s_bias[C::NG][3][8];
   __shared__ __align__(16) Places s_places[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -657,12 +662,18 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   float* mineq = comb + warp * (C::COMB / 4);
   const uint32_t q_smem = dev::SmemAddr(smem) + kWarps * C::RING + C::JOIN;
   const uint32_t k_lane = KLaneOffset<C>(lane), v_lane = VLaneOffset<C>(lane);
+  // What changes with the item only is kept per warp in shared memory.
+  if (lane == 0) {
+    s_use[warp] = s_fill[warp] = use;
+    s_item0[warp] = item0;
+  }
+  __syncwarp();
   Filler<C> fill;
-  fill.at = use;
+  fill.at = &s_fill[warp];
   fill.left = left;
   fill.places = fill.place = dev::SmemAddr(&s_places[warp]);
   const int64_t lane_off = static_cast<int64_t>(lane / C::CPR) * p.kv.pos_stride + (lane % C::CPR) * 16;
-  fill.Request(p, warp, lane);
+  fill.Request(p, use, warp, lane);
 
   const uint32_t kslot = ring, vslot = ring + C::KSLOT;
   uint32_t bad_now = 0;  // the step's halves that have rows in range but no page
@@ -670,14 +681,16 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   const bool two_terms = p.type == ElemType::kF32;
   for (bool begin = true;; begin = false) {
     // ---- an item: its queries, as B fragments
-    const int queries = min(per_chunk, group - use.chunk * per_chunk);
-    const int64_t col = (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
-    const int seg = use.tile;
+    int n, lo, hi;  // tiles of the item that are this block's; the range, from this warp's first row
     float x[D / 4] = {};
     {
+      const Cursor<C> c = s_use[warp];
+      n = min(left, c.span.tiles - c.tile);
+      lo = c.span.start - (c.span.base + c.tile * C::TILE + warp * C::R);
+      hi = c.span.len - (c.span.base + c.tile * C::TILE + warp * C::R);
       const int qi = C::PACK ? g & 3 : g;
-      if (qi < queries) {
-        const int64_t o = use.seq * p.q_stride + col + qi * D;
+      if (qi < min(per_chunk, group - c.chunk * per_chunk)) {
+        const int64_t o = c.seq * p.q_stride + (static_cast<int64_t>(c.head) * group + c.chunk * per_chunk + qi) * D;
         switch (p.type) {
           case ElemType::kF32: ReadQ<C>(x, static_cast<const float*>(p.q) + o, t); break;
           case ElemType::kF16: ReadQ<C>(x, static_cast<const __half*>(p.q) + o, t); break;
@@ -723,9 +736,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     __syncthreads();
 
     // ---- its tiles
-    for (;;) {
-    const int pos = use.span.base + use.tile * C::TILE + warp * C::R;
-    const int lo = use.span.start - pos, hi = use.span.len - pos;
+    left -= n + C::BORDER;  // (past the end where the share ends inside the item: what counts is whether any is left)
+#pragma unroll 1
+    for (int i = n; i > 0; --i, lo -= C::TILE, hi -= C::TILE) {
     const bool work = lo < C::R && hi > 0;
     const bool edge = lo > 0 || hi < C::R || bad_now != 0;
 
@@ -963,9 +976,6 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     __syncwarp();
     fill.template Issue<true>(p, vslot, lane, lane_off);
     bad_now = fill.Pop();
-    --left;
-    if (left <= 0 || use.tile + 1 == use.span.tiles) break;
-    ++use.tile;
     }
 
     // ---- the end of the item, or of this block's share of it
@@ -993,8 +1003,11 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         }
       }
       __syncthreads();
-      const bool whole = seg == 0 && use.tile + 1 == use.span.tiles;
-      const int64_t out = use.seq * p.out_stride + col;
+      const Cursor<C> use = s_use[warp];
+      const long long item0 = s_item0[warp];
+      const bool whole = use.tile == 0 && n == use.span.tiles;
+      const int queries = min(per_chunk, group - use.chunk * per_chunk);
+      const int64_t out = use.seq * p.out_stride + (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
       const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
       // The warps' shares joined: values 4 i .. 4 i + 3 of the item's queries.
@@ -1151,12 +1164,18 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           put(i, v, sum);
         }
       }
+      if (left > 0) {
+        Cursor<C> c = use;
+        c.Next(p, chunks, n);
+        __syncwarp();
+        if (lane == 0) {
+          s_use[warp] = c;
+          s_item0[warp] = item0 + use.span.tiles + C::BORDER;
+        }
+      }
       __syncthreads();  // the next item writes the join area again
     }
-    left -= C::BORDER;  // (a share that ends inside the item ends all the same)
     if (left <= 0) break;
-    item0 += use.span.tiles + C::BORDER;
-    use.Next(p, chunks);
   }
   CopyWait<0>();
 }
