@@ -64,6 +64,7 @@ struct Cfg {
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;  // 16-byte chunks of a row
+  static constexpr int LEAST = 2;
   static constexpr int BORDER = QUANT ? 1 : 2;  // the end of an item costs a block about as much as so many tiles
   static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
   static constexpr int KSLOT = R * ROW + 2 * SC;     // K codes, K scales, V scales
@@ -204,6 +205,13 @@ __device__ __forceinline__ void Sts64(uint32_t a, uint64_t x) {
 }
 __device__ __forceinline__ void Sts128Zero(uint32_t a) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
+}
+// An atomic that releases what the block wrote (after a barrier) and acquires
+// what the blocks before it released.
+__device__ __forceinline__ unsigned AddAcqRel(unsigned* p, unsigned v) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
 }
 __device__ __forceinline__ float Exp2(float x) {
   float y;
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     if (w == warp) upto += total;
     total += s_sum[w];
   }
-  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + C::LEAST - 1) / C::LEAST));
   if (static_cast<int>(blockIdx.x) >= blocks) return;
   const long long first = ShareBegin(total, blockIdx.x, blocks);
   int left = static_cast<int>(ShareBegin(total, blockIdx.x + 1, blocks) - first);  // tiles to do
@@ -1058,11 +1066,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           }
         }
         __syncthreads();
-        if (tid == 0) {
-          __threadfence();  // the whole block's record, after the barrier
-          s_last = atomicAdd(count, 1u) == static_cast<unsigned>(b1 - b0);
-          __threadfence();
-        }
+        if (tid == 0) s_last = AddAcqRel(count, 1u) == static_cast<unsigned>(b1 - b0);
         __syncthreads();
         finish = s_last != 0;
         if (finish && tid == 0) *count = 0;
@@ -1108,13 +1112,21 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           float* factor = comb;  // [query][record]
           for (int q = warp; q < queries; q += kWarps) {
             float top = -INFINITY, sum = 0.f;
-            for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, __ldcg(record(b) + kKvMaxQueries * D + q));
-            top = dev::WarpMax(top);
-            for (int b = b0 + lane; b <= b1; b += 32) {
+            for (int b = b0 + lane; b <= b1; b += 64) {  // (a second record per lane at once)
               const float* r = record(b) + kKvMaxQueries * D + q;
-              const float f = Exp2(__ldcg(r) - (top == -INFINITY ? 0.f : top));
-              factor[q * kKvMaxBlocks + b - b0] = f;
-              sum += f * __ldcg(r + kKvMaxQueries);
+              const float* r2 = record(min(b + 32, b1)) + kKvMaxQueries * D + q;
+              const float ma = __ldcg(r), mb = __ldcg(r2), la = __ldcg(r + kKvMaxQueries), lb = __ldcg(r2 + kKvMaxQueries);
+              const float now = fmaxf(top, fmaxf(ma, mb)), ref = now == -INFINITY ? 0.f : now;
+              sum = sum * Exp2(top - ref) + Exp2(ma - ref) * la + (b + 32 <= b1 ? Exp2(mb - ref) * lb : 0.f);
+              top = now;
+              factor[q * kKvMaxBlocks + b - b0] = ma;
+              if (b + 32 <= b1) factor[q * kKvMaxBlocks + b + 32 - b0] = mb;
+            }
+            const float all = dev::WarpMax(top), ref = all == -INFINITY ? 0.f : all;
+            sum *= Exp2(top - ref);
+            top = all;
+            for (int b = lane; b <= b1 - b0; b += 32) {  // (the lane's own: b and b + 32 keep their lane)
+              factor[q * kKvMaxBlocks + b] = Exp2(factor[q * kKvMaxBlocks + b] - ref);
             }
             sum = dev::WarpSum(sum);
             if (lane < kWarps) {
