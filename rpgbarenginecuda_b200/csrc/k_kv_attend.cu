@@ -220,6 +220,11 @@ __device__ __forceinline__ float Exp2(float x) {
 }
 using kvd::BitsHalf;
 using kvd::HalfBits;
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 Both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return HalfBits(__floats2half2_rn(lo, hi)); }
 
 using kvd::High4;
@@ -712,10 +717,10 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
       fill.template Issue<true>(p, vslot, lane, lane_off);
       bad_now = fill.Pop();
     }
-    float cs[2];            // from products to scores in log2 units
-    float m[2], ref[2];     // of columns 2 t, 2 t + 1: largest score; weights are 2^(score - ref)
-    float l[2];             // sum of this lane's weights
-    float acc[D / 16][4];
+    // of columns 2 t, 2 t + 1: from products to scores in log2 units; largest
+    // score; weights are 2^(score - ref); sum of this lane's weights
+    float2 cs, m = Both(-INFINITY), ref = m, l = Both(0.f);
+    float2 acc[D / 16][2];  // rows g and g + 8 of a tile
     int nu = 127 - 25;      // biased exponent of the power of two over the V scales seen
     {
       float bias[C::NG][C::QTILES];
@@ -727,19 +732,12 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           for (int n = 0; n < C::QTILES; ++n) s_bias[gp][n][g] = bias[gp][n];
         }
       }
+      cs.x = __shfl_sync(0xFFFFFFFFu, up, 4 * (C::PACK ? (2 * t) & 3 : 2 * t));
+      cs.y = __shfl_sync(0xFFFFFFFFu, up, 4 * (C::PACK ? (2 * t + 1) & 3 : 2 * t + 1));
+      // (lanes that join the digits from the lower one have 256 times the product)
+      if (C::QUANT && C::PACK && t >= 2) cs = Mul2(cs, Both(1.f / 256));
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        cs[c] = __shfl_sync(0xFFFFFFFFu, up, 4 * (C::PACK ? (2 * t + c) & 3 : 2 * t + c));
-        // (lanes that join the digits from the lower one have 256 times the product)
-        if (C::QUANT && C::PACK && t >= 2) cs[c] *= 1.f / 256;
-        m[c] = ref[c] = -INFINITY;
-        l[c] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
-      }
+      for (int i = 0; i < D / 16; ++i) acc[i][0] = acc[i][1] = Both(0.f);
     }
     __syncthreads();
 
@@ -753,12 +751,13 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     // ---- scores (and the V scales)
     CopyWait<1>();
     __syncwarp();
-    float s[C::MT][4];
+    float2 s[C::MT][2];  // rows g and g + 8 of a tile, columns 2 t and 2 t + 1
     uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
     if (work) {
       const uint32_t kbase = kslot + k_lane, sbase = kslot + C::R * C::ROW + g * (2 * C::NG);
       const uint32_t qbase = q_smem + lane * 16;
       if (!C::QUANT) {
+        float sum[C::MT][4];
 #pragma unroll
         for (int k4 = 0; k4 < C::QWORDS / 4; ++k4) {
           const uint4 q = Lds128(qbase + k4 * 512);
@@ -771,10 +770,15 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
             for (int mt = 0; mt < C::MT; ++mt) {
               uint32_t a[4];
               LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
-              ks == 0 ? MmaFirst(s[mt], a, q.x, q.y) : Mma(s[mt], a, j == 0 ? q.x : q.z, j == 0 ? q.y : q.w);
-              if (!C::PACK && two_terms) Mma(s[mt], a, j == 0 ? r.x : r.z, j == 0 ? r.y : r.w);
+              ks == 0 ? MmaFirst(sum[mt], a, q.x, q.y) : Mma(sum[mt], a, j == 0 ? q.x : q.z, j == 0 ? q.y : q.w);
+              if (!C::PACK && two_terms) Mma(sum[mt], a, j == 0 ? r.x : r.z, j == 0 ? r.y : r.w);
             }
           }
+        }
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+          s[mt][0] = make_float2(sum[mt][0], sum[mt][1]);
+          s[mt][1] = make_float2(sum[mt][2], sum[mt][3]);
         }
       } else {
         constexpr bool kU = C::KIND == KvType::kQ4;
@@ -804,27 +808,27 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           for (int mt = 0; mt < C::MT; ++mt) {
             uint32_t a[2][4];
             KFragments<C>(a, kbase, mt, gp);
-            auto product = [&](const uint4& q, const float2& b, float (&v)[4]) {
+            auto product = [&](const uint4& q, const float2& b, float2 (&v)[2]) {
               int n[4];
               MmaIntFirst<kU>(n, a[0], q.x, q.y, kIntStart);
               MmaInt<kU>(n, a[1], q.z, q.w);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) v[c] = __int_as_float(n[c]) - ((c & 1) ? b.y : b.x);
+              const float2 less = make_float2(-b.x, -b.y);
+              v[0] = Add2(make_float2(__int_as_float(n[0]), __int_as_float(n[1])), less);
+              v[1] = Add2(make_float2(__int_as_float(n[2]), __int_as_float(n[3])), less);
             };
-            float v[4], r[4];
+            float2 v[2], r[2];
             product(q0, b0, v);
             product(q1, b1, r);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = fmaf(r[c], C::PACK ? 1.f / 65536 : 1.f / 256, v[c]);
+            for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(C::PACK ? 1.f / 65536 : 1.f / 256), v[i]);
             if (!C::PACK) {
               product(q2, b2, r);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) v[c] = fmaf(r[c], 1.f / 65536, v[c]);
+              for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(1.f / 65536), v[i]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float f = gp == 0 ? d[mt][c >> 1].x : d[mt][c >> 1].y;
-              s[mt][c] = gp == 0 ? v[c] * f : fmaf(v[c], f, s[mt][c]);
+            for (int i = 0; i < 2; ++i) {
+              s[mt][i] = gp == 0 ? Mul2(v[i], Both(d[mt][i].x)) : Fma2(v[i], Both(d[mt][i].y), s[mt][i]);
             }
           }
         }
@@ -832,13 +836,19 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
       for (int mt = 0; mt < C::MT; ++mt) {
         if (C::PACK && C::QUANT) {  // lanes t < 2 hold the first digit, the others the second
-          const float f = t < 2 ? 1.f / 256 : 256.f;
+          const float2 f = Both(t < 2 ? 1.f / 256 : 256.f);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[mt][c] = fmaf(__shfl_xor_sync(0xFFFFFFFFu, s[mt][c], 2), f, s[mt][c]);
+          for (int i = 0; i < 2; ++i) {
+            s[mt][i] = Fma2(make_float2(__shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2), __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2)),
+                            f, s[mt][i]);
+          }
         }
         if (C::PACK && !C::QUANT && two_terms) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[mt][c] += __shfl_xor_sync(0xFFFFFFFFu, s[mt][c], 2);
+          for (int i = 0; i < 2; ++i) {
+            s[mt][i].x += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2);
+            s[mt][i].y += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2);
+          }
         }
       }
     }
@@ -857,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     // ---- weights: 2^(score - ref) with ref a power of two over the largest,
     // so that a weight times its V scale is at most 2^14 and small ones stay
     // normal f16 numbers
-    float alpha[2] = {1.f, 1.f};
+    float2 alpha = Both(1.f);
     if (work) {
       if (edge) {
         asm volatile("" ::: "memory");  // a branch, not predicates: few steps come here
@@ -866,9 +876,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = 16 * mt + 8 * i + g;
-            if ((bad_now >> mt) & 1) s[mt][2 * i] = s[mt][2 * i + 1] = kvd::Nan();
+            if ((bad_now >> mt) & 1) s[mt][i] = Both(kvd::Nan());
             if (r < lo || r >= hi) {
-              s[mt][2 * i] = s[mt][2 * i + 1] = -INFINITY;
+              s[mt][i] = Both(-INFINITY);
               vsc[mt][i] = 0;  // a scale out of range may be anything
             }
           }
@@ -887,27 +897,32 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         nu = max(nu, min(static_cast<int>(__float_as_uint(d) >> 23), 127 + 16) + 1);
       }
       const float shift = C::QUANT ? static_cast<float>(nu - 127 - kWeightBits) : -static_cast<float>(kWeightBits);
+      float2 top = s[0][0], now;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float top = fmaxf(s[0][c], s[0][2 + c]);
+      for (int j = 1; j < 2 * C::MT; ++j) {
+        top.x = fmaxf(top.x, s[j >> 1][j & 1].x);
+        top.y = fmaxf(top.y, s[j >> 1][j & 1].y);
+      }
 #pragma unroll
-        for (int mt = 1; mt < C::MT; ++mt) top = fmaxf(top, fmaxf(s[mt][c], s[mt][2 + c]));
+      for (int o = 4; o < 32; o <<= 1) {
+        top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, o));
+        top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, o));
+      }
+      m.x = fmaxf(m.x, top.x * cs.x);
+      m.y = fmaxf(m.y, top.y * cs.y);
+      now.x = (m.x == -INFINITY ? 0.f : m.x) + shift;
+      now.y = (m.y == -INFINITY ? 0.f : m.y) + shift;
+      alpha = make_float2(Exp2(ref.x - now.x), Exp2(ref.y - now.y));
+      ref.x = m.x == -INFINITY ? -INFINITY : now.x;
+      ref.y = m.y == -INFINITY ? -INFINITY : now.y;
+      l = Mul2(l, alpha);
+      const float2 less = make_float2(-now.x, -now.y);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        m[c] = fmaxf(m[c], top * cs[c]);
-        const float now = (m[c] == -INFINITY ? 0.f : m[c]) + shift;
-        alpha[c] = Exp2(ref[c] - now);
-        ref[c] = m[c] == -INFINITY ? -INFINITY : now;
-        l[c] *= alpha[c];
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float w = Exp2(fmaf(s[mt][2 * i + c], cs[c], -now));
-            s[mt][2 * i + c] = w;
-            l[c] += w;
-          }
-        }
+      for (int j = 0; j < 2 * C::MT; ++j) {
+        const float2 e = Fma2(s[j >> 1][j & 1], cs, less);
+        const float2 w = make_float2(Exp2(e.x), Exp2(e.y));
+        s[j >> 1][j & 1] = w;
+        l = Add2(l, w);
       }
     }
 
@@ -922,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         __syncwarp();
       }
       const uint32_t vbase = vslot + v_lane;
-      const float of_rest = t >= 2 ? 1.f : 0.f, of_lead = t >= 2 ? -1.f : 1.f;  // which term this lane's columns take
+      const float2 of_rest = Both(t >= 2 ? 1.f : 0.f), of_lead = Both(t >= 2 ? -1.f : 1.f);  // the lane's columns' term
 #pragma unroll
       for (int gp = 0; gp < C::NG; ++gp) {
         uint32_t b[C::MT][2][C::PACK ? 1 : 2];
@@ -930,20 +945,20 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float u = s[mt][2 * i], v = s[mt][2 * i + 1];
+            float2 u = s[mt][i];
             if (C::QUANT) {
               const float2 d = __half22float2(BitsHalf(vsc[mt][i]));
-              u *= gp == 0 ? d.x : d.y;
-              v *= gp == 0 ? d.x : d.y;
+              u = Mul2(u, Both(gp == 0 ? d.x : d.y));
             }
             // the first term is the leading 11 bits, the second the rest
-            const float uh = __uint_as_float(__float_as_uint(u) & 0xFFFFE000u);
-            const float vh = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
+            const float2 h = make_float2(__uint_as_float(__float_as_uint(u.x) & 0xFFFFE000u),
+                                         __uint_as_float(__float_as_uint(u.y) & 0xFFFFE000u));
             if (C::PACK) {
-              b[mt][i][0] = Transposed(PackHalf(fmaf(u, of_rest, uh * of_lead), fmaf(v, of_rest, vh * of_lead)));
+              const float2 w = Fma2(u, of_rest, Mul2(h, of_lead));
+              b[mt][i][0] = Transposed(PackHalf(w.x, w.y));
             } else {
-              b[mt][i][0] = Transposed(PackHalf(uh, vh));
-              b[mt][i][C::PACK ? 0 : 1] = Transposed(PackHalf(u - uh, v - vh));
+              b[mt][i][0] = Transposed(PackHalf(h.x, h.y));
+              b[mt][i][C::PACK ? 0 : 1] = Transposed(PackHalf(u.x - h.x, u.y - h.y));
             }
           }
         }
@@ -962,7 +977,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[4 * gp + i][c] = fmaf(acc[4 * gp + i][c], alpha[c & 1], part[i][c]);
+            for (int c = 0; c < 2; ++c) {
+              acc[4 * gp + i][c] = Fma2(acc[4 * gp + i][c], alpha, make_float2(part[i][2 * c], part[i][2 * c + 1]));
+            }
           }
         } else {
 #pragma unroll
@@ -976,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
               if (!C::PACK) Mma(part, a, b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][c] = fmaf(acc[i][c], alpha[c & 1], part[c]);
+            for (int c = 0; c < 2; ++c) acc[i][c] = Fma2(acc[i][c], alpha, make_float2(part[2 * c], part[2 * c + 1]));
           }
         }
       }
@@ -989,26 +1006,31 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
     // ---- the end of the item, or of this block's share of it
     {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], o);
+      for (int o = 4; o < 32; o <<= 1) {
+        l.x += __shfl_xor_sync(0xFFFFFFFFu, l.x, o);
+        l.y += __shfl_xor_sync(0xFFFFFFFFu, l.y, o);
       }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v = acc[i][c];
-          if (C::PACK) v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-          const int value = C::QUANT ? 64 * (i >> 2) + 8 * g + 4 * (c >> 1) + (i & 3) : 16 * i + 8 * (c >> 1) + g;
-          if (!C::PACK || t < 2) mineq[(2 * t + (c & 1)) * D + value] = v;
+        for (int c = 0; c < 2; ++c) {
+          float2 v = acc[i][c];
+          if (C::PACK) {  // the two terms
+            v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, 2);
+            v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, 2);
+          }
+          const int value = C::QUANT ? 64 * (i >> 2) + 8 * g + 4 * c + (i & 3) : 16 * i + 8 * c + g;
+          if (!C::PACK || t < 2) {
+            mineq[2 * t * D + value] = v.x;
+            mineq[(2 * t + 1) * D + value] = v.y;
+          }
         }
       }
       if (g == 0 && (!C::PACK || t < 2)) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          s_m[warp][2 * t + c] = ref[c];
-          s_l[warp][2 * t + c] = l[c];
-        }
+        s_m[warp][2 * t] = ref.x;
+        s_m[warp][2 * t + 1] = ref.y;
+        s_l[warp][2 * t] = l.x;
+        s_l[warp][2 * t + 1] = l.y;
       }
       __syncthreads();
       const Cursor<C> use = s_use[warp];
