@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
 // block's threads cover (values of a head) x (k heads, then v heads) x (rows),
 // and each takes kRows rows of every blockDim.z at once, so that their chains
 // of loads (position, page, codes) run side by side.
-constexpr int kRows = 4;
+constexpr int kRows = 2;
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
   dev::GridLaunchDependents();
