@@ -242,7 +242,8 @@ typedef struct rpgb_kv_pages {
   int64_t scale_page_stride, scale_head_stride;
 } rpgb_kv_pages;
 
-/* Page table of n_seq conversations (int32 [n_seq][stride], max_pages used). */
+/* Page table of n_seq conversations (int32 [n_seq][stride], max_pages used,
+ * at most 2^30 positions). */
 typedef struct rpgb_kv_table {
   const int32_t* pages;
   int64_t stride;

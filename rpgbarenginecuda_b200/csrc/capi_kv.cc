@@ -63,12 +63,14 @@ KvPages Pages(const rpgb_kv_pages* d) {
   return p;
 }
 
-KvTable Table(const rpgb_kv_table* d) {
+KvTable Table(const rpgb_kv_table* d, int page_log2) {
   RPGB_CHECK(d != nullptr, "kv: table is NULL");
   RPGB_CHECK(d->n_seq >= 0 && d->n_seq <= (1 << 20), "kv: bad conversation count %d", d->n_seq);
   RPGB_CHECK(d->max_pages > 0 && d->stride >= d->max_pages, "kv: bad page table (%d pages, stride %lld)", d->max_pages,
              static_cast<long long>(d->stride));
   RPGB_CHECK(d->pages != nullptr || d->n_seq == 0, "kv: page table is NULL");
+  RPGB_CHECK(d->max_pages <= (1 << 30) >> page_log2, "kv: %d pages of %d positions; at most 2^30 positions are taken",
+             d->max_pages, 1 << page_log2);
   CheckAligned(d->pages, 4, "kv: page table");
   KvTable t;
   t.pages = d->pages;
@@ -121,7 +123,7 @@ int32_t rpgb_kv_append(const rpgb_kv_pages* kv, const rpgb_kv_table* table, cons
     SetLastError("");
     KvAppendParams p;
     p.kv = Pages(kv);
-    p.table = Table(table);
+    p.table = Table(table, p.kv.page_log2);
     p.type = Type(type);
     CheckTokens(pos_dev, n_tok, seq_dev, p.table);
     RPGB_CHECK(n_heads >= 0 && n_heads <= 65535, "kv: bad head count %d", n_heads);
@@ -164,7 +166,7 @@ int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
     SetLastError("");
     KvGatherParams p;
     p.kv = Pages(kv);
-    p.table = Table(table);
+    p.table = Table(table, p.kv.page_log2);
     p.type = Type(type);
     CheckTokens(pos_dev, n_tok, seq_dev, p.table);
     if (n_tok == 0) return 0;
@@ -203,7 +205,7 @@ int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
     SetLastError("");
     KvAttendParams p;
     p.kv = Pages(kv);
-    p.table = Table(table);
+    p.table = Table(table, p.kv.page_log2);
     p.type = Type(type);
     RPGB_CHECK(n_heads > 0 && n_heads <= 65535 && n_heads % p.kv.n_kv == 0, "kv: %d q heads over %d KV heads", n_heads,
                p.kv.n_kv);

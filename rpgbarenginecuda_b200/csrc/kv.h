@@ -39,7 +39,7 @@ inline int64_t KvRowBytes(KvType t, int head_dim) {
 inline int64_t KvScaleRowBytes(int head_dim) { return 2 * (head_dim / kKvGroup); }
 
 struct KvTable {
-  const int32_t* pages = nullptr;  // [n_seq][stride]: pool page of each kKvPage run of positions
+  const int32_t* pages = nullptr;  // [n_seq][stride]: pool page of each page-sized run of positions
   int32_t n_seq = 0, max_pages = 0;
   int64_t stride = 0;  // entries between conversations
 };

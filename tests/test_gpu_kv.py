@@ -117,7 +117,7 @@ def attend(pool, q, lens=None, starts=None, scale=None, act="f32", stream=0, ws=
     if out is None:
         out = torch.full((rows, width), 7.0, dtype=dt, device="cuda")
     torch.cuda.synchronize()
-    pool.kv.attend(pool.pt, code, q.data_ptr(), n_heads, lens.data_ptr(), scale or pool.dim ** -0.5, out.data_ptr(),
+    pool.kv.attend(pool.pt, code, q.data_ptr(), n_heads, lens.data_ptr(), pool.dim ** -0.5 if scale is None else scale, out.data_ptr(),
                    ws.data_ptr(), ws.numel(), starts_ptr=st.data_ptr() if st is not None else 0, stream=stream,
                    q_stride=q.stride(0), out_stride=out.stride(0))
     torch.cuda.synchronize()
@@ -135,7 +135,7 @@ def expected(pool, q, lens=None, starts=None, scale=None):
             continue
         qi = q[i].view(pool.n_kv, -1, pool.dim)
         k, v = pool.value["k"][i][:, s0:n], pool.value["v"][i][:, s0:n]
-        w = torch.softmax(qi @ k.transpose(1, 2) * (scale or pool.dim ** -0.5), -1)
+        w = torch.softmax(qi @ k.transpose(1, 2) * (pool.dim ** -0.5 if scale is None else scale), -1)
         out[i] = (w @ v).reshape(-1)
     return out
 
@@ -252,6 +252,46 @@ def test_attend_extreme_scores():
     # scores of rows 0 and 1 are 1000 and 300 times the others', and so is their error
     for i, f in enumerate((1000.0, 300.0, 1.0, 1.0)):
         assert float((got[i].double().cpu() - want[i]).abs().max()) <= 4e-5 * f * top
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("heads", [4, 14])
+def test_attend_softmax_scales(kind, heads):
+    """Zero (the mean of the values), negative, and a hundredth of the usual one."""
+    lens = [0, 1, 90, 200]
+    pool = Pool(kind, lens, 16, seed=8)
+    q = queries(4, heads, 128, "f32")
+    for scale in (0.0, -(128 ** -0.5), 1e-2 * 128 ** -0.5):
+        check(attend(pool, q, scale=scale), expected(pool, q, scale=scale), pool, "f32")
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+def test_attend_many_queries_to_one_head(kind):
+    """37 query heads over one KV head: five passes of at most eight."""
+    pool = Pool(kind, [333, 20], 16, n_kv=1, seed=8)
+    q = queries(2, 37, 128, "f16")
+    check(attend(pool, q, act="f16"), expected(pool, q), pool, "f16")
+
+
+def test_attend_very_many_conversations():
+    """70000 conversations of 64 heads, most of them empty: more than 2^22 shares of work."""
+    n, heads = 70000, 64
+    lens = [0] * n
+    for i in range(0, n, 7001):
+        lens[i] = 1 + i % 40
+    pool = Pool("f16", lens, 16, n_kv=heads, dim=64, seed=3)
+    q = torch.zeros(n, heads * 64, dtype=torch.float16, device="cuda")
+    some = [i for i in range(n) if lens[i]]
+    q[some] = queries(len(some), heads, 64, "f16")
+    got = attend(pool, q, act="f16")
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[some] = False
+    assert int((got[rest] != 0).sum()) == 0
+    few = Pool.__new__(Pool)
+    few.__dict__.update(pool.__dict__)
+    few.value = {k: [pool.value[k][i] for i in some] for k in pool.value}
+    few.lens = [lens[i] for i in some]
+    check(got[some], expected(few, q[some]), few, "f16")
 
 
 @pytest.mark.parametrize("kind", ["q8", "q4"])

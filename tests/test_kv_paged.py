@@ -55,7 +55,7 @@ def test_bad_caches_are_refused(call, bad, why):
 @pytest.mark.parametrize("call", [attend, append, gather])
 def test_bad_tables_and_types_are_refused(call):
     for t in (rpg.PageTable(0, 2, 4), rpg.PageTable(FAKE + 2, 2, 4), rpg.PageTable(FAKE, -1, 4),
-              rpg.PageTable(FAKE, 2, 0), rpg.PageTable(FAKE, 2, 4, 3), rpg.PageTable(FAKE, (1 << 20) + 1, 4)):
+              rpg.PageTable(FAKE, 2, 0), rpg.PageTable(FAKE, 2, 4, 3), rpg.PageTable(FAKE, 2, 1 << 27), rpg.PageTable(FAKE, (1 << 20) + 1, 4)):
         with pytest.raises(EngineError):
             call(cache(), table=t)
     with pytest.raises(EngineError, match="element type"):
