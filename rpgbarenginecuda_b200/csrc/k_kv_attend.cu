@@ -45,40 +45,47 @@
 namespace rpgb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWeightBits = 14;  // weights are scaled by 2^14
 
-template <int D_, KvType KIND_, bool PACK_>
+template <int D_, KvType KIND_, bool PACK_, int WARPS_>
 struct Cfg {
+  static constexpr int WARPS = WARPS_;  // of a block: they share an item
+  static constexpr int THREADS = 32 * WARPS;
   static constexpr int D = D_;
   static constexpr KvType KIND = KIND_;
   static constexpr bool PACK = PACK_;  // at most 4 query heads: first and second terms share 8 columns
   static constexpr bool QUANT = KIND != KvType::kF16;
   static constexpr int QUERIES = PACK ? 4 : 8;
   static constexpr int R = QUANT || D == 64 ? 32 : 16;  // positions of a warp's step
-  static constexpr int TILE = kWarps * R;
+  static constexpr int TILE = WARPS * R;
   static constexpr int MT = R / 16;     // 16-position tiles of a step
   static constexpr int KS = D / 16;     // 16-value slices of a head
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;  // 16-byte chunks of a row
-  static constexpr int LEAST = 2;
-  static constexpr int BORDER = QUANT ? 1 : 2;  // the end of an item costs a block about as much as so many tiles
+  static constexpr int LEAST = 2;  // tiles (borders included) a block is started for
+  // the end of an item costs a block about as much as so many tiles
+  static constexpr int BORDER = (QUANT ? 1 : 2) * (WARPS == 1 ? 2 : 1);
   static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
   static constexpr int KSLOT = R * ROW + 2 * SC;     // K codes, K scales, V scales
   static constexpr int VSLOT = R * ROW;
   static constexpr int RING = KSLOT + VSLOT;  // per warp
   static_assert(KSLOT % 128 == 0 && VSLOT % 128 == 0, "tiles are 128-byte lines");
   static constexpr int COMB = QUERIES * D * 4;   // per warp
-  static constexpr int JOIN = kWarps * COMB > QUERIES * kKvMaxBlocks * 4 ? kWarps * COMB : QUERIES * kKvMaxBlocks * 4;
+  static constexpr int MAXBLOCKS = WARPS == 1 ? kKvMaxBlocks : 512;
+  // the join area: the warps' vectors, then the factors of up to BATCH records
+  static constexpr int JOIN = WARPS == 1 || WARPS * COMB > QUERIES * MAXBLOCKS * 4 ? WARPS * COMB : QUERIES * MAXBLOCKS * 4;
+  static constexpr int BATCH = JOIN / (QUERIES * 4);
   // q as B fragments: f16 terms, or up to three digit tiles of 8-bit integers
   static constexpr int QTILES = QUANT ? (PACK ? 2 : 3) : (PACK ? 1 : 2);
   static constexpr int QWORDS = QUANT ? 4 * NG : 2 * KS;  // of a lane and tile
   static constexpr int QBYTES = QTILES * QWORDS * 128;
-  static constexpr int SMEM = kWarps * RING + JOIN + QBYTES;
-  static constexpr int BLOCKS = PACK || D == 64 ? 3 : 2;  // resident per SM: what registers and shared memory allow
+  static constexpr int SMEM = WARPS * RING + JOIN + QBYTES;
+  // Resident per SM: 12 warps where registers allow (168 a thread).  With 64
+  // conversations to 16384 in 4 bits, 8 warps take 187 us, 12 take 175 and 16
+  // (128 registers, which spill) 185.
+  static constexpr int BLOCKS = (PACK || D == 64 ? 12 : 8) / WARPS;
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte lines.  The
@@ -377,13 +384,13 @@ struct Filler {
 };
 
 // Block b of n takes tiles [total b / n, total (b + 1) / n); ShareOf is the
-// block that has tile x.  Few tiles need no 64-bit division.
+// block that has tile x.  Few tiles (blocks are fewer than 2^11) need no 64-bit division.
 __device__ __forceinline__ long long ShareBegin(long long total, int b, int n) {
-  if (total < (1 << 22)) return static_cast<uint32_t>(total) * static_cast<uint32_t>(b) / static_cast<uint32_t>(n);
+  if (total < (1 << 21)) return static_cast<uint32_t>(total) * static_cast<uint32_t>(b) / static_cast<uint32_t>(n);
   return total * b / n;
 }
 __device__ __forceinline__ int ShareOf(long long x, long long total, int n) {
-  if (total < (1 << 22)) {
+  if (total < (1 << 21)) {
     return (static_cast<uint32_t>(x + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint32_t>(total);
   }
   return static_cast<int>(((x + 1) * n - 1) / total);
@@ -496,7 +503,7 @@ __device__ __forceinline__ void ReadQ(float (&x)[C::D / 4], const T* row, int t)
 
 // The lanes' q rows (lane g: column g's query) as B fragments in shared
 // memory: word i of tile n, lane at base + ((n * QWORDS + i) / 4 * 32 + lane) *
-// 16 + i % 4 * 4, written by warp i % kWarps.  Returns what turns a product
+// 16 + i % 4 * 4, written by warp i % C::WARPS.  Returns what turns a product
 // back into a score in log2 units (the scale's magnitude included; its sign
 // goes into the fragments, so that the largest product is the largest score).
 //
@@ -517,7 +524,7 @@ __device__ __forceinline__ float WriteQ(uint32_t base, const float (&x)[C::D / 4
   auto back = [&](float f) { return top_bits >= 0x7F800000u ? kvd::Nan() : fmaxf(f, 1e-30f); };
   auto put = [&](int n, int i, uint32_t w) {
     const int k = n * C::QWORDS + i;
-    if (i % kWarps == warp) Sts32(base + ((k >> 2) * 32 + lane) * 16 + (k & 3) * 4, w);
+    if (i % C::WARPS == warp) Sts32(base + ((k >> 2) * 32 + lane) * 16 + (k & 3) * 4, w);
   };
   if (!C::QUANT) {
     const int e = min(max(static_cast<int>(top_bits >> 23), 1), 253);  // kept in f32's normal range
@@ -594,15 +601,15 @@ __device__ __forceinline__ void AddScaled(float4& v, float f, const float4& x) {
 }
 
 template <typename C>
-__global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAttendParams p) {
+__global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const KvAttendParams p) {
   constexpr int D = C::D;
   extern __shared__ __align__(128) char smem[];
-  __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-  __shared__ long long s_sum[kWarps], s_begin, s_item0[kWarps];
+  __shared__ float s_m[C::WARPS][8], s_l[C::WARPS][8], s_keep[8];
+  __shared__ long long s_sum[C::WARPS], s_begin, s_item0[C::WARPS];
   __shared__ int s_seq, s_last;
-  __shared__ Cursor<C> s_use[kWarps], s_fill[kWarps];
+  __shared__ Cursor<C> s_use[C::WARPS], s_fill[C::WARPS];
   __shared__ __align__(8) float s_bias[C::NG][3][8];
-  __shared__ __align__(16) Places s_places[kWarps];
+  __shared__ __align__(16) Places s_places[C::WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.kv.n_kv;
   const int chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
@@ -613,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   dev::GridWait();  // (launched before the stream's previous kernel has finished)
   // This block's share of the tiles: prefix sums of the conversations' tiles
   // (and their items' borders), a run of conversations per thread.
-  const int run = (p.table.n_seq + kThreads - 1) / kThreads;
+  const int run = (p.table.n_seq + C::THREADS - 1) / C::THREADS;
   long long mine = 0;
   for (int i = 0; i < run; ++i) {
     const int s = tid * run + i;
@@ -629,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   __syncthreads();
   long long total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < C::WARPS; ++w) {
     if (w == warp) upto += total;
     total += s_sum[w];
   }
@@ -671,9 +678,9 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   }
 
   const uint32_t ring = dev::SmemAddr(smem) + warp * C::RING;
-  float* comb = reinterpret_cast<float*>(smem + kWarps * C::RING);
+  float* comb = reinterpret_cast<float*>(smem + C::WARPS * C::RING);
   float* mineq = comb + warp * (C::COMB / 4);
-  const uint32_t q_smem = dev::SmemAddr(smem) + kWarps * C::RING + C::JOIN;
+  const uint32_t q_smem = dev::SmemAddr(smem) + C::WARPS * C::RING + C::JOIN;
   const uint32_t k_lane = KLaneOffset<C>(lane), v_lane = VLaneOffset<C>(lane);
   // What changes with the item only is kept per warp in shared memory.
   if (lane == 0) {
@@ -1045,12 +1052,12 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         const int q = 4 * i / D;
         top = s_m[0][q];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][q]);
+        for (int w = 1; w < C::WARPS; ++w) top = fmaxf(top, s_m[w][q]);
         const float ref = top == -INFINITY ? 0.f : top;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < C::WARPS; ++w) {
           AddScaled(v, Exp2(s_m[w][q] - ref), reinterpret_cast<const float4*>(comb + w * (C::COMB / 4))[i]);
           sum += Exp2(s_m[w][q] - ref) * s_l[w][q];
         }
@@ -1073,18 +1080,18 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         // This block's record: one for an item that began in an earlier block,
         // one for an item that begins here.  Blocks b0 .. b1 hold the parts.
         const int b0 = ShareOf(item0, total, blocks), b1 = ShareOf(item0 + use.span.tiles - 1, total, blocks);
-        constexpr int kRecord = kKvMaxQueries * (D + 2);
+        const int record_size = KvRecordFloats(per_chunk, D), ms = per_chunk * D, ls = ms + per_chunk;
         float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
                                                   (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256);
-        auto record = [&](int b) { return records + (2 * b + (b == b0 ? 1 : 0)) * kRecord; };
+        auto record = [&](int b) { return records + static_cast<int64_t>(2 * b + (b == b0 ? 1 : 0)) * record_size; };
         unsigned* count = static_cast<unsigned*>(p.workspace) + (static_cast<int64_t>(use.seq) * p.kv.n_kv + use.head) * chunks + use.chunk;
         float* rec = record(blockIdx.x);
-        for (int i = tid; i < vecs; i += kThreads) {
+        for (int i = tid; i < vecs; i += C::THREADS) {
           float sum, top;
           reinterpret_cast<float4*>(rec)[i] = join(i, sum, top);
           if (i % (D / 4) == 0) {
-            rec[kKvMaxQueries * D + i / (D / 4)] = top;
-            rec[kKvMaxQueries * (D + 1) + i / (D / 4)] = sum;
+            rec[ms + i / (D / 4)] = top;
+            rec[ls + i / (D / 4)] = sum;
           }
         }
         __syncthreads();
@@ -1096,7 +1103,7 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
         if (finish && b1 - b0 < kFew) {
           // Few records: every thread reads what it needs of all of them at once.
           finish = false;
-          for (int i = tid; i < vecs; i += kThreads) {
+          for (int i = tid; i < vecs; i += C::THREADS) {
             const int q = 4 * i / D;
             float top = -INFINITY, m_[kFew], l_[kFew];
             float4 v[kFew];
@@ -1107,8 +1114,8 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
               v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
               if (b0 + n <= b1) {
                 const float* r = record(b0 + n);
-                m_[n] = __ldcg(r + kKvMaxQueries * D + q);
-                l_[n] = __ldcg(r + kKvMaxQueries * (D + 1) + q);
+                m_[n] = __ldcg(r + ms + q);
+                l_[n] = __ldcg(r + ls + q);
                 v[n] = __ldcg(reinterpret_cast<const float4*>(r) + i);
               }
             }
@@ -1127,72 +1134,84 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
           }
         }
         if (finish) {
-          // The last block joins all records under the maximum of all.  First
-          // the records' factors, a query per warp and a record per lane, into
-          // the join area; then warp w adds up records b0 + w, b0 + w + 4, ...
-          // in that order, a few of them in flight.
-          float* factor = comb;  // [query][record]
-          for (int q = warp; q < queries; q += kWarps) {
-            float top = -INFINITY, sum = 0.f;
-            for (int b = b0 + lane; b <= b1; b += 64) {  // (a second record per lane at once)
-              const float* r = record(b) + kKvMaxQueries * D + q;
-              const float* r2 = record(min(b + 32, b1)) + kKvMaxQueries * D + q;
-              const float ma = __ldcg(r), mb = __ldcg(r2), la = __ldcg(r + kKvMaxQueries), lb = __ldcg(r2 + kKvMaxQueries);
-              const float now = fmaxf(top, fmaxf(ma, mb)), ref = now == -INFINITY ? 0.f : now;
-              sum = sum * Exp2(top - ref) + Exp2(ma - ref) * la + (b + 32 <= b1 ? Exp2(mb - ref) * lb : 0.f);
-              top = now;
-              factor[q * kKvMaxBlocks + b - b0] = ma;
-              if (b + 32 <= b1) factor[q * kKvMaxBlocks + b + 32 - b0] = mb;
-            }
-            const float all = dev::WarpMax(top), ref = all == -INFINITY ? 0.f : all;
-            sum *= Exp2(top - ref);
-            top = all;
-            for (int b = lane; b <= b1 - b0; b += 32) {  // (the lane's own: b and b + 32 keep their lane)
-              factor[q * kKvMaxBlocks + b] = Exp2(factor[q * kKvMaxBlocks + b] - ref);
-            }
-            sum = dev::WarpSum(sum);
-            if (lane < kWarps) {
-              s_m[lane][q] = top;
-              s_l[lane][q] = lane == 0 ? sum : 0.f;
-            }
-          }
-          __syncthreads();
+          // The last block joins all records, BATCH of them at a time: their
+          // factors under the largest maximum so far into the join area, a
+          // query per warp and a record per lane; then warp w adds up records
+          // w, w + WARPS, ... in that order, a few of them in flight.
+          float* factor = comb;  // [query][record of the batch]
           constexpr int kVec = C::QUERIES * D / 128, kFlight = 8 / kVec;  // float4 of a lane; records in flight
           float4 v[kVec];
 #pragma unroll
           for (int k = 0; k < kVec; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int b = b0 + warp; b <= b1; b += kWarps * kFlight) {
-            float4 r[kFlight][kVec];
-#pragma unroll
-            for (int n = 0; n < kFlight; ++n) {
+          for (int c0 = b0; c0 <= b1; c0 += C::BATCH) {
+            const int c1 = min(c0 + C::BATCH - 1, b1);
+            for (int q = warp; q < queries; q += C::WARPS) {
+              const float before = c0 == b0 ? -INFINITY : s_m[0][q];
+              float top = before, sum = 0.f;  // the lane's
+              for (int b = c0 + lane; b <= c1; b += 64) {  // (a second record per lane at once)
+                const bool two = b + 32 <= c1;
+                const float *r = record(b) + q, *r2 = record(two ? b + 32 : b) + q;
+                const float ma = __ldcg(r + ms), mb = __ldcg(r2 + ms), la = __ldcg(r + ls), lb = __ldcg(r2 + ls);
+                const float now = fmaxf(top, fmaxf(ma, mb)), ref = now == -INFINITY ? 0.f : now;
+                sum = sum * Exp2(top - ref) + Exp2(ma - ref) * la + (two ? Exp2(mb - ref) * lb : 0.f);
+                top = now;
+                factor[q * C::BATCH + b - c0] = ma;
+                if (two) factor[q * C::BATCH + b + 32 - c0] = mb;
+              }
+              const float all = dev::WarpMax(top), ref = all == -INFINITY ? 0.f : all;
+              sum = dev::WarpSum(sum * Exp2(top - ref));
+              for (int b = lane; b <= c1 - c0; b += 32) {  // (the lane's own: b and b + 32 keep their lane)
+                factor[q * C::BATCH + b] = Exp2(factor[q * C::BATCH + b] - ref);
+              }
+              const float keep = Exp2(before - ref), was = c0 == b0 ? 0.f : s_l[0][q];
+              __syncwarp();
+              if (lane < C::WARPS) {
+                s_m[lane][q] = all;
+                s_l[lane][q] = lane == 0 ? was * keep + sum : 0.f;
+              }
+              if (lane == 0) s_keep[q] = keep;
+            }
+            __syncthreads();
+            if (c0 != b0) {
 #pragma unroll
               for (int k = 0; k < kVec; ++k) {
                 const int q = D == 128 ? k : 2 * k + (lane >> 4);
-                if (b + n * kWarps <= b1 && q < queries) {
-                  r[n][k] = __ldcg(reinterpret_cast<const float4*>(record(b + n * kWarps)) + 32 * k + lane);
+                const float f = q < queries ? s_keep[q] : 0.f;
+                v[k] = make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f);
+              }
+            }
+            for (int b = c0 + warp; b <= c1; b += C::WARPS * kFlight) {
+              float4 r[kFlight][kVec];
+#pragma unroll
+              for (int n = 0; n < kFlight; ++n) {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                  const int q = D == 128 ? k : 2 * k + (lane >> 4);
+                  if (b + n * C::WARPS <= c1 && q < queries) {
+                    r[n][k] = __ldcg(reinterpret_cast<const float4*>(record(b + n * C::WARPS)) + 32 * k + lane);
+                  }
+                }
+              }
+#pragma unroll
+              for (int n = 0; n < kFlight; ++n) {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                  const int q = D == 128 ? k : 2 * k + (lane >> 4);
+                  if (b + n * C::WARPS <= c1 && q < queries) {
+                    AddScaled(v[k], factor[q * C::BATCH + b - c0 + n * C::WARPS], r[n][k]);
+                  }
                 }
               }
             }
-#pragma unroll
-            for (int n = 0; n < kFlight; ++n) {
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) {
-                const int q = D == 128 ? k : 2 * k + (lane >> 4);
-                if (b + n * kWarps <= b1 && q < queries) {
-                  const float f = factor[q * kKvMaxBlocks + b - b0 + n * kWarps];
-                  AddScaled(v[k], f, r[n][k]);
-                }
-              }
-            }
+            __syncthreads();  // the factors have been read
           }
-          __syncthreads();  // the factors have been read
 #pragma unroll
           for (int k = 0; k < kVec; ++k) reinterpret_cast<float4*>(mineq)[32 * k + lane] = v[k];
           __syncthreads();
         }
       }
       if (finish) {
-        for (int i = tid; i < vecs; i += kThreads) {
+        for (int i = tid; i < vecs; i += C::THREADS) {
           float sum, top;
           const float4 v = join(i, sum, top);
           put(i, v, sum);
@@ -1214,10 +1233,10 @@ __global__ void __launch_bounds__(kThreads, C::BLOCKS) KvAttendKernel(const KvAt
   CopyWait<0>();
 }
 
-template <int D, KvType KIND, bool PACK>
-void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
-  using C = Cfg<D, KIND, PACK>;
-  static std::atomic<int> resident[64];  // blocks the device holds at once
+// Blocks of the kernel that the current device holds at once.
+template <typename C>
+int Resident() {
+  static std::atomic<int> resident[64];
   int dev = 0;
   RPGB_CUDA(cudaGetDevice(&dev));
   RPGB_CHECK(dev < 64, "kv: device %d", dev);
@@ -1226,11 +1245,17 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
     int sms = 0, per = 0;
     RPGB_CUDA(cudaFuncSetAttribute(KvAttendKernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     RPGB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    RPGB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, KvAttendKernel<C>, kThreads, C::SMEM));
+    RPGB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, KvAttendKernel<C>, C::THREADS, C::SMEM));
     RPGB_CHECK(per > 0, "kv: the attend kernel does not fit device %d", dev);
-    grid = sms * per < kKvMaxBlocks ? sms * per : kKvMaxBlocks;
+    grid = sms * per < C::MAXBLOCKS ? sms * per : C::MAXBLOCKS;
     resident[dev].store(grid, std::memory_order_release);
   }
+  return grid;
+}
+
+template <typename C>
+void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
+  int grid = Resident<C>();
   // no more blocks than tiles there can be
   const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
   const int64_t tiles = ((cap + 15) / C::TILE + 1 + C::BORDER) * p.kv.n_kv * chunks;
@@ -1242,16 +1267,31 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   a.pos16 = static_cast<uint32_t>(p.kv.pos_stride / 16);
   a.spage16 = static_cast<uint32_t>(p.kv.scale_page_stride / 16);
   a.shead16 = static_cast<uint32_t>(p.kv.scale_head_stride / 16);
-  LaunchKernelArgs(reinterpret_cast<const void*>(KvAttendKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, a);
+  LaunchKernelArgs(reinterpret_cast<const void*>(KvAttendKernel<C>), dim3(grid), dim3(C::THREADS), C::SMEM, s, true, a);
 }
 
+// Blocks of four warps that share an item, or of one: with at least as many
+// items as warps that run at once, a warp for itself needs no barriers and
+// joins less.  256 conversations to 200 positions of 16 / 8 heads in 8 bits:
+// 40.0 us with four, 26.2 with one; 512 to 60 of 32 / 8 in 4 bits: 52.3 and
+// 27.8.  With few items a warp's records are many: one conversation of 65521
+// positions takes 36 us with four warps a block, 50 already with two.
+template <int D, KvType KIND, bool PACK>
+void ByItems(const KvAttendParams& p, int chunks, cudaStream_t s) {
+  using One = Cfg<D, KIND, PACK, 1>;
+  if (static_cast<int64_t>(p.table.n_seq) * p.kv.n_kv * chunks >= Resident<One>()) {
+    Launch<One>(p, chunks, s);
+  } else {
+    Launch<Cfg<D, KIND, PACK, 4>>(p, chunks, s);
+  }
+}
 template <int D, KvType KIND>
 void ByQueries(const KvAttendParams& p, cudaStream_t s) {
   const int group = p.n_heads / p.kv.n_kv, chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
   if (group <= 4) {
-    Launch<D, KIND, true>(p, chunks, s);
+    ByItems<D, KIND, true>(p, chunks, s);
   } else {
-    Launch<D, KIND, false>(p, chunks, s);
+    ByItems<D, KIND, false>(p, chunks, s);
   }
 }
 template <int D>
@@ -1268,7 +1308,7 @@ void ByKind(const KvAttendParams& p, cudaStream_t s) {
 int64_t KvAttendWorkspace(int64_t n_seq, int n_heads, int n_kv, int head_dim) {
   const int group = n_heads / n_kv, chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
   const int64_t counters = (n_seq * n_kv * chunks * 4 + 255) / 256 * 256;
-  return counters + static_cast<int64_t>(2 * kKvMaxBlocks) * kKvMaxQueries * (head_dim + 2) * 4;
+  return counters + static_cast<int64_t>(2 * kKvMaxBlocks) * KvRecordFloats((group + chunks - 1) / chunks, head_dim) * 4;
 }
 
 void LaunchKvAttend(const KvAttendParams& p, cudaStream_t s) {

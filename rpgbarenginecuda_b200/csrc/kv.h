@@ -21,7 +21,14 @@ constexpr int kKvMinPage = 16;       // a page holds whole 16-position units
 constexpr int kKvMaxPage = 4096;
 constexpr int kKvMaxQueries = 8;     // query heads of a KV head that one attend pass takes
 constexpr int64_t kKvMaxStride = int64_t{1} << 35;  // bytes; a sixteenth of it fits 32 bits
-constexpr int kKvMaxBlocks = 512;    // bound of the attend grid (sizes the workspace)
+constexpr int kKvMaxBlocks = 1792;   // bound of the attend grid (sizes the workspace)
+// Floats of one attend record: a vector, a maximum and a sum per query, in whole 16 bytes.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+constexpr int KvRecordFloats(int queries, int head_dim) {
+  return (queries * (head_dim + 2) + 3) / 4 * 4;
+}
 
 struct KvPages {
   KvType type = KvType::kF16;

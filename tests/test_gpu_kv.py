@@ -194,6 +194,19 @@ def test_attend_many_conversations(kind):
 
 
 @pytest.mark.parametrize("kind", ["f16", "q8", "q4"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_attend_many_short_and_one_long(kind, dim, group):
+    """900 conversations of two KV heads, nearly all a page or two long, one of 30000 positions, windows on some."""
+    lens = [(i * 29) % 41 for i in range(900)]
+    lens[411] = 30000
+    starts = [3 if i % 5 == 0 else (29990 if i == 411 and group == 3 else 0) for i in range(900)]
+    pool = Pool(kind, lens, 16, n_kv=2, dim=dim, seed=group)
+    q = queries(900, 2 * group, dim, "f32")
+    check(attend(pool, q, starts=starts), expected(pool, q, starts=starts), pool, "f32")
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8", "q4"])
 def test_attend_windows(kind):
     """Starts inside a page and a tile, on their edges, at and past the length, negative; pages before them may be gone."""
     lens = [300, 300, 300, 300, 300, 300, 300, 40, 300]
@@ -274,7 +287,7 @@ def test_attend_many_queries_to_one_head(kind):
 
 
 def test_attend_very_many_conversations():
-    """70000 conversations of 64 heads, most of them empty: more than 2^22 shares of work."""
+    """70000 conversations of 64 heads, most of them empty: more than 2^21 tiles of work."""
     n, heads = 70000, 64
     lens = [0] * n
     for i in range(0, n, 7001):
