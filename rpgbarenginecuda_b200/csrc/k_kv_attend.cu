@@ -2,40 +2,58 @@
 // key-value cache: o = softmax(scale q K^T) V per q head, over positions
 // [start, len) of each conversation.
 //
-// What it has to do is read the cache once: 4 G flops per cached byte pair at
-// most (G query heads share a KV head), far under what the tensor cores do in
-// the time HBM takes, so the kernel is a stream of cache pages with the math
-// kept off its way.
+// What it has to do is read the cache once: 4 G flops per cached pair of
+// values (G query heads share a KV head), far under what the tensor cores do
+// in the time HBM takes.  So the kernel is a stream of cache pages with the
+// math kept out of its way, and what bounds it is HBM (f16, 8 bits) or the
+// rate at which the SMs issue the conversions (4 bits).
 //
 //  * Work.  An item is a (conversation, KV head, chunk of at most 8 query
-//    heads); its positions are cut into tiles and the tiles of all items, in
+//    heads); its positions are cut into tiles, and the tiles of all items, in
 //    order, are dealt evenly over a persistent grid, wherever the item borders
-//    fall.  Every block finds its share from the lengths on the device, so the
-//    host needs to know none, ragged batches stay balanced and one long
+//    fall.  A border is weighed as a tile or two, which is what ending an item
+//    costs.  Every block finds its share from the lengths on the device, so
+//    the host needs to know none, ragged batches stay balanced and one long
 //    conversation fills the GPU.  An item inside one block is written at once;
-//    otherwise the blocks leave (max, sum, vector) records in the workspace
-//    and the last of them to finish joins them in block order.
-//  * Data.  Each warp takes R consecutive positions of a tile and owns a ring
-//    of shared-memory slots filled with 16-byte asynchronous copies, DEPTH
-//    steps ahead of the math, across item borders.  Rows outside the range
-//    are not read but filled with zeros.  16-byte chunks are permuted so that
-//    every read of a tile is free of bank conflicts.
-//  * Math.  S^T = K q^T and O^T += V^T P^T as m16n8k16 tensor-core products
-//    with the positions (S) or value dimensions (O) as the 16 rows and 8
-//    query columns, so a group of 2 to 8 query heads wastes little; tcgen05
-//    has 128 rows but would need V and the converted codes staged through
-//    shared or tensor memory again for a product that is not the bound.
-//    Codes become exact f16 integers with two instructions per pair; a scale
-//    multiplies the group's partial score (K) or the weight of its position (V).
-//  * Precision.  f16 operands, f32 accumulation.  q is scaled by a power of
-//    two to a largest value in [1, 2) and split into two f16 terms (one when
-//    it is 16-bit, which is then exact), the softmax weights are split into
-//    two f16 terms, and scaled up by 2^14 (and by the power of two above the
-//    largest V scale seen) so that small ones stay normal numbers: 22 bits
-//    throughout.  With at most 4 query heads the second terms ride in the
-//    other 4 columns at no cost.  Each step's product starts from zero and is
-//    added to the running output in f32 registers: the tensor cores truncate
-//    when they add, which over a long conversation would add up.
+//    otherwise the blocks leave (vector, max, sum) records in the workspace
+//    and the last of them to finish joins them in block order, so the result
+//    does not depend on which is last.
+//  * Data.  A warp takes R consecutive positions of a tile and has a slot of
+//    shared memory for their K and one for their V, filled by 16-byte
+//    asynchronous copies: the next step's K while this step's V is at work and
+//    the other way round, across item borders.  (One step ahead is enough: 12
+//    warps keep about 100 KB in flight per SM; two steps ahead took 119 us
+//    where one takes 113.)  Page lookups and offsets of up to 16 steps are
+//    worked out at once, one 16-position half per lane.  Positions out of
+//    range are not used whatever they hold: their scores become -infinity,
+//    their V scales or rows zero.  16-byte chunks are permuted so that every
+//    read of a tile is free of bank conflicts.
+//  * Math.  S^T = K q^T and O^T += V^T P^T on mma.sync with the positions (S)
+//    or value dimensions (O) as the 16 rows and 8 query columns, so 2 to 8
+//    query heads waste little.  tcgen05 has 128 rows for a query side of 8 and
+//    would need codes staged once more through shared or tensor memory, for
+//    products that take a fifth of the time as they are.  Codes of K go to
+//    the integer tensor cores as they are (4-bit ones spread to bytes), with q
+//    as three signed base-256 digits; codes of V become exact f16 integers,
+//    two instructions per pair.  A scale multiplies the group's partial score
+//    (K) or the weight of its position (V).
+//  * Precision.  f32 sums throughout.  With an f16 cache q is scaled by a power
+//    of two to a largest value in [1, 2) and split into two f16 terms (a 16-bit
+//    q needs one); with a quantised one it is a 24-bit integer relative to its
+//    largest value.  The softmax weights are split into two f16 terms and
+//    carry a power of two that keeps small ones (times the largest V scale
+//    seen) normal numbers: 22 bits.  With at most 4 query heads the second
+//    terms and digits ride in the other 4 columns at no cost.  Each step's
+//    product starts from zero and is added to the running output in f32
+//    registers: the tensor cores truncate when they add, which would grow over
+//    a long conversation.
+//
+// Measured on one B200 (floor: bytes at the measured copy rate of 6.55 TB/s):
+// 32 conversations of 32 / 8 heads to 8192 positions in f16 107 us (104.5),
+// 16 to 3840 in 8 bits 25 us (12.9), one of 65521 in 8 bits 36 us (21.2), 64
+// to 4096 in 4 bits 56 us (27.7), one of 21 positions of 16 / 8 heads 6 us.  A
+// launch costs about 4 us before its first data (lengths, pages, data: three
+// round trips) and 3 us after its last.
 #include <atomic>
 
 #include "common.h"
@@ -90,8 +108,8 @@ struct Cfg {
 
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte lines.  The
 // chunk's place in its line is permuted (an exclusive or with bits of the row)
-// so that the lanes of one load (8 rows of one chunk for ldmatrix; see KRows
-// and VFragments for the codes) touch different banks.
+// so that the lanes of one load (8 rows of one chunk for ldmatrix; see
+// KFragments and VFragments for the codes) touch different banks.
 template <typename C, bool V>
 __host__ __device__ constexpr int ChunkAt(int r, int c) {
   const int key = C::KIND == KvType::kF16  ? r & 7
@@ -409,7 +427,7 @@ __device__ __forceinline__ int KLaneOffset(int lane) {
 // K codes of 16 positions (rows g, g + 8 of tile mt) and a 64-value group as A
 // fragments of two 32-value slices.  The columns of a slice are the lanes'
 // runs, 8 values of each: q8 codes as they are, 4-bit codes spread to bytes,
-// the even values of the 8, then the odd ones (LaneDigits takes q the same way).
+// the even values of the 8, then the odd ones (WriteQ takes q the same way).
 template <typename C>
 __device__ __forceinline__ void KFragments(uint32_t (&a)[2][4], uint32_t base, int mt, int gp) {
 #pragma unroll
