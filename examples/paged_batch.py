@@ -121,7 +121,8 @@ class PagedModel:
         self.free = list(range(n_pages))[::-1]
         self.table = np.full((max_conversations, self.max_pages), -1, np.int32)
         self.lengths: dict[int, int] = {}
-        self.workspace = torch.zeros(0, dtype=torch.uint8, device="cuda")
+        self.workspace = torch.zeros(rpg.attend_workspace(self.n_heads, self.n_kv, self.dim), dtype=torch.uint8,
+                                     device="cuda")
 
     def open(self) -> int:
         """A new conversation."""
@@ -153,9 +154,6 @@ class PagedModel:
         pages = rpg.PageTable(table.data_ptr(), n, self.max_pages)
         pos = torch.tensor(pos, dtype=torch.int32, device="cuda")
         lens = pos + 1
-        need = rpg.attend_workspace(n, self.n_heads, self.n_kv, self.dim)
-        if self.workspace.numel() < need:
-            self.workspace = torch.zeros(need, dtype=torch.uint8, device="cuda")
         x = torch.empty(n, self.embd.cols, device="cuda")
         for i, (_, token) in enumerate(tokens):
             self.embd.dequant(token, 1, x[i].data_ptr())

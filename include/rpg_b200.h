@@ -286,9 +286,10 @@ RPGB_API int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* ta
  * of conversation s (starts_dev NULL: from 0; pages wholly before the start
  * are not looked at).  An empty range gives zeros.  n_heads is any multiple
  * of n_kv; q head h reads KV head h / (n_heads / n_kv).  The sums are in f32.
- * workspace_dev: rpgb_kv_attend_workspace bytes, 256-byte aligned, zeroed
- * once before its first use; calls that may overlap need one each. */
-RPGB_API int64_t rpgb_kv_attend_workspace(int32_t n_seq, int32_t n_heads, int32_t n_kv, int32_t head_dim);
+ * workspace_dev: rpgb_kv_attend_workspace bytes (or more), 256-byte aligned,
+ * zeroed once before its first use; calls of any shapes may follow one another
+ * on it, calls that may overlap need one each. */
+RPGB_API int64_t rpgb_kv_attend_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim);
 RPGB_API int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type, const void* q_dev,
                                 int64_t q_stride, int32_t n_heads, const int32_t* lens_dev, const int32_t* starts_dev,
                                 float scale, void* out_dev, int64_t out_stride, void* workspace_dev,

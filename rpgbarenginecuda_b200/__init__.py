@@ -319,9 +319,9 @@ class PagedKv:
             check(-1, "kv_attend")
 
 
-def attend_workspace(n_seq: int, n_heads: int, n_kv: int, head_dim: int) -> int:
-    """Bytes of the workspace `PagedKv.attend` needs (zeroed once by the caller)."""
-    n = int(load_engine().rpgb_kv_attend_workspace(n_seq, n_heads, n_kv, head_dim))
+def attend_workspace(n_heads: int, n_kv: int, head_dim: int) -> int:
+    """Bytes of the workspace `PagedKv.attend` needs, whatever the batch (zeroed once by the caller)."""
+    n = int(load_engine().rpgb_kv_attend_workspace(n_heads, n_kv, head_dim))
     if n < 0:
         check(-1, "kv_attend_workspace")
     return n

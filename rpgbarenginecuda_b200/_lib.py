@@ -84,7 +84,7 @@ _SIGS = {
     "rpgb_counter_uniform": (c_f32, [c_u64, c_u64]),
     "rpgb_kv_append": (c_i32, [c_p, c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_i64, c_p, c_i64, c_p]),
     "rpgb_kv_gather": (c_i32, [c_p, c_p, c_i32, c_p, c_p, c_i64, c_p, c_p, c_i64, c_p]),
-    "rpgb_kv_attend_workspace": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "rpgb_kv_attend_workspace": (c_i64, [c_i32, c_i32, c_i32]),
     "rpgb_kv_attend": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_f32, c_p, c_i64, c_p, c_i64, c_p]),
     "rpgb_text_open": (c_p, [ctypes.c_char_p]),
     "rpgb_text_close": (None, [c_p]),

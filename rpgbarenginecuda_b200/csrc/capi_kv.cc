@@ -186,13 +186,13 @@ int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
   RPGB_CATCH(-1)
 }
 
-int64_t rpgb_kv_attend_workspace(int32_t n_seq, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+int64_t rpgb_kv_attend_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim) {
   try {
     SetLastError("");
-    RPGB_CHECK(n_seq >= 0 && n_seq <= (1 << 20) && n_kv > 0 && n_kv <= 4096 && n_heads > 0 && n_heads <= 65535 &&
-                   n_heads % n_kv == 0 && (head_dim == 64 || head_dim == 128),
-               "kv: bad shape (%d conversations, %d heads over %d KV heads of %d)", n_seq, n_heads, n_kv, head_dim);
-    return KvAttendWorkspace(n_seq, n_heads, n_kv, head_dim);
+    RPGB_CHECK(n_kv > 0 && n_kv <= 4096 && n_heads > 0 && n_heads <= 65535 && n_heads % n_kv == 0 &&
+                   (head_dim == 64 || head_dim == 128),
+               "kv: bad shape (%d heads over %d KV heads of %d)", n_heads, n_kv, head_dim);
+    return KvAttendWorkspace(n_heads, n_kv, head_dim);
   }
   RPGB_CATCH(-1)
 }
@@ -215,7 +215,7 @@ int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
     CheckRows(out_dev, out_stride, cols, p.type, "out");
     RPGB_CHECK(lens_dev != nullptr, "kv: lengths are NULL");
     RPGB_CHECK(std::isfinite(scale), "kv: the scale is not finite");
-    const int64_t need = KvAttendWorkspace(p.table.n_seq, n_heads, p.kv.n_kv, p.kv.head_dim);
+    const int64_t need = KvAttendWorkspace(n_heads, p.kv.n_kv, p.kv.head_dim);
     RPGB_CHECK(workspace_dev != nullptr && workspace_bytes >= need, "kv: workspace of %lld bytes; %lld are needed",
                static_cast<long long>(workspace_dev != nullptr ? workspace_bytes : 0), static_cast<long long>(need));
     CheckAligned(workspace_dev, 256, "kv: workspace");

@@ -1099,10 +1099,10 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         // one for an item that begins here.  Blocks b0 .. b1 hold the parts.
         const int b0 = ShareOf(item0, total, blocks), b1 = ShareOf(item0 + use.span.tiles - 1, total, blocks);
         const int record_size = KvRecordFloats(per_chunk, D), ms = per_chunk * D, ls = ms + per_chunk;
-        float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
-                                                  (static_cast<int64_t>(p.table.n_seq) * items * 4 + 255) / 256 * 256);
+        float* records = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + kKvMaxBlocks * 4);
         auto record = [&](int b) { return records + static_cast<int64_t>(2 * b + (b == b0 ? 1 : 0)) * record_size; };
-        unsigned* count = static_cast<unsigned*>(p.workspace) + (static_cast<int64_t>(use.seq) * p.kv.n_kv + use.head) * chunks + use.chunk;
+        // (one item at most begins in a block and goes on past it, so the block numbers its counter)
+        unsigned* count = static_cast<unsigned*>(p.workspace) + b0;
         float* rec = record(blockIdx.x);
         for (int i = tid; i < vecs; i += C::THREADS) {
           float sum, top;
@@ -1323,10 +1323,9 @@ void ByKind(const KvAttendParams& p, cudaStream_t s) {
 
 }  // namespace
 
-int64_t KvAttendWorkspace(int64_t n_seq, int n_heads, int n_kv, int head_dim) {
+int64_t KvAttendWorkspace(int n_heads, int n_kv, int head_dim) {
   const int group = n_heads / n_kv, chunks = (group + kKvMaxQueries - 1) / kKvMaxQueries;
-  const int64_t counters = (n_seq * n_kv * chunks * 4 + 255) / 256 * 256;
-  return counters + static_cast<int64_t>(2 * kKvMaxBlocks) * KvRecordFloats((group + chunks - 1) / chunks, head_dim) * 4;
+  return kKvMaxBlocks * (4 + 8ll * KvRecordFloats((group + chunks - 1) / chunks, head_dim));
 }
 
 void LaunchKvAttend(const KvAttendParams& p, cudaStream_t s) {

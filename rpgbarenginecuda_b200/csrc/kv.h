@@ -100,9 +100,11 @@ struct KvAttendParams {
   // kv in units of 16 bytes
   uint32_t magic = 0, page16 = 0, head16 = 0, pos16 = 0, spage16 = 0, shead16 = 0;
 };
-// Workspace bytes of LaunchKvAttend (its first bytes are counters that start
-// at zero and are zero again after every call).
-int64_t KvAttendWorkspace(int64_t n_seq, int n_heads, int n_kv, int head_dim);
+// Workspace bytes of LaunchKvAttend: kKvMaxBlocks counters, which start at
+// zero and are zero again after every call, then two records per block.  The
+// counters' place does not depend on the shape, so calls of any shapes may
+// follow one another on one workspace.
+int64_t KvAttendWorkspace(int n_heads, int n_kv, int head_dim);
 void LaunchKvAttend(const KvAttendParams& p, cudaStream_t s);
 
 }  // namespace rpgb

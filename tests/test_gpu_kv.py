@@ -113,7 +113,7 @@ def attend(pool, q, lens=None, starts=None, scale=None, act="f32", stream=0, ws=
     st = i32(starts) if starts is not None else None
     n_heads = width // pool.dim
     if ws is None:
-        ws = torch.zeros(rpg.attend_workspace(rows, n_heads, pool.n_kv, pool.dim), dtype=torch.uint8, device="cuda")
+        ws = torch.zeros(rpg.attend_workspace(n_heads, pool.n_kv, pool.dim), dtype=torch.uint8, device="cuda")
     if out is None:
         out = torch.full((rows, width), 7.0, dtype=dt, device="cuda")
     torch.cuda.synchronize()
@@ -364,6 +364,19 @@ def test_attend_repeats_and_leaves_the_workspace_ready(kind):
         assert torch.equal(out, first)
 
 
+def test_attend_one_workspace_for_batches_of_all_sizes():
+    """Batches that grow and shrink, of other head layouts, one after another on one workspace."""
+    ws = torch.zeros(rpg.attend_workspace(24, 3, 128), dtype=torch.uint8, device="cuda")
+    for rows, longest, n_kv, group, dim, kind in ((1, 4000, 1, 2, 128, "f16"), (400, 50, 5, 4, 64, "q8"),
+                                                  (3, 3000, 3, 8, 128, "q4"), (900, 20, 8, 1, 64, "f16"),
+                                                  (17, 700, 8, 3, 128, "q8"), (1, 9000, 2, 8, 64, "q4"),
+                                                  (150, 60, 3, 7, 128, "f16")):
+        lens = [1 + (i * 31) % longest for i in range(rows - 1)] + [longest]
+        pool = Pool(kind, lens, 16, n_kv=n_kv, dim=dim, seed=rows)
+        q = queries(rows, n_kv * group, dim, "f32")
+        check(attend(pool, q, ws=ws), expected(pool, q), pool, "f32")
+
+
 def test_attend_on_another_stream():
     pool = Pool("q8", [3000, 50], 16, seed=1)
     q = queries(2, 4, 128, "f32")
@@ -604,7 +617,7 @@ def test_a_conversation_step_by_step(kind, tol):
     dev = table.cuda()
     rot = rpg.Rotary(dev.data_ptr(), n)
     x, x64 = x.view(n, 2, -1), x64.view(n, 2, -1, dim)
-    ws = torch.zeros(rpg.attend_workspace(2, n_heads, n_kv, dim), dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(rpg.attend_workspace(n_heads, n_kv, dim), dtype=torch.uint8, device="cuda")
     out = torch.empty(n, 2, n_heads * dim, device="cuda")
     q = torch.empty(2, n_heads * dim, device="cuda")
     for t in range(n):

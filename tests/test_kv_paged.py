@@ -106,10 +106,10 @@ def test_nothing_to_do_is_no_error():
 
 
 def test_workspace_size():
-    n = rpg.attend_workspace(4, 16, 8, 128)
+    n = rpg.attend_workspace(16, 8, 128)
     assert 0 < n <= 16 << 20
-    assert rpg.attend_workspace(4096, 64, 8, 128) > rpg.attend_workspace(4, 64, 8, 128)
-    for bad in ((-1, 16, 8, 128), (4, 12, 8, 128), (4, 16, 0, 128), (4, 16, 8, 80)):
+    assert rpg.attend_workspace(64, 8, 128) > n > rpg.attend_workspace(16, 8, 64)
+    for bad in ((0, 8, 128), (12, 8, 128), (16, 0, 128), (16, 8, 80)):
         with pytest.raises(EngineError):
             rpg.attend_workspace(*bad)
 
