@@ -93,7 +93,8 @@ struct Cfg {
   static constexpr int COMB = QUERIES * D * 4;   // per warp
   static constexpr int MAXBLOCKS = WARPS == 1 ? kKvMaxBlocks : 512;
   // the join area: the warps' vectors, then the factors of up to BATCH records
-  static constexpr int JOIN = WARPS == 1 || WARPS * COMB > QUERIES * MAXBLOCKS * 4 ? WARPS * COMB : QUERIES * MAXBLOCKS * 4;
+  static constexpr int FACTORS = WARPS == 1 ? 0 : QUERIES * MAXBLOCKS * 4;
+  static constexpr int JOIN = WARPS * COMB > FACTORS ? WARPS * COMB : FACTORS;
   static constexpr int BATCH = JOIN / (QUERIES * 4);
   // q as B fragments: f16 terms, or up to three digit tiles of 8-bit integers
   static constexpr int QTILES = QUANT ? (PACK ? 2 : 3) : (PACK ? 1 : 2);
@@ -209,7 +210,10 @@ __device__ __forceinline__ uint2 Lds64(uint32_t a) {
 }
 __device__ __forceinline__ uint4 Lds128(uint32_t a) {
   uint4 x;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "r"(a)
+               : "memory");
   return x;
 }
 __device__ __forceinline__ void Sts32(uint32_t a, uint32_t x) {
@@ -454,7 +458,9 @@ __device__ __forceinline__ void KFragments(uint32_t (&a)[2][4], uint32_t base, i
 template <typename C>
 __device__ __forceinline__ int VLaneOffset(int lane) {
   const int g = lane >> 2, t = lane & 3;
-  if (C::KIND == KvType::kF16) return ChunkAt<C, true>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);  // for ldmatrix
+  if (C::KIND == KvType::kF16) {  // for ldmatrix
+    return ChunkAt<C, true>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+  }
   return C::KIND == KvType::kQ8 ? ChunkAt<C, true>(2 * t, g >> 1) + (g & 1) * 8
                                 : ChunkAt<C, true>(2 * t, g >> 2) + (g & 3) * 4;
 }
@@ -770,262 +776,265 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
     left -= n + C::BORDER;  // (past the end where the share ends inside the item: what counts is whether any is left)
 #pragma unroll 1
     for (int i = n; i > 0; --i, lo -= C::TILE, hi -= C::TILE) {
-    const bool work = lo < C::R && hi > 0;
-    const bool edge = lo > 0 || hi < C::R || bad_now != 0;
+      const bool work = lo < C::R && hi > 0;
+      const bool edge = lo > 0 || hi < C::R || bad_now != 0;
 
-    // ---- scores (and the V scales)
-    CopyWait<1>();
-    __syncwarp();
-    float2 s[C::MT][2];  // rows g and g + 8 of a tile, columns 2 t and 2 t + 1
-    uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
-    if (work) {
-      const uint32_t kbase = kslot + k_lane, sbase = kslot + C::R * C::ROW + g * (2 * C::NG);
-      const uint32_t qbase = q_smem + lane * 16;
-      if (!C::QUANT) {
-        float sum[C::MT][4];
+      // ---- scores (and the V scales)
+      CopyWait<1>();
+      __syncwarp();
+      float2 s[C::MT][2];  // rows g and g + 8 of a tile, columns 2 t and 2 t + 1
+      uint32_t vsc[C::MT][2];  // V scales of the lane's rows, one or two f16
+      if (work) {
+        const uint32_t kbase = kslot + k_lane, sbase = kslot + C::R * C::ROW + g * (2 * C::NG);
+        const uint32_t qbase = q_smem + lane * 16;
+        if (!C::QUANT) {
+          float sum[C::MT][4];
 #pragma unroll
-        for (int k4 = 0; k4 < C::QWORDS / 4; ++k4) {
-          const uint4 q = Lds128(qbase + k4 * 512);
-          uint4 r = q;
-          if (!C::PACK && two_terms) r = Lds128(qbase + (C::QWORDS / 4 + k4) * 512);
+          for (int k4 = 0; k4 < C::QWORDS / 4; ++k4) {
+            const uint4 q = Lds128(qbase + k4 * 512);
+            uint4 r = q;
+            if (!C::PACK && two_terms) r = Lds128(qbase + (C::QWORDS / 4 + k4) * 512);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int ks = 2 * k4 + j;
+            for (int j = 0; j < 2; ++j) {
+              const int ks = 2 * k4 + j;
 #pragma unroll
-            for (int mt = 0; mt < C::MT; ++mt) {
-              uint32_t a[4];
-              LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
-              ks == 0 ? MmaFirst(sum[mt], a, q.x, q.y) : Mma(sum[mt], a, j == 0 ? q.x : q.z, j == 0 ? q.y : q.w);
-              if (!C::PACK && two_terms) Mma(sum[mt], a, j == 0 ? r.x : r.z, j == 0 ? r.y : r.w);
+              for (int mt = 0; mt < C::MT; ++mt) {
+                uint32_t a[4];
+                LdMatrix(a, Moved<C, false>(kbase, 16 * mt, 2 * ks));
+                ks == 0 ? MmaFirst(sum[mt], a, q.x, q.y) : Mma(sum[mt], a, j == 0 ? q.x : q.z, j == 0 ? q.y : q.w);
+                if (!C::PACK && two_terms) Mma(sum[mt], a, j == 0 ? r.x : r.z, j == 0 ? r.y : r.w);
+              }
             }
-          }
-        }
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-          s[mt][0] = make_float2(sum[mt][0], sum[mt][1]);
-          s[mt][1] = make_float2(sum[mt][2], sum[mt][3]);
-        }
-      } else {
-        constexpr bool kU = C::KIND == KvType::kQ4;
-        float2 d[C::MT][2];
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t a = sbase + (16 * mt + 8 * i) * (2 * C::NG);
-            const uint32_t k = C::NG == 2 ? Lds32(a) : Lds16(a);
-            vsc[mt][i] = C::NG == 2 ? Lds32(a + C::SC) : Lds16(a + C::SC);
-            d[mt][i] = __half22float2(BitsHalf(k));
-          }
-        }
-#pragma unroll
-        for (int gp = 0; gp < C::NG; ++gp) {
-          const uint4 q0 = Lds128(qbase + gp * 512);
-          const uint4 q1 = Lds128(qbase + (C::NG + gp) * 512);
-          const uint4 q2 = C::PACK ? q1 : Lds128(qbase + (2 * C::NG + gp) * 512);
-          float2 b0 = make_float2(kIntBias, kIntBias), b1 = b0, b2 = b0;
-          if (kU) {
-            b0 = *reinterpret_cast<const float2*>(&s_bias[gp][0][2 * t]);
-            b1 = *reinterpret_cast<const float2*>(&s_bias[gp][1][2 * t]);
-            b2 = *reinterpret_cast<const float2*>(&s_bias[gp][C::QTILES - 1][2 * t]);
           }
 #pragma unroll
           for (int mt = 0; mt < C::MT; ++mt) {
-            uint32_t a[2][4];
-            KFragments<C>(a, kbase, mt, gp);
-            auto product = [&](const uint4& q, const float2& b, float2 (&v)[2]) {
-              int n[4];
-              MmaIntFirst<kU>(n, a[0], q.x, q.y, kIntStart);
-              MmaInt<kU>(n, a[1], q.z, q.w);
-              const float2 less = make_float2(-b.x, -b.y);
-              v[0] = Add2(make_float2(__int_as_float(n[0]), __int_as_float(n[1])), less);
-              v[1] = Add2(make_float2(__int_as_float(n[2]), __int_as_float(n[3])), less);
-            };
-            float2 v[2], r[2];
-            product(q0, b0, v);
-            product(q1, b1, r);
+            s[mt][0] = make_float2(sum[mt][0], sum[mt][1]);
+            s[mt][1] = make_float2(sum[mt][2], sum[mt][3]);
+          }
+        } else {
+          constexpr bool kU = C::KIND == KvType::kQ4;
+          float2 d[C::MT][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(C::PACK ? 1.f / 65536 : 1.f / 256), v[i]);
-            if (!C::PACK) {
-              product(q2, b2, r);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(1.f / 65536), v[i]);
-            }
+          for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              s[mt][i] = gp == 0 ? Mul2(v[i], Both(d[mt][i].x)) : Fma2(v[i], Both(d[mt][i].y), s[mt][i]);
+              const uint32_t a = sbase + (16 * mt + 8 * i) * (2 * C::NG);
+              const uint32_t k = C::NG == 2 ? Lds32(a) : Lds16(a);
+              vsc[mt][i] = C::NG == 2 ? Lds32(a + C::SC) : Lds16(a + C::SC);
+              d[mt][i] = __half22float2(BitsHalf(k));
+            }
+          }
+#pragma unroll
+          for (int gp = 0; gp < C::NG; ++gp) {
+            const uint4 q0 = Lds128(qbase + gp * 512);
+            const uint4 q1 = Lds128(qbase + (C::NG + gp) * 512);
+            const uint4 q2 = C::PACK ? q1 : Lds128(qbase + (2 * C::NG + gp) * 512);
+            float2 b0 = make_float2(kIntBias, kIntBias), b1 = b0, b2 = b0;
+            if (kU) {
+              b0 = *reinterpret_cast<const float2*>(&s_bias[gp][0][2 * t]);
+              b1 = *reinterpret_cast<const float2*>(&s_bias[gp][1][2 * t]);
+              b2 = *reinterpret_cast<const float2*>(&s_bias[gp][C::QTILES - 1][2 * t]);
+            }
+#pragma unroll
+            for (int mt = 0; mt < C::MT; ++mt) {
+              uint32_t a[2][4];
+              KFragments<C>(a, kbase, mt, gp);
+              auto product = [&](const uint4& q, const float2& b, float2 (&v)[2]) {
+                int n[4];
+                MmaIntFirst<kU>(n, a[0], q.x, q.y, kIntStart);
+                MmaInt<kU>(n, a[1], q.z, q.w);
+                const float2 less = make_float2(-b.x, -b.y);
+                v[0] = Add2(make_float2(__int_as_float(n[0]), __int_as_float(n[1])), less);
+                v[1] = Add2(make_float2(__int_as_float(n[2]), __int_as_float(n[3])), less);
+              };
+              float2 v[2], r[2];
+              product(q0, b0, v);
+              product(q1, b1, r);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(C::PACK ? 1.f / 65536 : 1.f / 256), v[i]);
+              if (!C::PACK) {
+                product(q2, b2, r);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[i] = Fma2(r[i], Both(1.f / 65536), v[i]);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                s[mt][i] = gp == 0 ? Mul2(v[i], Both(d[mt][i].x)) : Fma2(v[i], Both(d[mt][i].y), s[mt][i]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+          if (C::PACK && C::QUANT) {  // lanes t < 2 hold the first digit, the others the second
+            const float2 f = Both(t < 2 ? 1.f / 256 : 256.f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 other = make_float2(__shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2),
+                                               __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2));
+              s[mt][i] = Fma2(other, f, s[mt][i]);
+            }
+          }
+          if (C::PACK && !C::QUANT && two_terms) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              s[mt][i].x += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2);
+              s[mt][i].y += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2);
             }
           }
         }
       }
-#pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
-        if (C::PACK && C::QUANT) {  // lanes t < 2 hold the first digit, the others the second
-          const float2 f = Both(t < 2 ? 1.f / 256 : 256.f);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            s[mt][i] = Fma2(make_float2(__shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2), __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2)),
-                            f, s[mt][i]);
-          }
-        }
-        if (C::PACK && !C::QUANT && two_terms) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            s[mt][i].x += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].x, 2);
-            s[mt][i].y += __shfl_xor_sync(0xFFFFFFFFu, s[mt][i].y, 2);
-          }
+      __syncwarp();
+      if (fill.count == 0) {
+        if (fill.left > 0) {
+          fill.Batch(p, warp, lane, chunks);
+        } else {
+          fill.have = 0;  // no more steps
         }
       }
-    }
-    __syncwarp();
-    if (fill.count == 0) {
-      if (fill.left > 0) {
-        fill.Batch(p, warp, lane, chunks);
-      } else {
-        fill.have = 0;  // no more steps
-      }
-    }
-    fill.template Issue<false>(p, kslot, lane, lane_off);
-    CopyWait<1>();  // V
-    __syncwarp();
+      fill.template Issue<false>(p, kslot, lane, lane_off);
+      CopyWait<1>();  // V
+      __syncwarp();
 
-    // ---- weights: 2^(score - ref) with ref a power of two over the largest,
-    // so that a weight times its V scale is at most 2^14 and small ones stay
-    // normal f16 numbers
-    float2 alpha = Both(1.f);
-    if (work) {
-      if (edge) {
-        asm volatile("" ::: "memory");  // a branch, not predicates: few steps come here
+      // ---- weights: 2^(score - ref) with ref a power of two over the largest,
+      // so that a weight times its V scale is at most 2^14 and small ones stay
+      // normal f16 numbers
+      float2 alpha = Both(1.f);
+      if (work) {
+        if (edge) {
+          asm volatile("" ::: "memory");  // a branch, not predicates: few steps come here
 #pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
+          for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = 16 * mt + 8 * i + g;
-            if ((bad_now >> mt) & 1) s[mt][i] = Both(kvd::Nan());
-            if (r < lo || r >= hi) {
-              s[mt][i] = Both(-INFINITY);
-              vsc[mt][i] = 0;  // a scale out of range may be anything
-            }
-          }
-        }
-      }
-      if (C::QUANT) {
-        __half2 top = BitsHalf(0);
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) top = __hmax2(top, __habs2(BitsHalf(vsc[mt][i])));
-        }
-        const uint32_t u = HalfBits(top);
-        const uint32_t f16 = __reduce_max_sync(0xFFFFFFFFu, max(u & 0xFFFFu, u >> 16));
-        const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(f16)));
-        nu = max(nu, min(static_cast<int>(__float_as_uint(d) >> 23), 127 + 16) + 1);
-      }
-      const float shift = C::QUANT ? static_cast<float>(nu - 127 - kWeightBits) : -static_cast<float>(kWeightBits);
-      float2 top = s[0][0], now;
-#pragma unroll
-      for (int j = 1; j < 2 * C::MT; ++j) {
-        top.x = fmaxf(top.x, s[j >> 1][j & 1].x);
-        top.y = fmaxf(top.y, s[j >> 1][j & 1].y);
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, o));
-        top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, o));
-      }
-      m.x = fmaxf(m.x, top.x * cs.x);
-      m.y = fmaxf(m.y, top.y * cs.y);
-      now.x = (m.x == -INFINITY ? 0.f : m.x) + shift;
-      now.y = (m.y == -INFINITY ? 0.f : m.y) + shift;
-      alpha = make_float2(Exp2(ref.x - now.x), Exp2(ref.y - now.y));
-      ref.x = m.x == -INFINITY ? -INFINITY : now.x;
-      ref.y = m.y == -INFINITY ? -INFINITY : now.y;
-      l = Mul2(l, alpha);
-      const float2 less = make_float2(-now.x, -now.y);
-#pragma unroll
-      for (int j = 0; j < 2 * C::MT; ++j) {
-        const float2 e = Fma2(s[j >> 1][j & 1], cs, less);
-        const float2 w = make_float2(Exp2(e.x), Exp2(e.y));
-        s[j >> 1][j & 1] = w;
-        l = Add2(l, w);
-      }
-    }
-
-    // ---- values
-    if (work) {
-      if (!C::QUANT && edge) {  // what lies out of range may be anything, NaN too: zeros
-#pragma unroll 1
-        for (int i = lane; i < C::R * C::CPR; i += 32) {
-          const int r = i / C::CPR;
-          if (r < lo || r >= hi) Sts128Zero(vslot + ChunkAt<C, true>(r, i % C::CPR));
-        }
-        __syncwarp();
-      }
-      const uint32_t vbase = vslot + v_lane;
-      const float2 of_rest = Both(t >= 2 ? 1.f : 0.f), of_lead = Both(t >= 2 ? -1.f : 1.f);  // the lane's columns' term
-#pragma unroll
-      for (int gp = 0; gp < C::NG; ++gp) {
-        uint32_t b[C::MT][2][C::PACK ? 1 : 2];
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float2 u = s[mt][i];
-            if (C::QUANT) {
-              const float2 d = __half22float2(BitsHalf(vsc[mt][i]));
-              u = Mul2(u, Both(gp == 0 ? d.x : d.y));
-            }
-            // the first term is the leading 11 bits, the second the rest
-            const float2 h = make_float2(__uint_as_float(__float_as_uint(u.x) & 0xFFFFE000u),
-                                         __uint_as_float(__float_as_uint(u.y) & 0xFFFFE000u));
-            if (C::PACK) {
-              const float2 w = Fma2(u, of_rest, Mul2(h, of_lead));
-              b[mt][i][0] = Transposed(PackHalf(w.x, w.y));
-            } else {
-              b[mt][i][0] = Transposed(PackHalf(h.x, h.y));
-              b[mt][i][C::PACK ? 0 : 1] = Transposed(PackHalf(u.x - h.x, u.y - h.y));
+            for (int i = 0; i < 2; ++i) {
+              const int r = 16 * mt + 8 * i + g;
+              if ((bad_now >> mt) & 1) s[mt][i] = Both(kvd::Nan());
+              if (r < lo || r >= hi) {
+                s[mt][i] = Both(-INFINITY);
+                vsc[mt][i] = 0;  // a scale out of range may be anything
+              }
             }
           }
         }
         if (C::QUANT) {
-          float part[4][4];
+          __half2 top = BitsHalf(0);
 #pragma unroll
-          for (int kt = 0; kt < C::MT; ++kt) {
-            uint32_t a[4][4];
-            VFragments<C>(a, vbase, kt, gp, magic);
+          for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              kt == 0 ? MmaFirst(part[i], a[i], b[kt][0][0], b[kt][1][0]) : Mma(part[i], a[i], b[kt][0][0], b[kt][1][0]);
-              if (!C::PACK) Mma(part[i], a[i], b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
+            for (int i = 0; i < 2; ++i) top = __hmax2(top, __habs2(BitsHalf(vsc[mt][i])));
+          }
+          const uint32_t u = HalfBits(top);
+          const uint32_t f16 = __reduce_max_sync(0xFFFFFFFFu, max(u & 0xFFFFu, u >> 16));
+          const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(f16)));
+          nu = max(nu, min(static_cast<int>(__float_as_uint(d) >> 23), 127 + 16) + 1);
+        }
+        const float shift = C::QUANT ? static_cast<float>(nu - 127 - kWeightBits) : -static_cast<float>(kWeightBits);
+        float2 top = s[0][0], now;
+#pragma unroll
+        for (int j = 1; j < 2 * C::MT; ++j) {
+          top.x = fmaxf(top.x, s[j >> 1][j & 1].x);
+          top.y = fmaxf(top.y, s[j >> 1][j & 1].y);
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, o));
+          top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, o));
+        }
+        m.x = fmaxf(m.x, top.x * cs.x);
+        m.y = fmaxf(m.y, top.y * cs.y);
+        now.x = (m.x == -INFINITY ? 0.f : m.x) + shift;
+        now.y = (m.y == -INFINITY ? 0.f : m.y) + shift;
+        alpha = make_float2(Exp2(ref.x - now.x), Exp2(ref.y - now.y));
+        ref.x = m.x == -INFINITY ? -INFINITY : now.x;
+        ref.y = m.y == -INFINITY ? -INFINITY : now.y;
+        l = Mul2(l, alpha);
+        const float2 less = make_float2(-now.x, -now.y);
+#pragma unroll
+        for (int j = 0; j < 2 * C::MT; ++j) {
+          const float2 e = Fma2(s[j >> 1][j & 1], cs, less);
+          const float2 w = make_float2(Exp2(e.x), Exp2(e.y));
+          s[j >> 1][j & 1] = w;
+          l = Add2(l, w);
+        }
+      }
+
+      // ---- values
+      if (work) {
+        if (!C::QUANT && edge) {  // what lies out of range may be anything, NaN too: zeros
+#pragma unroll 1
+          for (int i = lane; i < C::R * C::CPR; i += 32) {
+            const int r = i / C::CPR;
+            if (r < lo || r >= hi) Sts128Zero(vslot + ChunkAt<C, true>(r, i % C::CPR));
+          }
+          __syncwarp();
+        }
+        const uint32_t vbase = vslot + v_lane;
+        // the term that the lane's columns take
+        const float2 of_rest = Both(t >= 2 ? 1.f : 0.f), of_lead = Both(t >= 2 ? -1.f : 1.f);
+#pragma unroll
+        for (int gp = 0; gp < C::NG; ++gp) {
+          uint32_t b[C::MT][2][C::PACK ? 1 : 2];
+#pragma unroll
+          for (int mt = 0; mt < C::MT; ++mt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float2 u = s[mt][i];
+              if (C::QUANT) {
+                const float2 d = __half22float2(BitsHalf(vsc[mt][i]));
+                u = Mul2(u, Both(gp == 0 ? d.x : d.y));
+              }
+              // the first term is the leading 11 bits, the second the rest
+              const float2 h = make_float2(__uint_as_float(__float_as_uint(u.x) & 0xFFFFE000u),
+                                           __uint_as_float(__float_as_uint(u.y) & 0xFFFFE000u));
+              if (C::PACK) {
+                const float2 w = Fma2(u, of_rest, Mul2(h, of_lead));
+                b[mt][i][0] = Transposed(PackHalf(w.x, w.y));
+              } else {
+                b[mt][i][0] = Transposed(PackHalf(h.x, h.y));
+                b[mt][i][C::PACK ? 0 : 1] = Transposed(PackHalf(u.x - h.x, u.y - h.y));
+              }
             }
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              acc[4 * gp + i][c] = Fma2(acc[4 * gp + i][c], alpha, make_float2(part[i][2 * c], part[i][2 * c + 1]));
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            float part[4];
+          if (C::QUANT) {
+            float part[4][4];
 #pragma unroll
             for (int kt = 0; kt < C::MT; ++kt) {
-              uint32_t a[4];
-              LdMatrixT(a, Moved<C, true>(vbase, 16 * kt, 2 * i));
-              kt == 0 ? MmaFirst(part, a, b[kt][0][0], b[kt][1][0]) : Mma(part, a, b[kt][0][0], b[kt][1][0]);
-              if (!C::PACK) Mma(part, a, b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
+              uint32_t a[4][4];
+              VFragments<C>(a, vbase, kt, gp, magic);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                kt == 0 ? MmaFirst(part[i], a[i], b[kt][0][0], b[kt][1][0])
+                        : Mma(part[i], a[i], b[kt][0][0], b[kt][1][0]);
+                if (!C::PACK) Mma(part[i], a[i], b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
+              }
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) acc[i][c] = Fma2(acc[i][c], alpha, make_float2(part[2 * c], part[2 * c + 1]));
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                acc[4 * gp + i][c] = Fma2(acc[4 * gp + i][c], alpha, make_float2(part[i][2 * c], part[i][2 * c + 1]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              float part[4];
+#pragma unroll
+              for (int kt = 0; kt < C::MT; ++kt) {
+                uint32_t a[4];
+                LdMatrixT(a, Moved<C, true>(vbase, 16 * kt, 2 * i));
+                kt == 0 ? MmaFirst(part, a, b[kt][0][0], b[kt][1][0]) : Mma(part, a, b[kt][0][0], b[kt][1][0]);
+                if (!C::PACK) Mma(part, a, b[kt][0][C::PACK ? 0 : 1], b[kt][1][C::PACK ? 0 : 1]);
+              }
+#pragma unroll
+              for (int c = 0; c < 2; ++c) acc[i][c] = Fma2(acc[i][c], alpha, make_float2(part[2 * c], part[2 * c + 1]));
+            }
           }
         }
       }
-    }
-    __syncwarp();
-    fill.template Issue<true>(p, vslot, lane, lane_off);
-    bad_now = fill.Pop();
+      __syncwarp();
+      fill.template Issue<true>(p, vslot, lane, lane_off);
+      bad_now = fill.Pop();
     }
 
     // ---- the end of the item, or of this block's share of it
