@@ -1297,16 +1297,19 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
   LaunchKernelArgs(reinterpret_cast<const void*>(KvAttendKernel<C>), dim3(grid), dim3(C::THREADS), C::SMEM, s, true, a);
 }
 
-// Blocks of four warps that share an item, or of one: with at least as many
+// Blocks of four warps that share an item, or of one.  With about as many
 // items as warps that run at once, a warp for itself needs no barriers and
-// joins less.  256 conversations to 200 positions of 16 / 8 heads in 8 bits:
-// 40.0 us with four, 26.2 with one; 512 to 60 of 32 / 8 in 4 bits: 52.3 and
-// 27.8.  With few items a warp's records are many: one conversation of 65521
-// positions takes 36 us with four warps a block, 50 already with two.
+// joins less; with few, a warp's records are many.  32 / 8 heads, four warps
+// and one: 128 conversations to 100 positions in 8 bits 20.3 and 15.3 us, to
+// 2000 70 and 67, 96 to 400 25.0 and 23.1, 64 to 400 18.4 and 18.6, 32 to 100
+// 9.2 and 12.7.  In f16, where a step is shorter, 220 to 100 25.5 and 23.1, to
+// 400 47.0 and 47.7, to 2000 172 and 181, 128 to 400 31.7 and 33.1.  So half
+// the running warps' number of items is the border for codes, and their whole
+// number for f16.
 template <int D, KvType KIND, bool PACK>
 void ByItems(const KvAttendParams& p, int chunks, cudaStream_t s) {
   using One = Cfg<D, KIND, PACK, 1>;
-  if (static_cast<int64_t>(p.table.n_seq) * p.kv.n_kv * chunks >= Resident<One>()) {
+  if (static_cast<int64_t>(p.table.n_seq) * p.kv.n_kv * chunks >= Resident<One>() / (One::QUANT ? 2 : 1)) {
     Launch<One>(p, chunks, s);
   } else {
     Launch<Cfg<D, KIND, PACK, 4>>(p, chunks, s);
