@@ -3,8 +3,8 @@
 // Both are bound by memory and by the issue of what goes with it.  append
 // reads a q|k|v row and writes q and the cache: the 2811 rows of 16 / 8 heads
 // in f32 take 16.5 us (floor 12.5 us at the measured copy rate of 6.55 TB/s);
-// 10544 rows of 32 / 8 heads in f16 into 4 bits 55 us (35), where the norm,
-// the rotation and the codes keep the SMs issuing 77 % of the time.  gather
+// 10624 rows of 32 / 8 heads in f16 into 4 bits 51 us (35), where the norm,
+// the rotation and the codes keep the SMs issuing three quarters of the time.  gather
 // reads 41000 rows of 8 heads in 4 bits and writes them in f16 in 42.5 us
 // (33).  A single row takes 2 to 2.5 us on the GPU.
 #include <atomic>
@@ -16,7 +16,9 @@
 namespace rpgb {
 namespace {
 
-constexpr int kThreads = 128;
+// Threads of an append block: 10624 rows of 32 / 8 heads in f16 into 4 bits
+// take 51.1 us with 64, 53.4 with 128, 78.8 with 256.
+constexpr int kThreads = 64;
 
 template <KvType KIND>
 __host__ __device__ constexpr float MostCode() {
