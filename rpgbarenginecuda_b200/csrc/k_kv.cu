@@ -4,8 +4,8 @@
 // reads a q|k|v row and writes q and the cache: the 2811 rows of 16 / 8 heads
 // in f32 take 16.5 us (floor 12.5 us at the measured copy rate of 6.55 TB/s);
 // 10624 rows of 32 / 8 heads in f16 into 4 bits 51 us (35), where the norm,
-// the rotation and the codes keep the SMs issuing three quarters of the time.  gather
-// reads 41000 rows of 8 heads in 4 bits and writes them in f16 in 42.5 us
+// the rotation and the codes keep the SMs issuing three quarters of the time.
+// gather reads 41000 rows of 8 heads in 4 bits and writes them in f16 in 42 us
 // (33).  A single row takes 2 to 2.5 us on the GPU.
 #include <atomic>
 
@@ -270,12 +270,12 @@ __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
     t[r] = (static_cast<int64_t>(blockIdx.x) * kRows + r) * blockDim.z + threadIdx.z;
     pos[r] = -1;
     page[r] = -1;
-    if (t[r] < p.n_tok) pos[r] = __ldg(p.pos + t[r]);
+    if (t[r] < p.n_tok) pos[r] = p.pos[t[r]];
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     if (pos[r] >= 0) {
-      const int seq = p.seq != nullptr ? __ldg(p.seq + t[r]) : static_cast<int>(t[r]);
+      const int seq = p.seq != nullptr ? p.seq[t[r]] : static_cast<int>(t[r]);
       page[r] = kvd::PageOf(p.table, p.kv.n_pages, seq, pos[r] >> p.kv.page_log2);
     }
   }

@@ -274,8 +274,8 @@ template <typename C>
 __device__ __forceinline__ Span SpanOf(const KvAttendParams& p, int seq) {
   const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
   Span s;
-  s.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(p.lens + seq), 0)), cap));
-  s.start = p.starts != nullptr ? max(__ldg(p.starts + seq), 0) : 0;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(p.lens[seq], 0)), cap));
+  s.start = p.starts != nullptr ? max(p.starts[seq], 0) : 0;
   if (s.start >= s.len) s.start = s.len = 0;
   s.base = s.start & ~(C::R - 1);  // a step lies in one page, or its halves in two of 16
   s.tiles = max(1, (s.len - s.base + C::TILE - 1) / C::TILE);  // an empty item still writes its zeros
@@ -328,7 +328,7 @@ struct Filler {
     const int pos = Pos(c, warp, lane);
     // (positions in range lie inside the table: SpanOf)
     if (left > 0 && InRange(c, pos, lane)) {
-      page = __ldg(p.table.pages + c.seq * p.table.stride + (pos >> p.kv.page_log2));
+      page = p.table.pages[c.seq * p.table.stride + (pos >> p.kv.page_log2)];
     }
   }
   __device__ __forceinline__ void Batch(const KvAttendParams& p, int warp, int lane, int chunks) {
@@ -1072,7 +1072,7 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
       const bool whole = use.tile == 0 && n == use.span.tiles;
       const int queries = min(per_chunk, group - use.chunk * per_chunk);
       const int64_t out = use.seq * p.out_stride + (static_cast<int64_t>(use.head) * group + use.chunk * per_chunk) * D;
-      const bool past = static_cast<int64_t>(max(__ldg(p.lens + use.seq), 0)) >
+      const bool past = static_cast<int64_t>(max(p.lens[use.seq], 0)) >
                         (static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2);
       // The warps' shares joined: values 4 i .. 4 i + 3 of the item's queries.
       auto join = [&](int i, float& sum, float& top) {

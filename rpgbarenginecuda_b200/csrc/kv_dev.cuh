@@ -9,6 +9,10 @@
 #include "kernels.cuh"
 #include "kv.h"
 
+// The kernels of the paged cache start before the stream's previous kernel has
+// ended and wait for it; what it may have written is read by plain loads after
+// the wait, not by the read-only path, which promises nothing about such data.
+
 namespace rpgb {
 namespace kvd {
 
@@ -17,7 +21,7 @@ __device__ __forceinline__ float Nan() { return __uint_as_float(0x7FC00000u); }
 // Pool page of position `pos` of conversation `seq`, or -1 where the table has none.
 __device__ __forceinline__ int PageOf(const KvTable& t, int n_pages, int seq, int64_t page) {
   if (seq < 0 || seq >= t.n_seq || page >= t.max_pages) return -1;
-  const int id = __ldg(t.pages + seq * t.stride + page);
+  const int id = t.pages[seq * t.stride + page];
   return static_cast<unsigned>(id) < static_cast<unsigned>(n_pages) ? id : -1;
 }
 
