@@ -634,3 +634,37 @@ def test_a_conversation_step_by_step(kind, tol):
         scores = scores.masked_fill(~torch.tril(torch.ones(n, n, dtype=torch.bool)), float("-inf"))
         want = torch.einsum("hgtn,nhd->thgd", torch.softmax(scores, -1), qkv[:, n_heads + n_kv:]).reshape(n, -1)
         assert float((out[:, s].double().cpu() - want).abs().max()) <= tol * 3.5
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+def test_buffers_updated_in_place_between_calls(kind):
+    """200 steps on the same buffers, lengths, positions and rows updated by other kernels in between and nothing
+    waited for: each step sees what was written before it."""
+    n_seq, n_heads, n_kv, dim, steps = 40, 8, 2, 128, 200
+    pool = Pool(kind, [208] * n_seq, 16, n_kv=n_kv, dim=dim, seed=5)
+    cols = (n_heads + 2 * n_kv) * dim
+    x = torch.randn(steps, n_seq, cols, generator=torch.Generator().manual_seed(4)).cuda()
+    row = torch.empty(n_seq, cols, device="cuda")
+    pos, lens = i32([-1] * n_seq), i32([0] * n_seq)
+    ws = torch.zeros(rpg.attend_workspace(n_heads, n_kv, dim), dtype=torch.uint8, device="cuda")
+    out = torch.empty(n_seq, n_heads * dim, device="cuda")
+    kept = torch.empty(steps, n_seq, n_heads * dim, device="cuda")
+    for t in range(steps):
+        row.copy_(x[t])
+        pos += 1
+        lens += 1
+        pool.kv.append(pool.pt, None, rpg.F32, row.data_ptr(), n_heads, pos.data_ptr(), n_seq, row.data_ptr(),
+                       q_stride=cols)
+        pool.kv.attend(pool.pt, rpg.F32, row.data_ptr(), n_heads, lens.data_ptr(), dim ** -0.5, out.data_ptr(),
+                       ws.data_ptr(), ws.numel(), q_stride=cols)
+        kept[t].copy_(out)
+    torch.cuda.synchronize()
+    seq = [s for s in range(n_seq) for _ in range(steps)]
+    k, v = read(pool, seq, list(range(steps)) * n_seq)
+    k, v = (y.double().view(n_seq, steps, n_kv, dim).transpose(1, 2) for y in (k, v))
+    top = float(v.abs().max())
+    q = x[:, :, :n_heads * dim].double().cpu().view(steps, n_seq, n_kv, -1, dim)
+    for t in (0, 1, 15, 16, 63, 64, 127, 128, steps - 1):
+        w = torch.softmax(torch.einsum("shgd,shnd->shgn", q[t], k[:, :, :t + 1]) * dim ** -0.5, -1)
+        want = torch.einsum("shgn,shnd->shgd", w, v[:, :, :t + 1]).reshape(n_seq, -1)
+        assert float((kept[t].double().cpu() - want).abs().max()) <= 4e-5 * top, t
