@@ -232,7 +232,7 @@ RPGB_API float rpgb_counter_uniform(uint64_t seed, uint64_t counter);
 /* Pages of one layer.  head_dim is 64 or 128, page_size a power of two from
  * 16 to 4096.  Strides are in bytes: [page][kv head][position] of codes
  * (multiples of 16, at least a row: 2, 1 or 1/2 byte per value).  Quantised
- * caches have a scale d (f16) for every 64 values of a row, dense
+ * caches have a scale d (f16, finite or NaN) for every 64 values of a row, dense
  * [position][head_dim / 64] inside a head's page, with strides of their own.
  * k and v share the strides; k, v and the scales are 16-byte aligned. */
 typedef struct rpgb_kv_pages {
@@ -285,7 +285,13 @@ RPGB_API int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* ta
  * softmax(scale q K^T) V per head over positions [starts_dev[s], lens_dev[s])
  * of conversation s (starts_dev NULL: from 0; pages wholly before the start
  * are not looked at).  An empty range gives zeros.  n_heads is any multiple
- * of n_kv; q head h reads KV head h / (n_heads / n_kv).  The sums are in f32.
+ * of n_kv; q head h reads KV head h / (n_heads / n_kv).  The sums are in f32;
+ * q is held to 2^-24 of its head's largest value.  A q head that holds a NaN
+ * or an infinity gives NaN.  Infinities and NaN in the range count as the
+ * formula in f32 has them: a score of minus infinity drops its position, a NaN
+ * or plus infinity makes the head's row NaN, an infinite value its dimension
+ * infinite; a range with no score above minus infinity gives zeros, as an
+ * empty one.
  * workspace_dev: rpgb_kv_attend_workspace bytes (or more), 256-byte aligned,
  * zeroed once before its first use; calls of any shapes may follow one another
  * on it, calls that may overlap need one each. */

@@ -47,6 +47,8 @@
 //    product starts from zero and is added to the running output in f32
 //    registers: the tensor cores truncate when they add, which would grow over
 //    a long conversation.
+//  * Infinities in an f16 cache give what the formula gives in f32: a warp
+//    whose share came out NaN does it again without splits (PlainShare).
 //
 // Measured on one B200 (floor: bytes at the measured copy rate of 6.55 TB/s):
 // 32 conversations of 32 / 8 heads to 8192 positions in f16 107 us (104.5),
@@ -624,6 +626,64 @@ __device__ __forceinline__ void AddScaled(float4& v, float f, const float4& x) {
   v.w += f * x.w;
 }
 
+// A warp's share of an item (its rows of n tiles from c's) by the formula as
+// it stands: one value at a time in f32.  With an f16 cache the split terms of
+// q and of the weights give the formula's results for finite values only
+// (infinity times a term that is zero, or times terms of both signs, is NaN),
+// so a share that came out NaN is done again here; its vectors, maxima and
+// sums replace the first ones.  (A quantised cache holds no infinity, and a
+// NaN is its group's scale.)
+template <typename C>
+__device__ __forceinline__ void PlainShare(const KvAttendParams& p, const Cursor<C>& c, int n, int warp, int lane,
+                                           int64_t q_row, int queries, float* vec, float* maxima, float* sums) {
+  constexpr int N = C::D / 32;  // values of a lane
+  using Row = kvd::Pack<__half, N>;
+#pragma unroll 1
+  for (int qi = 0; qi < queries; ++qi) {
+    const int64_t o = q_row + static_cast<int64_t>(qi) * C::D + lane * N;
+    float x[N], acc[N] = {}, m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      switch (p.type) {
+        case ElemType::kF32: x[e] = static_cast<const float*>(p.q)[o + e]; break;
+        case ElemType::kF16: x[e] = kvd::ToFloat(static_cast<const __half*>(p.q)[o + e]); break;
+        case ElemType::kBF16: x[e] = kvd::ToFloat(static_cast<const __nv_bfloat16*>(p.q)[o + e]); break;
+      }
+      l += x[e] * 0.f;  // NaN with a NaN or an infinity in q
+    }
+    l = dev::WarpSum(l);
+#pragma unroll 1
+    for (int k = 0; k < n * C::R && l == l; ++k) {
+      const int pos = c.span.base + (c.tile + k / C::R) * C::TILE + warp * C::R + k % C::R;
+      if (pos < c.span.start || pos >= c.span.len) continue;
+      const int page = kvd::PageOf(p.table, p.kv.n_pages, c.seq, pos >> p.kv.page_log2);
+      if (page < 0) {
+        l = kvd::Nan();
+        break;
+      }
+      const int64_t at =
+          kvd::CodeOffset(p.kv, page, c.head, pos & ((1 << p.kv.page_log2) - 1)) + lane * static_cast<int>(sizeof(Row));
+      const Row kr = *reinterpret_cast<const Row*>(p.kv.k + at), vr = *reinterpret_cast<const Row*>(p.kv.v + at);
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) dot += x[e] * __half2float(kr.v[e]);
+      const float s = dev::WarpSum(dot) * (p.scale * kLog2e);
+      const float now = fmaxf(m, s), ref = now == -INFINITY ? 0.f : now;
+      const float alpha = Exp2(m - ref), w = Exp2(s - ref);
+      m = now;
+      l = l * alpha + w;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = acc[e] * alpha + w * __half2float(vr.v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) vec[qi * C::D + lane * N + e] = l == l ? acc[e] : l;
+    if (lane == 0) {
+      maxima[qi] = m;
+      sums[qi] = l;
+    }
+  }
+}
+
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const KvAttendParams p) {
   constexpr int D = C::D;
@@ -1044,6 +1104,7 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         l.x += __shfl_xor_sync(0xFFFFFFFFu, l.x, o);
         l.y += __shfl_xor_sync(0xFFFFFFFFu, l.y, o);
       }
+      float2 any = l;  // NaN where one of the lane's results is
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
@@ -1053,6 +1114,7 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
             v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, 2);
             v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, 2);
           }
+          if (!C::QUANT) any = Add2(any, v);
           const int value = C::QUANT ? 64 * (i >> 2) + 8 * g + 4 * c + (i & 3) : 16 * i + 8 * c + g;
           if (!C::PACK || t < 2) {
             mineq[2 * t * D + value] = v.x;
@@ -1065,6 +1127,13 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         s_m[warp][2 * t + 1] = ref.y;
         s_l[warp][2 * t] = l.x;
         s_l[warp][2 * t + 1] = l.y;
+      }
+      if (!C::QUANT && __any_sync(0xFFFFFFFFu, !(any.x == any.x && any.y == any.y))) {
+        const Cursor<C> c = s_use[warp];
+        const int first = c.chunk * per_chunk;
+        __syncwarp();
+        PlainShare(p, c, n, warp, lane, c.seq * p.q_stride + (static_cast<int64_t>(c.head) * group + first) * D,
+                   min(per_chunk, group - first), mineq, s_m[warp], s_l[warp]);
       }
       __syncthreads();
       const Cursor<C> use = s_use[warp];
