@@ -265,7 +265,8 @@ typedef struct rpgb_kv_rotary {
  * pos_dev[t] (value j of a head pairs with j + head_dim / 2); k and v go to
  * that position of conversation seq_dev[t] (seq_dev NULL: row t belongs to
  * conversation t), q to q_out_dev in the rows' type (NULL: not wanted; it may
- * be the q part of qkv_dev itself).  A quantised cache rounds to the nearest
+ * be the q part of qkv_dev itself).  An f16 cache rounds to f16, magnitudes
+ * from 65520 on to infinity.  A quantised cache rounds to the nearest
  * code of d = f16(max |x| * (1 / 127) or (1 / 7)); magnitudes past 127 or 7 times 65504
  * saturate, a group that holds a NaN reads back as NaN.  Rows must not name
  * the same position twice.  rotary NULL: k and q go through as they are. */

@@ -9,6 +9,8 @@ half a unit of the output type.
 
 import pytest
 
+import rpgbarenginecuda_b200 as rpg
+
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
@@ -122,3 +124,18 @@ def test_nan_scales_of_a_quantised_cache(kind, group):
         fine = torch.isfinite(got[i])
         assert int(fine.sum()) == group * (128, 192, 256)[i]
         assert float((got[i].double() - want).abs()[fine].max()) <= 4e-5 * top
+
+def test_append_of_values_past_f16():
+    """The f16 cache rounds as f16 does: past 65504 to infinity; the quantised ones saturate."""
+    for kind, most in (("f16", INF), ("q8", 127 * 65504.0), ("q4", 7 * 65504.0)):
+        pool = Pool(kind, [16], 16, n_kv=1, dim=64, seed=1)
+        x = torch.ones(1, 128, device="cuda")
+        x[0, 3], x[0, 70], x[0, 71] = 1e9, -1e9, 65504.0
+        pos = torch.tensor([4], dtype=torch.int32, device="cuda")
+        pool.kv.append(pool.pt, None, rpg.F32, x.data_ptr(), 0, pos.data_ptr(), 1)
+        k, v = (torch.empty(1, 64, device="cuda") for _ in range(2))
+        pool.kv.gather(pool.pt, rpg.F32, pos.data_ptr(), 1, k.data_ptr(), v.data_ptr())
+        torch.cuda.synchronize()
+        assert float(k[0, 3]) == most and float(v[0, 6]) == -most
+        if kind == "f16":
+            assert float(v[0, 7]) == 65504.0
