@@ -264,12 +264,18 @@ typedef struct rpgb_kv_rotary {
  * heads.  The q and k heads are normalised and rotated for position
  * pos_dev[t] (value j of a head pairs with j + head_dim / 2); k and v go to
  * that position of conversation seq_dev[t] (seq_dev NULL: row t belongs to
- * conversation t), q to q_out_dev in the rows' type (NULL: not wanted; it may
- * be the q part of qkv_dev itself).  An f16 cache rounds to f16, magnitudes
- * from 65520 on to infinity.  A quantised cache rounds to the nearest
- * code of d = f16(max |x| * (1 / 127) or (1 / 7)); magnitudes past 127 or 7 times 65504
- * saturate, a group that holds a NaN reads back as NaN.  Rows must not name
- * the same position twice.  rotary NULL: k and q go through as they are. */
+ * conversation t).  Norm and rotation are f32 operations that round one by one:
+ * (x * r) * w with r the reciprocal root of (sum of squares) * (1 / head_dim) +
+ * eps, then a cos - b sin and b cos + a sin.  The squares are added in a fixed
+ * order, so that the codes do not depend on the batch: head_dim 128 in runs of
+ * four values from the left, then runs 64, 32, 16, 8 and 4 values apart;
+ * head_dim 64 values 32, 16, 8, 4, 2 and 1 apart.  q goes to q_out_dev in the
+ * rows' type (NULL: not wanted; it may be the q part of qkv_dev itself).  An
+ * f16 cache rounds to f16, magnitudes from 65520 on to infinity.  A quantised
+ * cache rounds to the nearest code of d = f16(max |x| * (1 / 127) or (1 / 7));
+ * magnitudes past 127 or 7 times 65504 saturate, a group that holds a NaN reads
+ * back as NaN.  Rows must not name the same position twice.  rotary NULL: k and
+ * q go through as they are. */
 RPGB_API int32_t rpgb_kv_append(const rpgb_kv_pages* kv, const rpgb_kv_table* table, const rpgb_kv_rotary* rotary,
                                 int32_t type, const void* qkv_dev, int64_t qkv_stride, int32_t n_heads,
                                 const int32_t* seq_dev, const int32_t* pos_dev, int64_t n_tok, void* q_out_dev,

@@ -92,7 +92,11 @@ __device__ __forceinline__ void StoreCodes(char* row, int i, const float (&x)[8]
 }
 
 // 1 / sqrt(mean x^2 + eps) of a head, in f32.  The squares and sums round one
-// by one (no fused multiply-add) in a fixed tree.
+// by one (no fused multiply-add), in an order that is part of the operator's
+// definition: it decides the code of a value that falls beside a rounding
+// boundary (a sum from the left gives another 8-bit code for 5 values in a
+// million).  The orders are those of torch.mean over rows of 64 and of 128 on
+// this GPU, so that codes can be held against an evaluation there.
 template <int D>
 __device__ __forceinline__ float InvRms(const float (&a)[8], const float (&b)[8], float eps) {
   float s;
@@ -134,8 +138,8 @@ __device__ __forceinline__ float InvRms(const float (&a)[8], const float (&b)[8]
 // first half (a) and of the second (b), so a rotation pair (j, j + D / 2) sits
 // in one lane and a scale group of 64 values in the same lanes; the rotation
 // stays in registers for all heads.  Norm and rotation round every product and
-// sum on its own, so a value that falls near a rounding boundary of the cache
-// gets the code of the formulas evaluated step by step in f32.
+// sum on its own, in the order of InvRms and of the formulas as written, so
+// equal rows get equal codes whatever the launch.
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams p) {
   constexpr int L = D / 16, kHeads = kThreads / L;

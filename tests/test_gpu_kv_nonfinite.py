@@ -125,6 +125,7 @@ def test_nan_scales_of_a_quantised_cache(kind, group):
         assert int(fine.sum()) == group * (128, 192, 256)[i]
         assert float((got[i].double() - want).abs()[fine].max()) <= 4e-5 * top
 
+
 def test_append_of_values_past_f16():
     """The f16 cache rounds as f16 does: past 65504 to infinity; the quantised ones saturate."""
     for kind, most in (("f16", INF), ("q8", 127 * 65504.0), ("q4", 7 * 65504.0)):
