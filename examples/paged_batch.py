@@ -137,20 +137,24 @@ class PagedModel:
         del self.lengths[c]
 
     def forward(self, tokens: list[tuple[int, int]]) -> torch.Tensor:
-        """Appends (conversation, token id) rows, in order, and returns their logits [row][vocabulary]."""
-        seq, pos = [], []
+        """Appends (conversation, token id) rows, in order, and returns their logits [row][vocabulary].
+
+        A call that raises leaves the conversations as they were."""
+        seq, pos, lengths, places = [], [], dict(self.lengths), self.table.copy()
+        taken = 0
         for c, _ in tokens:
-            p = self.lengths[c]
-            if p // self.page >= self.max_pages or (p % self.page == 0 and not self.free):
+            p = lengths[c]
+            if p // self.page >= self.max_pages or (p % self.page == 0 and taken == len(self.free)):
                 raise RuntimeError(f"no page for position {p} of conversation {c}")
             if p % self.page == 0:
-                self.table[c, p // self.page] = self.free.pop()
+                taken += 1
+                places[c, p // self.page] = self.free[-taken]
             seq.append(c)
             pos.append(p)
-            self.lengths[c] = p + 1
+            lengths[c] = p + 1
         n = len(tokens)
         # every row has its own page list and length: a prompt's rows see what comes before them
-        table = torch.from_numpy(self.table[seq]).cuda()
+        table = torch.from_numpy(places[seq]).cuda()
         pages = rpg.PageTable(table.data_ptr(), n, self.max_pages)
         pos = torch.tensor(pos, dtype=torch.int32, device="cuda")
         lens = pos + 1
@@ -178,7 +182,10 @@ class PagedModel:
             y = norm(x, w["ffn_norm"])
             h = torch.nn.functional.silu(product(w["ffn_gate"], y)) * product(w["ffn_up"], y)
             x = x + product(w["ffn_down"], h)
-        return product(self.head, norm(x, self.out_norm))
+        logits = product(self.head, norm(x, self.out_norm))
+        del self.free[len(self.free) - taken:]
+        self.table, self.lengths = places, lengths
+        return logits
 
 
 def main(argv=None):

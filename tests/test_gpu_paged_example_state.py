@@ -49,37 +49,3 @@ def test_a_bad_token_changes_nothing(tiny_model):
         m.forward(rows(0, 15, 2) + [(0, m.embd.rows)])
     assert state(m) == before
     assert torch.equal(m.forward(rows(0, 3, 3)), calm.forward(rows(0, 3, 3)))
-
-
-def test_the_last_position(tiny_model):
-    """max_positions that is no multiple of the page: all of them work, the next one raises."""
-    m = model(tiny_model, n_pages=10, max_positions=50)
-    a = m.open()
-    logits = m.forward(rows(a, 49, 1))
-    assert torch.isfinite(logits).all()
-    assert torch.isfinite(m.forward(rows(a, 1, 2))).all()
-    before = state(m)
-    with pytest.raises(RuntimeError, match="full"):
-        m.forward(rows(a, 1, 3))
-    assert state(m) == before
-
-
-def test_all_conversations_open(tiny_model):
-    m = model(tiny_model)
-    m.open(), m.open()
-    with pytest.raises(RuntimeError, match="open"):
-        m.open()
-    m.close(1)
-    assert m.open() == 1
-
-
-def test_on_another_stream(tiny_model):
-    m, calm = model(tiny_model), model(tiny_model)
-    a = (m.open(), calm.open())[0]
-    side = torch.cuda.Stream()
-    for n in (30, 1, 1, 9):
-        want = calm.forward(rows(a, n, n))
-        with torch.cuda.stream(side):
-            got = m.forward(rows(a, n, n))
-        side.synchronize()
-        assert torch.equal(got, want)
