@@ -89,7 +89,7 @@ class PagedModel:
         g = lambda key: meta[f"{arch}.{key}"]  # noqa: E731
         self.n_layers, self.n_heads, self.n_kv = g("block_count"), g("attention.head_count"), g("attention.head_count_kv")
         self.dim, self.eps = g("attention.key_length"), g("attention.layer_norm_rms_epsilon")
-        self.page, self.max_pages = page, -(-max_positions // page)
+        self.page, self.max_pages, self.max_positions = page, -(-max_positions // page), max_positions
 
         def matrix(name):
             kind, (cols, rows), data = tensors[name]
@@ -144,7 +144,9 @@ class PagedModel:
         taken = 0
         for c, _ in tokens:
             p = lengths[c]
-            if p // self.page >= self.max_pages or (p % self.page == 0 and taken == len(self.free)):
+            if p >= self.max_positions:  # (the rotation table ends there)
+                raise RuntimeError(f"conversation {c} is full ({p} positions)")
+            if p % self.page == 0 and taken == len(self.free):
                 raise RuntimeError(f"no page for position {p} of conversation {c}")
             if p % self.page == 0:
                 taken += 1

@@ -49,3 +49,16 @@ def test_a_bad_token_changes_nothing(tiny_model):
         m.forward(rows(0, 15, 2) + [(0, m.embd.rows)])
     assert state(m) == before
     assert torch.equal(m.forward(rows(0, 3, 3)), calm.forward(rows(0, 3, 3)))
+
+
+def test_the_last_position(tiny_model):
+    """max_positions that is no multiple of the page: all of them work, the next one raises."""
+    m = model(tiny_model, n_pages=10, max_positions=50)
+    a = m.open()
+    logits = m.forward(rows(a, 49, 1))
+    assert torch.isfinite(logits).all()
+    assert torch.isfinite(m.forward(rows(a, 1, 2))).all()
+    before = state(m)
+    with pytest.raises(RuntimeError, match="full"):
+        m.forward(rows(a, 1, 3))
+    assert state(m) == before
