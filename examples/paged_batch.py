@@ -126,7 +126,9 @@ class PagedModel:
 
     def open(self) -> int:
         """A new conversation."""
-        c = next(i for i in range(len(self.table)) if i not in self.lengths)
+        c = next((i for i in range(len(self.table)) if i not in self.lengths), None)
+        if c is None:
+            raise RuntimeError(f"all {len(self.table)} conversations are open")
         self.lengths[c] = 0
         return c
 

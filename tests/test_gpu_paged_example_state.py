@@ -62,3 +62,12 @@ def test_the_last_position(tiny_model):
     with pytest.raises(RuntimeError, match="full"):
         m.forward(rows(a, 1, 3))
     assert state(m) == before
+
+
+def test_all_conversations_open(tiny_model):
+    m = model(tiny_model)
+    m.open(), m.open()
+    with pytest.raises(RuntimeError, match="open"):
+        m.open()
+    m.close(1)
+    assert m.open() == 1
