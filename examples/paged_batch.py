@@ -123,6 +123,7 @@ class PagedModel:
         self.lengths: dict[int, int] = {}
         self.workspace = torch.zeros(rpg.attend_workspace(self.n_heads, self.n_kv, self.dim), dtype=torch.uint8,
                                      device="cuda")
+        torch.cuda.synchronize()  # forward may come on another stream
 
     def open(self) -> int:
         """A new conversation."""
@@ -141,7 +142,8 @@ class PagedModel:
     def forward(self, tokens: list[tuple[int, int]]) -> torch.Tensor:
         """Appends (conversation, token id) rows, in order, and returns their logits [row][vocabulary].
 
-        A call that raises leaves the conversations as they were."""
+        Runs on torch's current stream.  A call that raises leaves the conversations as they were."""
+        stream = torch.cuda.current_stream().cuda_stream
         seq, pos, lengths, places = [], [], dict(self.lengths), self.table.copy()
         taken = 0
         for c, _ in tokens:
@@ -164,11 +166,11 @@ class PagedModel:
         lens = pos + 1
         x = torch.empty(n, self.embd.cols, device="cuda")
         for i, (_, token) in enumerate(tokens):
-            self.embd.dequant(token, 1, x[i].data_ptr())
+            self.embd.dequant(token, 1, x[i].data_ptr(), stream)
 
         def product(m, y):
             out = torch.empty(n, m.rows, device="cuda")
-            m.matvec(y.data_ptr(), n, out.data_ptr())
+            m.matvec(y.data_ptr(), n, out.data_ptr(), stream)
             return out
 
         def norm(y, w):
@@ -179,9 +181,10 @@ class PagedModel:
         for w in self.layers:
             y = norm(x, w["attn_norm"])
             qkv = torch.cat([product(w[m], y) for m in ("attn_q", "attn_k", "attn_v")], 1)
-            w["kv"].append(pages, w["rotary"], rpg.F32, qkv.data_ptr(), self.n_heads, pos.data_ptr(), n, q.data_ptr())
+            w["kv"].append(pages, w["rotary"], rpg.F32, qkv.data_ptr(), self.n_heads, pos.data_ptr(), n, q.data_ptr(),
+                           stream=stream)
             w["kv"].attend(pages, rpg.F32, q.data_ptr(), self.n_heads, lens.data_ptr(), self.dim ** -0.5, att.data_ptr(),
-                           self.workspace.data_ptr(), self.workspace.numel())
+                           self.workspace.data_ptr(), self.workspace.numel(), stream=stream)
             x = x + product(w["attn_output"], att)
             y = norm(x, w["ffn_norm"])
             h = torch.nn.functional.silu(product(w["ffn_gate"], y)) * product(w["ffn_up"], y)

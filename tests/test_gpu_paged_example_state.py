@@ -71,3 +71,15 @@ def test_all_conversations_open(tiny_model):
         m.open()
     m.close(1)
     assert m.open() == 1
+
+
+def test_on_another_stream(tiny_model):
+    m, calm = model(tiny_model), model(tiny_model)
+    a = (m.open(), calm.open())[0]
+    side = torch.cuda.Stream()
+    for n in (30, 1, 1, 9):
+        want = calm.forward(rows(a, n, n))
+        with torch.cuda.stream(side):
+            got = m.forward(rows(a, n, n))
+        side.synchronize()
+        assert torch.equal(got, want)
