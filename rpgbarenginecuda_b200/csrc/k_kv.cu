@@ -251,7 +251,9 @@ __global__ void __launch_bounds__(kThreads) KvAppendKernel(const KvAppendParams 
 // Sixteen consecutive values of one head's k or v row per thread and row; the
 // block's threads cover (values of a head) x (k heads, then v heads) x (rows),
 // and each takes kRows rows of every blockDim.z at once, so that their chains
-// of loads (position, page, codes) run side by side.
+// of loads (position, page, codes) run side by side.  41000 rows of 8 heads to
+// f16 with one row a thread, two and four: f16 63.9, 56.2 and 54.5 us, 8 bits
+// 58.8, 56.2 and 62.7, 4 bits 55.8, 41.7 and 41.7; 40 rows 1.8, 2.1 and 2.5.
 constexpr int kRows = 2;
 template <int D, KvType KIND, typename T>
 __global__ void __launch_bounds__(256) KvGatherKernel(const KvGatherParams p) {
@@ -349,24 +351,35 @@ int NumSms() {
   return n;
 }
 
+// While all blocks run at once (32 to an SM), a row's heads go to blocks of
+// their own (latency); past that a block keeps its row's rotation for all its
+// heads.  Rows of 32 / 8 heads in f16 to f16, a row in blocks of 8 heads and in
+// one: 1 row 1.7 and 3.8 us, 300 3.2 and 5.3, 600 4.6 and 7.6, 1200 10.1 and
+// 9.3, 9600 62 and 44; of 16 / 2 heads in f32 to 4 bits 1200 rows 7.1 and 7.6,
+// 2400 13.5 and 13.3; the border is at 789 and at 1578 rows.
 template <int D, KvType KIND, typename T>
 struct Append {
   static void Run(const KvAppendParams& p, cudaStream_t s) {
     constexpr int kHeads = kThreads / (D / 16);
     const int heads = (p.q_out != nullptr ? p.n_heads : 0) + 2 * p.kv.n_kv;
-    // few rows: their heads go to blocks of their own (latency); many: a block keeps its row's rotation
     const int parts = (heads + kHeads - 1) / kHeads;
-    const dim3 grid(static_cast<unsigned>(p.n_tok), p.n_tok * parts <= 4 * NumSms() ? parts : 1);
+    const dim3 grid(static_cast<unsigned>(p.n_tok), p.n_tok * parts <= 32 * NumSms() ? parts : 1);
     LaunchKernelArgs(reinterpret_cast<const void*>(KvAppendKernel<D, KIND, T>), grid, dim3(kThreads), 0, s, true, p);
   }
 };
+
+// While about all blocks run at once (24 to an SM), a block takes kRows rows;
+// past that as many more as fit its threads.  Rows of 2 heads from 8 to 16
+// bits: 600 rows 2.3 and 2.6 us, 6000 3.4 and 3.7, 7000 4.0 and 3.7, 12000 6.7
+// and 4.9, 41000 24.9 and 16.7; to f32 7000 5.3 and 7.3, 12000 9.7 and 8.8; the
+// border is at 7104 rows.  (8 heads fill a block's threads either way.)
 template <int D, KvType KIND, typename T>
 struct Gather {
   static void Run(const KvGatherParams& p, cudaStream_t s) {
     constexpr int L = D / 16;
     const int heads = 2 * p.kv.n_kv, y = heads < 256 / L ? heads : 256 / L;
-    // few rows: a block takes kRows at most; many: as many as fit its threads
-    const int64_t fit = 256 / (L * y), z = p.n_tok < 2 * NumSms() ? 1 : fit;
+    const int64_t blocks = (p.n_tok + kRows - 1) / kRows * ((heads + y - 1) / y);
+    const int64_t z = blocks <= 24 * NumSms() ? 1 : 256 / (L * y);
     const dim3 block(L, y, static_cast<unsigned>(z));
     const dim3 grid(static_cast<unsigned>((p.n_tok + kRows * z - 1) / (kRows * z)), (heads + y - 1) / y);
     LaunchKernelArgs(reinterpret_cast<const void*>(KvGatherKernel<D, KIND, T>), grid, block, 0, s, true, p);
