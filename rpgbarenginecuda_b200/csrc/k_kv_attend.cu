@@ -84,7 +84,11 @@ struct Cfg {
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;  // 16-byte chunks of a row
-  static constexpr int LEAST = 2;  // tiles (borders included) a block is started for
+  // Tiles (borders included) a block is started for.  One conversation of 16 /
+  // 8 heads in f16 with 1, 2, 3 and 4: 100 positions 7.0, 6.1, 7.0 and 6.0 us,
+  // 300 8.2, 7.5, 8.0 and 10.4, 2851 11.8, 10.8, 11.3 and 13.4; of 32 / 8 heads
+  // in 8 bits to 500 8.3, 9.1, 12.0 and 13.6.
+  static constexpr int LEAST = 2;
   // the end of an item costs a block about as much as so many tiles
   static constexpr int BORDER = (QUANT ? 1 : 2) * (WARPS == 1 ? 2 : 1);
   static constexpr int SC = QUANT ? R * NG * 2 : 0;  // scales of a step
@@ -1197,7 +1201,12 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         if (finish && tid == 0) *count = 0;
         constexpr int kFew = 4;
         if (finish && b1 - b0 < kFew) {
-          // Few records: every thread reads what it needs of all of them at once.
+          // Few records: every thread reads what it needs of all of them at
+          // once.  Against the join below: one conversation of 16 / 8 heads to
+          // 300 in f16 7.5 and 8.5 us, of 32 / 8 to 500 in 8 bits 9.1 and 10.0,
+          // 64 to 4096 in 4 bits 56.3 and 57.6.  (Up to eight records so: 8 of
+          // 64 / 8 heads to 1000 in f16 11.5 us against 13.2, but 11.1 against
+          // 10.8 for one of 16 / 8 to 2851, for the registers it takes.)
           finish = false;
           for (int i = tid; i < vecs; i += C::THREADS) {
             const int q = 4 * i / D;
@@ -1374,7 +1383,12 @@ void Launch(const KvAttendParams& p, int chunks, cudaStream_t s) {
 // 9.2 and 12.7.  In f16, where a step is shorter, 220 to 100 25.5 and 23.1, to
 // 400 47.0 and 47.7, to 2000 172 and 181, 128 to 400 31.7 and 33.1.  So half
 // the running warps' number of items is the border for codes, and their whole
-// number for f16.
+// number for f16.  Other layouts, 220 conversations of 40 / 8 heads: in 8 bits
+// to 400 58 and 38, to 2000 130 and 113, in f16 to 400 56 and 50, to 2000 182
+// and 183; 96 in 4 bits to 400 26 and 23; 192 of 24 / 4 heads of 64 in 8 bits
+// to 400 18.3 and 17.8, 320 25 and 22.  Near the border short conversations
+// would take one warp earlier (160 to 100 of 8 / 8 heads of 64 in f16 15.3 and
+// 10.3) and long ones later (192 to 2000 of 24 / 4 in f16 45.5 and 49.4).
 template <int D, KvType KIND, bool PACK>
 void ByItems(const KvAttendParams& p, int chunks, cudaStream_t s) {
   using One = Cfg<D, KIND, PACK, 1>;
