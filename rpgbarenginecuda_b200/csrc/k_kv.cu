@@ -6,7 +6,7 @@
 // 10624 rows of 32 / 8 heads in f16 into 4 bits 51 us (35), where the norm,
 // the rotation and the codes keep the SMs issuing three quarters of the time.
 // gather reads 41000 rows of 8 heads in 4 bits and writes them in f16 in 42 us
-// (33).  A single row takes 2 to 2.5 us on the GPU.
+// (33).  A single row takes 1.7 to 2.4 us on the GPU (calls in a graph).
 #include <atomic>
 
 #include "common.h"
@@ -351,7 +351,7 @@ int NumSms() {
   return n;
 }
 
-// While all blocks run at once (32 to an SM), a row's heads go to blocks of
+// Up to 32 blocks for every SM (14 run at once) a row's heads go to blocks of
 // their own (latency); past that a block keeps its row's rotation for all its
 // heads.  Rows of 32 / 8 heads in f16 to f16, a row in blocks of 8 heads and in
 // one: 1 row 1.7 and 3.8 us, 300 3.2 and 5.3, 600 4.6 and 7.6, 1200 10.1 and
@@ -368,8 +368,8 @@ struct Append {
   }
 };
 
-// While about all blocks run at once (24 to an SM), a block takes kRows rows;
-// past that as many more as fit its threads.  Rows of 2 heads from 8 to 16
+// Up to 24 blocks for every SM a block takes kRows rows; past that as many more
+// as fit its threads.  Rows of 2 heads from 8 to 16
 // bits: 600 rows 2.3 and 2.6 us, 6000 3.4 and 3.7, 7000 4.0 and 3.7, 12000 6.7
 // and 4.9, 41000 24.9 and 16.7; to f32 7000 5.3 and 7.3, 12000 9.7 and 8.8; the
 // border is at 7104 rows.  (8 heads fill a block's threads either way.)

@@ -23,11 +23,11 @@
 //    asynchronous copies: the next step's K while this step's V is at work and
 //    the other way round, across item borders.  (One step ahead is enough: 12
 //    warps keep about 100 KB in flight per SM; two steps ahead took 119 us
-//    where one takes 113.)  Page lookups and offsets of up to 16 steps are
-//    worked out at once, one 16-position half per lane.  Positions out of
-//    range are not used whatever they hold: their scores become -infinity,
-//    their V scales or rows zero.  16-byte chunks are permuted so that every
-//    read of a tile is free of bank conflicts.
+//    where one takes 113.)  Page lookups and offsets of up to 32 steps of 16
+//    positions, 16 of 32, are worked out at once, one 16-position half per
+//    lane.  Positions out of range are not used whatever they hold: their
+//    scores become -infinity, their V scales or rows zero.  16-byte chunks are
+//    permuted so that every read of a tile is free of bank conflicts.
 //  * Math.  S^T = K q^T and O^T += V^T P^T on mma.sync with the positions (S)
 //    or value dimensions (O) as the 16 rows and 8 query columns, so 2 to 8
 //    query heads waste little.  tcgen05 has 128 rows for a query side of 8 and
@@ -53,9 +53,11 @@
 // Measured on one B200 (floor: bytes at the measured copy rate of 6.55 TB/s):
 // 32 conversations of 32 / 8 heads to 8192 positions in f16 107 us (104.5),
 // 16 to 3840 in 8 bits 25 us (12.9), one of 65521 in 8 bits 36 us (21.2), 64
-// to 4096 in 4 bits 56 us (27.7), one of 21 positions of 16 / 8 heads 6 us.  A
-// launch costs about 4 us before its first data (lengths, pages, data: three
-// round trips) and 3 us after its last.
+// to 4096 in 4 bits 56 us (27.7), one of 21 positions of 16 / 8 heads 5.4 us.
+// Between 4096 and 16384 positions the time grows as the floor does in f16 and
+// 8 bits and 1.5 times as fast in 4 bits; the line through these times leaves
+// 8 us for no data in f16, 13 in 8 and 4 bits and 15 for one conversation: the
+// start (lengths, pages, data: three round trips) and the joins.
 #include <atomic>
 
 #include "common.h"
@@ -107,9 +109,11 @@ struct Cfg {
   static constexpr int QWORDS = QUANT ? 4 * NG : 2 * KS;  // of a lane and tile
   static constexpr int QBYTES = QTILES * QWORDS * 128;
   static constexpr int SMEM = WARPS * RING + JOIN + QBYTES;
-  // Resident per SM: 12 warps where registers allow (168 a thread).  With 64
-  // conversations to 16384 in 4 bits, 8 warps take 187 us, 12 take 175 and 16
-  // (128 registers, which spill) 185.
+  // Resident per SM: 12 warps where registers allow (168 a thread; of these
+  // the 8-bit form for up to 4 queries of 128 values spills 4 or 5), 8 for more
+  // queries of 128 values (200 to 223).  With 64 conversations to 16384 in 4
+  // bits, 8 warps take 187 us, 12 take 175 and 16 (128 registers, which spill)
+  // 185.
   static constexpr int BLOCKS = (PACK || D == 64 ? 12 : 8) / WARPS;
 };
 
