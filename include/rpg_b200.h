@@ -293,7 +293,7 @@ RPGB_API int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* ta
  * of conversation s (starts_dev NULL: from 0; pages wholly before the start
  * are not looked at).  An empty range gives zeros.  n_heads is any multiple
  * of n_kv; q head h reads KV head h / (n_heads / n_kv).  The sums are in f32;
- * q is held to 2^-24 of its head's largest value.  A q head that holds a NaN
+ * q is held to 2^-23 of its head's largest value.  A q head that holds a NaN
  * or an infinity gives NaN.  Infinities and NaN in the range count as the
  * formula in f32 has them: a score of minus infinity drops its position, a NaN
  * or plus infinity makes the head's row NaN, an infinite value its dimension

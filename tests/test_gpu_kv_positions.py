@@ -123,8 +123,8 @@ def test_extreme_scores(kind, heads):
     """Queries from 1e-20 to a thousand times the usual, of both signs, zero, and with one value far over the others.
 
     A score is an f32 sum of D products in at most 16 steps that may truncate, of partial sums under a quarter of the
-    sum of the magnitudes: off by 8 * 2^-24 of that, and by 2^-24 of the row's largest |q| times the sum of |k|, since
-    q is held to that.  An error e of the scores moves the output by at most 2 e max |v|; 4e-5 of max |v| is the rest."""
+    sum of the magnitudes: off by 8 * 2^-24 of that, and by 2^-24 of the row's largest |q| times the sum of |k|: q is
+    held to 2^-23, and these errors do not all align.  An error e of the scores moves the output by at most 2 e max |v|; 4e-5 of max |v| is the rest."""
     pool = Pool(kind, [200] * 7, 16, n_kv=2, seed=8)
     q = queries(7, heads, 128, "f32")
     for i, f in enumerate((1000.0, -300.0, 30.0, 1e-20, 0.0, 1e-3)):
