@@ -83,6 +83,39 @@ def test_infinities_of_an_f16_cache(dim, group, act, n):
     assert (got[5] == 0).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [3, 8])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_infinities_among_many_conversations(dim, group, act):
+    """900 short conversations and one that is split over many blocks, windows on some, infinities in a few: those are
+    the formula's, the others the same bits as without."""
+    lens = [1 + (i * 29) % 41 for i in range(900)]
+    lens[411] = 6000
+    starts = [3 if i % 5 == 0 else 0 for i in range(900)]
+    pool = Pool("f16", lens, 16, n_kv=2, dim=dim, seed=group)
+    q = queries(900, 2 * group, dim, act)
+    assert (q != 0).all()
+    before = attend(pool, q, starts=starts, act=act).clone()
+    put(pool, "v", 411, 5999, 0, 7, INF)
+    put(pool, "v", 411, 20, 1, 9, -INF)
+    put(pool, "k", 411, 3333, 0, 1, -INF)
+    marked = {411}
+    for j, i in enumerate(range(3, 900, 37)):
+        if lens[i] > 4:
+            marked.add(i)
+            put(pool, "kv"[j % 2], i, lens[i] - 1, j % 2, j % dim, (INF, -INF)[j // 2 % 2])
+    put(pool, "v", 10, 1, 0, 0, INF)  # before the window: not looked at
+    got = attend(pool, q, starts=starts, act=act)
+    rest = torch.ones(900, dtype=torch.bool, device="cuda")
+    rest[sorted(marked)] = False
+    assert torch.equal(got[rest], before[rest])
+    top = max(float(v[torch.isfinite(v)].abs().max()) for v in pool.value["v"])
+    for i in marked:
+        for name in ("k", "v"):
+            pool.value[name][i] = pool.value[name][i][:, starts[i]:]
+        same(got[i], formula(pool, q, i, lambda h: h // group, dim ** -0.5), top, ACT[act][2])
+
+
 @pytest.mark.parametrize("kind", ["f16", "q8", "q4"])
 @pytest.mark.parametrize("group", [3, 8])
 def test_queries_that_are_not_finite(kind, group):
