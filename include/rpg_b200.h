@@ -308,6 +308,96 @@ RPGB_API int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* ta
                                 float scale, void* out_dev, int64_t out_stride, void* workspace_dev,
                                 int64_t workspace_bytes, void* stream);
 
+/* How a score is made from a product: x = scale (q . k); with cap > 0 x = cap
+ * tanh(x / cap); with slopes (f32 [n_heads], one per q head) x - slopes[head]
+ * |pos[row] - position|, pos (int32 [n_rows], needed with slopes only) being
+ * the rows' own positions.  slopes and pos are device pointers. */
+typedef struct rpgb_kv_scores {
+  float scale, cap;
+  const float* slopes;
+  const int32_t* pos;
+} rpgb_kv_scores;
+
+/* Attention of several new tokens per conversation: prompts, appended turns,
+ * chunks of them.  Rows rows_dev[s] .. rows_dev[s + 1] - 1 of q_dev and out_dev
+ * (rows_dev int32 [n_seq + 1], not decreasing, within [0, n_rows]) belong to
+ * conversation s of the table; rows of no conversation are left as they are.
+ * Row r sees positions [starts_dev[r], ends_dev[r]) (starts_dev NULL: from 0):
+ * its position + 1 as the end makes a causal prompt, a start behind it a window
+ * or packed documents, the length of a prefix as the least end a prefix whose
+ * rows see all of it.  Along a conversation's rows neither starts nor ends may
+ * decrease; a row whose range lies outside the first row's start and the last
+ * row's end of its neighbours gives NaN.  An empty range gives zeros, one past
+ * the table NaN.  Rows whose k and v are to be seen are appended before.
+ *
+ * Sums are in f32.  q is held to 2^-22 of its head's largest value where it is
+ * f32 and to 2^-11 of each value where it has 16 bits, and so are the softmax
+ * weights.  NaN and infinities count as in rpgb_kv_attend.
+ * workspace_dev: rpgb_kv_attend_rows_workspace bytes (or more), 256-byte
+ * aligned; it need not be zeroed, and calls that may overlap need one each. */
+RPGB_API int64_t rpgb_kv_attend_rows_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim);
+RPGB_API int32_t rpgb_kv_attend_rows(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type,
+                                     const void* q_dev, int64_t q_stride, int32_t n_heads, const int32_t* rows_dev,
+                                     int64_t n_rows, const int32_t* ends_dev, const int32_t* starts_dev,
+                                     const rpgb_kv_scores* scores, void* out_dev, int64_t out_stride,
+                                     void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* rpgb_kv_attend for conversations that begin alike (the same instructions,
+ * the same world): what they share is read and multiplied once for all.
+ * Conversations groups_dev[g] .. groups_dev[g + 1] - 1 (int32 [n_groups + 1], not
+ * decreasing, within [0, n_seq]) hold the same k and v at positions [0,
+ * prefix_dev[s]) (int32 [n_seq], one value per group), which are read through
+ * the page list of the group's first conversation; the positions behind through
+ * each conversation's own list.  The page lists may hold the same pages there
+ * or copies, and prefix need not end a page.  A conversation whose prefix is
+ * above that of its group's first gives NaN.  Conversations of no group are
+ * left as they are.  A group of one and a prefix of 0 are taken.
+ * Results are those of rpgb_kv_attend, to the precision of
+ * rpgb_kv_attend_rows.  workspace_dev: rpgb_kv_attend_shared_workspace bytes
+ * (or more) for n_seq conversations, 256-byte aligned, zeroed once before its
+ * first use; calls of any shapes of at most n_seq conversations may follow one
+ * another on it, calls that may overlap need one each. */
+RPGB_API int64_t rpgb_kv_attend_shared_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t n_seq);
+RPGB_API int32_t rpgb_kv_attend_shared(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type,
+                                       const void* q_dev, int64_t q_stride, int32_t n_heads, const int32_t* lens_dev,
+                                       const int32_t* starts_dev, const int32_t* groups_dev, int32_t n_groups,
+                                       const int32_t* prefix_dev, float scale, void* out_dev, int64_t out_stride,
+                                       void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ sampling of a batch */
+
+/* Options of each row, device arrays of n_rows entries; NULL leaves a filter
+ * out (temperature NULL: 1).  Meanings are rpgb_sample's, and min_p:
+ *   temperature  <= 0 (or NaN): the largest logit, ties to the lowest index
+ *   top_k        active iff 1 < k < vocab: logits under the k-th largest are
+ *                dropped (those equal to it stay)
+ *   top_p        active iff 0 < p < 1: a value is dropped when the tokens of
+ *                larger values already have p of the probability that is left
+ *   min_p        active iff 0 < p <= 1: tokens of less than p times the
+ *                largest probability are dropped
+ *   u            random numbers in [0, 1), needed unless every row is greedy:
+ *                the token is the first whose probabilities, added in index
+ *                order, exceed u */
+typedef struct rpgb_sample_rows_options {
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p, *u;
+} rpgb_sample_rows_options;
+
+/* Draws one token per row of logits_dev (n_rows rows of vocab values of
+ * `type`, `stride` elements apart, aligned as their type is) into
+ * tok_out_dev[r]; prob_out_dev[r] (NULL: not wanted) receives the probability
+ * it was drawn with.  Weights and their sums hold 2^-32 or better where they
+ * decide a draw.  NaN and minus infinity are never drawn; rows that hold
+ * nothing else give -1 and NaN; where there are plus infinities, they alone
+ * are drawn, each alike.  Rows are independent of one another: a row's token
+ * does not depend on the batch.  Allocates nothing, needs no workspace, returns
+ * without waiting, can be captured in a graph. */
+#define RPGB_SAMPLE_ROWS_MAX_VOCAB 262144
+RPGB_API int32_t rpgb_sample_rows(int32_t type, const void* logits_dev, int64_t stride, int32_t n_rows, int32_t vocab,
+                                  const rpgb_sample_rows_options* options, int32_t* tok_out_dev, float* prob_out_dev,
+                                  void* stream);
+
 /* ------------------------------------------------------------------ text layer
  *
  * The host text layer rpg_engine_generate runs, without a GPU: the same token

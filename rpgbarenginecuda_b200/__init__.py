@@ -15,13 +15,13 @@ import ctypes
 
 import numpy as np
 
-from ._lib import (EngineError, KvPagesDesc, KvRotaryDesc, KvTableDesc, SampleOptions, check,  # noqa: F401
-                   load_engine)
+from ._lib import (EngineError, KvPagesDesc, KvRotaryDesc, KvScoresDesc, KvTableDesc, SampleOptions,  # noqa: F401
+                   SampleRowsDesc, check, load_engine)
 
 __all__ = ["Model", "Session", "Matrix", "SampleOptions", "EngineError", "TpGroup", "shard_plan", "sample",
            "counter_uniform", "launch_count", "library_path", "GGML_Q4_K", "GGML_Q5_K", "GGML_Q6_K", "GGML_Q8_0",
-           "PagedKv", "PageTable", "Rotary", "attend_workspace", "rope_table", "F32", "F16", "BF16", "KV_F16", "KV_Q8",
-           "KV_Q4", "KV_GROUP"]
+           "PagedKv", "PageTable", "Rotary", "attend_workspace", "attend_rows_workspace", "attend_shared_workspace",
+           "sample_rows", "rope_table", "F32", "F16", "BF16", "KV_F16", "KV_Q8", "KV_Q4", "KV_GROUP"]
 
 GGML_Q8_0 = 8
 GGML_Q4_K = 12
@@ -250,6 +250,20 @@ def sample(logits_ptr: int, n: int, opts: SampleOptions, seed: int, counter: int
           "sample")
 
 
+def sample_rows(logits_ptr: int, dtype: int, n_rows: int, vocab: int, tok_ptr: int, u_ptr: int = 0,
+                temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0, min_p_ptr: int = 0, prob_ptr: int = 0,
+                stride: int = 0, stream: int = 0):
+    """One token per row of logits, with every row's own options and random number (rpgb_sample_rows).
+
+    Options are device arrays of n_rows entries (f32, top_k int32); 0 leaves one out."""
+    lib = load_engine()
+    options = SampleRowsDesc(temperature_ptr or None, top_k_ptr or None, top_p_ptr or None, min_p_ptr or None,
+                             u_ptr or None)
+    if lib.rpgb_sample_rows(dtype, logits_ptr, stride or vocab, n_rows, vocab, ctypes.addressof(options), tok_ptr,
+                            prob_ptr or None, stream or None) < 0:
+        check(-1, "sample_rows")
+
+
 class PageTable:
     """Page table of a batch: int32 [n_seq][stride] on the device, `max_pages` entries of a row used."""
 
@@ -317,6 +331,47 @@ class PagedKv:
                                     starts_ptr or None, scale, out_ptr, out_stride or row, workspace_ptr,
                                     workspace_bytes, stream or None) < 0:
             check(-1, "kv_attend")
+
+
+    def attend_rows(self, table: PageTable, dtype: int, q_ptr: int, n_heads: int, rows_ptr: int, n_rows: int,
+                    ends_ptr: int, scale: float, out_ptr: int, workspace_ptr: int, workspace_bytes: int,
+                    starts_ptr: int = 0, cap: float = 0.0, slopes_ptr: int = 0, pos_ptr: int = 0, q_stride: int = 0,
+                    out_stride: int = 0, stream: int = 0):
+        """Attention of several new tokens per conversation (rpgb_kv_attend_rows)."""
+        row = n_heads * self.head_dim
+        scores = KvScoresDesc(scale, cap, slopes_ptr or None, pos_ptr or None)
+        if self._lib.rpgb_kv_attend_rows(self._ref, table._ref, dtype, q_ptr, q_stride or row, n_heads, rows_ptr, n_rows,
+                                         ends_ptr, starts_ptr or None, ctypes.addressof(scores), out_ptr,
+                                         out_stride or row, workspace_ptr, workspace_bytes, stream or None) < 0:
+            check(-1, "kv_attend_rows")
+
+    def attend_shared(self, table: PageTable, dtype: int, q_ptr: int, n_heads: int, lens_ptr: int, groups_ptr: int,
+                      n_groups: int, prefix_ptr: int, scale: float, out_ptr: int, workspace_ptr: int,
+                      workspace_bytes: int, starts_ptr: int = 0, q_stride: int = 0, out_stride: int = 0,
+                      stream: int = 0):
+        """Attention of one new token per conversation, what groups of them begin with read once
+        (rpgb_kv_attend_shared)."""
+        row = n_heads * self.head_dim
+        if self._lib.rpgb_kv_attend_shared(self._ref, table._ref, dtype, q_ptr, q_stride or row, n_heads, lens_ptr,
+                                           starts_ptr or None, groups_ptr, n_groups, prefix_ptr, scale, out_ptr,
+                                           out_stride or row, workspace_ptr, workspace_bytes, stream or None) < 0:
+            check(-1, "kv_attend_shared")
+
+
+def attend_rows_workspace(n_heads: int, n_kv: int, head_dim: int) -> int:
+    """Bytes of the workspace `PagedKv.attend_rows` needs, whatever the batch."""
+    n = int(load_engine().rpgb_kv_attend_rows_workspace(n_heads, n_kv, head_dim))
+    if n < 0:
+        check(-1, "kv_attend_rows_workspace")
+    return n
+
+
+def attend_shared_workspace(n_heads: int, n_kv: int, head_dim: int, n_seq: int) -> int:
+    """Bytes of the workspace `PagedKv.attend_shared` needs for up to n_seq conversations (zeroed once by the caller)."""
+    n = int(load_engine().rpgb_kv_attend_shared_workspace(n_heads, n_kv, head_dim, n_seq))
+    if n < 0:
+        check(-1, "kv_attend_shared_workspace")
+    return n
 
 
 def attend_workspace(n_heads: int, n_kv: int, head_dim: int) -> int:

@@ -49,6 +49,18 @@ class KvRotaryDesc(ctypes.Structure):
     _fields_ = [("rope", c_p), ("q_norm", c_p), ("k_norm", c_p), ("rope_positions", c_i32), ("eps", c_f32)]
 
 
+class KvScoresDesc(ctypes.Structure):
+    """rpgb_kv_scores."""
+
+    _fields_ = [("scale", c_f32), ("cap", c_f32), ("slopes", c_p), ("pos", c_p)]
+
+
+class SampleRowsDesc(ctypes.Structure):
+    """rpgb_sample_rows_options."""
+
+    _fields_ = [(n, c_p) for n in ("temperature", "top_k", "top_p", "min_p", "u")]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "rpgb_version": (ctypes.c_char_p, []),
@@ -86,6 +98,13 @@ _SIGS = {
     "rpgb_kv_gather": (c_i32, [c_p, c_p, c_i32, c_p, c_p, c_i64, c_p, c_p, c_i64, c_p]),
     "rpgb_kv_attend_workspace": (c_i64, [c_i32, c_i32, c_i32]),
     "rpgb_kv_attend": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_f32, c_p, c_i64, c_p, c_i64, c_p]),
+    "rpgb_kv_attend_rows_workspace": (c_i64, [c_i32, c_i32, c_i32]),
+    "rpgb_kv_attend_rows": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_i64, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64,
+                                    c_p]),
+    "rpgb_kv_attend_shared_workspace": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "rpgb_kv_attend_shared": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_p, c_p, c_i32, c_p, c_f32, c_p, c_i64,
+                                      c_p, c_i64, c_p]),
+    "rpgb_sample_rows": (c_i32, [c_i32, c_p, c_i64, c_i32, c_i32, c_p, c_p, c_p, c_p]),
     "rpgb_text_open": (c_p, [ctypes.c_char_p]),
     "rpgb_text_close": (None, [c_p]),
     "rpgb_text_encode": (c_i64, [c_p, ctypes.c_char_p, c_i64, c_i32, c_p, c_i64]),

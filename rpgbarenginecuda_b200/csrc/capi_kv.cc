@@ -1,11 +1,13 @@
-// capi_kv.cc -- extern "C" entry points of the paged key-value cache
-// (include/rpg_b200.h): argument checks, then the launchers of kv.h.
+// capi_kv.cc -- extern "C" entry points of the paged key-value cache and of the
+// sampling of a batch (include/rpg_b200.h): argument checks, then the launchers
+// of kv.h and sample_rows.h.
 #include <climits>
 #include <cmath>
 
 #include "../../include/rpg_b200.h"
 #include "common.h"
 #include "kv.h"
+#include "sample_rows.h"
 
 using namespace rpgb;
 
@@ -102,6 +104,32 @@ void CheckTokens(const int32_t* pos, int64_t n_tok, const int32_t* seq, const Kv
              static_cast<long long>(n_tok), t.n_seq);
 }
 
+void CheckShape(int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+  RPGB_CHECK(n_kv > 0 && n_kv <= 4096 && n_heads > 0 && n_heads <= 65535 && n_heads % n_kv == 0 &&
+                 (head_dim == 64 || head_dim == 128),
+             "kv: bad shape (%d heads over %d KV heads of %d)", n_heads, n_kv, head_dim);
+}
+void CheckWorkspace(const void* p, int64_t bytes, int64_t need) {
+  RPGB_CHECK(p != nullptr && bytes >= need, "kv: workspace of %lld bytes; %lld are needed",
+             static_cast<long long>(p != nullptr ? bytes : 0), static_cast<long long>(need));
+  CheckAligned(p, 256, "kv: workspace");
+}
+
+// Parts of the workspace of rpgb_kv_attend_shared.  The counters of the attend
+// kernel, which stay zero between calls, come first whatever the batch.
+struct SharedWorkspace {
+  int64_t attend = 0, rows, own, own_lse, total;
+};
+SharedWorkspace SharedParts(int n_heads, int n_kv, int head_dim, int n_seq) {
+  auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  SharedWorkspace w;
+  w.rows = up(KvAttendWorkspace(n_heads, n_kv, head_dim));
+  w.own = w.rows + up(KvRowsWorkspace(n_heads, n_kv, head_dim));
+  w.own_lse = w.own + up(4ll * n_seq * n_heads * head_dim);
+  w.total = w.own_lse + up(4ll * n_seq * n_heads);
+  return w;
+}
+
 }  // namespace
 
 #define RPGB_CATCH(ret)                                     \
@@ -189,9 +217,7 @@ int32_t rpgb_kv_gather(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
 int64_t rpgb_kv_attend_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim) {
   try {
     SetLastError("");
-    RPGB_CHECK(n_kv > 0 && n_kv <= 4096 && n_heads > 0 && n_heads <= 65535 && n_heads % n_kv == 0 &&
-                   (head_dim == 64 || head_dim == 128),
-               "kv: bad shape (%d heads over %d KV heads of %d)", n_heads, n_kv, head_dim);
+    CheckShape(n_heads, n_kv, head_dim);
     return KvAttendWorkspace(n_heads, n_kv, head_dim);
   }
   RPGB_CATCH(-1)
@@ -215,10 +241,7 @@ int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
     CheckRows(out_dev, out_stride, cols, p.type, "out");
     RPGB_CHECK(lens_dev != nullptr, "kv: lengths are NULL");
     RPGB_CHECK(std::isfinite(scale), "kv: the scale is not finite");
-    const int64_t need = KvAttendWorkspace(n_heads, p.kv.n_kv, p.kv.head_dim);
-    RPGB_CHECK(workspace_dev != nullptr && workspace_bytes >= need, "kv: workspace of %lld bytes; %lld are needed",
-               static_cast<long long>(workspace_dev != nullptr ? workspace_bytes : 0), static_cast<long long>(need));
-    CheckAligned(workspace_dev, 256, "kv: workspace");
+    CheckWorkspace(workspace_dev, workspace_bytes, KvAttendWorkspace(n_heads, p.kv.n_kv, p.kv.head_dim));
     p.lens = lens_dev;
     p.starts = starts_dev;
     p.q = q_dev;
@@ -226,9 +249,189 @@ int32_t rpgb_kv_attend(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int3
     p.n_heads = n_heads;
     p.scale = scale;
     p.out = out_dev;
+    p.out_type = p.type;
     p.out_stride = out_stride;
     p.workspace = workspace_dev;
     LaunchKvAttend(p, static_cast<cudaStream_t>(stream));
+    return 0;
+  }
+  RPGB_CATCH(-1)
+}
+
+int64_t rpgb_kv_attend_rows_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+  try {
+    SetLastError("");
+    CheckShape(n_heads, n_kv, head_dim);
+    return KvRowsWorkspace(n_heads, n_kv, head_dim);
+  }
+  RPGB_CATCH(-1)
+}
+
+int32_t rpgb_kv_attend_rows(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type, const void* q_dev,
+                            int64_t q_stride, int32_t n_heads, const int32_t* rows_dev, int64_t n_rows,
+                            const int32_t* ends_dev, const int32_t* starts_dev, const rpgb_kv_scores* scores,
+                            void* out_dev, int64_t out_stride, void* workspace_dev, int64_t workspace_bytes,
+                            void* stream) {
+  try {
+    SetLastError("");
+    KvRowsParams p;
+    p.kv = Pages(kv);
+    p.table = Table(table, p.kv.page_log2);
+    p.type = Type(type);
+    RPGB_CHECK(n_heads > 0 && n_heads <= 65535 && n_heads % p.kv.n_kv == 0, "kv: %d q heads over %d KV heads", n_heads,
+               p.kv.n_kv);
+    RPGB_CHECK(n_rows >= 0 && n_rows <= kKvMaxRows, "kv: bad row count %lld", static_cast<long long>(n_rows));
+    RPGB_CHECK(scores != nullptr, "kv: scores is NULL");
+    RPGB_CHECK(std::isfinite(scores->scale), "kv: the scale is not finite");
+    RPGB_CHECK(std::isfinite(scores->cap) && scores->cap >= 0.f, "kv: bad cap %g", static_cast<double>(scores->cap));
+    RPGB_CHECK(scores->slopes == nullptr || scores->pos != nullptr, "kv: slopes need the rows' positions");
+    CheckAligned(scores->slopes, 4, "kv: slopes");
+    CheckAligned(scores->pos, 4, "kv: row positions");
+    if (p.table.n_seq == 0 || n_rows == 0) return 0;
+    const int64_t cols = static_cast<int64_t>(n_heads) * p.kv.head_dim;
+    CheckRows(q_dev, q_stride, cols, p.type, "q");
+    CheckRows(out_dev, out_stride, cols, p.type, "out");
+    RPGB_CHECK(rows_dev != nullptr && ends_dev != nullptr, "kv: rows or ends are NULL");
+    CheckAligned(rows_dev, 4, "kv: rows");
+    CheckAligned(ends_dev, 4, "kv: ends");
+    CheckAligned(starts_dev, 4, "kv: starts");
+    CheckWorkspace(workspace_dev, workspace_bytes, KvRowsWorkspace(n_heads, p.kv.n_kv, p.kv.head_dim));
+    p.rows = rows_dev;
+    p.n_lists = p.table.n_seq;
+    p.n_rows = static_cast<int32_t>(n_rows);
+    p.starts = starts_dev;
+    p.ends = ends_dev;
+    p.q = q_dev;
+    p.q_stride = q_stride;
+    p.n_heads = n_heads;
+    p.scale = scores->scale;
+    p.cap = scores->cap;
+    p.slopes = scores->slopes;
+    p.pos = scores->pos;
+    p.out = out_dev;
+    p.out_stride = out_stride;
+    p.workspace = workspace_dev;
+    LaunchKvRows(p, static_cast<cudaStream_t>(stream));
+    return 0;
+  }
+  RPGB_CATCH(-1)
+}
+
+int64_t rpgb_kv_attend_shared_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t n_seq) {
+  try {
+    SetLastError("");
+    CheckShape(n_heads, n_kv, head_dim);
+    RPGB_CHECK(n_seq >= 0 && n_seq <= (1 << 20), "kv: bad conversation count %d", n_seq);
+    return SharedParts(n_heads, n_kv, head_dim, n_seq).total;
+  }
+  RPGB_CATCH(-1)
+}
+
+int32_t rpgb_kv_attend_shared(const rpgb_kv_pages* kv, const rpgb_kv_table* table, int32_t type, const void* q_dev,
+                              int64_t q_stride, int32_t n_heads, const int32_t* lens_dev, const int32_t* starts_dev,
+                              const int32_t* groups_dev, int32_t n_groups, const int32_t* prefix_dev, float scale,
+                              void* out_dev, int64_t out_stride, void* workspace_dev, int64_t workspace_bytes,
+                              void* stream) {
+  try {
+    SetLastError("");
+    KvRowsParams p;
+    p.kv = Pages(kv);
+    p.table = Table(table, p.kv.page_log2);
+    p.type = Type(type);
+    RPGB_CHECK(n_heads > 0 && n_heads <= 65535 && n_heads % p.kv.n_kv == 0, "kv: %d q heads over %d KV heads", n_heads,
+               p.kv.n_kv);
+    RPGB_CHECK(n_groups >= 0 && n_groups <= (1 << 20), "kv: bad group count %d", n_groups);
+    if (p.table.n_seq == 0 || n_groups == 0) return 0;
+    const int64_t cols = static_cast<int64_t>(n_heads) * p.kv.head_dim;
+    CheckRows(q_dev, q_stride, cols, p.type, "q");
+    CheckRows(out_dev, out_stride, cols, p.type, "out");
+    RPGB_CHECK(lens_dev != nullptr && groups_dev != nullptr && prefix_dev != nullptr,
+               "kv: lengths, groups or prefixes are NULL");
+    CheckAligned(lens_dev, 4, "kv: lengths");
+    CheckAligned(starts_dev, 4, "kv: starts");
+    CheckAligned(groups_dev, 4, "kv: groups");
+    CheckAligned(prefix_dev, 4, "kv: prefixes");
+    RPGB_CHECK(std::isfinite(scale), "kv: the scale is not finite");
+    const SharedWorkspace w = SharedParts(n_heads, p.kv.n_kv, p.kv.head_dim, p.table.n_seq);
+    CheckWorkspace(workspace_dev, workspace_bytes, w.total);
+    char* base = static_cast<char*>(workspace_dev);
+    // first what follows the common positions, by the operator for one token of each
+    KvAttendParams a;
+    a.kv = p.kv;
+    a.table = p.table;
+    a.type = p.type;
+    a.lens = lens_dev;
+    a.starts = starts_dev;
+    a.prefix = prefix_dev;
+    a.q = q_dev;
+    a.q_stride = q_stride;
+    a.n_heads = n_heads;
+    a.scale = scale;
+    a.out = base + w.own;
+    a.out_type = ElemType::kF32;
+    a.out_stride = cols;
+    a.lse = reinterpret_cast<float*>(base + w.own_lse);
+    a.workspace = base + w.attend;
+    LaunchKvAttend(a, static_cast<cudaStream_t>(stream));
+    // then the common positions, for all of a group at once, and the two together
+    p.rows = groups_dev;
+    p.n_lists = n_groups;
+    p.n_rows = p.table.n_seq;
+    p.starts = starts_dev;
+    p.ends = lens_dev;
+    p.prefix = prefix_dev;
+    p.q = q_dev;
+    p.q_stride = q_stride;
+    p.n_heads = n_heads;
+    p.scale = scale;
+    p.out = out_dev;
+    p.out_stride = out_stride;
+    p.own = static_cast<const float*>(a.out);
+    p.own_lse = a.lse;
+    p.workspace = base + w.rows;
+    LaunchKvRows(p, static_cast<cudaStream_t>(stream));
+    return 0;
+  }
+  RPGB_CATCH(-1)
+}
+
+int32_t rpgb_sample_rows(int32_t type, const void* logits_dev, int64_t stride, int32_t n_rows, int32_t vocab,
+                         const rpgb_sample_rows_options* options, int32_t* tok_out_dev, float* prob_out_dev,
+                         void* stream) {
+  try {
+    SetLastError("");
+    SampleRowsParams p;
+    RPGB_CHECK(type == RPGB_F32 || type == RPGB_F16 || type == RPGB_BF16, "sample_rows: unknown element type %d", type);
+    p.type = static_cast<ElemType>(type);
+    RPGB_CHECK(n_rows >= 0, "sample_rows: bad row count %d", n_rows);
+    RPGB_CHECK(vocab > 0 && vocab <= RPGB_SAMPLE_ROWS_MAX_VOCAB, "sample_rows: vocabulary of %d; 1 to %d are taken", vocab,
+               RPGB_SAMPLE_ROWS_MAX_VOCAB);
+    RPGB_CHECK(stride >= vocab, "sample_rows: stride %lld under the vocabulary's %d", static_cast<long long>(stride),
+               vocab);
+    RPGB_CHECK(options != nullptr, "sample_rows: options is NULL");
+    RPGB_CHECK(options->u != nullptr || options->temperature != nullptr,
+               "sample_rows: rows that are not greedy need random numbers");
+    for (const void* x : {static_cast<const void*>(options->temperature), static_cast<const void*>(options->top_k),
+                          static_cast<const void*>(options->top_p), static_cast<const void*>(options->min_p),
+                          static_cast<const void*>(options->u), static_cast<const void*>(tok_out_dev),
+                          static_cast<const void*>(prob_out_dev)}) {
+      CheckAligned(x, 4, "sample_rows: an array of options or results");
+    }
+    if (n_rows == 0) return 0;
+    RPGB_CHECK(logits_dev != nullptr && tok_out_dev != nullptr, "sample_rows: logits or tokens are NULL");
+    CheckAligned(logits_dev, type == RPGB_F32 ? 4 : 2, "sample_rows: logits");
+    p.logits = logits_dev;
+    p.stride = stride;
+    p.n_rows = n_rows;
+    p.vocab = vocab;
+    p.temperature = options->temperature;
+    p.top_k = options->top_k;
+    p.top_p = options->top_p;
+    p.min_p = options->min_p;
+    p.u = options->u;
+    p.tok = tok_out_dev;
+    p.prob = prob_out_dev;
+    LaunchSampleRows(p, static_cast<cudaStream_t>(stream));
     return 0;
   }
   RPGB_CATCH(-1)

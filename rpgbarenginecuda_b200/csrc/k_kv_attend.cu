@@ -286,6 +286,7 @@ __device__ __forceinline__ Span SpanOf(const KvAttendParams& p, int seq) {
   Span s;
   s.len = static_cast<int>(min(static_cast<int64_t>(max(p.lens[seq], 0)), cap));
   s.start = p.starts != nullptr ? max(p.starts[seq], 0) : 0;
+  if (p.prefix != nullptr) s.start = max(s.start, p.prefix[seq]);
   if (s.start >= s.len) s.start = s.len = 0;
   s.base = s.start & ~(C::R - 1);  // a step lies in one page, or its halves in two of 16
   s.tiles = max(1, (s.len - s.base + C::TILE - 1) / C::TILE);  // an empty item still writes its zeros
@@ -1167,12 +1168,16 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         }
         return v;
       };
-      auto put = [&](int i, const float4& v, float sum) {
+      auto put = [&](int i, const float4& v, float sum, float top) {
         const float f = sum != 0.f ? 1.f / sum : 0.f;  // nothing in range: zero
         float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = past ? kvd::Nan() : y[e];
-        switch (p.type) {
+        if (p.lse != nullptr && i % (D / 4) == 0) {
+          p.lse[static_cast<int64_t>(use.seq) * p.n_heads + use.head * group + use.chunk * per_chunk + i / (D / 4)] =
+              top + log2f(sum);
+        }
+        switch (p.out_type) {
           case ElemType::kF32: kvd::Store4(static_cast<float*>(p.out) + out + 4 * i, y); break;
           case ElemType::kF16: kvd::Store4(static_cast<__half*>(p.out) + out + 4 * i, y); break;
           case ElemType::kBF16: kvd::Store4(static_cast<__nv_bfloat16*>(p.out) + out + 4 * i, y); break;
@@ -1239,7 +1244,7 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
               AddScaled(sumv, f, v[n]);
               sum += f * l_[n];
             }
-            put(i, sumv, sum);
+            put(i, sumv, sum, top);
           }
         }
         if (finish) {
@@ -1323,7 +1328,7 @@ __global__ void __launch_bounds__(C::THREADS, C::BLOCKS) KvAttendKernel(const Kv
         for (int i = tid; i < vecs; i += C::THREADS) {
           float sum, top;
           const float4 v = join(i, sum, top);
-          put(i, v, sum);
+          put(i, v, sum, top);
         }
       }
       if (left > 0) {

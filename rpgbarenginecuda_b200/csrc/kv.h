@@ -21,6 +21,7 @@ constexpr int kKvMinPage = 16;       // a page holds whole 16-position units
 constexpr int kKvMaxPage = 4096;
 constexpr int kKvMaxQueries = 8;     // query heads of a KV head that one attend pass takes
 constexpr int64_t kKvMaxStride = int64_t{1} << 35;  // bytes; a sixteenth of it fits 32 bits
+constexpr int kKvMaxRows = 1 << 24;  // rows of one call over shared page lists
 constexpr int kKvMaxBlocks = 1792;   // bound of the attend grid (sizes the workspace)
 // Floats of one attend record: a vector, a maximum and a sum per query, in whole 16 bytes.
 #ifdef __CUDACC__
@@ -96,6 +97,11 @@ struct KvAttendParams {
   void* out = nullptr;
   int64_t out_stride = 0;  // elements
   void* workspace = nullptr;
+  // Positions under prefix[seq] are left out (null: none); out is of out_type;
+  // lse[seq][q head] = log2 of the sum of 2^(score log2 e) (null: not wanted).
+  const int32_t* prefix = nullptr;
+  ElemType out_type = ElemType::kF32;
+  float* lse = nullptr;
   // filled in by LaunchKvAttend: a constant of the kernel, and the strides of
   // kv in units of 16 bytes
   uint32_t magic = 0, page16 = 0, head16 = 0, pos16 = 0, spage16 = 0, shead16 = 0;
@@ -106,5 +112,34 @@ struct KvAttendParams {
 // follow one another on one workspace.
 int64_t KvAttendWorkspace(int n_heads, int n_kv, int head_dim);
 void LaunchKvAttend(const KvAttendParams& p, cudaStream_t s);
+
+// Attention of several rows that read one page list: the new tokens of a
+// conversation (prefix null: lists are the table's rows), or the conversations
+// of a group over the positions that they share (the list is that of the
+// group's first; ends are the lengths).
+struct KvRowsParams {
+  KvPages kv;
+  KvTable table;
+  ElemType type = ElemType::kF32;
+  const int32_t* rows = nullptr;  // [n_lists + 1]
+  int32_t n_lists = 0;
+  int32_t n_rows = 0;
+  const int32_t *starts = nullptr, *ends = nullptr;  // [n_rows]; starts null: 0
+  const int32_t* prefix = nullptr;                   // [n_rows]
+  const void* q = nullptr;
+  int64_t q_stride = 0;  // elements
+  int32_t n_heads = 0;
+  float scale = 0.f, cap = 0.f;
+  const float* slopes = nullptr;
+  const int32_t* pos = nullptr;
+  void* out = nullptr;
+  int64_t out_stride = 0;  // elements
+  // the rest of a row's attention, to be added: f32 [n_rows][n_heads][head_dim]
+  // and its sums [n_rows][n_heads] (KvAttendParams::lse); null: none
+  const float *own = nullptr, *own_lse = nullptr;
+  void* workspace = nullptr;
+};
+int64_t KvRowsWorkspace(int n_heads, int n_kv, int head_dim);
+void LaunchKvRows(const KvRowsParams& p, cudaStream_t s);
 
 }  // namespace rpgb
