@@ -1,8 +1,11 @@
 // k_kv_rows.cu -- attention of several rows that read one page list: new tokens
 // of a conversation, or the conversations of a group over what they share.
+#include <atomic>
+
 #include "common.h"
 #include "kv_dev.cuh"
 #include "launch.h"
+#include "tc_dev.cuh"
 
 namespace rpgb {
 namespace {
@@ -58,9 +61,8 @@ __device__ __forceinline__ void Put(void* out, ElemType t, int64_t i, float x) {
   }
 }
 
-// A score in units of log2 from a product of q and k.
-__device__ __forceinline__ float Score(const KvRowsParams& p, float x, float slope, int distance) {
-  x *= p.scale;
+// A score of the formula (capped, biased) in units of log2.
+__device__ __forceinline__ float Bent(const KvRowsParams& p, float x, float slope, int distance) {
   if (p.cap > 0.f) {
     // tanh |t| = (1 - e) / (1 + e) with e = exp(-2 |t|)
     const float e = Exp2(fabsf(x) * (-2.f * kLog2e) / p.cap);
@@ -125,7 +127,7 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
     float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) dot += x[e] * k[e];
-    const float s = Score(p, dev::WarpSum(dot), slope, pos - at);
+    const float s = Bent(p, dev::WarpSum(dot) * p.scale, slope, pos - at);
     const float now = fmaxf(m, s), ref = now == -INFINITY ? 0.f : now;
     const float alpha = Exp2(m - ref), w = Exp2(s - ref);
     m = now;
@@ -135,71 +137,1131 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
   }
 }
 
-template <int D, KvType KIND>
-__global__ void __launch_bounds__(256) PlainKernel(const KvRowsParams p) {
-  constexpr int N = D / 32;
+
+// ------------------------------------------------------------------ shapes
+
+constexpr int kTileRows = 128;            // rows of a tile: the lanes of tensor memory
+constexpr int kItemRows = 2 * kTileRows;  // two tiles share the positions that pass through
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kThreads = 32 * (kSoftWarps + kLoadWarps + 2);  // and one that issues products, one that deals out items
+constexpr int kMaxBlocks = 160;
+constexpr int kItems = 4;    // items described ahead
+constexpr int kNotes = 8;    // steps whose scales and bad pages are held
+constexpr int kLeast = 2;    // steps that a block is started for
+constexpr int kHeadroom = 15, kSlack = 8;  // weights are at most 2^15, and 2^7 when their reference was set
+
+template <int D_, KvType KIND_, bool TWO_>
+struct Cfg {
+  static constexpr int D = D_;
+  static constexpr KvType KIND = KIND_;
+  static constexpr bool QUANT = KIND != KvType::kF16;
+  static constexpr bool TWO = TWO_;  // q and weights in two f16 terms (f32 activations)
+  static constexpr int TERMS = TWO ? 2 : 1;
+  static constexpr int KT = QUANT || TWO ? 64 : 128;  // positions of a step
+  static constexpr int NG = QUANT ? D / kKvGroup : 1;
+  static constexpr int BOX = D / 64;                  // 128-byte columns of a tile of f16
+  static constexpr int QTERM = BOX * kTileRows * 128, QTILE = TERMS * QTERM;
+  static constexpr int PLANE = BOX * KT * 128;
+  static constexpr int STAGES = QUANT && !TWO ? 3 : 2;
+  static constexpr int LAG = QUANT && !TWO ? 4 : 2;  // copies begun before the oldest is waited for
+  static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
+  static constexpr int CPR = ROW / 16;
+  static constexpr int PER = KT * CPR / (32 * kLoadWarps);  // 16-byte pieces of a thread
+  static constexpr int RAW = QUANT ? KT * ROW : 0;
+  static constexpr int NOTE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
+  static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kNotes * NOTE;
+  static constexpr int PBASE = KT == 128 ? 64 : 0;  // weights lie over scores already read
+  static_assert(SMEM <= 230 * 1024, "shared memory");
+};
+
+struct Item {
+  int table_row, row0, n_tok, head, chunk;
+  int base, lo, hi;      // first position of step 0; positions that any row may see
+  int step0, steps;      // 0: no more items
+  int first_prefix;
+  bool begins, ends;
+};
+// A piece that begins an item that further blocks end.
+struct Job {
+  int row0, n_tok, head, chunk, last, pad[3];
+};
+
+__host__ __device__ constexpr int64_t RecordFloats(int d) { return static_cast<int64_t>(kItemRows) * (d + 2); }
+constexpr int64_t kJobBytes = kMaxBlocks * static_cast<int64_t>(sizeof(Job));
+
+// Query heads of a KV head in chunks of at most kItemRows.
+struct Split {
+  int group, chunks, per, tokens, items;  // of a chunk; tokens of an item; items of a slot
+  __device__ __forceinline__ explicit Split(const KvRowsParams& p) {
+    group = p.n_heads / p.kv.n_kv;
+    chunks = (group + kItemRows - 1) / kItemRows;
+    per = (group + chunks - 1) / chunks;
+    tokens = kItemRows / per;
+    items = p.kv.n_kv * chunks;
+  }
+};
+
+// Slots number the items of a head: list s begins at slot rows[s] / tokens + s,
+// which leaves room for all its pieces whatever the lists before it hold.
+__device__ __forceinline__ int SlotOf(const KvRowsParams& p, const Split& sp, int list) {
+  return RowBegin(p, list) / sp.tokens + list;
+}
+template <typename C>
+struct Slots {
+  int list = 0;
+  __device__ __forceinline__ void Seek(const KvRowsParams& p, const Split& sp, int slot) {
+    int lo = 0, hi = p.n_lists - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      SlotOf(p, sp, mid) <= slot ? lo = mid : hi = mid - 1;
+    }
+    list = lo;
+  }
+  // Item of the slot (head and steps taken are the caller's); returns its steps, 0 where there is none.
+  __device__ __forceinline__ int Get(const KvRowsParams& p, const Split& sp, int slot, Item& it) {
+    while (list + 1 < p.n_lists && SlotOf(p, sp, list + 1) <= slot) ++list;
+    const int begin = RowBegin(p, list), end = RowEnd(p, list);
+    const int64_t j = slot - (begin / sp.tokens + list), row0 = begin + j * sp.tokens;
+    if (j < 0 || row0 >= end) return 0;
+    it.table_row = TableRow(p, list);
+    it.row0 = static_cast<int>(row0);
+    it.n_tok = min(sp.tokens, end - it.row0);
+    const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
+    it.first_prefix = 0;
+    if (p.prefix != nullptr) {
+      it.first_prefix = max(p.prefix[begin], 0);
+      it.lo = 0;
+      it.hi = static_cast<int>(min(static_cast<int64_t>(it.first_prefix), cap));
+    } else {
+      it.lo = p.starts != nullptr ? max(p.starts[it.row0], 0) : 0;
+      it.hi = static_cast<int>(min(static_cast<int64_t>(max(p.ends[it.row0 + it.n_tok - 1], 0)), cap));
+    }
+    if (it.lo >= it.hi) it.lo = it.hi = 0;
+    it.base = it.lo & ~15;
+    return max(1, (it.hi - it.base + C::KT - 1) / C::KT);
+  }
+};
+
+// Block b of n has steps [total b / n, total (b + 1) / n); ShareOf is the block that has step x.
+__device__ __forceinline__ int ShareOf(long long x, long long total, int n) {
+  return static_cast<int>(((x + 1) * n - 1) / total);
+}
+
+// ------------------------------------------------------------------ instructions
+
+__device__ __forceinline__ uint32_t Swz(int row, int chunk) {
+  return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void CopyWait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ bool MbarTest(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(dev::SmemAddr(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void TmemLoad32(uint32_t a, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void TmemLoadWait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void TmemStore32(uint32_t a, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// A in tensor memory, B in shared memory.
+__device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of 16 positions of a V tile: values are contiguous (128-byte
+// rows, swizzled), 8 positions 1024 bytes apart, the next 64 values `box` bytes on.
+__device__ __forceinline__ uint64_t DescV(uint32_t a, int box) {
+  return static_cast<uint64_t>((a >> 4) & 0x3FFFu) | static_cast<uint64_t>(box >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+__device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return kvd::HalfBits(__floats2half2_rn(lo, hi)); }
+
+// ------------------------------------------------------------------ kernel
+
+struct Bars {
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t s_full[2], p_full[2], q_full[2], pv_done[2];
+  uint64_t item_full[kItems], item_empty[kItems], fin;
+};
+
+// The ring of items, as a reader sees it.
+struct Reader {
+  int n = 0;
+  __device__ __forceinline__ bool Next(Bars& b, const Item* items, Item& it, int lane) {
+    const int i = n % kItems;
+    if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&b.item_full[i], (n / kItems) & 1))) return false;
+    it = items[i];
+    __syncwarp();
+    if (lane == 0) tc::MbarArrive(&b.item_empty[i]);
+    ++n;
+    return it.steps > 0;
+  }
+};
+
+template <typename C>
+__device__ __forceinline__ float* RecordOf(const KvRowsParams& p, int block, bool begins) {
+  return reinterpret_cast<float*>(static_cast<char*>(p.workspace) + kJobBytes) +
+         (2 * block + (begins ? 1 : 0)) * RecordFloats(C::D);
+}
+
+// How a row's result and what was found elsewhere add up.
+struct Join {
+  float f = 0.f, g = 0.f;  // of this result, of the other
+  __device__ __forceinline__ Join(const KvRowsParams& p, int64_t row_head, float ref, float l) {
+    f = l != 0.f ? 1.f / l : 0.f;
+    if (p.own != nullptr) {
+      const float a = ref + log2f(l), b = p.own_lse[row_head];
+      const float top = fmaxf(a, b), base = top == -INFINITY ? 0.f : top;
+      const float wa = exp2f(a - base), wb = exp2f(b - base), sum = wa + wb;
+      f = sum != 0.f ? f * (wa / sum) : 0.f;
+      g = sum != 0.f ? wb / sum : 0.f;
+    }
+  }
+};
+
+// 32 values of an output row.
+__device__ __forceinline__ void Put32(const KvRowsParams& p, bool wide, int64_t at, const float* y) {
+  if (p.type == ElemType::kF32) {
+    float* o = static_cast<float*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(y[i + e]);
+      if (wide) {
+        kvd::Store32(o + i, w);
+      } else {
+        reinterpret_cast<uint4*>(o + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(o + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+  } else {
+    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < 32; i += 16) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (p.type == ElemType::kF16) {
+          w[e] = PackHalf(y[i + 2 * e], y[i + 2 * e + 1]);
+        } else {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(y[i + 2 * e], y[i + 2 * e + 1]);
+          w[e] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      if (wide) {
+        kvd::Store32(o + i, w);
+      } else {
+        reinterpret_cast<uint4*>(o + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(o + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+  }
+}
+
+// Queries of one row: f16 terms of q times 2^-e (a largest value in [2^12,
+// 2^13), the sign of the softmax scale in them) into the tile.  Returns the
+// factor from products to scores in units of log2 (scores of the formula where
+// they are capped or biased), NaN for a row that is not finite.
+template <typename C, typename T>
+__device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char* tile, int row) {
+  const T* q = static_cast<const T*>(p.q) + at;
+  float most = 0.f, bad = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < C::D; c += 8) {
+    float x[8];
+    kvd::Load8(q + c, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(x[i]));
+      bad += x[i] * 0.f;
+    }
+  }
+  const int e = most > 0.f ? min(max(static_cast<int>(__float_as_uint(most) >> 23), 1), 254) - 127 - 12 : 0;
+  // 2^-e in two factors: each is a normal number
+  const float f0 = __uint_as_float(static_cast<uint32_t>(127 - e / 2) << 23);
+  const float f1 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
+  const float s1 = p.scale < 0.f ? -f1 : f1;
+#pragma unroll 4
+  for (int c = 0; c < C::D; c += 8) {
+    float x[8];
+    kvd::Load8(q + c, x);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = x[2 * i] * f0 * s1, b = x[2 * i + 1] * f0 * s1;
+      hi[i] = PackHalf(a, b);
+      const float2 h = __half22float2(kvd::BitsHalf(hi[i]));
+      lo[i] = PackHalf(a - h.x, b - h.y);
+    }
+    char* dst = tile + (c >> 6) * (kTileRows * 128) + Swz(row, (c >> 3) & 7);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (C::TWO) *reinterpret_cast<uint4*>(dst + C::QTERM) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  return fabsf(p.scale) / f0 / f1 + bad;
+}
+
+template <typename C>
+__global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, uint32_t magic) {
+  using namespace tc;
+  constexpr int D = C::D, KT = C::KT;
+  extern __shared__ char smem_raw[];
+  __shared__ Bars bars;
+  __shared__ Item items[kItems];
+  __shared__ uint32_t s_tmem, s_bad[kNotes];
+  __shared__ long long s_part[kThreads / 32], s_before;
+  __shared__ int s_slot;
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* s_q = smem;
+  char* s_k = s_q + 2 * C::QTILE;
+  char* s_v = s_k + C::STAGES * C::PLANE;
+  char* s_raw = s_v + C::STAGES * C::PLANE;
+  char* s_note = s_raw + (C::LAG + 1) * C::RAW;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Split sp(p);
+
+  if (warp == 0) TmemAlloc(&s_tmem, 512u);
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      dev::MbarInit(&bars.k_full[i], kLoadWarps);
+      dev::MbarInit(&bars.v_full[i], kLoadWarps);
+      dev::MbarInit(&bars.k_empty[i], 1);
+      dev::MbarInit(&bars.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      dev::MbarInit(&bars.s_full[i], 1);
+      dev::MbarInit(&bars.pv_done[i], 1);
+      dev::MbarInit(&bars.p_full[i], kSoftWarps / 2);
+      dev::MbarInit(&bars.q_full[i], kSoftWarps / 2);
+    }
+    for (int i = 0; i < kItems; ++i) {
+      dev::MbarInit(&bars.item_full[i], 1);
+      dev::MbarInit(&bars.item_empty[i], kSoftWarps + kLoadWarps + 1);
+    }
+    dev::MbarInit(&bars.fin, 1);
+    dev::MbarInitFence();
+  }
   dev::GridLaunchDependents();
   dev::GridWait();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int row = static_cast<int>(item / p.n_heads), h = static_cast<int>(item % p.n_heads);
-  if (row >= p.n_rows) return;
-  int lo = 0, hi = p.n_lists;  // the first list that ends behind the row
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    RowEnd(p, mid) > row ? hi = mid : lo = mid + 1;
+
+  // ---- this block's share of the steps: a run of slots per thread, their steps added up
+  const int n_slots = p.n_rows / sp.tokens + p.n_lists;
+  const int run = (n_slots + kThreads - 1) / kThreads;
+  const int slot_lo = min(tid * run, n_slots), slot_hi = min(slot_lo + run, n_slots);
+  long long mine = 0;
+  {
+    Slots<C> sl;
+    Item it;
+    if (slot_lo < slot_hi) sl.Seek(p, sp, slot_lo);
+    for (int i = slot_lo; i < slot_hi; ++i) mine += sl.Get(p, sp, i, it);
   }
-  if (lo == p.n_lists || RowBegin(p, lo) > row) return;
-  const int head = h / (p.n_heads / p.kv.n_kv);
-  const Seen s = SeenBy(p, row);
-  float acc[N], m, l;
-  const float slope = p.slopes != nullptr ? p.slopes[h] : 0.f;
-  const int pos = p.slopes != nullptr ? p.pos[row] : 0;
-  const int64_t in_head = static_cast<int64_t>(h) * D + lane * N;
-  PlainRow<D, KIND>(p, TableRow(p, lo), head, row * p.q_stride + static_cast<int64_t>(h) * D, slope, pos, s.start, s.end,
-                    acc, m, l);
-  if (p.prefix != nullptr && p.prefix[row] > p.prefix[RowBegin(p, lo)]) l = kvd::Nan();
-  if (s.past) l = kvd::Nan();
-  float f = l != 0.f ? 1.f / l : 0.f, g = 0.f;
-  if (p.own != nullptr) {
-    const float a = m + log2f(l), b = p.own_lse[static_cast<int64_t>(row) * p.n_heads + h];
-    const float top = fmaxf(a, b), ref = top == -INFINITY ? 0.f : top;
-    const float wa = Exp2(a - ref), wb = Exp2(b - ref), sum = wa + wb;
-    f = sum != 0.f ? f * wa / sum : 0.f;
-    g = sum != 0.f ? wb / sum : 0.f;
-  }
+  long long incl = mine;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    float y = acc[e] * f;
-    if (p.own != nullptr) y += g * p.own[static_cast<int64_t>(row) * p.n_heads * D + in_head + e];
-    Put(p.out, p.type, row * p.out_stride + in_head + e, y);
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
   }
+  if (lane == 31) s_part[warp] = incl;
+  FenceBeforeSync();
+  __syncthreads();
+  FenceAfterSync();
+  const uint32_t tmem = s_tmem;
+  long long before = incl - mine, per_head = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_part[w];
+    per_head += s_part[w];
+  }
+  const long long total = per_head * sp.items;
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), max(total / kLeast, 1ll)));
+  const int block = blockIdx.x;
+  const long long x0 = block < blocks ? total * block / blocks : total;
+  const long long x1 = block < blocks ? total * (block + 1) / blocks : total;
+  const long long rem = per_head > 0 ? x0 % per_head : 0;
+  if (x0 < x1 && before <= rem && rem < before + mine) {
+    s_slot = slot_lo;
+    s_before = before;
+  }
+  __syncthreads();
+
+  if (warp == kSoftWarps + kLoadWarps + 1) {
+    // ---- items of this block, in order
+    Job job{};
+    Slots<C> sl;
+    int n = 0, slot = 0, hc = 0;
+    long long x = x0, skip = 0;
+    if (x0 < x1) {
+      slot = s_slot;
+      skip = rem - s_before;  // steps of the run to leave out
+      hc = static_cast<int>(x0 / per_head);
+      sl.Seek(p, sp, slot);
+    }
+    bool ok = true;
+    for (bool more = true; more && ok;) {
+      Item it;
+      it.steps = 0;
+      if (x < x1) {
+        const int steps = sl.Get(p, sp, slot, it);
+        if (steps <= skip) {  // (an empty slot too)
+          skip -= steps;
+          it.steps = -1;
+        } else {
+          it.step0 = static_cast<int>(skip);
+          it.steps = static_cast<int>(min(static_cast<long long>(steps) - skip, x1 - x));
+          it.head = hc / sp.chunks;
+          it.chunk = hc % sp.chunks;
+          it.begins = it.step0 == 0;
+          it.ends = it.step0 + it.steps == steps;
+          if (it.begins && !it.ends) {
+            job.row0 = it.row0;
+            job.n_tok = it.n_tok;
+            job.head = it.head;
+            job.chunk = it.chunk;
+            job.last = min(max(ShareOf(x + steps - 1, total, blocks), block), blocks - 1);
+          }
+          x += it.steps;
+          skip = 0;
+        }
+        if (++slot == n_slots) {
+          slot = 0;
+          ++hc;
+          sl.list = 0;
+        }
+        if (it.steps < 0) continue;
+      } else {
+        more = false;
+      }
+      const int i = n % kItems;
+      if (n >= kItems) ok = __all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.item_empty[i], (n / kItems - 1) & 1));
+      if (!ok) break;
+      if (lane == 0) {
+        items[i] = it;
+        MbarArrive(&bars.item_full[i]);
+      }
+      __syncwarp();
+      ++n;
+    }
+    if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
+  } else if (warp == kSoftWarps + kLoadWarps) {
+    // ---- products: per step and tile O += P V of the step before, then S = Q K^T
+    if (lane == 0) {
+      constexpr uint32_t id_s = InstrDesc(128, KT);
+      constexpr uint32_t id_o = InstrDesc(128, C::NG == 1 ? D : 64) | 1u << 16;  // (V: values contiguous)
+      const uint64_t d_q = DescSw128(s_q), d_k = DescSw128(s_k);
+      const uint32_t a_v = dev::SmemAddr(s_v);
+      int n = 0;
+      uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
+      int c = 0;  // steps so far
+      bool ok = true;
+      while (ok) {
+        const int i = n % kItems;
+        if (!dev::MbarWait(&bars.item_full[i], (n / kItems) & 1)) break;
+        const int steps = items[i].steps, rows = items[i].n_tok * sp.per;
+        MbarArrive(&bars.item_empty[i]);
+        ++n;
+        if (steps <= 0) break;
+        const int tiles = rows > kTileRows ? 2 : 1;
+        for (int j = 0; j <= steps && ok; ++j) {
+          for (int t = 0; t < tiles && ok; ++t) {
+            if (j > 0) {
+              const int st = (c + j - 1) % C::STAGES, par = ((c + j - 1) / C::STAGES) & 1;
+              ok = (t > 0 || dev::MbarWait(&bars.v_full[st], par)) && dev::MbarWait(&bars.p_full[t], p_parity[t]);
+              if (!ok) break;
+              p_parity[t] ^= 1;
+              FenceAfterSync();
+              const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128 + C::PBASE;
+#pragma unroll
+              for (int g = 0; g < C::NG; ++g) {
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k) {
+                  const uint64_t v = DescV(a_v + st * C::PLANE + g * (KT * 128) + k * 2048, KT * 128);
+#pragma unroll
+                  for (int term = 0; term < C::TERMS; ++term) {
+                    MmaTs(o + 64 * g, w + (g * C::TERMS + term) * (KT / 2) + 8 * k, v, id_o,
+                          j > 1 || k > 0 || term > 0 ? 1u : 0u);
+                  }
+                }
+              }
+              MmaCommit(&bars.pv_done[t]);
+              if (t == tiles - 1) MmaCommit(&bars.v_empty[st]);
+            }
+            if (j < steps) {
+              const int st = (c + j) % C::STAGES, par = ((c + j) / C::STAGES) & 1;
+              ok = (j > 0 || dev::MbarWait(&bars.q_full[t], q_parity[t])) &&
+                   (t > 0 || dev::MbarWait(&bars.k_full[st], par));
+              if (!ok) break;
+              if (j == 0) q_parity[t] ^= 1;
+              FenceAfterSync();
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const int g = C::NG == 1 ? 0 : k / 4;
+                const uint64_t adv = static_cast<uint64_t>((k & 3) * 2);
+                const uint64_t kd = d_k + ((st * C::PLANE + (k >> 2) * (KT * 128)) >> 4) + adv;
+#pragma unroll
+                for (int term = 0; term < C::TERMS; ++term) {
+                  Mma(tmem + t * 128 + 64 * g,
+                      d_q + ((t * C::QTILE + term * C::QTERM + (k >> 2) * (kTileRows * 128)) >> 4) + adv, kd, id_s,
+                      (C::NG == 1 ? k > 0 : (k & 3) > 0) || term > 0 ? 1u : 0u);
+                }
+              }
+              MmaCommit(&bars.s_full[t]);
+              if (t == tiles - 1) MmaCommit(&bars.k_empty[st]);
+            }
+          }
+        }
+        c += steps;
+      }
+      MmaCommit(&bars.fin);  // no product is under way when the block ends
+      dev::MbarWait(&bars.fin, 0);
+    }
+    __syncwarp();
+  } else if (warp >= kSoftWarps) {
+    // ---- copies
+    const int lt = tid - 32 * kSoftWarps, lw = lt >> 5;
+    const uint32_t a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v), a_raw = dev::SmemAddr(s_raw),
+                   a_note = dev::SmemAddr(s_note);
+    const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
+    constexpr int kRowStep = 32 * kLoadWarps / C::CPR;
+    const int mask = (1 << p.kv.page_log2) - 1;
+    int begun = 0, ended = 0;  // copies: step 2 n is K's, 2 n + 1 V's
+    bool ok = true;
+    // the oldest copy has arrived: for codes, spread them to f16; tell the products
+    auto finish = [&]() {
+      const int step = ended >> 1, st = step % C::STAGES;
+      const bool v = ended & 1;
+      if (C::QUANT) {
+        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(v ? &bars.v_empty[st] : &bars.k_empty[st],
+                                                   ((step / C::STAGES) & 1) ^ 1))) {
+          ok = false;
+          return;
+        }
+        const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
+        char* dst = (v ? s_v : s_k) + st * C::PLANE;
+#pragma unroll
+        for (int i = 0; i < C::PER; ++i) {
+          const int r = r0 + i * kRowStep;
+          const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
+          constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            kvd::Codes16<C::KIND> code;
+            if (C::KIND == KvType::kQ8) {
+              code.w[0] = w.x;
+              code.w[1] = w.y;
+              code.w[C::KIND == KvType::kQ8 ? 2 : 0] = w.z;
+              code.w[C::KIND == KvType::kQ8 ? 3 : 0] = w.w;
+            } else {
+              code.w[0] = h == 0 ? w.x : w.z;
+              code.w[1] = h == 0 ? w.y : w.w;
+            }
+            uint32_t y[8];
+            code.Pairs(y, magic);
+            const int u = (c0 * kHalves + h) * 2;  // 8-value chunk of the row
+            char* d = dst + (u >> 3) * (KT * 128);
+            *reinterpret_cast<uint4*>(d + Swz(r, u & 7)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+        }
+      }
+      dev::FenceProxyAsync();
+      __syncwarp();
+      if (lane == 0) MbarArrive(v ? &bars.v_full[st] : &bars.k_full[st]);
+      ++ended;
+    };
+    Reader rd;
+    Item it;
+    while (ok && rd.Next(bars, items, it, lane)) {
+      int page = -1, next = -1;
+      auto lookup = [&](int pos) {  // page of the lane's 16 positions
+        return lane < KT / 16 && pos + 16 > it.lo && pos < it.hi
+                   ? p.table.pages[it.table_row * p.table.stride + (pos >> p.kv.page_log2)]
+                   : -1;
+      };
+      next = lookup(it.base + it.step0 * KT + 16 * lane);
+      for (int j = 0; j < it.steps && ok; ++j) {
+        const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
+        page = next;
+        if (j + 1 < it.steps) next = lookup(at + KT);
+        const bool used = lane < KT / 16 && at + 16 > it.lo && at < it.hi;
+        const bool there = used && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
+        const uint32_t have = __ballot_sync(0xFFFFFFFFu, there);
+        const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
+        const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
+        if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int st = (begun >> 1) % C::STAGES;
+          if (!C::QUANT) {
+            uint64_t* bar = v ? &bars.v_empty[st] : &bars.k_empty[st];
+            const uint32_t parity = (((begun >> 1) / C::STAGES) & 1) ^ 1;
+            if (!__all_sync(0xFFFFFFFFu, MbarTest(bar, parity))) {
+              if (ended < begun) {  // what has been begun is of use before there is room for more
+                CopyWait<0>();
+                while (ended < begun) finish();
+              }
+              if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(bar, parity))) {
+                ok = false;
+                break;
+              }
+            }
+          }
+          const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
+          uint32_t dst;
+          if (C::QUANT) {
+            dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
+          } else {
+            dst = (v ? a_v : a_k) + st * C::PLANE + (c0 >> 3) * (KT * 128);
+          }
+#pragma unroll
+          for (int i = 0; i < C::PER; ++i) {
+            const int r = r0 + i * kRowStep, pos = pos0 + r;
+            const int64_t o = __shfl_sync(0xFFFFFFFFu, off, r >> 4) + (r & 15) * p.kv.pos_stride;
+            const bool in = ((have >> (r >> 4)) & 1) && pos >= it.lo && pos < it.hi;
+            CopyAsync16(C::QUANT ? dst + i * (32 * kLoadWarps * 16) : dst + Swz(r, c0 & 7), in ? plane + o : plane, in);
+          }
+          if (C::QUANT && v == 0) {
+            // scales of K and V: 16 positions are dense, 2 NG 16-byte pieces
+            constexpr int kPer = 2 * C::NG;
+            const int i = lane / kPer % (KT / 16);
+            const int64_t so = there ? kvd::ScaleOffset(p.kv, page, it.head, at & mask) : 0;
+            const int64_t o = __shfl_sync(0xFFFFFFFFu, so, i) + lane % kPer * 16;
+            if (lw < 2 && lane < KT / 16 * kPer) {
+              const bool in = (have >> i) & 1;
+              const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
+              CopyAsync16(a_note + (begun >> 1) % kNotes * C::NOTE + lw * (C::NOTE / 2) + lane * 16, in ? src + o : src, in);
+            }
+          }
+          CopyCommit();
+          ++begun;
+          if (begun - ended > C::LAG) {
+            CopyWait<C::LAG>();
+            finish();
+            if (!ok) break;
+          }
+        }
+      }
+    }
+    CopyWait<0>();
+    while (ok && ended < begun) finish();
+  } else {
+    // ---- softmax: a thread per row
+    const int t = warp >> 2, in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128;
+    const int size = p.type == ElemType::kF32 ? 4 : 2;
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.out_stride * size)) & 31) == 0;
+    const bool bent = p.cap > 0.f || p.slopes != nullptr;
+    uint32_t s_parity = 0;
+    int c = 0, note = 0;  // products with V begun for this tile; steps so far
+    bool ok = true;
+    Reader rd;
+    Item it;
+    while (ok && rd.Next(bars, items, it, lane)) {
+      const int steps = it.steps, note0 = note;
+      note += steps;
+      if (t == 1 && it.n_tok * sp.per <= kTileRows) continue;
+      const int tok = r / sp.per, g = r - tok * sp.per + it.chunk * sp.per;
+      const bool valid = tok < it.n_tok && g < sp.group;
+      const bool active = __any_sync(0xFFFFFFFFu, valid);
+      const int row = it.row0 + tok, qh = it.head * sp.group + g;
+      const int64_t q_at = row * p.q_stride + static_cast<int64_t>(qh) * D;
+      Seen seen{0, 0, false};
+      float cs = 0.f, slope = 0.f;
+      int pos = 0;
+      bool nan_row = false;
+      if (valid) {
+        seen = SeenBy(p, row);
+        nan_row = seen.past || (seen.start < seen.end && (seen.start < it.lo || seen.end > it.hi)) ||
+                  (p.prefix != nullptr && p.prefix[row] > it.first_prefix);
+        char* tile = s_q + t * C::QTILE;
+        cs = p.type == ElemType::kF32 ? WriteQ<C, float>(p, q_at, tile, in_tile)
+                                      : (p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
+                                                                  : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile));
+        if (!(cs == cs)) nan_row = true;
+        if (!bent) cs *= kLog2e;
+        if (p.slopes != nullptr) {
+          slope = p.slopes[qh];
+          pos = p.pos[row];
+        }
+      }
+      dev::FenceProxyAsync();
+      __syncwarp();
+      if (lane == 0) MbarArrive(&bars.q_full[t]);
+
+      float m = -INFINITY, ref = -INFINITY, l = 0.f;
+      int nu = C::QUANT ? -30 : 0;
+      for (int j = 0; j < steps; ++j) {
+        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.s_full[t], s_parity))) {
+          ok = false;
+          break;
+        }
+        s_parity ^= 1;
+        FenceAfterSync();
+        if (active) {
+          const int pos0 = it.base + (it.step0 + j) * KT;
+          const int from = min(max(seen.start - pos0, 0), KT), to = min(max(seen.end - pos0, 0), KT);  // columns seen
+          const uint32_t bad = s_bad[(note0 + j) % kNotes];
+          if (bad != 0 && from < to) {
+            // columns from .. to - 1 in units of 16
+            const uint32_t mine_ = ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u);
+            if (bad & mine_) nan_row = true;
+          }
+          const bool edge = __any_sync(0xFFFFFFFFu, from > 0 || to < KT);
+          const char* scales = s_note + (note0 + j) % kNotes * C::NOTE;
+          uint32_t u[64];
+          float mx = -INFINITY;
+          // scores of 64 columns from c0 into u, in units of log2 where they are bent
+          auto columns = [&](int c0) {
+            TmemLoad32(a_s + c0, u);
+            TmemLoad32(a_s + c0 + 32, u + 32);
+            TmemLoadWait();
+          };
+          auto groups = [&]() {  // the same from the parts of two groups, each with its scale
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t b[32];
+              TmemLoad32(a_s + 32 * h, u + 32 * h);
+              if (C::NG == 2) TmemLoad32(a_s + 64 + 32 * h, b);
+              TmemLoadWait();
+#pragma unroll
+              for (int i = 0; i < 32; i += 4 / C::NG * 2) {
+                const uint4 w = *reinterpret_cast<const uint4*>(scales + (32 * h + i) * 2 * C::NG);
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 8 / C::NG; ++e) {
+                  const int k = 32 * h + i + e;
+                  if (C::NG == 2) {
+                    const float2 d = __half22float2(kvd::BitsHalf(ww[e % 4]));
+                    u[k] = __float_as_uint(__uint_as_float(u[k]) * d.x + __uint_as_float(b[(i + e) % 32]) * d.y);
+                  } else {
+                    const float2 d = __half22float2(kvd::BitsHalf(ww[e / 2 % 4]));
+                    u[k] = __float_as_uint(__uint_as_float(u[k]) * (e & 1 ? d.y : d.x));
+                  }
+                }
+              }
+            }
+          };
+          auto bend = [&](int c0) {
+            if (bent) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) u[i] = __float_as_uint(Bent(p, __uint_as_float(u[i]) * cs, slope, pos - pos0 - c0 - i));
+            }
+          };
+          auto hide = [&](int c0) {
+            if (edge) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                if (c0 + i < from || c0 + i >= to) u[i] = __float_as_uint(-INFINITY);
+              }
+            }
+          };
+          auto largest = [&]() {
+            float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              a = fmaxf(a, __uint_as_float(u[i]));
+              b = fmaxf(b, __uint_as_float(u[i + 1]));
+            }
+            mx = fmaxf(mx, fmaxf(a, b));
+          };
+          if (KT == 128) {
+            columns(0);
+            bend(0);
+            hide(0);
+            largest();
+            columns(64);
+            bend(64);
+            hide(64);
+            largest();
+          } else {
+            if (C::QUANT) {
+              groups();
+            } else {
+              columns(0);
+            }
+            bend(0);
+            hide(0);
+            largest();
+          }
+          const float to_log2 = bent ? 1.f : cs;
+          if (C::QUANT) {
+            // an exponent over the V scales that count
+            float top = 0.f;
+            if (edge) {
+              for (int i = from * C::NG; i < to * C::NG; ++i) {
+                top = fmaxf(top, fabsf(__half2float(reinterpret_cast<const __half*>(scales + C::NOTE / 2)[i])));
+              }
+            } else {
+              for (int i = lane; i < KT * C::NG / 2; i += 32) {
+                const float2 d = __half22float2(__habs2(reinterpret_cast<const __half2*>(scales + C::NOTE / 2)[i]));
+                top = fmaxf(top, fmaxf(d.x, d.y));
+              }
+              top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
+            }
+            nu = max(nu, static_cast<int>(__float_as_uint(top) >> 23) - 126);
+          }
+          m = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * to_log2);
+          const float over = m + static_cast<float>(nu);
+          const bool grow = over > ref + static_cast<float>(kHeadroom);
+          if (__any_sync(0xFFFFFFFFu, grow)) {
+            const float now = grow ? over - static_cast<float>(kHeadroom - kSlack) : ref;
+            const float alpha = grow && ref != -INFINITY ? exp2f(ref - now) : 1.f;
+            ref = now;
+            if (__any_sync(0xFFFFFFFFu, alpha != 1.f)) {
+              l *= alpha;
+              if (j > 0) {
+                if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) {
+                  ok = false;
+                  break;
+                }
+                FenceAfterSync();
+#pragma unroll 1
+                for (int k = 0; k < D; k += 32) {
+                  uint32_t o[32];
+                  TmemLoad32(a_o + k, o);
+                  TmemLoadWait();
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                  TmemStore32(a_o + k, o);
+                }
+                TmemStoreWait();
+              }
+            }
+          }
+          const float less = ref == -INFINITY ? 0.f : ref;
+          // weights of the 64 columns in u (hidden ones are minus infinity, whose product with a scale of 0 is not)
+          auto weights = [&](int c0) {
+            float a = 0.f, b = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              float x = Exp2(__uint_as_float(u[i]) * to_log2 - less), y = Exp2(__uint_as_float(u[i + 1]) * to_log2 - less);
+              if (edge) {
+                if (c0 + i < from || c0 + i >= to) x = 0.f;
+                if (c0 + i + 1 < from || c0 + i + 1 >= to) y = 0.f;
+              }
+              a += x;
+              b += y;
+              u[i] = __float_as_uint(x);
+              u[i + 1] = __float_as_uint(y);
+            }
+            l += a + b;
+          };
+          // to f16 and into tensor memory
+          auto store = [&](uint32_t dst) {
+            uint32_t h[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) h[i] = PackHalf(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+            TmemStore32(dst, h);
+            if (C::TWO) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float2 f = __half22float2(kvd::BitsHalf(h[i]));
+                h[i] = PackHalf(__uint_as_float(u[2 * i]) - f.x, __uint_as_float(u[2 * i + 1]) - f.y);
+              }
+              TmemStore32(dst + 32, h);
+            }
+          };
+          if (KT == 128) {
+            weights(64);
+            store(a_s + C::PBASE + 32);
+            columns(0);
+            bend(0);
+            hide(0);
+            weights(0);
+            store(a_s + C::PBASE);
+          } else if (C::QUANT) {
+            weights(0);
+#pragma unroll
+            for (int gp = 0; gp < C::NG; ++gp) {
+              // times the scales of the group's values
+#pragma unroll
+              for (int term = 0; term < C::TERMS; ++term) {
+                uint32_t h[32];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  float d[4];
+                  const char* sc = scales + C::NOTE / 2 + 2 * i * 2 * C::NG;
+                  if (C::NG == 2) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(sc);
+                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      const float2 f = __half22float2(kvd::BitsHalf(ww[e]));
+                      d[e] = gp == 0 ? f.x : f.y;
+                    }
+                  } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(sc);
+                    const float2 f = __half22float2(kvd::BitsHalf(w.x)), f2 = __half22float2(kvd::BitsHalf(w.y));
+                    d[0] = f.x;
+                    d[1] = f.y;
+                    d[2] = f2.x;
+                    d[3] = f2.y;
+                  }
+                  float y[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    y[e] = __uint_as_float(u[2 * i + e]) * d[e];
+                    if (edge && (2 * i + e < from || 2 * i + e >= to)) y[e] = 0.f;
+                  }
+                  h[i] = PackHalf(y[0], y[1]);
+                  h[i + 1] = PackHalf(y[2], y[3]);
+                  if (term == 1) {
+                    const float2 f = __half22float2(kvd::BitsHalf(h[i])), f2 = __half22float2(kvd::BitsHalf(h[i + 1]));
+                    h[i] = PackHalf(y[0] - f.x, y[1] - f.y);
+                    h[i + 1] = PackHalf(y[2] - f2.x, y[3] - f2.y);
+                  }
+                }
+                TmemStore32(a_s + (gp * C::TERMS + term) * 32, h);
+              }
+            }
+          } else {
+            weights(0);
+            store(a_s);
+          }
+          TmemStoreWait();
+          FenceBeforeSync();
+        }
+        __syncwarp();
+        if (lane == 0) MbarArrive(&bars.p_full[t]);
+        ++c;
+      }
+      // ---- the end of the item, or of this block's piece of it
+      if (ok && !__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) ok = false;
+      FenceAfterSync();
+      const int64_t row_head = static_cast<int64_t>(row) * p.n_heads + qh;
+      const int64_t out = row * p.out_stride + static_cast<int64_t>(qh) * D;
+      const bool whole = it.begins && it.ends;
+      float* rec = RecordOf<C>(p, block, it.begins);
+      if (nan_row || !ok) l = kvd::Nan();  // (a wait that gave up is not to pass for a result)
+      if (active) {
+        const Join jn = valid && whole ? Join(p, row_head, ref, l) : Join(p, 0, 0.f, 0.f);
+        float check = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < D; k += 32) {
+          uint32_t o[32];
+          TmemLoad32(a_o + k, o);
+          TmemLoadWait();
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            y[i] = __uint_as_float(o[i]);
+            check += y[i] * 0.f;
+          }
+          if (valid && whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = l == 0.f ? 0.f : y[i] * jn.f;
+            if (p.own != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(p.own + row_head * D + k + i);
+                y[i] += jn.g * w.x;
+                y[i + 1] += jn.g * w.y;
+                y[i + 2] += jn.g * w.z;
+                y[i + 3] += jn.g * w.w;
+              }
+            }
+            Put32(p, wide, out + k, y);
+          } else if (valid) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = o[i + e];
+              kvd::Store32(rec + r * D + k + i, w);
+            }
+          }
+        }
+        if (valid && !whole) {
+          rec[kItemRows * D + r] = ref;
+          rec[kItemRows * (D + 1) + r] = l;
+        }
+        if (!C::QUANT) {
+          // infinities and NaN: such rows again, by the formula
+          uint32_t again = __ballot_sync(0xFFFFFFFFu, valid && !nan_row && ok && !(check + l * 0.f == 0.f));
+          const int from = it.base + it.step0 * KT, to = from + steps * KT;
+          while (again != 0) {
+            const int w = __ffs(again) - 1;
+            again &= again - 1;
+            const int start = __shfl_sync(0xFFFFFFFFu, seen.start, w), end = __shfl_sync(0xFFFFFFFFu, seen.end, w);
+            constexpr int N = D / 32;
+            float acc[N], pm, pl;
+            PlainRow<D, C::KIND>(p, it.table_row, it.head, __shfl_sync(0xFFFFFFFFu, q_at, w),
+                                 __shfl_sync(0xFFFFFFFFu, slope, w), __shfl_sync(0xFFFFFFFFu, pos, w), max(start, from),
+                                 min(end, to), acc, pm, pl);
+            const int rr = __shfl_sync(0xFFFFFFFFu, r, w);
+            const int64_t rh = __shfl_sync(0xFFFFFFFFu, row_head, w), oo = __shfl_sync(0xFFFFFFFFu, out, w);
+            if (whole) {
+              const Join jp(p, rh, pm, pl);
+#pragma unroll
+              for (int e = 0; e < N; ++e) {
+                float y = pl == 0.f ? 0.f : acc[e] * jp.f;
+                if (p.own != nullptr) y += jp.g * p.own[rh * D + lane * N + e];
+                Put(p.out, p.type, oo + lane * N + e, y);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < N; ++e) rec[rr * D + lane * N + e] = acc[e];
+              if (lane == 0) {
+                rec[kItemRows * D + rr] = pm;
+                rec[kItemRows * (D + 1) + rr] = pl;
+              }
+            }
+          }
+        }
+      }
+      FenceBeforeSync();  // (what was read of tensor memory, before the next item's products)
+    }
+  }
+  __syncthreads();
+  if (warp == 0) TmemDealloc(tmem, 512u);
+}
+
+// Joins the pieces of the items that several blocks had, in block order.
+template <typename C>
+__global__ void __launch_bounds__(256) RowsJoinKernel(const KvRowsParams p) {
+  constexpr int D = C::D;
+  dev::GridLaunchDependents();
+  dev::GridWait();
+  const Job job = static_cast<const Job*>(p.workspace)[blockIdx.x];
+  const Split sp(p);
+  const int b0 = blockIdx.x, n = job.last - b0 + 1;
+  constexpr int kVec = D / 4;  // threads of a row
+  for (int r = blockIdx.y * (256 / kVec) + threadIdx.x / kVec; r < job.n_tok * sp.per; r += gridDim.y * (256 / kVec)) {
+    const int tok = r / sp.per, g = r - tok * sp.per + job.chunk * sp.per, i = threadIdx.x % kVec;
+    if (g >= sp.group) continue;
+    auto rec = [&](int k) { return RecordOf<C>(p, b0 + k, k == 0); };
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kFlight = 4;
+    for (int k0 = 0; k0 < n; k0 += kFlight) {
+      float ref[kFlight], l[kFlight];
+      float4 x[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        ref[k] = -INFINITY;
+        l[k] = 0.f;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < n) {
+          const float* q = rec(k0 + k);
+          ref[k] = q[kItemRows * D + r];
+          l[k] = q[kItemRows * (D + 1) + r];
+          x[k] = reinterpret_cast<const float4*>(q + r * D)[i];
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) now = fmaxf(now, ref[k]);
+      const float base = now == -INFINITY ? 0.f : now, keep = exp2f(top - base);
+      v = make_float4(v.x * keep, v.y * keep, v.z * keep, v.w * keep);
+      sum *= keep;
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const float f = exp2f(ref[k] - base);
+        sum += l[k] == 0.f ? 0.f : f * l[k];
+        if (l[k] != 0.f) {
+          v.x += f * x[k].x;
+          v.y += f * x[k].y;
+          v.z += f * x[k].z;
+          v.w += f * x[k].w;
+        }
+      }
+      top = now;
+    }
+    const int row = job.row0 + tok, qh = job.head * sp.group + g;
+    const int64_t row_head = static_cast<int64_t>(row) * p.n_heads + qh;
+    const Join jn(p, row_head, top, sum);
+    float y[4] = {v.x * jn.f, v.y * jn.f, v.z * jn.f, v.w * jn.f};
+    if (sum == 0.f) y[0] = y[1] = y[2] = y[3] = 0.f;
+    if (p.own != nullptr) {
+      const float4 w = reinterpret_cast<const float4*>(p.own + row_head * D)[i];
+      y[0] += jn.g * w.x;
+      y[1] += jn.g * w.y;
+      y[2] += jn.g * w.z;
+      y[3] += jn.g * w.w;
+    }
+    const int64_t out = row * p.out_stride + static_cast<int64_t>(qh) * D + 4 * i;
+    switch (p.type) {
+      case ElemType::kF32: kvd::Store4(static_cast<float*>(p.out) + out, y); break;
+      case ElemType::kF16: kvd::Store4(static_cast<__half*>(p.out) + out, y); break;
+      case ElemType::kBF16: kvd::Store4(static_cast<__nv_bfloat16*>(p.out) + out, y); break;
+    }
+  }
+}
+
+template <typename C>
+int Grid() {
+  static std::atomic<int> grids[64];
+  int dev = 0;
+  RPGB_CUDA(cudaGetDevice(&dev));
+  RPGB_CHECK(dev < 64, "kv: device %d", dev);
+  int grid = grids[dev].load(std::memory_order_acquire);
+  if (grid == 0) {
+    int sms = 0;
+    RPGB_CUDA(cudaFuncSetAttribute(RowsKernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    RPGB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    grid = sms < kMaxBlocks ? sms : kMaxBlocks;
+    grids[dev].store(grid, std::memory_order_release);
+  }
+  return grid;
+}
+
+template <typename C>
+void Launch(const KvRowsParams& p, cudaStream_t s) {
+  const int grid = Grid<C>();
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, p,
+                   kvd::kMagic);
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, 8), dim3(256), 0, s, true, p);
 }
 
 template <int D, KvType KIND>
-void Launch(const KvRowsParams& p, cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(p.n_rows) * p.n_heads;
-  LaunchKernelArgs(reinterpret_cast<const void*>(PlainKernel<D, KIND>), dim3(static_cast<unsigned>((warps + 7) / 8)),
-                   dim3(256), 0, s, true, p);
+void ByType(const KvRowsParams& p, cudaStream_t s) {
+  p.type == ElemType::kF32 ? Launch<Cfg<D, KIND, true>>(p, s) : Launch<Cfg<D, KIND, false>>(p, s);
 }
-
 template <int D>
 void ByKind(const KvRowsParams& p, cudaStream_t s) {
   switch (p.kv.type) {
-    case KvType::kF16: return Launch<D, KvType::kF16>(p, s);
-    case KvType::kQ8: return Launch<D, KvType::kQ8>(p, s);
-    case KvType::kQ4: return Launch<D, KvType::kQ4>(p, s);
+    case KvType::kF16: return ByType<D, KvType::kF16>(p, s);
+    case KvType::kQ8: return ByType<D, KvType::kQ8>(p, s);
+    case KvType::kQ4: return ByType<D, KvType::kQ4>(p, s);
   }
 }
 
 }  // namespace
 
-int64_t KvRowsWorkspace(int, int, int head_dim) { return 2ll * 160 * 256 * (head_dim + 2) * 4 + 65536; }
+int64_t KvRowsWorkspace(int, int, int head_dim) { return kJobBytes + 2ll * kMaxBlocks * RecordFloats(head_dim) * 4; }
 
 void LaunchKvRows(const KvRowsParams& p, cudaStream_t s) {
   p.kv.head_dim == 64 ? ByKind<64>(p, s) : ByKind<128>(p, s);
   RPGB_CUDA(cudaGetLastError());
-  CountLaunches(1);
+  CountLaunches(2);
 }
 
 }  // namespace rpgb
