@@ -1,6 +1,7 @@
 // k_kv_rows.cu -- attention of several rows that read one page list: new tokens
 // of a conversation, or the conversations of a group over what they share.
 #include <atomic>
+#include <type_traits>
 
 #include "common.h"
 #include "kv_dev.cuh"
@@ -142,12 +143,17 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
 
 constexpr int kTileRows = 128;            // rows of a tile: the lanes of tensor memory
 constexpr int kItemRows = 2 * kTileRows;  // two tiles share the positions that pass through
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = 32 * (kSoftWarps + kLoadWarps + 2);  // and one that issues products, one that deals out items
+constexpr int kSoftWarps = 8, kLoadWarps = 2;
+constexpr int kMmaWarp = kSoftWarps, kDealWarp = kMmaWarp + 1, kLoadWarp0 = kDealWarp + 1;
+constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
+// Registers: 168 a thread at launch; the rows' warps take what the last four leave: 216 * 256 + 72 * 128 = 168 * 384.
+constexpr int kSoftRegs = 216, kOtherRegs = 72;
+static_assert(kThreads == 384 && kSoftRegs * 256 + kOtherRegs * 128 <= 168 * kThreads, "registers");
 constexpr int kMaxBlocks = 160;
 constexpr int kItems = 4;    // items described ahead
 constexpr int kNotes = 8;    // steps whose scales and bad pages are held
 constexpr int kLeast = 2;    // steps that a block is started for
+constexpr int kBorder = 2;   // steps that the end of an item is worth
 constexpr int kHeadroom = 15, kSlack = 8;  // weights are at most 2^15, and 2^7 when their reference was set
 
 template <int D_, KvType KIND_, bool TWO_>
@@ -170,7 +176,6 @@ struct Cfg {
   static constexpr int RAW = QUANT ? KT * ROW : 0;
   static constexpr int NOTE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
   static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kNotes * NOTE;
-  static constexpr int PBASE = KT == 128 ? 64 : 0;  // weights lie over scores already read
   static_assert(SMEM <= 230 * 1024, "shared memory");
 };
 
@@ -242,7 +247,8 @@ struct Slots {
   }
 };
 
-// Block b of n has steps [total b / n, total (b + 1) / n); ShareOf is the block that has step x.
+// Block b of n has steps [total b / n, total (b + 1) / n), the borders of items
+// counted; ShareOf is the block that has step x.
 __device__ __forceinline__ int ShareOf(long long x, long long total, int n) {
   return static_cast<int>(((x + 1) * n - 1) / total);
 }
@@ -394,12 +400,14 @@ __device__ __forceinline__ void Put32(const KvRowsParams& p, bool wide, int64_t 
 // they are capped or biased), NaN for a row that is not finite.
 template <typename C, typename T>
 __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char* tile, int row) {
-  const T* q = static_cast<const T*>(p.q) + at;
+  kvd::Raw8<T> q[C::D / 8];  // all of the row on its way at once
+#pragma unroll
+  for (int c = 0; c < C::D / 8; ++c) q[c].Load(static_cast<const T*>(p.q) + at + 8 * c);
   float most = 0.f, bad = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < C::D; c += 8) {
+#pragma unroll
+  for (int c = 0; c < C::D / 8; ++c) {
     float x[8];
-    kvd::Load8(q + c, x);
+    q[c].Floats(x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       most = fmaxf(most, fabsf(x[i]));
@@ -411,10 +419,10 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
   const float f0 = __uint_as_float(static_cast<uint32_t>(127 - e / 2) << 23);
   const float f1 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
   const float s1 = p.scale < 0.f ? -f1 : f1;
-#pragma unroll 4
-  for (int c = 0; c < C::D; c += 8) {
+#pragma unroll
+  for (int c = 0; c < C::D / 8; ++c) {
     float x[8];
-    kvd::Load8(q + c, x);
+    q[c].Floats(x);
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -423,7 +431,7 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
       const float2 h = __half22float2(kvd::BitsHalf(hi[i]));
       lo[i] = PackHalf(a - h.x, b - h.y);
     }
-    char* dst = tile + (c >> 6) * (kTileRows * 128) + Swz(row, (c >> 3) & 7);
+    char* dst = tile + (c >> 3) * (kTileRows * 128) + Swz(row, c & 7);
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (C::TWO) *reinterpret_cast<uint4*>(dst + C::QTERM) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
@@ -482,7 +490,10 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     Slots<C> sl;
     Item it;
     if (slot_lo < slot_hi) sl.Seek(p, sp, slot_lo);
-    for (int i = slot_lo; i < slot_hi; ++i) mine += sl.Get(p, sp, i, it);
+    for (int i = slot_lo; i < slot_hi; ++i) {
+      const int steps = sl.Get(p, sp, i, it);
+      mine += steps > 0 ? steps + kBorder : 0;
+    }
   }
   long long incl = mine;
 #pragma unroll
@@ -511,8 +522,9 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     s_before = before;
   }
   __syncthreads();
-
-  if (warp == kSoftWarps + kLoadWarps + 1) {
+  if (warp >= kSoftWarps) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == kDealWarp) {
     // ---- items of this block, in order
     Job job{};
     Slots<C> sl;
@@ -530,8 +542,10 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
       it.steps = 0;
       if (x < x1) {
         const int steps = sl.Get(p, sp, slot, it);
-        if (steps <= skip) {  // (an empty slot too)
-          skip -= steps;
+        const int weight = steps > 0 ? steps + kBorder : 0;
+        if (steps <= skip) {  // nothing of it, or its border alone
+          x += weight > skip ? weight - skip : 0;
+          skip -= min(skip, static_cast<long long>(weight));
           it.steps = -1;
         } else {
           it.step0 = static_cast<int>(skip);
@@ -547,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
             job.chunk = it.chunk;
             job.last = min(max(ShareOf(x + steps - 1, total, blocks), block), blocks - 1);
           }
-          x += it.steps;
+          x += it.steps + (it.ends ? kBorder : 0);
           skip = 0;
         }
         if (++slot == n_slots) {
@@ -570,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
       ++n;
     }
     if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
-  } else if (warp == kSoftWarps + kLoadWarps) {
+  } else if (warp == kMmaWarp) {
     // ---- products: per step and tile O += P V of the step before, then S = Q K^T
     if (lane == 0) {
       constexpr uint32_t id_s = InstrDesc(128, KT);
@@ -597,16 +611,17 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
               if (!ok) break;
               p_parity[t] ^= 1;
               FenceAfterSync();
-              const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128 + C::PBASE;
+              const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128;
 #pragma unroll
               for (int g = 0; g < C::NG; ++g) {
 #pragma unroll
-                for (int k = 0; k < KT / 16; ++k) {
-                  const uint64_t v = DescV(a_v + st * C::PLANE + g * (KT * 128) + k * 2048, KT * 128);
+                for (int term = C::TERMS - 1; term >= 0; --term) {
 #pragma unroll
-                  for (int term = 0; term < C::TERMS; ++term) {
+                  for (int k = 0; k < KT / 16; ++k) {
+                    const uint64_t v = DescV(a_v + st * C::PLANE + g * (KT * 128) + k * 2048, KT * 128);
+                    // with two terms every step's product starts anew (it is added up in registers)
                     MmaTs(o + 64 * g, w + (g * C::TERMS + term) * (KT / 2) + 8 * k, v, id_o,
-                          j > 1 || k > 0 || term > 0 ? 1u : 0u);
+                          (!C::TWO && j > 1) || k > 0 || term < C::TERMS - 1 ? 1u : 0u);
                   }
                 }
               }
@@ -620,16 +635,17 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
               if (!ok) break;
               if (j == 0) q_parity[t] ^= 1;
               FenceAfterSync();
+              // (second terms first: the sums that the tensor cores cut short are small then)
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const int g = C::NG == 1 ? 0 : k / 4;
-                const uint64_t adv = static_cast<uint64_t>((k & 3) * 2);
-                const uint64_t kd = d_k + ((st * C::PLANE + (k >> 2) * (KT * 128)) >> 4) + adv;
+              for (int term = C::TERMS - 1; term >= 0; --term) {
 #pragma unroll
-                for (int term = 0; term < C::TERMS; ++term) {
+                for (int k = 0; k < D / 16; ++k) {
+                  const int g = C::NG == 1 ? 0 : k / 4;
+                  const uint64_t adv = static_cast<uint64_t>((k & 3) * 2);
+                  const uint64_t kd = d_k + ((st * C::PLANE + (k >> 2) * (KT * 128)) >> 4) + adv;
                   Mma(tmem + t * 128 + 64 * g,
                       d_q + ((t * C::QTILE + term * C::QTERM + (k >> 2) * (kTileRows * 128)) >> 4) + adv, kd, id_s,
-                      (C::NG == 1 ? k > 0 : (k & 3) > 0) || term > 0 ? 1u : 0u);
+                      (C::NG == 1 ? k > 0 : (k & 3) > 0) || term < C::TERMS - 1 ? 1u : 0u);
                 }
               }
               MmaCommit(&bars.s_full[t]);
@@ -643,9 +659,9 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
       dev::MbarWait(&bars.fin, 0);
     }
     __syncwarp();
-  } else if (warp >= kSoftWarps) {
+  } else {
     // ---- copies
-    const int lt = tid - 32 * kSoftWarps, lw = lt >> 5;
+    const int lt = tid - 32 * kLoadWarp0, lw = lt >> 5;
     const uint32_t a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v), a_raw = dev::SmemAddr(s_raw),
                    a_note = dev::SmemAddr(s_note);
     const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
@@ -665,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
         }
         const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
         char* dst = (v ? s_v : s_k) + st * C::PLANE;
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < C::PER; ++i) {
           const int r = r0 + i * kRowStep;
           const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
@@ -716,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
         const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
         const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
         if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
-#pragma unroll
+#pragma unroll 1
         for (int v = 0; v < 2; ++v) {
           const int st = (begun >> 1) % C::STAGES;
           if (!C::QUANT) {
@@ -740,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
           } else {
             dst = (v ? a_v : a_k) + st * C::PLANE + (c0 >> 3) * (KT * 128);
           }
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < C::PER; ++i) {
             const int r = r0 + i * kRowStep, pos = pos0 + r;
             const int64_t o = __shfl_sync(0xFFFFFFFFu, off, r >> 4) + (r & 15) * p.kv.pos_stride;
@@ -771,8 +787,10 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     }
     CopyWait<0>();
     while (ok && ended < begun) finish();
+  }
   } else {
     // ---- softmax: a thread per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int t = warp >> 2, in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128;
@@ -806,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
                                       : (p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
                                                                   : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile));
         if (!(cs == cs)) nan_row = true;
-        if (!bent) cs *= kLog2e;
+        if (!bent) cs = fmaxf(cs * kLog2e, 1e-37f);  // (a scale of 0: minus infinity times it is to stay)
         if (p.slopes != nullptr) {
           slope = p.slopes[qh];
           pos = p.pos[row];
@@ -818,6 +836,210 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
 
       float m = -INFINITY, ref = -INFINITY, l = 0.f;
       int nu = C::QUANT ? -30 : 0;
+      float2 acc[C::TWO ? D / 2 : 1];  // the result of the steps before the last
+      if (C::TWO) {
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) acc[i % (C::TWO ? D / 2 : 1)] = make_float2(0.f, 0.f);
+      }
+      auto ProductsDone = [&]() {  // those with V of the last step
+        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) return false;
+        FenceAfterSync();
+        return true;
+      };
+      // Softmax of a step's scores, weights into tensor memory.  EDGE: some row of the warp does not see all positions.
+      auto step = [&](auto edge, int j, int from, int to, int pos0, const char* scales) {
+        constexpr bool EDGE = decltype(edge)::value;
+        if (C::TWO && j > 0) {
+          if (!ProductsDone()) return false;  // (they came before these scores)
+#pragma unroll
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            TmemLoad32(a_o + k, o);
+            TmemLoadWait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2& a = acc[(k / 2 + i) % (C::TWO ? D / 2 : 1)];
+              a = __fadd2_rn(a, make_float2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
+            }
+          }
+        }
+        float2 s[KT / 2];
+        uint32_t* u = reinterpret_cast<uint32_t*>(s);
+        if (C::NG == 2) {
+          // the parts of the two groups, each times its scale
+#pragma unroll
+          for (int h = 0; h < KT; h += 16) {
+            uint32_t b[16];
+            TmemLoad16(a_s + h, *reinterpret_cast<uint32_t(*)[16]>(u + h));
+            TmemLoad16(a_s + 64 + h, b);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const uint4 w = *reinterpret_cast<const uint4*>(scales + (h + i) * 4);
+              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 d = __half22float2(kvd::BitsHalf(ww[e]));
+                u[h + i + e] = __float_as_uint(__uint_as_float(u[h + i + e]) * d.x + __uint_as_float(b[i + e]) * d.y);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < KT; h += 32) TmemLoad32(a_s + h, u + h);
+          TmemLoadWait();
+          if (C::QUANT) {
+#pragma unroll
+            for (int i = 0; i < KT / 2; i += 4) {
+              const uint4 w = *reinterpret_cast<const uint4*>(scales + i * 4);
+              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[i + e] = __fmul2_rn(s[i + e], __half22float2(kvd::BitsHalf(ww[e])));
+            }
+          }
+        }
+        if (bent) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i) u[i] = __float_as_uint(Bent(p, __uint_as_float(u[i]) * cs, slope, pos - pos0 - i));
+        }
+        if (EDGE) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i) {
+            if (i < from || i >= to) u[i] = __float_as_uint(-INFINITY);
+          }
+        }
+        float2 top = s[0], top2 = s[1];
+#pragma unroll
+        for (int i = 2; i < KT / 2; i += 2) {
+          top.x = fmaxf(top.x, s[i].x);
+          top.y = fmaxf(top.y, s[i].y);
+          top2.x = fmaxf(top2.x, s[i + 1].x);
+          top2.y = fmaxf(top2.y, s[i + 1].y);
+        }
+        const float mx = fmaxf(fmaxf(top.x, top.y), fmaxf(top2.x, top2.y));
+        const float to_log2 = bent ? 1.f : cs;
+        if (C::QUANT) {
+          // an exponent over the V scales that count
+          const char* vs = scales + C::NOTE / 2;
+          float most = 0.f;
+          if (EDGE) {
+            for (int i = from * C::NG; i < to * C::NG; ++i) {
+              most = fmaxf(most, fabsf(__half2float(reinterpret_cast<const __half*>(vs)[i])));
+            }
+          } else {
+            for (int i = lane; i < KT * C::NG / 2; i += 32) {
+              const float2 d = __half22float2(__habs2(reinterpret_cast<const __half2*>(vs)[i]));
+              most = fmaxf(most, fmaxf(d.x, d.y));
+            }
+            most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
+          }
+          nu = max(nu, static_cast<int>(__float_as_uint(most) >> 23) - 126);
+        }
+        m = fmaxf(m, mx * to_log2);
+        const float over = m + static_cast<float>(nu);
+        const bool grow = over > ref + static_cast<float>(kHeadroom);
+        float alpha = 1.f;
+        bool rescale = false;
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+          const float now = grow ? over - static_cast<float>(kHeadroom - kSlack) : ref;
+          if (grow && ref != -INFINITY) alpha = exp2f(ref - now);
+          ref = now;
+          l *= alpha;
+          rescale = __any_sync(0xFFFFFFFFu, alpha != 1.f);
+        }
+        if (rescale && C::TWO) {
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i) {
+            float2& a = acc[i % (C::TWO ? D / 2 : 1)];
+            a = __fmul2_rn(a, make_float2(alpha, alpha));
+          }
+        }
+        if (rescale && !C::TWO && j > 0) {
+          if (!ProductsDone()) return false;
+#pragma unroll 1
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            TmemLoad32(a_o + k, o);
+            TmemLoadWait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            TmemStore32(a_o + k, o);
+          }
+        }
+        const float less = ref == -INFINITY ? 0.f : -ref;
+        const float2 f2 = make_float2(to_log2, to_log2), less2 = make_float2(less, less);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < KT; h += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2& x = s[h / 2 + i];
+            x = __ffma2_rn(x, f2, less2);
+            x = make_float2(Exp2(x.x), Exp2(x.y));
+            if (C::TWO || C::QUANT) sum = __fadd2_rn(sum, x);
+            if (!C::QUANT) {
+              w[i] = PackHalf(x.x, x.y);
+              // (weights of one term are added up as they are used)
+              if (!C::TWO) sum = __fadd2_rn(sum, __half22float2(kvd::BitsHalf(w[i])));
+            }
+          }
+          if (!C::QUANT) {
+            TmemStore16(a_s + h / 2, w);
+            if (C::TWO) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = s[h / 2 + i], f = __half22float2(kvd::BitsHalf(w[i]));
+                w[i] = PackHalf(x.x - f.x, x.y - f.y);
+              }
+              TmemStore16(a_s + 32 + h / 2, w);
+            }
+          }
+        }
+        l += sum.x + sum.y;
+        if (C::QUANT) {
+          // times the scales of each group's values
+          const char* vs = scales + C::NOTE / 2;
+#pragma unroll
+          for (int gp = 0; gp < C::NG; ++gp) {
+#pragma unroll
+            for (int h = 0; h < KT; h += 32) {
+              uint32_t w[16], w2[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 8 / C::NG) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vs + (h + i) * 2 * C::NG);
+                const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4 / C::NG; ++e) {
+                  float2 d;
+                  if (C::NG == 2) {
+                    const float2 d0 = __half22float2(kvd::BitsHalf(xx[2 * e % 4])), d1 = __half22float2(kvd::BitsHalf(xx[(2 * e + 1) % 4]));
+                    d = gp == 0 ? make_float2(d0.x, d1.x) : make_float2(d0.y, d1.y);
+                  } else {
+                    d = __half22float2(kvd::BitsHalf(xx[e]));
+                  }
+                  const int k = h + i + 2 * e;
+                  float2 y = __fmul2_rn(s[k / 2], d);
+                  if (EDGE) {  // (a scale that the row does not see may be NaN)
+                    if (k < from || k >= to) y.x = 0.f;
+                    if (k + 1 < from || k + 1 >= to) y.y = 0.f;
+                  }
+                  const int at = (i + 2 * e) / 2;
+                  w[at] = PackHalf(y.x, y.y);
+                  if (C::TWO) {
+                    const float2 f = __half22float2(kvd::BitsHalf(w[at]));
+                    w2[at] = PackHalf(y.x - f.x, y.y - f.y);
+                  }
+                }
+              }
+              TmemStore16(a_s + gp * C::TERMS * 32 + h / 2, w);
+              if (C::TWO) TmemStore16(a_s + (gp * C::TERMS + 1) * 32 + h / 2, w2);
+            }
+          }
+        }
+        TmemStoreWait();
+        FenceBeforeSync();
+        return true;
+      };
       for (int j = 0; j < steps; ++j) {
         if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.s_full[t], s_parity))) {
           ok = false;
@@ -831,223 +1053,12 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
           const uint32_t bad = s_bad[(note0 + j) % kNotes];
           if (bad != 0 && from < to) {
             // columns from .. to - 1 in units of 16
-            const uint32_t mine_ = ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u);
-            if (bad & mine_) nan_row = true;
+            if (bad & ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u)) nan_row = true;
           }
-          const bool edge = __any_sync(0xFFFFFFFFu, from > 0 || to < KT);
           const char* scales = s_note + (note0 + j) % kNotes * C::NOTE;
-          uint32_t u[64];
-          float mx = -INFINITY;
-          // scores of 64 columns from c0 into u, in units of log2 where they are bent
-          auto columns = [&](int c0) {
-            TmemLoad32(a_s + c0, u);
-            TmemLoad32(a_s + c0 + 32, u + 32);
-            TmemLoadWait();
-          };
-          auto groups = [&]() {  // the same from the parts of two groups, each with its scale
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t b[32];
-              TmemLoad32(a_s + 32 * h, u + 32 * h);
-              if (C::NG == 2) TmemLoad32(a_s + 64 + 32 * h, b);
-              TmemLoadWait();
-#pragma unroll
-              for (int i = 0; i < 32; i += 4 / C::NG * 2) {
-                const uint4 w = *reinterpret_cast<const uint4*>(scales + (32 * h + i) * 2 * C::NG);
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 8 / C::NG; ++e) {
-                  const int k = 32 * h + i + e;
-                  if (C::NG == 2) {
-                    const float2 d = __half22float2(kvd::BitsHalf(ww[e % 4]));
-                    u[k] = __float_as_uint(__uint_as_float(u[k]) * d.x + __uint_as_float(b[(i + e) % 32]) * d.y);
-                  } else {
-                    const float2 d = __half22float2(kvd::BitsHalf(ww[e / 2 % 4]));
-                    u[k] = __float_as_uint(__uint_as_float(u[k]) * (e & 1 ? d.y : d.x));
-                  }
-                }
-              }
-            }
-          };
-          auto bend = [&](int c0) {
-            if (bent) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i) u[i] = __float_as_uint(Bent(p, __uint_as_float(u[i]) * cs, slope, pos - pos0 - c0 - i));
-            }
-          };
-          auto hide = [&](int c0) {
-            if (edge) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i) {
-                if (c0 + i < from || c0 + i >= to) u[i] = __float_as_uint(-INFINITY);
-              }
-            }
-          };
-          auto largest = [&]() {
-            float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              a = fmaxf(a, __uint_as_float(u[i]));
-              b = fmaxf(b, __uint_as_float(u[i + 1]));
-            }
-            mx = fmaxf(mx, fmaxf(a, b));
-          };
-          if (KT == 128) {
-            columns(0);
-            bend(0);
-            hide(0);
-            largest();
-            columns(64);
-            bend(64);
-            hide(64);
-            largest();
-          } else {
-            if (C::QUANT) {
-              groups();
-            } else {
-              columns(0);
-            }
-            bend(0);
-            hide(0);
-            largest();
-          }
-          const float to_log2 = bent ? 1.f : cs;
-          if (C::QUANT) {
-            // an exponent over the V scales that count
-            float top = 0.f;
-            if (edge) {
-              for (int i = from * C::NG; i < to * C::NG; ++i) {
-                top = fmaxf(top, fabsf(__half2float(reinterpret_cast<const __half*>(scales + C::NOTE / 2)[i])));
-              }
-            } else {
-              for (int i = lane; i < KT * C::NG / 2; i += 32) {
-                const float2 d = __half22float2(__habs2(reinterpret_cast<const __half2*>(scales + C::NOTE / 2)[i]));
-                top = fmaxf(top, fmaxf(d.x, d.y));
-              }
-              top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
-            }
-            nu = max(nu, static_cast<int>(__float_as_uint(top) >> 23) - 126);
-          }
-          m = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * to_log2);
-          const float over = m + static_cast<float>(nu);
-          const bool grow = over > ref + static_cast<float>(kHeadroom);
-          if (__any_sync(0xFFFFFFFFu, grow)) {
-            const float now = grow ? over - static_cast<float>(kHeadroom - kSlack) : ref;
-            const float alpha = grow && ref != -INFINITY ? exp2f(ref - now) : 1.f;
-            ref = now;
-            if (__any_sync(0xFFFFFFFFu, alpha != 1.f)) {
-              l *= alpha;
-              if (j > 0) {
-                if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) {
-                  ok = false;
-                  break;
-                }
-                FenceAfterSync();
-#pragma unroll 1
-                for (int k = 0; k < D; k += 32) {
-                  uint32_t o[32];
-                  TmemLoad32(a_o + k, o);
-                  TmemLoadWait();
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                  TmemStore32(a_o + k, o);
-                }
-                TmemStoreWait();
-              }
-            }
-          }
-          const float less = ref == -INFINITY ? 0.f : ref;
-          // weights of the 64 columns in u (hidden ones are minus infinity, whose product with a scale of 0 is not)
-          auto weights = [&](int c0) {
-            float a = 0.f, b = 0.f;
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              float x = Exp2(__uint_as_float(u[i]) * to_log2 - less), y = Exp2(__uint_as_float(u[i + 1]) * to_log2 - less);
-              if (edge) {
-                if (c0 + i < from || c0 + i >= to) x = 0.f;
-                if (c0 + i + 1 < from || c0 + i + 1 >= to) y = 0.f;
-              }
-              a += x;
-              b += y;
-              u[i] = __float_as_uint(x);
-              u[i + 1] = __float_as_uint(y);
-            }
-            l += a + b;
-          };
-          // to f16 and into tensor memory
-          auto store = [&](uint32_t dst) {
-            uint32_t h[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) h[i] = PackHalf(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-            TmemStore32(dst, h);
-            if (C::TWO) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float2 f = __half22float2(kvd::BitsHalf(h[i]));
-                h[i] = PackHalf(__uint_as_float(u[2 * i]) - f.x, __uint_as_float(u[2 * i + 1]) - f.y);
-              }
-              TmemStore32(dst + 32, h);
-            }
-          };
-          if (KT == 128) {
-            weights(64);
-            store(a_s + C::PBASE + 32);
-            columns(0);
-            bend(0);
-            hide(0);
-            weights(0);
-            store(a_s + C::PBASE);
-          } else if (C::QUANT) {
-            weights(0);
-#pragma unroll
-            for (int gp = 0; gp < C::NG; ++gp) {
-              // times the scales of the group's values
-#pragma unroll
-              for (int term = 0; term < C::TERMS; ++term) {
-                uint32_t h[32];
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  float d[4];
-                  const char* sc = scales + C::NOTE / 2 + 2 * i * 2 * C::NG;
-                  if (C::NG == 2) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(sc);
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      const float2 f = __half22float2(kvd::BitsHalf(ww[e]));
-                      d[e] = gp == 0 ? f.x : f.y;
-                    }
-                  } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(sc);
-                    const float2 f = __half22float2(kvd::BitsHalf(w.x)), f2 = __half22float2(kvd::BitsHalf(w.y));
-                    d[0] = f.x;
-                    d[1] = f.y;
-                    d[2] = f2.x;
-                    d[3] = f2.y;
-                  }
-                  float y[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    y[e] = __uint_as_float(u[2 * i + e]) * d[e];
-                    if (edge && (2 * i + e < from || 2 * i + e >= to)) y[e] = 0.f;
-                  }
-                  h[i] = PackHalf(y[0], y[1]);
-                  h[i + 1] = PackHalf(y[2], y[3]);
-                  if (term == 1) {
-                    const float2 f = __half22float2(kvd::BitsHalf(h[i])), f2 = __half22float2(kvd::BitsHalf(h[i + 1]));
-                    h[i] = PackHalf(y[0] - f.x, y[1] - f.y);
-                    h[i + 1] = PackHalf(y[2] - f2.x, y[3] - f2.y);
-                  }
-                }
-                TmemStore32(a_s + (gp * C::TERMS + term) * 32, h);
-              }
-            }
-          } else {
-            weights(0);
-            store(a_s);
-          }
-          TmemStoreWait();
-          FenceBeforeSync();
+          ok = __any_sync(0xFFFFFFFFu, valid && (from > 0 || to < KT)) ? step(std::true_type(), j, from, to, pos0, scales)
+                                                                       : step(std::false_type(), j, from, to, pos0, scales);
+          if (!ok) break;
         }
         __syncwarp();
         if (lane == 0) MbarArrive(&bars.p_full[t]);
@@ -1064,7 +1075,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
       if (active) {
         const Join jn = valid && whole ? Join(p, row_head, ref, l) : Join(p, 0, 0.f, 0.f);
         float check = 0.f;
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < D; k += 32) {
           uint32_t o[32];
           TmemLoad32(a_o + k, o);
@@ -1073,6 +1084,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             y[i] = __uint_as_float(o[i]);
+            if (C::TWO) y[i] += reinterpret_cast<const float*>(acc)[(k + i) % (C::TWO ? D : 1)];
             check += y[i] * 0.f;
           }
           if (valid && whole) {
@@ -1094,7 +1106,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
             for (int i = 0; i < 32; i += 8) {
               uint32_t w[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = o[i + e];
+              for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(y[i + e]);
               kvd::Store32(rec + r * D + k + i, w);
             }
           }
