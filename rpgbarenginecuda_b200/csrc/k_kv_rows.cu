@@ -1,6 +1,10 @@
 // k_kv_rows.cu -- attention of several rows that read one page list: new tokens
 // of a conversation, or the conversations of a group over what they share.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "common.h"
@@ -62,15 +66,23 @@ __device__ __forceinline__ void Put(void* out, ElemType t, int64_t i, float x) {
   }
 }
 
-// A score of the formula (capped, biased) in units of log2.
-__device__ __forceinline__ float Bent(const KvRowsParams& p, float x, float slope, int distance) {
-  if (p.cap > 0.f) {
-    // tanh |t| = (1 - e) / (1 + e) with e = exp(-2 |t|)
-    const float e = Exp2(fabsf(x) * (-2.f * kLog2e) / p.cap);
-    x = copysignf(p.cap * __fdividef(1.f - e, 1.f + e), x) + x * 0.f;  // (NaN stays NaN)
+// What scores are bent by, in units of log2.
+struct Bend {
+  float rate, cap, slope;
+  bool capped, biased;
+  __device__ __forceinline__ explicit Bend(const KvRowsParams& p, float slope_)
+      : rate(p.cap > 0.f ? -2.f * kLog2e / p.cap : 0.f), cap(p.cap * kLog2e), slope(slope_ * kLog2e), capped(p.cap > 0.f),
+        biased(p.slopes != nullptr) {}
+  // cap tanh(x / cap) of a score of the formula: tanh |t| = (1 - e) / (1 + e) with e = exp(-2 |t|)
+  __device__ __forceinline__ float Capped(float x) const {
+    const float e = Exp2(fabsf(x) * rate);
+    return copysignf(cap * __fdividef(1.f - e, 1.f + e), x);
   }
-  return (x - slope * static_cast<float>(abs(distance))) * kLog2e;
-}
+  __device__ __forceinline__ float operator()(float x, int distance) const {
+    x = capped ? Capped(x) : x * kLog2e;
+    return biased ? x - slope * fabsf(static_cast<float>(distance)) : x;
+  }
+};
 
 // One row by the formula, a position at a time, by a warp.
 template <int D, KvType KIND>
@@ -78,6 +90,7 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
                                          int from, int to, float (&acc)[D / 32], float& m, float& l) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
+  const Bend bend(p, slope);
   float x[N];
   l = 0.f;
   m = -INFINITY;
@@ -128,7 +141,7 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
     float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) dot += x[e] * k[e];
-    const float s = Bent(p, dev::WarpSum(dot) * p.scale, slope, pos - at);
+    const float s = bend(dev::WarpSum(dot) * p.scale, pos - at);
     const float now = fmaxf(m, s), ref = now == -INFINITY ? 0.f : now;
     const float alpha = Exp2(m - ref), w = Exp2(s - ref);
     m = now;
@@ -169,7 +182,7 @@ struct Cfg {
   static constexpr int QTERM = BOX * kTileRows * 128, QTILE = TERMS * QTERM;
   static constexpr int PLANE = BOX * KT * 128;
   static constexpr int STAGES = QUANT && !TWO ? 3 : 2;
-  static constexpr int LAG = QUANT && !TWO ? 4 : 2;  // copies begun before the oldest is waited for
+  static constexpr int LAG = QUANT && !TWO ? 4 : 2;  // copies of codes begun before the oldest is waited for
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;
   static constexpr int PER = KT * CPR / (32 * kLoadWarps);  // 16-byte pieces of a thread
@@ -266,13 +279,14 @@ template <int N>
 __device__ __forceinline__ void CopyWait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ bool MbarTest(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-               : "=r"(ok)
-               : "r"(dev::SmemAddr(bar)), "r"(parity)
-               : "memory");
-  return ok != 0;
+// 16 positions of 64 values of a head's page.
+__device__ __forceinline__ void LoadTile(void* dst, const CUtensorMap* map, int value, int at, int head, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dev::SmemAddr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(value), "r"(at), "r"(head), "r"(page), "r"(dev::SmemAddr(bar))
+      : "memory");
 }
 __device__ __forceinline__ void TmemLoad32(uint32_t a, uint32_t* r) {
   asm volatile(
@@ -295,19 +309,36 @@ __device__ __forceinline__ void TmemStore32(uint32_t a, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// A in tensor memory, B in shared memory.
-__device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Operands in shared memory as the low words of their descriptors; the high
+// word is the same for all: 1024 bytes between groups of eight 128-byte rows,
+// version 1, the 128-byte swizzle.  One thread issues a product in about 115
+// cycles where it works out 64-bit descriptors, loops and branches for each,
+// which is twice what the product takes; unrolled and with 32-bit sums it keeps
+// up.
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+// A tile whose rows are 128 bytes along the sum (q and K).
+__device__ __forceinline__ uint32_t DescRows(uint32_t a) { return a >> 4 | 1u << 16; }
+// V: the sum runs over rows, and the next 64 values are `box` bytes on.
+__device__ __forceinline__ uint32_t DescV(uint32_t a, int box) { return a >> 4 | static_cast<uint32_t>(box >> 4) << 16; }
+__device__ __forceinline__ void MmaSs(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(kDescHigh)
       : "memory");
 }
-// Descriptor of 16 positions of a V tile: values are contiguous (128-byte
-// rows, swizzled), 8 positions 1024 bytes apart, the next 64 values `box` bytes on.
-__device__ __forceinline__ uint64_t DescV(uint32_t a, int box) {
-  return static_cast<uint64_t>((a >> 4) & 0x3FFFu) | static_cast<uint64_t>(box >> 4) << 16 |
-         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+// A in tensor memory.
+__device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(kDescHigh)
+      : "memory");
+}
+// A value that is worked out here and not kept over loops (32 of them would be spilled).
+__device__ __forceinline__ uint32_t Here(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return kvd::HalfBits(__floats2half2_rn(lo, hi)); }
 
@@ -394,52 +425,81 @@ __device__ __forceinline__ void Put32(const KvRowsParams& p, bool wide, int64_t 
   }
 }
 
-// Queries of one row: f16 terms of q times 2^-e (a largest value in [2^12,
-// 2^13), the sign of the softmax scale in them) into the tile.  Returns the
-// factor from products to scores in units of log2 (scores of the formula where
-// they are capped or biased), NaN for a row that is not finite.
+// Queries of one row into the tile, the sign of the softmax scale in them:
+// f16 ones as they are, others times 2^-e (a largest value in [2^12, 2^13)) as
+// f16 terms.  Returns the factor from products to scores, NaN for a row that is
+// not finite.
 template <typename C, typename T>
 __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char* tile, int row) {
+  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, __half>::value;
   kvd::Raw8<T> q[C::D / 8];  // all of the row on its way at once
 #pragma unroll
   for (int c = 0; c < C::D / 8; ++c) q[c].Load(static_cast<const T*>(p.q) + at + 8 * c);
-  float most = 0.f, bad = 0.f;
+  // the bits of the largest magnitude: those of infinity and NaN are above all others
+  uint32_t most = 0;
 #pragma unroll
   for (int c = 0; c < C::D / 8; ++c) {
-    float x[8];
-    q[c].Floats(x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = fmaxf(most, fabsf(x[i]));
-      bad += x[i] * 0.f;
+    for (int i = 0; i < kvd::Raw8<T>::N; ++i) {
+      for (const uint32_t w : {q[c].w[i].x, q[c].w[i].y, q[c].w[i].z, q[c].w[i].w}) {
+        most = kF32 ? max(most, w & 0x7FFFFFFFu) : __vmaxu2(most, w & 0x7FFF7FFFu);
+      }
     }
   }
-  const int e = most > 0.f ? min(max(static_cast<int>(__float_as_uint(most) >> 23), 1), 254) - 127 - 12 : 0;
-  // 2^-e in two factors: each is a normal number
-  const float f0 = __uint_as_float(static_cast<uint32_t>(127 - e / 2) << 23);
-  const float f1 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
-  const float s1 = p.scale < 0.f ? -f1 : f1;
+  if (!kF32) most = max(most & 0xFFFFu, most >> 16) << 16;
+  const bool finite = most < (kF16 ? 0x7C000000u : 0x7F800000u);
+  const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0;
+  float f0 = 1.f, f1 = 1.f;
+  if (!kF16) {
+    const int e = most > 0 && finite ? max(static_cast<int>(most >> 23), 1) - 127 - 12 : 0;
+    // 2^-e in two factors: each is a normal number
+    f0 = __uint_as_float(static_cast<uint32_t>(127 - e / 2) << 23);
+    f1 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
+  }
 #pragma unroll
   for (int c = 0; c < C::D / 8; ++c) {
-    float x[8];
-    q[c].Floats(x);
     uint32_t hi[4], lo[4];
+    if (kF16) {
+      const uint4 w = q[c].w[0];
+      hi[0] = w.x ^ sign;
+      hi[1] = w.y ^ sign;
+      hi[2] = w.z ^ sign;
+      hi[3] = w.w ^ sign;
+    } else {
+      float x[8];
+      q[c].Floats(x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = x[2 * i] * f0 * s1, b = x[2 * i + 1] * f0 * s1;
-      hi[i] = PackHalf(a, b);
-      const float2 h = __half22float2(kvd::BitsHalf(hi[i]));
-      lo[i] = PackHalf(a - h.x, b - h.y);
+      for (int i = 0; i < 4; ++i) {
+        const float2 y = __fmul2_rn(__fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(f0, f0)), make_float2(f1, f1));
+        hi[i] = PackHalf(y.x, y.y);
+        if (C::TWO) {
+          const float2 h = __half22float2(kvd::BitsHalf(hi[i]));
+          lo[i] = PackHalf(y.x - h.x, y.y - h.y) ^ sign;
+        }
+        hi[i] ^= sign;
+      }
     }
     char* dst = tile + (c >> 3) * (kTileRows * 128) + Swz(row, c & 7);
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (C::TWO) *reinterpret_cast<uint4*>(dst + C::QTERM) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  return fabsf(p.scale) / f0 / f1 + bad;
+  return finite ? fabsf(p.scale) / f0 / f1 : kvd::Nan();
 }
 
+// A row of an item, as the thread that has it sees it.
+struct RowState {
+  Item it;
+  int note0;  // steps before the item
+  int row, qh;
+  Seen seen;
+  float cs, slope;  // scores (in units of log2 where they are not capped) are products times cs
+  int pos;
+  bool valid, active, is_nan;  // active: some row of the warp is valid
+};
+
 template <typename C>
-__global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, uint32_t magic) {
+__global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const KvRowsParams p,
+               uint32_t magic) {
   using namespace tc;
   constexpr int D = C::D, KT = C::KT;
   extern __shared__ char smem_raw[];
@@ -589,8 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     if (lane == 0) {
       constexpr uint32_t id_s = InstrDesc(128, KT);
       constexpr uint32_t id_o = InstrDesc(128, C::NG == 1 ? D : 64) | 1u << 16;  // (V: values contiguous)
-      const uint64_t d_q = DescSw128(s_q), d_k = DescSw128(s_k);
-      const uint32_t a_v = dev::SmemAddr(s_v);
+      const uint32_t a_q = dev::SmemAddr(s_q), a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v);
       int n = 0;
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
       int c = 0;  // steps so far
@@ -612,16 +671,17 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
               p_parity[t] ^= 1;
               FenceAfterSync();
               const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128;
+              // with two terms every step's product starts anew (it is added up in registers)
+              const bool going_on = !C::TWO && j > 1;
 #pragma unroll
               for (int g = 0; g < C::NG; ++g) {
 #pragma unroll
                 for (int term = C::TERMS - 1; term >= 0; --term) {
+                  const uint32_t v = Here(DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
+                  const uint32_t a = Here(w + (g * C::TERMS + term) * (KT / 2)), d = Here(o + 64 * g);
 #pragma unroll
                   for (int k = 0; k < KT / 16; ++k) {
-                    const uint64_t v = DescV(a_v + st * C::PLANE + g * (KT * 128) + k * 2048, KT * 128);
-                    // with two terms every step's product starts anew (it is added up in registers)
-                    MmaTs(o + 64 * g, w + (g * C::TERMS + term) * (KT / 2) + 8 * k, v, id_o,
-                          (!C::TWO && j > 1) || k > 0 || term < C::TERMS - 1 ? 1u : 0u);
+                    MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
                   }
                 }
               }
@@ -639,13 +699,14 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
 #pragma unroll
               for (int term = C::TERMS - 1; term >= 0; --term) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                  const int g = C::NG == 1 ? 0 : k / 4;
-                  const uint64_t adv = static_cast<uint64_t>((k & 3) * 2);
-                  const uint64_t kd = d_k + ((st * C::PLANE + (k >> 2) * (KT * 128)) >> 4) + adv;
-                  Mma(tmem + t * 128 + 64 * g,
-                      d_q + ((t * C::QTILE + term * C::QTERM + (k >> 2) * (kTileRows * 128)) >> 4) + adv, kd, id_s,
-                      (C::NG == 1 ? k > 0 : (k & 3) > 0) || term < C::TERMS - 1 ? 1u : 0u);
+                for (int box = 0; box < C::BOX; ++box) {
+                  const uint32_t d = Here(tmem + t * 128 + (C::NG == 2 ? 64 * box : 0));
+                  const uint32_t q = Here(DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
+                  const uint32_t kk = Here(DescRows(a_k + st * C::PLANE + box * (KT * 128)));
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
+                  }
                 }
               }
               MmaCommit(&bars.s_full[t]);
@@ -662,49 +723,46 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
   } else {
     // ---- copies
     const int lt = tid - 32 * kLoadWarp0, lw = lt >> 5;
-    const uint32_t a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v), a_raw = dev::SmemAddr(s_raw),
-                   a_note = dev::SmemAddr(s_note);
+    const int mask = (1 << p.kv.page_log2) - 1;
+    int begun = 0, ended = 0;  // copies: 2 n is K's of step n, 2 n + 1 V's
+    bool ok = true;
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // (what kernels before this one stored is read by copies)
+    const uint32_t a_raw = dev::SmemAddr(s_raw), a_note = dev::SmemAddr(s_note);
     const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
     constexpr int kRowStep = 32 * kLoadWarps / C::CPR;
-    const int mask = (1 << p.kv.page_log2) - 1;
-    int begun = 0, ended = 0;  // copies: step 2 n is K's, 2 n + 1 V's
-    bool ok = true;
-    // the oldest copy has arrived: for codes, spread them to f16; tell the products
+    // The oldest copy of codes has arrived: spread them to f16, tell the products.
     auto finish = [&]() {
       const int step = ended >> 1, st = step % C::STAGES;
       const bool v = ended & 1;
-      if (C::QUANT) {
-        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(v ? &bars.v_empty[st] : &bars.k_empty[st],
-                                                   ((step / C::STAGES) & 1) ^ 1))) {
-          ok = false;
-          return;
-        }
-        const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
-        char* dst = (v ? s_v : s_k) + st * C::PLANE;
+      if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(v ? &bars.v_empty[st] : &bars.k_empty[st], ((step / C::STAGES) & 1) ^ 1))) {
+        ok = false;
+        return;
+      }
+      const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
+      char* dst = (v ? s_v : s_k) + st * C::PLANE;
 #pragma unroll 2
-        for (int i = 0; i < C::PER; ++i) {
-          const int r = r0 + i * kRowStep;
-          const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
-          constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
+      for (int i = 0; i < C::PER; ++i) {
+        const int r = r0 + i * kRowStep;
+        const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
+        constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            kvd::Codes16<C::KIND> code;
-            if (C::KIND == KvType::kQ8) {
-              code.w[0] = w.x;
-              code.w[1] = w.y;
-              code.w[C::KIND == KvType::kQ8 ? 2 : 0] = w.z;
-              code.w[C::KIND == KvType::kQ8 ? 3 : 0] = w.w;
-            } else {
-              code.w[0] = h == 0 ? w.x : w.z;
-              code.w[1] = h == 0 ? w.y : w.w;
-            }
-            uint32_t y[8];
-            code.Pairs(y, magic);
-            const int u = (c0 * kHalves + h) * 2;  // 8-value chunk of the row
-            char* d = dst + (u >> 3) * (KT * 128);
-            *reinterpret_cast<uint4*>(d + Swz(r, u & 7)) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+        for (int h = 0; h < kHalves; ++h) {
+          kvd::Codes16<C::KIND> code;
+          if (C::KIND == KvType::kQ8) {
+            code.w[0] = w.x;
+            code.w[1] = w.y;
+            code.w[C::KIND == KvType::kQ8 ? 2 : 0] = w.z;
+            code.w[C::KIND == KvType::kQ8 ? 3 : 0] = w.w;
+          } else {
+            code.w[0] = h == 0 ? w.x : w.z;
+            code.w[1] = h == 0 ? w.y : w.w;
           }
+          uint32_t y[8];
+          code.Pairs(y, magic);
+          const int u = (c0 * kHalves + h) * 2;  // 8-value chunk of the row
+          char* d = dst + (u >> 3) * (KT * 128);
+          *reinterpret_cast<uint4*>(d + Swz(r, u & 7)) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
         }
       }
       dev::FenceProxyAsync();
@@ -715,16 +773,16 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     Reader rd;
     Item it;
     while (ok && rd.Next(bars, items, it, lane)) {
-      int page = -1, next = -1;
-      auto lookup = [&](int pos) {  // page of the lane's 16 positions
+      // lane g has to do with positions 16 g .. 16 g + 15 of a step: their page
+      auto lookup = [&](int pos) {
         return lane < KT / 16 && pos + 16 > it.lo && pos < it.hi
                    ? p.table.pages[it.table_row * p.table.stride + (pos >> p.kv.page_log2)]
                    : -1;
       };
-      next = lookup(it.base + it.step0 * KT + 16 * lane);
+      int next = lookup(it.base + it.step0 * KT + 16 * lane);
       for (int j = 0; j < it.steps && ok; ++j) {
         const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
-        page = next;
+        const int page = next;
         if (j + 1 < it.steps) next = lookup(at + KT);
         const bool used = lane < KT / 16 && at + 16 > it.lo && at < it.hi;
         const bool there = used && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
@@ -732,61 +790,107 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
         const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
         const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
         if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
+        if (!C::QUANT) {
+          // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
+          const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
+          constexpr uint32_t kEvery = 0x55555555u & ((1u << KT / 16) - 1);  // groups of warp 0
+          const uint32_t groups = kEvery << lw;
+          const int g = lw + 2 * (lane / C::BOX), box = lane % C::BOX;
+          const int pg = __shfl_sync(0xFFFFFFFFu, page, g & 31), in = (pos0 + 16 * g) & mask;
 #pragma unroll 1
-        for (int v = 0; v < 2; ++v) {
-          const int st = (begun >> 1) % C::STAGES;
-          if (!C::QUANT) {
-            uint64_t* bar = v ? &bars.v_empty[st] : &bars.k_empty[st];
-            const uint32_t parity = (((begun >> 1) / C::STAGES) & 1) ^ 1;
-            if (!__all_sync(0xFFFFFFFFu, MbarTest(bar, parity))) {
-              if (ended < begun) {  // what has been begun is of use before there is room for more
-                CopyWait<0>();
-                while (ended < begun) finish();
+          for (int v = 0; v < 2; ++v) {
+            const int st = (begun >> 1) % C::STAGES;
+            uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
+            if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
+              ok = false;
+              break;
+            }
+            char* dst = (v ? s_v : s_k) + st * C::PLANE;
+            const uint32_t take = (v ? full : have) & groups;
+            uint32_t rest = v ? groups & ~full : 0;
+            if (rest != 0) {
+              // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
+              while (rest != 0) {
+                const int q = __ffs(rest) - 1;
+                rest &= rest - 1;
+                const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
+#pragma unroll 1
+                for (int i = lane; i < 16 * C::CPR; i += 32) {
+                  const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
+                  const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
+                  CopyAsync16(dev::SmemAddr(dst + (c >> 3) * (KT * 128) + Swz(16 * q + r, c & 7)),
+                              seen ? src + r * p.kv.pos_stride + c * 16 : p.kv.v, seen);
+                }
               }
-              if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(bar, parity))) {
-                ok = false;
-                break;
+              CopyCommit();
+              CopyWait<0>();
+              dev::FenceProxyAsync();
+            }
+            __syncwarp();
+            if (lane == 0) dev::MbarExpectTx(whole, __popc(take) * (C::BOX * 2048));  // (an arrival too)
+            __syncwarp();
+            if (lane < KT / 32 * C::BOX && ((take >> g) & 1)) {
+              LoadTile(dst + box * (KT * 128) + g * 2048, v ? &map_v : &map_k, 64 * box, in, it.head, pg, whole);
+            }
+            ++begun;
+          }
+          ended = begun;
+        } else {
+#pragma unroll 1
+          for (int v = 0; v < 2 && ok; ++v) {
+            const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
+            const uint32_t dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
+            // 16 positions at a time: rows r0 + k * kRowStep of them are this thread's
+#pragma unroll 1
+            for (int g = 0; g < KT / 16; ++g) {
+              const char* src = plane + __shfl_sync(0xFFFFFFFFu, off, g);
+              const bool have_g = (have >> g) & 1;
+              const int first = pos0 + 16 * g;
+              auto copy = [&](uint32_t to, int r) {
+                const bool in = have_g && first + r >= it.lo && first + r < it.hi;
+                CopyAsync16(to, in ? src + r * p.kv.pos_stride : plane, in);
+              };
+              if (kRowStep > 16) {  // (a thread has rows of every other sixteen)
+                constexpr int kSkip = kRowStep > 16 ? kRowStep / 16 : 1;
+                if ((r0 >> 4) == g % kSkip) copy(dst + g / kSkip * (32 * kLoadWarps * 16), r0 & 15);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 16 / kRowStep; ++k) copy(dst + g * (16 * C::ROW) + k * (kRowStep * C::ROW), r0 + k * kRowStep);
               }
             }
-          }
-          const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
-          uint32_t dst;
-          if (C::QUANT) {
-            dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
-          } else {
-            dst = (v ? a_v : a_k) + st * C::PLANE + (c0 >> 3) * (KT * 128);
-          }
-#pragma unroll 4
-          for (int i = 0; i < C::PER; ++i) {
-            const int r = r0 + i * kRowStep, pos = pos0 + r;
-            const int64_t o = __shfl_sync(0xFFFFFFFFu, off, r >> 4) + (r & 15) * p.kv.pos_stride;
-            const bool in = ((have >> (r >> 4)) & 1) && pos >= it.lo && pos < it.hi;
-            CopyAsync16(C::QUANT ? dst + i * (32 * kLoadWarps * 16) : dst + Swz(r, c0 & 7), in ? plane + o : plane, in);
-          }
-          if (C::QUANT && v == 0) {
-            // scales of K and V: 16 positions are dense, 2 NG 16-byte pieces
-            constexpr int kPer = 2 * C::NG;
-            const int i = lane / kPer % (KT / 16);
-            const int64_t so = there ? kvd::ScaleOffset(p.kv, page, it.head, at & mask) : 0;
-            const int64_t o = __shfl_sync(0xFFFFFFFFu, so, i) + lane % kPer * 16;
-            if (lw < 2 && lane < KT / 16 * kPer) {
-              const bool in = (have >> i) & 1;
-              const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
-              CopyAsync16(a_note + (begun >> 1) % kNotes * C::NOTE + lw * (C::NOTE / 2) + lane * 16, in ? src + o : src, in);
+            if (v == 0) {
+              // scales of K and V: 16 positions are dense, 2 NG 16-byte pieces
+              constexpr int kPer = 2 * C::NG;
+              const int i = lane / kPer % (KT / 16);
+              const int64_t so = there ? kvd::ScaleOffset(p.kv, page, it.head, at & mask) : 0;
+              const int64_t o = __shfl_sync(0xFFFFFFFFu, so, i) + lane % kPer * 16;
+              if (lane < KT / 16 * kPer) {
+                const bool in = (have >> i) & 1;
+                const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
+                CopyAsync16(a_note + (begun >> 1) % kNotes * C::NOTE + lw * (C::NOTE / 2) + lane * 16, in ? src + o : src, in);
+              }
             }
-          }
-          CopyCommit();
-          ++begun;
-          if (begun - ended > C::LAG) {
-            CopyWait<C::LAG>();
-            finish();
-            if (!ok) break;
+            CopyCommit();
+            ++begun;
+            if (begun - ended > C::LAG) {
+              CopyWait<C::LAG>();
+              finish();
+            }
           }
         }
       }
     }
-    CopyWait<0>();
-    while (ok && ended < begun) finish();
+    if (C::QUANT) {
+      CopyWait<0>();
+      while (ok && ended < begun) finish();
+    } else if (begun > 0) {
+      // copies that nobody waits for any more have landed before the block ends
+      for (int n = max(0, begun / 2 - C::STAGES); n < begun / 2; ++n) {
+        const int st = n % C::STAGES;
+        dev::MbarWait(&bars.k_full[st], (n / C::STAGES) & 1);
+        dev::MbarWait(&bars.v_full[st], (n / C::STAGES) & 1);
+      }
+    }
   }
   } else {
     // ---- softmax: a thread per row
@@ -796,44 +900,64 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
     const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128;
     const int size = p.type == ElemType::kF32 ? 4 : 2;
     const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.out_stride * size)) & 31) == 0;
-    const bool bent = p.cap > 0.f || p.slopes != nullptr;
     uint32_t s_parity = 0;
     int c = 0, note = 0;  // products with V begun for this tile; steps so far
     bool ok = true;
     Reader rd;
-    Item it;
-    while (ok && rd.Next(bars, items, it, lane)) {
-      const int steps = it.steps, note0 = note;
-      note += steps;
-      if (t == 1 && it.n_tok * sp.per <= kTileRows) continue;
-      const int tok = r / sp.per, g = r - tok * sp.per + it.chunk * sp.per;
-      const bool valid = tok < it.n_tok && g < sp.group;
-      const bool active = __any_sync(0xFFFFFFFFu, valid);
-      const int row = it.row0 + tok, qh = it.head * sp.group + g;
-      const int64_t q_at = row * p.q_stride + static_cast<int64_t>(qh) * D;
-      Seen seen{0, 0, false};
-      float cs = 0.f, slope = 0.f;
-      int pos = 0;
-      bool nan_row = false;
-      if (valid) {
-        seen = SeenBy(p, row);
-        nan_row = seen.past || (seen.start < seen.end && (seen.start < it.lo || seen.end > it.hi)) ||
-                  (p.prefix != nullptr && p.prefix[row] > it.first_prefix);
+    // The next item that this tile has rows of, and what the thread has to know of its row.
+    auto next_item = [&](RowState& w) {
+      do {
+        if (!rd.Next(bars, items, w.it, lane)) return false;
+        w.note0 = note;
+        note += w.it.steps;
+      } while (t == 1 && w.it.n_tok * sp.per <= kTileRows);
+      const int tok = r / sp.per, g = r - tok * sp.per + w.it.chunk * sp.per;
+      w.valid = tok < w.it.n_tok && g < sp.group;
+      w.active = __any_sync(0xFFFFFFFFu, w.valid);
+      w.row = w.it.row0 + tok;
+      w.qh = w.it.head * sp.group + g;
+      w.seen = Seen{0, 0, false};
+      w.cs = w.slope = 0.f;
+      w.pos = 0;
+      w.is_nan = false;
+      return true;
+    };
+    auto write_q = [&](RowState& w) {
+      if (w.valid) {
+        const int64_t q_at = w.row * p.q_stride + static_cast<int64_t>(w.qh) * D;
         char* tile = s_q + t * C::QTILE;
-        cs = p.type == ElemType::kF32 ? WriteQ<C, float>(p, q_at, tile, in_tile)
-                                      : (p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
-                                                                  : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile));
-        if (!(cs == cs)) nan_row = true;
-        if (!bent) cs = fmaxf(cs * kLog2e, 1e-37f);  // (a scale of 0: minus infinity times it is to stay)
+        if (C::TWO) {
+          w.cs = WriteQ<C, float>(p, q_at, tile, in_tile);
+        } else {
+          w.cs = p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
+                                          : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile);
+        }
+        w.seen = SeenBy(p, w.row);
+        const Seen& s = w.seen;
+        w.is_nan = s.past || (s.start < s.end && (s.start < w.it.lo || s.end > w.it.hi)) || !(w.cs == w.cs) ||
+                   (p.prefix != nullptr && p.prefix[w.row] > w.it.first_prefix);
+        if (!(p.cap > 0.f)) w.cs = fmaxf(w.cs * kLog2e, 1e-37f);  // (a scale of 0: minus infinity times it is to stay)
         if (p.slopes != nullptr) {
-          slope = p.slopes[qh];
-          pos = p.pos[row];
+          w.slope = p.slopes[w.qh];
+          w.pos = p.pos[w.row];
         }
       }
       dev::FenceProxyAsync();
       __syncwarp();
       if (lane == 0) MbarArrive(&bars.q_full[t]);
-
+    };
+    RowState now;
+    bool more = next_item(now);
+    if (more) write_q(now);
+    while (ok && more) {
+      const Item& it = now.it;
+      const int steps = it.steps, note0 = now.note0, row = now.row, qh = now.qh;
+      const Seen seen = now.seen;
+      const float cs = now.cs, slope = now.slope;
+      const int pos = now.pos;
+      const bool valid = now.valid, active = now.active;
+      bool nan_row = now.is_nan;
+      const Bend bend(p, slope);
       float m = -INFINITY, ref = -INFINITY, l = 0.f;
       int nu = C::QUANT ? -30 : 0;
       float2 acc[C::TWO ? D / 2 : 1];  // the result of the steps before the last
@@ -897,9 +1021,16 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
             }
           }
         }
-        if (bent) {
+        if (bend.capped) {
 #pragma unroll
-          for (int i = 0; i < KT; ++i) u[i] = __float_as_uint(Bent(p, __uint_as_float(u[i]) * cs, slope, pos - pos0 - i));
+          for (int i = 0; i < KT; ++i) u[i] = __float_as_uint(bend.Capped(__uint_as_float(u[i]) * cs));
+        }
+        if (bend.biased) {
+          const float first = static_cast<float>(pos - pos0), f = bend.capped ? 1.f : cs;
+#pragma unroll
+          for (int i = 0; i < KT; ++i) {
+            u[i] = __float_as_uint(__uint_as_float(u[i]) * f - bend.slope * fabsf(first - static_cast<float>(i)));
+          }
         }
         if (EDGE) {
 #pragma unroll
@@ -916,7 +1047,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
           top2.y = fmaxf(top2.y, s[i + 1].y);
         }
         const float mx = fmaxf(fmaxf(top.x, top.y), fmaxf(top2.x, top2.y));
-        const float to_log2 = bent ? 1.f : cs;
+        const float to_log2 = bend.capped || bend.biased ? 1.f : cs;
         if (C::QUANT) {
           // an exponent over the V scales that count
           const char* vs = scales + C::NOTE / 2;
@@ -1064,6 +1195,12 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
         if (lane == 0) MbarArrive(&bars.p_full[t]);
         ++c;
       }
+      // The next item's queries go into the place of this one's (whose products
+      // with K are done) before this one's result is taken, so that the tensor
+      // cores have work meanwhile.  (With two terms the registers do not hold both.)
+      RowState then;
+      more = ok && next_item(then);
+      if (!C::TWO && more) write_q(then);
       // ---- the end of the item, or of this block's piece of it
       if (ok && !__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) ok = false;
       FenceAfterSync();
@@ -1125,7 +1262,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
             const int start = __shfl_sync(0xFFFFFFFFu, seen.start, w), end = __shfl_sync(0xFFFFFFFFu, seen.end, w);
             constexpr int N = D / 32;
             float acc[N], pm, pl;
-            PlainRow<D, C::KIND>(p, it.table_row, it.head, __shfl_sync(0xFFFFFFFFu, q_at, w),
+            PlainRow<D, C::KIND>(p, it.table_row, it.head, __shfl_sync(0xFFFFFFFFu, row * p.q_stride + static_cast<int64_t>(qh) * D, w),
                                  __shfl_sync(0xFFFFFFFFu, slope, w), __shfl_sync(0xFFFFFFFFu, pos, w), max(start, from),
                                  min(end, to), acc, pm, pl);
             const int rr = __shfl_sync(0xFFFFFFFFu, r, w);
@@ -1150,6 +1287,8 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const KvRowsParams p, 
         }
       }
       FenceBeforeSync();  // (what was read of tensor memory, before the next item's products)
+      if (C::TWO && more) write_q(then);
+      now = then;
     }
   }
   __syncthreads();
@@ -1228,6 +1367,36 @@ __global__ void __launch_bounds__(256) RowsJoinKernel(const KvRowsParams p) {
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 Encode() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }
+  });
+  RPGB_CHECK(fn != nullptr, "kv: cuTensorMapEncodeTiled is unavailable");
+  return fn;
+}
+
+// A plane of an f16 cache, [page][head][position][value] by its strides.
+CUtensorMap PlaneMap(const KvPages& kv, char* plane) {
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), cuuint64_t{1} << kv.page_log2,
+                              static_cast<cuuint64_t>(kv.n_kv), static_cast<cuuint64_t>(kv.n_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv.pos_stride), static_cast<cuuint64_t>(kv.head_stride),
+                                 static_cast<cuuint64_t>(kv.page_stride)};
+  const cuuint32_t box[4] = {64, 16, 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUresult r = Encode()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, plane, dims, strides, box, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RPGB_CHECK(r == CUDA_SUCCESS, "kv: tensor map encoding failed (%d)", static_cast<int>(r));
+  return m;
+}
+
 template <typename C>
 int Grid() {
   static std::atomic<int> grids[64];
@@ -1248,8 +1417,13 @@ int Grid() {
 template <typename C>
 void Launch(const KvRowsParams& p, cudaStream_t s) {
   const int grid = Grid<C>();
-  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, p,
-                   kvd::kMagic);
+  CUtensorMap map_k{}, map_v{};
+  if (!C::QUANT) {
+    map_k = PlaneMap(p.kv, p.kv.k);
+    map_v = PlaneMap(p.kv, p.kv.v);
+  }
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, map_k, map_v,
+                   p, kvd::kMagic);
   LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, 8), dim3(256), 0, s, true, p);
 }
 
