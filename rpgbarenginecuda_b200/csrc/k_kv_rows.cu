@@ -166,7 +166,6 @@ constexpr int kMaxBlocks = 160;
 constexpr int kItems = 4;    // items described ahead
 constexpr int kNotes = 8;    // steps whose scales and bad pages are held
 constexpr int kLeast = 2;    // steps that a block is started for
-constexpr int kBorder = 2;   // steps that the end of an item is worth
 constexpr int kHeadroom = 15, kSlack = 8;  // weights are at most 2^15, and 2^7 when their reference was set
 
 template <int D_, KvType KIND_, bool TWO_>
@@ -188,6 +187,7 @@ struct Cfg {
   static constexpr int PER = KT * CPR / (32 * kLoadWarps);  // 16-byte pieces of a thread
   static constexpr int RAW = QUANT ? KT * ROW : 0;
   static constexpr int NOTE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
+  static constexpr int BORDER = TWO ? 5 : (QUANT ? 6 : 4);  // steps that the beginning and end of an item are worth
   static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kNotes * NOTE;
   static_assert(SMEM <= 230 * 1024, "shared memory");
 };
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     if (slot_lo < slot_hi) sl.Seek(p, sp, slot_lo);
     for (int i = slot_lo; i < slot_hi; ++i) {
       const int steps = sl.Get(p, sp, i, it);
-      mine += steps > 0 ? steps + kBorder : 0;
+      mine += steps > 0 ? steps + C::BORDER : 0;
     }
   }
   long long incl = mine;
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       it.steps = 0;
       if (x < x1) {
         const int steps = sl.Get(p, sp, slot, it);
-        const int weight = steps > 0 ? steps + kBorder : 0;
+        const int weight = steps > 0 ? steps + C::BORDER : 0;
         if (steps <= skip) {  // nothing of it, or its border alone
           x += weight > skip ? weight - skip : 0;
           skip -= min(skip, static_cast<long long>(weight));
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             job.chunk = it.chunk;
             job.last = min(max(ShareOf(x + steps - 1, total, blocks), block), blocks - 1);
           }
-          x += it.steps + (it.ends ? kBorder : 0);
+          x += it.steps + (it.ends ? C::BORDER : 0);
           skip = 0;
         }
         if (++slot == n_slots) {
@@ -1295,23 +1295,26 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
   if (warp == 0) TmemDealloc(tmem, 512u);
 }
 
-// Joins the pieces of the items that several blocks had, in block order.
+// Joins the pieces of the items that several blocks had, in block order: block
+// (b, y) the rows y, y + gridDim.y, ... (in units of 256 threads) of the item
+// that begins in block b.  What bounds it is the pieces' way through L2, so
+// eight of them are on their way at once.
+constexpr int kJoinBlocks = 16;
 template <typename C>
 __global__ void __launch_bounds__(256) RowsJoinKernel(const KvRowsParams p) {
-  constexpr int D = C::D;
+  constexpr int D = C::D, kVec = D / 4, kRows = 256 / kVec;  // threads of a row, rows of a block at once
   dev::GridLaunchDependents();
   dev::GridWait();
   const Job job = static_cast<const Job*>(p.workspace)[blockIdx.x];
+  if (job.n_tok == 0) return;
   const Split sp(p);
-  const int b0 = blockIdx.x, n = job.last - b0 + 1;
-  constexpr int kVec = D / 4;  // threads of a row
-  for (int r = blockIdx.y * (256 / kVec) + threadIdx.x / kVec; r < job.n_tok * sp.per; r += gridDim.y * (256 / kVec)) {
-    const int tok = r / sp.per, g = r - tok * sp.per + job.chunk * sp.per, i = threadIdx.x % kVec;
+  const int b0 = blockIdx.x, n = job.last - b0 + 1, i = threadIdx.x % kVec;
+  for (int r = blockIdx.y * kRows + threadIdx.x / kVec; r < job.n_tok * sp.per; r += kJoinBlocks * kRows) {
+    const int tok = r / sp.per, g = r - tok * sp.per + job.chunk * sp.per;
     if (g >= sp.group) continue;
-    auto rec = [&](int k) { return RecordOf<C>(p, b0 + k, k == 0); };
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kFlight = 4;
+    constexpr int kFlight = 8;
     for (int k0 = 0; k0 < n; k0 += kFlight) {
       float ref[kFlight], l[kFlight];
       float4 x[kFlight];
@@ -1319,9 +1322,8 @@ __global__ void __launch_bounds__(256) RowsJoinKernel(const KvRowsParams p) {
       for (int k = 0; k < kFlight; ++k) {
         ref[k] = -INFINITY;
         l[k] = 0.f;
-        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (k0 + k < n) {
-          const float* q = rec(k0 + k);
+          const float* q = RecordOf<C>(p, b0 + k0 + k, k0 + k == 0);
           ref[k] = q[kItemRows * D + r];
           l[k] = q[kItemRows * (D + 1) + r];
           x[k] = reinterpret_cast<const float4*>(q + r * D)[i];
@@ -1335,9 +1337,9 @@ __global__ void __launch_bounds__(256) RowsJoinKernel(const KvRowsParams p) {
       sum *= keep;
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const float f = exp2f(ref[k] - base);
-        sum += l[k] == 0.f ? 0.f : f * l[k];
         if (l[k] != 0.f) {
+          const float f = exp2f(ref[k] - base);
+          sum += f * l[k];
           v.x += f * x[k].x;
           v.y += f * x[k].y;
           v.z += f * x[k].z;
@@ -1424,7 +1426,7 @@ void Launch(const KvRowsParams& p, cudaStream_t s) {
   }
   LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, map_k, map_v,
                    p, kvd::kMagic);
-  LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, 8), dim3(256), 0, s, true, p);
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, kJoinBlocks), dim3(256), 0, s, true, p);
 }
 
 template <int D, KvType KIND>
