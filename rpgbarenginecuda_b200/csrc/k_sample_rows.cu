@@ -15,7 +15,8 @@
 //    bound on are gathered in the first block, sorted, cut and drawn from there;
 //  * where that list does not hold what the filters leave (a flat row and a
 //    large top-p, very many equal values, a large k): the least x by selection,
-//    eight bits at a time, over counts (top-k) or sums of weights (top-p);
+//    ten bits of its distance from the largest at a time, over counts (top-k) or
+//    sums of weights (top-p);
 //  * then, and without these filters at once, the weights of all that is left
 //    are added up, the warp that has the target in its share is found from the
 //    blocks' and warps' sums, and it finds the token.
@@ -34,9 +35,9 @@ using u64 = unsigned long long;
 constexpr int kCluster = 8;  // blocks that share a row
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 256;
-constexpr int kList = 1024;      // values that the first block sorts
-constexpr int kMostK = 512;      // the largest k that the list is tried for
+constexpr int kBins = 1024, kBinBits = 10;
+constexpr int kList = 2048;      // values that the first block sorts
+constexpr int kMostK = 1280;     // the largest k that the list is tried for
 constexpr int kFirst = 384;      // the K of rows with top-p alone
 constexpr double kFix = 17592186044416.0;  // 2^44
 
@@ -69,20 +70,19 @@ __device__ __forceinline__ float FromKey(uint32_t k) {
 struct Shared {
   double power[256];  // 2^(j / 256)
   union {
+    unsigned thread_top[kThreads];
     struct {
-      u64 mass[kBins], all_mass[kBins];
-      unsigned count[kBins], all_count[kBins];
-      unsigned thread_top[kThreads];
-    };
-    struct {
-      u64 list[kList], weight[kList];  // key and the complement of the index; weights in the list's order
-    };
+      // sums of weights in three parts of 15 bits, which 2^15 terms (a block's share) do not overflow
+      unsigned part[3][kBins];
+      u64 all[kBins / kCluster];  // of all blocks, this block's bins
+    } bins;
+    u64 list[kList];  // key and the complement of the index
   };
   u64 mine[kList / 4];  // what this block found for the list
-  u64 part[kWarps], sum, target;
-  unsigned wide[kWarps], top, n_mine, n_all;
+  u64 wsum[kWarps], sum, over;
+  unsigned wide[kWarps], top, n_mine;
   int first;
-  uint32_t least;
+  uint32_t least, most;
   int found;
 };
 
@@ -108,7 +108,9 @@ struct Weights {
     return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
   }
 };
-__device__ __forceinline__ u64 Fixed(double w) { return static_cast<u64>(__double2ll_rn(w * kFix)); }
+__device__ __forceinline__ u64 Fixed(double w) {  // (w 2^44 to the nearest integer, which 2^52 + it holds)
+  return static_cast<u64>(__double_as_longlong(fma(w, kFix, 4503599627370496.0)) - 0x4330000000000000ll);
+}
 
 __device__ __forceinline__ u64 WarpAdd(u64 v) {
 #pragma unroll
@@ -145,6 +147,125 @@ __device__ __forceinline__ void Sort(u64* x, int n) {
 __device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 total) {
   const double u = fmin(fmax(p.u != nullptr ? static_cast<double>(p.u[row]) : 0.0, 0.0), 1.0);
   return min(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+}
+
+// Among the row's values with keys from `cut` on: the key of the `need`-th
+// largest, or (by_mass) the largest key from which on the weights reach `share`
+// of their sum; `cut` where there is none.  First by the distance from the
+// largest value, in units of 2^-23 of a factor 2 of weight, ten bits at a time:
+// a row's values spread over many bins so.  Then, where distances round alike
+// and keys do not, by the keys.
+template <typename F>
+__device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, bool by_mass, float share, u64 need, uint32_t cut,
+                                           int n, F value, uint32_t rank) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto distance = [&](float v) -> uint32_t {  // (what is farther than a weight of 2^-127 counts as alike)
+    const double d = (weigh.top - static_cast<double>(v)) * weigh.c;
+    return static_cast<double>(v) == weigh.top ? 0u
+                                               : (d < 127.0 ? static_cast<uint32_t>(__double2int_rz(d * 8388608.0)) : 0x3FFFFFFFu);
+  };
+  u64 over = 0;          // counts or weights before the prefix's range
+  uint32_t prefix = 0, at = 0;
+  for (int digit = 0; digit < 7; ++digit) {
+    const bool by_key = digit >= 3;  // three digits of the distance, then four of 8 bits of the key's complement
+    const int bits = by_key ? 8 : kBinBits, shift = by_key ? 24 - 8 * (digit - 3) : 20 - 10 * digit;
+    if (digit == 3) {
+      at = prefix;
+      prefix = 0;
+      if (tid == 0) {
+        sh.least = 0xFFFFFFFFu;
+        sh.most = 0;
+      }
+      __syncthreads();
+      uint32_t a = 0xFFFFFFFFu, b = 0;
+      for (int i = tid; i < n; i += kThreads) {
+        const float v = value(i);
+        const uint32_t k = Key(v);
+        if (k >= cut && distance(v) == at) {
+          a = min(a, k);
+          b = max(b, k);
+        }
+      }
+      a = __reduce_min_sync(0xFFFFFFFFu, a);
+      b = __reduce_max_sync(0xFFFFFFFFu, b);
+      if (lane == 0) {
+        atomicMin(&sh.least, a);
+        atomicMax(&sh.most, b);
+      }
+      ClusterSync();
+      a = 0xFFFFFFFFu;
+      b = 0;
+      for (uint32_t c = 0; c < kCluster; ++c) {
+        a = min(a, *In(&sh.least, c));
+        b = max(b, *In(&sh.most, c));
+      }
+      ClusterSync();
+      if (a == b) return a;
+    }
+    for (int i = tid; i < kBins; i += kThreads) sh.bins.part[0][i] = sh.bins.part[1][i] = sh.bins.part[2][i] = 0;
+    if (tid == 0) sh.found = -1;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+      const float v = value(i);
+      const uint32_t k = Key(v);
+      if (k < cut) continue;
+      uint32_t code = distance(v);
+      if (by_key) {
+        if (code != at) continue;
+        code = ~k;
+      }
+      if (digit != 0 && digit != 3 && code >> (shift + bits) != prefix) continue;
+      const uint32_t bin = code >> shift & ((1u << bits) - 1);
+      if (by_mass) {
+        const u64 w = Fixed(weigh(v));
+        const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
+        if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
+        if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
+        if ((low & 0x7FFFu) != 0) atomicAdd(&sh.bins.part[2][bin], low & 0x7FFFu);
+      } else {
+        atomicAdd(&sh.bins.part[2][bin], 1u);
+      }
+    }
+    ClusterSync();
+    if (tid < kBins / kCluster) {
+      u64 sum = 0;
+      const int bin = rank * (kBins / kCluster) + tid;
+      for (uint32_t c = 0; c < kCluster; ++c) {
+        sum += (static_cast<u64>(In(sh.bins.part[0], c)[bin]) << 30) + (static_cast<u64>(In(sh.bins.part[1], c)[bin]) << 15) +
+               In(sh.bins.part[2], c)[bin];
+      }
+      sh.bins.all[tid] = sum;
+    }
+    ClusterSync();
+    // the bin in which the sum from the front reaches what is needed: two bins a thread
+    static_assert(kBins == 2 * kThreads, "bins of a thread");
+    const int bin = 2 * tid;
+    const u64* all = In(sh.bins.all, bin / (kBins / kCluster));
+    const u64 s0 = all[bin % (kBins / kCluster)], s1 = all[bin % (kBins / kCluster) + 1];
+    u64 before = WarpScan(s0 + s1, lane);
+    if (lane == 31) sh.wsum[warp] = before;
+    before -= s0 + s1;
+    __syncthreads();
+    u64 total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.wsum[w];
+      total += sh.wsum[w];
+    }
+    if (by_mass && digit == 0) need = static_cast<u64>(ceil(static_cast<double>(share) * static_cast<double>(total)));
+    before += over;
+    if (before < need && need <= before + s0) {
+      sh.found = bin;
+      sh.over = before;
+    } else if (before + s0 < need && need <= before + s0 + s1) {
+      sh.found = bin + 1;
+      sh.over = before + s0;
+    }
+    __syncthreads();
+    if (sh.found < 0) return cut;  // fewer values than are wanted: all stay
+    prefix = prefix << bits | static_cast<uint32_t>(sh.found);
+    over = sh.over;
+  }
+  return ~prefix;
 }
 
 template <typename T>
@@ -313,11 +434,11 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
       }
     }
     mass = WarpAdd(mass);
-    if (lane == 0) sh.part[warp] = mass;
+    if (lane == 0) sh.wsum[warp] = mass;
     __syncthreads();
     if (tid == 0) {
       u64 s = 0;
-      for (int k = 0; k < kWarps; ++k) s += sh.part[k];
+      for (int k = 0; k < kWarps; ++k) s += sh.wsum[k];
       sh.sum = s;
     }
     ClusterSync();
@@ -346,61 +467,71 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
         __syncthreads();
         Sort(sh.list, size);
         const uint32_t least_k = by_k ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
-        // weights of the values from least_k on, and their running sums: two values a thread
-        u64 w0 = 0, w1 = 0;
-        const int i = 2 * tid;
-        if (i < m && static_cast<uint32_t>(sh.list[i] >> 32) >= least_k) w0 = Fixed(weigh(FromKey(sh.list[i] >> 32)));
-        if (i + 1 < m && static_cast<uint32_t>(sh.list[i + 1] >> 32) >= least_k) {
-          w1 = Fixed(weigh(FromKey(sh.list[i + 1] >> 32)));
+        // weights of the values from least_k on, and their running sums: four values a thread
+        u64 w[4], own = 0;
+        const int i = 4 * tid;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
+          w[e] = k >= least_k ? Fixed(weigh(FromKey(k))) : 0;
+          own += w[e];
         }
-        u64 incl = WarpScan(w0 + w1, lane);
-        if (lane == 31) sh.part[warp] = incl;
+        u64 excl = WarpScan(own, lane);
+        if (lane == 31) sh.wsum[warp] = excl;
         __syncthreads();
-        u64 before = 0, sum = 0;
+        u64 sum = 0;
         for (int k = 0; k < kWarps; ++k) {
-          if (k < warp) before += sh.part[k];
-          sum += sh.part[k];
+          if (k < warp) excl += sh.wsum[k];
+          sum += sh.wsum[k];
         }
-        incl += before;
+        excl -= own;
         if (by_k) total = sum;
         // the first value with which the sum reaches its share is the last of the kept
         const u64 need = by_p ? static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))) : ~0ull;
         if (tid == 0) sh.least = by_p ? 0 : least_k;
         __syncthreads();
-        const u64 e0 = incl - w0 - w1, e1 = incl - w1;
-        if (w0 > 0 && e0 < need && need <= e0 + w0) sh.least = static_cast<uint32_t>(sh.list[i] >> 32);
-        if (w1 > 0 && e1 < need && need <= e1 + w1) sh.least = static_cast<uint32_t>(sh.list[i + 1] >> 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (excl < need && need <= excl + w[e]) sh.least = static_cast<uint32_t>(sh.list[i + e] >> 32);
+          excl += w[e];
+        }
         __syncthreads();
         // (0 where the list does not reach the share; with top-k it holds all that counts)
         if (sh.least != 0) {
           cut = sh.least;
-          // the kept, in the list's order
-          double d0 = 0.0, d1 = 0.0;
-          w0 = i < m ? kept(FromKey(sh.list[i] >> 32), d0) : 0;
-          w1 = i + 1 < m ? kept(FromKey(sh.list[i + 1] >> 32), d1) : 0;
-          sh.weight[i] = w0;
-          sh.weight[i + 1] = w1;
-          const u64 s = WarpAdd(w0 + w1);
-          const int last = __reduce_max_sync(0xFFFFFFFFu, w1 > 0 ? i + 2 : (w0 > 0 ? i + 1 : 0));
+          // the kept, in the list's order, over the row, which no one reads any more
+          u64* weight = reinterpret_cast<u64*>(raw);
+          own = 0;
+          int last = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            double d = 0.0;
+            w[e] = i + e < m ? kept(FromKey(sh.list[i + e] >> 32), d) : 0;
+            weight[i + e] = w[e];
+            own += w[e];
+            if (w[e] > 0) last = i + e + 1;
+          }
+          own = WarpAdd(own);
+          last = __reduce_max_sync(0xFFFFFFFFu, last);
+          __syncthreads();
           if (lane == 0) {
-            sh.part[warp] = s;
+            sh.wsum[warp] = own;
             sh.wide[warp] = static_cast<unsigned>(last);
           }
           __syncthreads();
           total = 0;
           int count = 0;
           for (int k = 0; k < kWarps; ++k) {
-            total += sh.part[k];
+            total += sh.wsum[k];
             count = max(count, static_cast<int>(sh.wide[k]));
           }
           const u64 target = Target(p, row, total);
           // what comes before a token by its index
           for (int k = tid; k < count; k += kThreads) {
             const uint32_t index = ~static_cast<uint32_t>(sh.list[k]);
-            const u64 own = sh.weight[k];
-            u64 sum_before = 0;
-            for (int j = 0; j < count; ++j) sum_before += ~static_cast<uint32_t>(sh.list[j]) < index ? sh.weight[j] : 0;
-            if (sum_before <= target && target - sum_before < own) {
+            u64 before = 0;
+            for (int j = 0; j < count; ++j) before += ~static_cast<uint32_t>(sh.list[j]) < index ? weight[j] : 0;
+            if (before <= target && target - before < weight[k]) {
               p.tok[row] = static_cast<int>(index);
               if (p.prob != nullptr) {
                 p.prob[row] = static_cast<float>(weigh(FromKey(sh.list[k] >> 32)) * kFix / static_cast<double>(total));
@@ -416,61 +547,12 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     ClusterSync();  // (it has been read: the first block may end, or go on to use its memory)
     if (found) return;
 
-    // ---- the least key that the filters leave, eight bits at a time
+    // ---- the least key that the filters leave
     for (int pass = 0; pass < 2; ++pass) {
-      const bool by_mass = pass == 1;
-      if (by_mass ? !by_p : !by_k) continue;
-      uint32_t prefix = 0;
-      unsigned wanted = static_cast<unsigned>(top_k);
-      u64 over = 0, need = 0;  // the mass above the prefix's range; the mass that has to be reached
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < kBins; i += kThreads) {
-          sh.mass[i] = 0;
-          sh.count[i] = 0;
-        }
-        __syncthreads();
-        for (int i = tid; i < n; i += kThreads) {
-          const float v = kvd::ToFloat(vals[i]);
-          const uint32_t k = Key(v);
-          if (k < cut || (shift < 24 && k >> (shift + 8) != prefix)) continue;
-          const int bin = k >> shift & 255;
-          if (by_mass) {
-            atomicAdd(&sh.mass[bin], Fixed(weigh(v)));
-          } else {
-            atomicAdd(&sh.count[bin], 1u);
-          }
-        }
-        ClusterSync();
-        for (int i = tid; i < kBins; i += kThreads) {
-          u64 m = 0;
-          unsigned c = 0;
-          for (uint32_t b = 0; b < kCluster; ++b) {
-            m += *In(&sh.mass[i], b);
-            c += *In(&sh.count[i], b);
-          }
-          sh.all_mass[i] = m;
-          sh.all_count[i] = c;
-        }
-        __syncthreads();
-        if (tid == 0) {
-          int bin = 255;
-          if (by_mass) {
-            if (shift == 24) {
-              u64 total = 0;
-              for (int i = 0; i < kBins; ++i) total += sh.all_mass[i];
-              need = static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total)));
-            }
-            // the lowest bin above which there is less than `need`
-            while (bin > 0 && over + sh.all_mass[bin] < need) over += sh.all_mass[bin--];
-          } else {
-            while (bin > 0 && sh.all_count[bin] < wanted) wanted -= sh.all_count[bin--];
-          }
-          sh.least = prefix << 8 | static_cast<uint32_t>(bin);
-        }
-        ClusterSync();  // (before the histograms are cleared too)
-        prefix = sh.least;
+      if (pass == 0 ? by_k : by_p) {
+        cut = Select(sh, weigh, pass == 1, top_p, static_cast<u64>(top_k), cut, n, [&](int i) { return kvd::ToFloat(vals[i]); },
+                     rank);
       }
-      cut = max(cut, prefix);  // (min-p does not count for the share)
     }
   }
 
@@ -480,11 +562,11 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
   u64 mine = 0;
   for (int i = lo + lane; i < hi; i += 32) mine += kept(kvd::ToFloat(vals[i]), w);
   mine = WarpAdd(mine);
-  if (lane == 0) sh.part[warp] = mine;
+  if (lane == 0) sh.wsum[warp] = mine;
   __syncthreads();
   if (tid == 0) {
     u64 s = 0;
-    for (int k = 0; k < kWarps; ++k) s += sh.part[k];
+    for (int k = 0; k < kWarps; ++k) s += sh.wsum[k];
     sh.sum = s;
   }
   ClusterSync();
@@ -494,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     if (b < rank) before += s;
     total += s;
   }
-  for (int k = 0; k < warp; ++k) before += sh.part[k];
+  for (int k = 0; k < warp; ++k) before += sh.wsum[k];
   const u64 target = Target(p, row, total);
   if (before <= target && target - before < mine) {
     // this warp has it: a run for each lane, then the values of that run
@@ -522,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
 template <typename T>
 void Launch(const SampleRowsParams& p, cudaStream_t s) {
   const int per = ((p.vocab + kCluster - 1) / kCluster + 15) / 16 * 16;
-  const size_t smem = static_cast<size_t>(per) * sizeof(T);
+  const size_t row = static_cast<size_t>(per) * sizeof(T), smem = row > 8 * kList ? row : 8 * kList;
   const void* fn = reinterpret_cast<const void*>(SampleRowsKernel<T>);
   RPGB_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
   LaunchKernelClusterArgs(fn, dim3(static_cast<unsigned>(p.n_rows) * kCluster), dim3(kThreads), smem, s, true, kCluster, p,
