@@ -1,0 +1,730 @@
+// k_sample_rows.cu -- one token per row of logits, every row with its own
+// temperature, top-k, top-p, min-p and random number.
+//
+// With z = x / T, m the largest z and w = exp(z - m) a token is kept when
+//   x >= the k-th largest x                         (top-k; equal ones stay)
+//   sum of w over larger x < p * sum of w           (top-p, of what top-k left)
+//   w >= min_p                                      (min-p)
+// and the draw is the first index whose kept weights, added in index order,
+// exceed u times their sum.  All three filters are a least x.
+//
+// What it has to do is read the logits once.  A cluster of eight blocks holds a
+// row in shared memory; what follows is the row's largest value, then
+//  * with top-k or top-p: the largest value of each of the cluster's 4096
+//    threads bounds the K-th largest from below, so the few values from that
+//    bound on are gathered in the first block, sorted, cut and drawn from there;
+//  * where that list does not hold what the filters leave (a flat row and a
+//    large top-p, very many equal values, a large k): the least x by selection,
+//    ten bits of its distance from the largest at a time, over counts (top-k) or
+//    sums of weights (top-p);
+//  * then, and without these filters at once, the weights of all that is left
+//    are added up, the warp that has the target in its share is found from the
+//    blocks' and warps' sums, and it finds the token.
+// A draw compares u with sums of up to 2^18 terms, so weights are held to 2^-37
+// in f64 and added as integers of 2^-44: no sum depends on its order.
+#include "common.h"
+#include "kv_dev.cuh"
+#include "launch.h"
+#include "sample_rows.h"
+
+namespace rpgb {
+__device__ unsigned long long g_probe[32];
+namespace {
+#define TK(i) { if(tid==0){ long long n_=clock64(); atomicAdd(&g_probe[i],(unsigned long long)(n_-_t)); _t=n_; } }
+
+using u64 = unsigned long long;
+
+constexpr int kCluster = 8;  // blocks that share a row
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 1024, kBinBits = 10;
+constexpr int kGroups = 512;     // of eight threads
+constexpr int kList = 2048;      // values that the first block sorts
+constexpr int kMostK = 1280;     // the largest k that the list is tried for
+constexpr int kFirst = 384;      // the K of rows with top-p alone
+constexpr double kFix = 17592186044416.0;  // 2^44
+
+__device__ __forceinline__ void ClusterSync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ClusterRank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of `p` in the shared memory of block `rank`.
+template <typename T>
+__device__ __forceinline__ T* In(T* p, uint32_t rank) {
+  uint64_t r;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<T*>(r);
+}
+
+// Floats in order as integers; NaN and minus infinity (never drawn) as 0.
+__device__ __forceinline__ uint32_t Key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return x > -INFINITY ? k : 0u;
+}
+constexpr uint32_t kLowest = 0x00800000u;  // of the lowest finite value
+__device__ __forceinline__ float FromKey(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+}
+
+struct Shared {
+  double power[1024];  // 2^(j / 1024)
+  union {
+    unsigned thread_top[kThreads];
+    struct {
+      // sums of weights in three parts of 15 bits, which 2^15 terms (a block's share) do not overflow
+      unsigned part[3][kBins];
+      u64 all[kBins / kCluster];  // of all blocks, this block's bins
+    } bins;
+    u64 list[kList];  // key and the complement of the index
+  };
+  u64 mine[kList / 4];  // what this block found for the list
+  u64 wsum[kWarps], sum, over;
+  alignas(16) unsigned group_top[kGroups / kCluster];
+  unsigned wide[2 * kWarps], top, n_mine;
+  int first;
+  uint32_t least, most;
+  int found;
+};
+
+// f32 to f64 by its bits, which costs less than the conversion (zeros and
+// subnormals become numbers under 2^-126, infinities and NaN above 2^127).
+__device__ __forceinline__ double Wide(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double(static_cast<int>((((u & 0x7FFFFFFFu) >> 3) + 0x38000000u) | (u & 0x80000000u)),
+                          static_cast<int>(u << 29));
+}
+
+// exp((x - top) / T) as 2^y with y = n + j / 1024 + r: 2^(j / 1024) from a table
+// and 2^r (|r| <= 2^-11) by its series to the second power, whose next term is
+// under 2^-37.  Products with f64 take two issue slots of a warp and about
+// forty cycles, so there are few of them and no branch between.
+struct Weights {
+  const double* power;
+  double top, c, base;
+  bool near_;  // one product holds y to 2^-43
+  __device__ __forceinline__ Weights(const Shared& sh, float top_, float temperature)
+      : power(sh.power), top(static_cast<double>(top_)), c(1.4426950408889634 / static_cast<double>(temperature)) {
+    base = -top * c;
+    near_ = fabs(base) < 1024.0;
+  }
+  // times 2^44, to the nearest integer; what is under 2^-60 and not finite is 0, but the infinite top's equals count alike
+  __device__ __forceinline__ u64 Fixed(float x) const {
+    double y = near_ ? fma(Wide(x), c, base) : (static_cast<double>(x) - top) * c;
+    const bool none = !(y >= -60.0 && y < 1.0);  // (NaN is far above)
+    y = none ? 0.0 : y;
+    const u64 f = static_cast<u64>(__double_as_longlong(Power(y, 44) + 4503599627370496.0) - 0x4330000000000000ll);
+    return none ? (x == INFINITY ? 1ull << 44 : 0) : f;
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    const double y = (static_cast<double>(x) - top) * c;
+    return y >= -60.0 ? Power(y, 0) : (x == INFINITY ? 1.0 : 0.0);
+  }
+  __device__ __forceinline__ double Power(double y, int up) const {  // 2^(y + up)
+    constexpr double kMagic = 6755399441055744.0 / 1024.0;           // 1.5 2^52 in units of 1 / 1024
+    const double t = y + kMagic;
+    const double r = y - (t - kMagic);
+    const int n = __double2loint(t);
+    const double q = fma(r, 0.24022650695910072, 0.69314718055994531) * r;
+    const double p = power[n & 1023];
+    const double w = fma(p, q, p);
+    return __hiloint2double(__double2hiint(w) + ((n >> 10) + up) * (1 << 20), __double2loint(w));
+  }
+};
+
+__device__ __forceinline__ u64 WarpAdd(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ u64 WarpScan(u64 v, int lane) {  // with the lane's own
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 w = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+
+// Sorts n (a power of two from 64) keys, the largest first.  Up to 128 one warp
+// does it without barriers for all.
+__device__ __forceinline__ void Sort(u64* x, int n) {
+  const bool small = n <= 128;
+  const int threads = small ? 32 : kThreads;
+  if (threadIdx.x < threads) {
+    for (int k = 2; k <= n; k <<= 1) {
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int i = threadIdx.x; i < n / 2; i += threads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const u64 u = x[a], v = x[b];
+          if ((u < v) == ((a & k) == 0)) {
+            x[a] = v;
+            x[b] = u;
+          }
+        }
+        small ? __syncwarp() : __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// `u` of a sum of weights: the target is exceeded by exactly one token's running sum.
+__device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 total) {
+  const double u = fmin(fmax(p.u != nullptr ? static_cast<double>(p.u[row]) : 0.0, 0.0), 1.0);
+  return min(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+}
+
+// Among the row's values with keys from `cut` on: the key of the `need`-th
+// largest, or (by_mass) the largest key from which on the weights reach `share`
+// of their sum; `cut` where there is none.  First by the distance from the
+// largest value, in units of 2^-23 of a factor 2 of weight, ten bits at a time:
+// a row's values spread over many bins so.  Then, where distances round alike
+// and keys do not, by the keys.
+template <typename F>
+__device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, bool by_mass, float share, u64 need, uint32_t cut,
+                                           int n, F value, uint32_t rank) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto distance = [&](float v) -> uint32_t {  // (what is farther than a weight of 2^-127 counts as alike)
+    const double d = (weigh.top - static_cast<double>(v)) * weigh.c;
+    return static_cast<double>(v) == weigh.top ? 0u
+                                               : (d < 127.0 ? static_cast<uint32_t>(__double2int_rz(d * 8388608.0)) : 0x3FFFFFFFu);
+  };
+  u64 over = 0;          // counts or weights before the prefix's range
+  uint32_t prefix = 0, at = 0;
+  for (int digit = 0; digit < 7; ++digit) {
+    const bool by_key = digit >= 3;  // three digits of the distance, then four of 8 bits of the key's complement
+    const int bits = by_key ? 8 : kBinBits, shift = by_key ? 24 - 8 * (digit - 3) : 20 - 10 * digit;
+    if (digit == 3) {
+      at = prefix;
+      prefix = 0;
+      if (tid == 0) {
+        sh.least = 0xFFFFFFFFu;
+        sh.most = 0;
+      }
+      __syncthreads();
+      uint32_t a = 0xFFFFFFFFu, b = 0;
+      for (int i = tid; i < n; i += kThreads) {
+        const float v = value(i);
+        const uint32_t k = Key(v);
+        if (k >= cut && distance(v) == at) {
+          a = min(a, k);
+          b = max(b, k);
+        }
+      }
+      a = __reduce_min_sync(0xFFFFFFFFu, a);
+      b = __reduce_max_sync(0xFFFFFFFFu, b);
+      if (lane == 0) {
+        atomicMin(&sh.least, a);
+        atomicMax(&sh.most, b);
+      }
+      ClusterSync();
+      a = 0xFFFFFFFFu;
+      b = 0;
+      for (uint32_t c = 0; c < kCluster; ++c) {
+        a = min(a, *In(&sh.least, c));
+        b = max(b, *In(&sh.most, c));
+      }
+      ClusterSync();
+      if (a == b) return a;
+    }
+    for (int i = tid; i < kBins; i += kThreads) sh.bins.part[0][i] = sh.bins.part[1][i] = sh.bins.part[2][i] = 0;
+    if (tid == 0) sh.found = -1;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+      const float v = value(i);
+      const uint32_t k = Key(v);
+      if (k < cut) continue;
+      uint32_t code = distance(v);
+      if (by_key) {
+        if (code != at) continue;
+        code = ~k;
+      }
+      if (digit != 0 && digit != 3 && code >> (shift + bits) != prefix) continue;
+      const uint32_t bin = code >> shift & ((1u << bits) - 1);
+      if (by_mass) {
+        const u64 w = weigh.Fixed(v);
+        const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
+        if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
+        if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
+        if ((low & 0x7FFFu) != 0) atomicAdd(&sh.bins.part[2][bin], low & 0x7FFFu);
+      } else {
+        atomicAdd(&sh.bins.part[2][bin], 1u);
+      }
+    }
+    ClusterSync();
+    if (tid < kBins / kCluster) {
+      u64 sum = 0;
+      const int bin = rank * (kBins / kCluster) + tid;
+      for (uint32_t c = 0; c < kCluster; ++c) {
+        sum += (static_cast<u64>(In(sh.bins.part[0], c)[bin]) << 30) + (static_cast<u64>(In(sh.bins.part[1], c)[bin]) << 15) +
+               In(sh.bins.part[2], c)[bin];
+      }
+      sh.bins.all[tid] = sum;
+    }
+    ClusterSync();
+    // the bin in which the sum from the front reaches what is needed: two bins a thread
+    static_assert(kBins == 2 * kThreads, "bins of a thread");
+    const int bin = 2 * tid;
+    const u64* all = In(sh.bins.all, bin / (kBins / kCluster));
+    const u64 s0 = all[bin % (kBins / kCluster)], s1 = all[bin % (kBins / kCluster) + 1];
+    u64 before = WarpScan(s0 + s1, lane);
+    if (lane == 31) sh.wsum[warp] = before;
+    before -= s0 + s1;
+    __syncthreads();
+    u64 total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.wsum[w];
+      total += sh.wsum[w];
+    }
+    if (by_mass && digit == 0) need = static_cast<u64>(ceil(static_cast<double>(share) * static_cast<double>(total)));
+    before += over;
+    if (before < need && need <= before + s0) {
+      sh.found = bin;
+      sh.over = before;
+    } else if (before + s0 < need && need <= before + s0 + s1) {
+      sh.found = bin + 1;
+      sh.over = before + s0;
+    }
+    __syncthreads();
+    if (sh.found < 0) return cut;  // fewer values than are wanted: all stay
+    prefix = prefix << bits | static_cast<uint32_t>(sh.found);
+    over = sh.over;
+  }
+  return ~prefix;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRowsParams p, int per) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ Shared sh;
+  T* vals = reinterpret_cast<T*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = ClusterRank();
+  const int row = blockIdx.x / kCluster;
+  for (int i = tid; i < 1024; i += kThreads) sh.power[i] = exp2(i / 1024.0);
+  if (tid == 0) sh.n_mine = 0;
+  dev::GridLaunchDependents();
+  dev::GridWait();
+  TK(0)
+  const int begin = min(static_cast<int>(rank) * per, p.vocab), n = min(per, p.vocab - begin);
+  const T* src = static_cast<const T*>(p.logits) + row * p.stride + begin;
+  const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.f;
+  const int top_k = p.top_k != nullptr ? p.top_k[row] : 0;
+  const float top_p = p.top_p != nullptr ? p.top_p[row] : 1.f;
+  const float min_p = p.min_p != nullptr ? p.min_p[row] : 0.f;
+  const bool greedy = !(temperature > 0.f);
+  const bool by_k = !greedy && top_k > 1 && top_k < p.vocab, by_p = !greedy && top_p > 0.f && top_p < 1.f;
+
+  // ---- the row into shared memory, and its largest value
+  float best = -INFINITY;
+  constexpr int kVec = 16 / sizeof(T);
+  if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+    const int vecs = n / kVec;
+    constexpr int kFlight = 4;
+    for (int i0 = tid; i0 < vecs; i0 += kThreads * kFlight) {
+      uint4 w[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        if (i0 + k * kThreads < vecs) w[k] = reinterpret_cast<const uint4*>(src)[i0 + k * kThreads];
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        if (i0 + k * kThreads < vecs) {
+          reinterpret_cast<uint4*>(vals)[i0 + k * kThreads] = w[k];
+          const kvd::Pack<T, kVec> x = *reinterpret_cast<const kvd::Pack<T, kVec>*>(&w[k]);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) best = fmaxf(best, kvd::ToFloat(x.v[e]));
+        }
+      }
+    }
+    for (int i = vecs * kVec + tid; i < n; i += kThreads) {
+      vals[i] = src[i];
+      best = fmaxf(best, kvd::ToFloat(vals[i]));
+    }
+  } else {
+    constexpr int kFlight = 8;
+    for (int i0 = tid; i0 < n; i0 += kThreads * kFlight) {
+      T w[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        if (i0 + k * kThreads < n) w[k] = src[i0 + k * kThreads];
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        if (i0 + k * kThreads < n) {
+          vals[i0 + k * kThreads] = w[k];
+          best = fmaxf(best, kvd::ToFloat(w[k]));
+        }
+      }
+    }
+  }
+  TK(1)
+  const unsigned my_key = Key(best);
+  sh.thread_top[tid] = my_key;
+  {
+    unsigned w = my_key;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) w = max(w, __shfl_xor_sync(0xFFFFFFFFu, w, o));
+    if (lane % 8 == 0) sh.group_top[tid / 8] = w;
+    w = __reduce_max_sync(0xFFFFFFFFu, w);
+    if (lane == 0) sh.wide[warp] = w;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    unsigned w = 0;
+    for (int k = 0; k < kWarps; ++k) w = max(w, sh.wide[k]);
+    sh.top = w;
+  }
+  ClusterSync();
+  TK(2)
+  unsigned top = 0;
+  for (uint32_t b = 0; b < kCluster; ++b) top = max(top, *In(&sh.top, b));
+  const float most = FromKey(top);
+
+  if (top == 0 || greedy) {
+    // ---- nothing to draw, or the largest value's lowest index
+    int at = INT_MAX;
+    if (top != 0 && sh.top == top) {
+      for (int i = tid; i < n; i += kThreads) {
+        if (Key(kvd::ToFloat(vals[i])) == top) {
+          at = begin + i;
+          break;
+        }
+      }
+    }
+    at = __reduce_min_sync(0xFFFFFFFFu, at);
+    __syncthreads();
+    if (lane == 0) sh.wide[warp] = static_cast<unsigned>(at);
+    __syncthreads();
+    if (tid == 0) {
+      for (int k = 0; k < kWarps; ++k) at = min(at, static_cast<int>(sh.wide[k]));
+      sh.first = at;
+    }
+    ClusterSync();
+    if (rank == 0 && tid == 0) {
+      for (uint32_t b = 1; b < kCluster; ++b) at = min(at, *In(&sh.first, b));
+      p.tok[row] = top == 0 ? -1 : at;
+      if (p.prob != nullptr) p.prob[row] = top == 0 ? kvd::Nan() : 1.f;
+    }
+    ClusterSync();
+    return;
+  }
+
+  const Weights weigh(sh, most, temperature);
+  uint32_t least_min = 1, cut = 1;
+  if (min_p > 0.f && min_p <= 1.f) {
+    // under x = top + T log(min_p), less a part in 2^20 of both, no weight reaches min_p; kept() decides the rest
+    const float cut = most + temperature * logf(min_p);
+    const float low = cut - (fabsf(most) + fabsf(temperature * logf(min_p))) * 9.5367431640625e-7f;
+    if (low > -INFINITY && most < INFINITY) least_min = max(1u, Key(low));
+  }
+  const bool by_min = min_p > 0.f && min_p <= 1.f;
+  // the weight of a value, 0 where a filter drops it
+  auto kept = [&](float v) -> u64 {
+    const uint32_t k = Key(v);
+    if (by_min && k >= least_min && weigh(v) < static_cast<double>(min_p)) return 0;
+    const u64 w = weigh.Fixed(v);
+    return k >= least_min && k >= cut ? w : 0;
+  };
+  if (by_k || by_p) {
+    // ---- a bound that at least `want` values reach: the want-th largest of the
+    // largest values of groups of the row (its upper 22 bits).  Of 512 groups of
+    // eight threads every warp finds it alone; where more are wanted, of all
+    // threads, together.
+    const int want = by_k ? min(top_k, kMostK + 1) : kFirst;
+    const bool listed = want <= kMostK;
+    uint32_t bound = 0;
+    if (want <= kGroups / 4 * 3) {
+      unsigned key[kGroups / 32];
+#pragma unroll
+      for (int i = 0; i < kGroups / 32; i += 4) {
+        const int at = lane * (kGroups / 32) + i;
+        const uint4 w = *reinterpret_cast<const uint4*>(In(sh.group_top, at / (kGroups / kCluster)) + at % (kGroups / kCluster));
+        key[i] = w.x;
+        key[i + 1] = w.y;
+        key[i + 2] = w.z;
+        key[i + 3] = w.w;
+      }
+      for (int bit = 31; bit >= 10; --bit) {
+        const uint32_t try_ = bound | 1u << bit;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups / 32; ++i) c += key[i] >= try_;
+        if (__reduce_add_sync(0xFFFFFFFFu, c) >= want) bound = try_;
+      }
+    } else if (listed) {
+      unsigned key[kCluster];
+#pragma unroll
+      for (uint32_t b = 0; b < kCluster; ++b) key[b] = In(sh.thread_top, b)[tid];
+      for (int bit = 31; bit >= 10; --bit) {
+        const uint32_t try_ = bound | 1u << bit;
+        int c = 0;
+#pragma unroll
+        for (int b = 0; b < kCluster; ++b) c += key[b] >= try_;
+        c = __reduce_add_sync(0xFFFFFFFFu, c);
+        unsigned* wide = sh.wide + (bit & 1) * kWarps;
+        if (lane == 0) wide[warp] = c;
+        __syncthreads();
+        int all = lane < kWarps ? static_cast<int>(wide[lane]) : 0;
+        if (__reduce_add_sync(0xFFFFFFFFu, all) >= want) bound = try_;
+      }
+    }
+    bound = max(bound, kLowest);
+    TK(3)
+    // ---- what reaches it, and the sum of all weights where the list may not hold all that counts
+    const float bound_value = listed ? FromKey(bound) : INFINITY;
+    u64 mass = 0;
+    constexpr int kAhead = 4;
+    for (int i0 = warp * 32 * kAhead; i0 < n; i0 += kThreads * kAhead) {
+      float v[kAhead];
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int i = i0 + e * 32 + lane;
+        v[e] = i < n ? kvd::ToFloat(vals[i]) : -INFINITY;
+        any |= v[e] >= bound_value;
+      }
+      if (!by_k) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) mass += weigh.Fixed(v[e]);
+      }
+      if (listed && __any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          const bool in = v[e] >= bound_value;
+          const uint32_t mask = __ballot_sync(0xFFFFFFFFu, in);
+          if (mask != 0) {
+            unsigned at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n_mine, __popc(mask));
+            at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(mask & ((1u << lane) - 1));
+            if (in && at < kList / 4) {
+              sh.mine[at] = static_cast<u64>(Key(v[e])) << 32 | ~static_cast<uint32_t>(begin + i0 + e * 32 + lane);
+            }
+          }
+        }
+      }
+    }
+    mass = WarpAdd(mass);
+    if (lane == 0) sh.wsum[warp] = mass;
+    __syncthreads();
+    if (tid == 0) {
+      u64 s = 0;
+      for (int k = 0; k < kWarps; ++k) s += sh.wsum[k];
+      sh.sum = s;
+    }
+    ClusterSync();
+    TK(4)
+    if (rank == 0) {
+      // ---- the first block sorts the list, cuts it and draws
+      unsigned start[kCluster + 1];
+      bool fits = listed;
+      u64 total = 0;
+      start[0] = 0;
+      for (uint32_t b = 0; b < kCluster; ++b) {
+        const unsigned c = *In(&sh.n_mine, b);
+        fits = fits && c <= kList / 4;
+        start[b + 1] = start[b] + c;
+        total += *In(&sh.sum, b);
+      }
+      const int m = static_cast<int>(start[kCluster]);
+      fits = fits && m <= kList;
+      if (tid == 0) sh.found = 0;
+      if (fits) {
+        int size = 64;
+        while (size < m) size <<= 1;
+        for (uint32_t b = 0; b < kCluster; ++b) {
+          for (int i = tid; i < static_cast<int>(start[b + 1] - start[b]); i += kThreads) sh.list[start[b] + i] = In(sh.mine, b)[i];
+        }
+        for (int i = m + tid; i < size; i += kThreads) sh.list[i] = 0;
+        __syncthreads();
+        TK(5)
+        Sort(sh.list, size);
+        TK(6)
+        const uint32_t least_k = by_k && top_k <= m ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
+        // weights of the values from least_k on, and their running sums: four values a thread
+        u64 w[4], own = 0;
+        const int i = 4 * tid;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
+          w[e] = k >= least_k && k != 0 ? weigh.Fixed(FromKey(k)) : 0;
+          own += w[e];
+        }
+        u64 excl = WarpScan(own, lane);
+        if (lane == 31) sh.wsum[warp] = excl;
+        __syncthreads();
+        u64 sum = 0;
+        for (int k = 0; k < kWarps; ++k) {
+          if (k < warp) excl += sh.wsum[k];
+          sum += sh.wsum[k];
+        }
+        excl -= own;
+        if (by_k) total = sum;
+        // the first value with which the sum reaches its share is the last of the kept
+        const u64 need = by_p ? static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))) : ~0ull;
+        if (tid == 0) sh.least = by_p ? 0 : least_k;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (excl < need && need <= excl + w[e]) sh.least = static_cast<uint32_t>(sh.list[i + e] >> 32);
+          excl += w[e];
+        }
+        __syncthreads();
+        // (0 where the list does not reach the share; with top-k it holds all that counts)
+        if (sh.least != 0) {
+          cut = sh.least;
+          // the kept, in the list's order, over the row, which no one reads any more
+          u64* weight = reinterpret_cast<u64*>(raw);
+          own = 0;
+          int last = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
+            if (k < cut || k < least_min || (by_min && weigh(FromKey(k)) < static_cast<double>(min_p))) w[e] = 0;
+            weight[i + e] = w[e];
+            own += w[e];
+            if (w[e] > 0) last = i + e + 1;
+          }
+          own = WarpAdd(own);
+          last = __reduce_max_sync(0xFFFFFFFFu, last);
+          __syncthreads();
+          if (lane == 0) {
+            sh.wsum[warp] = own;
+            sh.wide[warp] = static_cast<unsigned>(last);
+          }
+          __syncthreads();
+          total = 0;
+          int count = 0;
+          for (int k = 0; k < kWarps; ++k) {
+            total += sh.wsum[k];
+            count = max(count, static_cast<int>(sh.wide[k]));
+          }
+          const u64 target = Target(p, row, total);
+          // what comes before a token by its index
+          for (int k = tid; k < count; k += kThreads) {
+            const uint32_t index = ~static_cast<uint32_t>(sh.list[k]);
+            u64 before = 0;
+            for (int j = 0; j < count; ++j) before += ~static_cast<uint32_t>(sh.list[j]) < index ? weight[j] : 0;
+            if (before <= target && target - before < weight[k]) {
+              p.tok[row] = static_cast<int>(index);
+              if (p.prob != nullptr) {
+                p.prob[row] = static_cast<float>(weigh(FromKey(sh.list[k] >> 32)) * kFix / static_cast<double>(total));
+              }
+            }
+          }
+          if (tid == 0) sh.found = 1;
+        }
+      }
+    }
+    if(rank==0) TK(7)
+    ClusterSync();
+    const bool found = *In(&sh.found, 0) != 0;
+    ClusterSync();  // (it has been read: the first block may end, or go on to use its memory)
+    if (found) return;
+
+    // ---- the least key that the filters leave
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == 0 ? by_k : by_p) {
+        cut = Select(sh, weigh, pass == 1, top_p, static_cast<u64>(top_k), cut, n, [&](int i) { return kvd::ToFloat(vals[i]); },
+                     rank);
+      }
+    }
+  }
+
+  TK(8)
+  // ---- the kept weights: a run of the row for each warp
+  const int run = (per + kThreads - 1) / kThreads, lo = min(warp * 32 * run, n), hi = min(lo + 32 * run, n);
+  const float floor_ = fmaxf(cut > 1 ? FromKey(cut) : -INFINITY, least_min > 1 ? FromKey(least_min) : -INFINITY);
+  u64 mine = 0;
+  constexpr int kAhead = 4;
+  for (int i0 = lo; i0 < hi; i0 += 32 * kAhead) {
+    float v[kAhead];
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int i = i0 + e * 32 + lane;
+      v[e] = i < hi ? kvd::ToFloat(vals[i]) : -INFINITY;
+      any |= v[e] >= floor_;
+    }
+    if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) mine += kept(v[e]);
+    }
+  }
+  mine = WarpAdd(mine);
+  if (lane == 0) sh.wsum[warp] = mine;
+  __syncthreads();
+  if (tid == 0) {
+    u64 s = 0;
+    for (int k = 0; k < kWarps; ++k) s += sh.wsum[k];
+    sh.sum = s;
+  }
+  ClusterSync();
+  TK(9)
+  u64 before = 0, total = 0;
+  for (uint32_t b = 0; b < kCluster; ++b) {
+    const u64 s = *In(&sh.sum, b);
+    if (b < rank) before += s;
+    total += s;
+  }
+  for (int k = 0; k < warp; ++k) before += sh.wsum[k];
+  const u64 target = Target(p, row, total);
+  if (before <= target && target - before < mine) {
+    // this warp has it: a run for each lane, then the values of that run
+    u64 own = 0;
+    const int a = min(lo + lane * run, hi), b = min(a + run, hi);
+    for (int i0 = 0; i0 < run; i0 += kAhead) {
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) own += kept(a + i0 + e < b ? kvd::ToFloat(vals[a + i0 + e]) : -INFINITY);
+    }
+    const u64 excl = WarpScan(own, lane) - own + before;
+    const int who = __ffs(__ballot_sync(0xFFFFFFFFu, excl <= target && target - excl < own)) - 1;
+    const int a1 = __shfl_sync(0xFFFFFFFFu, a, who), b1 = __shfl_sync(0xFFFFFFFFu, b, who);
+    u64 so_far = __shfl_sync(0xFFFFFFFFu, excl, who);
+    for (int i0 = a1; i0 < b1; i0 += 32) {
+      const int i = i0 + lane;
+      const float x = i < b1 ? kvd::ToFloat(vals[i]) : -INFINITY;
+      const u64 v = kept(x);
+      const u64 incl = so_far + WarpScan(v, lane);
+      if (incl - v <= target && target < incl) {
+        p.tok[row] = begin + i;
+        if (p.prob != nullptr) p.prob[row] = static_cast<float>(weigh(x) * kFix / static_cast<double>(total));
+      }
+      so_far = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    }
+  }
+  TK(10)
+  ClusterSync();
+  TK(11)
+}
+
+template <typename T>
+void Launch(const SampleRowsParams& p, cudaStream_t s) {
+  const int per = ((p.vocab + kCluster - 1) / kCluster + 15) / 16 * 16;
+  const size_t row = static_cast<size_t>(per) * sizeof(T), smem = row > 8 * kList ? row : 8 * kList;
+  const void* fn = reinterpret_cast<const void*>(SampleRowsKernel<T>);
+  RPGB_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
+  LaunchKernelClusterArgs(fn, dim3(static_cast<unsigned>(p.n_rows) * kCluster), dim3(kThreads), smem, s, true, kCluster, p,
+                          per);
+}
+
+}  // namespace
+
+void LaunchSampleRows(const SampleRowsParams& p, cudaStream_t s) {
+  switch (p.type) {
+    case ElemType::kF32: Launch<float>(p, s); break;
+    case ElemType::kF16: Launch<__half>(p, s); break;
+    case ElemType::kBF16: Launch<__nv_bfloat16>(p, s); break;
+  }
+  RPGB_CUDA(cudaGetLastError());
+  CountLaunches(1);
+}
+
+}  // namespace rpgb
+
+extern "C" __attribute__((visibility("default"))) int rpgb_probe(unsigned long long* out){ cudaMemcpyFromSymbol(out, rpgb::g_probe, 256); unsigned long long z[32]={}; cudaMemcpyToSymbol(rpgb::g_probe, z, 256); return 0;}

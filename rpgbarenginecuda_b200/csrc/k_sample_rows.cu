@@ -20,8 +20,8 @@
 //  * then, and without these filters at once, the weights of all that is left
 //    are added up, the warp that has the target in its share is found from the
 //    blocks' and warps' sums, and it finds the token.
-// A draw compares u with sums of up to 2^18 terms, so weights are held to 2^-42
-// in f64 and added as integers of 2^-44: no sum depends on its order.
+// A draw compares u with sums of up to 2^18 terms, so weights are held to 2^-34,
+// and sums of them that are compared are integers of 2^-44.
 #include "common.h"
 #include "kv_dev.cuh"
 #include "launch.h"
@@ -36,6 +36,7 @@ constexpr int kCluster = 8;  // blocks that share a row
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024, kBinBits = 10;
+constexpr int kGroups = 512;     // of eight threads
 constexpr int kList = 2048;      // values that the first block sorts
 constexpr int kMostK = 1280;     // the largest k that the list is tried for
 constexpr int kFirst = 384;      // the K of rows with top-p alone
@@ -44,6 +45,10 @@ constexpr double kFix = 17592186044416.0;  // 2^44
 __device__ __forceinline__ void ClusterSync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of it: this block has read what it needs of the others; no
+// other block needs this one's memory any more.
+__device__ __forceinline__ void ClusterArrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ClusterWait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t ClusterRank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -63,12 +68,13 @@ __device__ __forceinline__ uint32_t Key(float x) {
   const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
   return x > -INFINITY ? k : 0u;
 }
+constexpr uint32_t kLowest = 0x00800000u;  // of the lowest finite value
 __device__ __forceinline__ float FromKey(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
 }
 
 struct Shared {
-  double power[256];  // 2^(j / 256)
+  float2 power[256];  // 2^(j / 256)
   union {
     unsigned thread_top[kThreads];
     struct {
@@ -80,37 +86,88 @@ struct Shared {
   };
   u64 mine[kList / 4];  // what this block found for the list
   u64 wsum[kWarps], sum, over;
-  unsigned wide[kWarps], top, n_mine;
+  alignas(16) unsigned group_top[kGroups / kCluster];
+  unsigned wide[2 * kWarps], top, n_mine;
   int first;
   uint32_t least, most;
   int found;
 };
 
-// exp((x - top) / T) as 2^y with y = n + j / 256 + r: 2^(j / 256) from a table
-// and 2^r (|r| <= 2^-9) by its series to the third power, whose next term is
-// under 2^-42.
+// Weights exp((x - top) / T) = 2^y as pairs of f32, hi + lo, good to about
+// 2^-34 (f64 to the same end took twice the time): x - top and its product with
+// c = log2(e) / T carry their rounding errors along, y = n + j / 256 + r, 2^(j /
+// 256) comes from a table of pairs and 2^r (|r| <= 2^-9) from its series to the
+// third power, whose next term is under 2^-42.  Two values at a time.
 struct Weights {
-  const double* power;
-  double top, c;
-  __device__ __forceinline__ Weights(const Shared& sh, float top_, float temperature)
-      : power(sh.power), top(static_cast<double>(top_)), c(1.4426950408889634 / static_cast<double>(temperature)) {}
+  const float2* power;
+  float top, c, c_low;
+  bool infinite;  // the largest value is: its equals count alike, nothing else does
+  __device__ __forceinline__ Weights(const Shared& sh, float top_, float temperature) : power(sh.power), top(top_) {
+    const double cc = fmin(1.4426950408889634 / static_cast<double>(temperature), 3e38);
+    c = static_cast<float>(cc);
+    c_low = static_cast<float>(cc - static_cast<double>(c));
+    infinite = top == INFINITY;
+  }
+  static __device__ __forceinline__ float2 Two(float x) { return make_float2(x, x); }
+  __device__ __forceinline__ void operator()(float2 x, float2& hi, float2& lo) const {
+    if (infinite) {
+      hi = make_float2(x.x == INFINITY ? 1.f : 0.f, x.y == INFINITY ? 1.f : 0.f);
+      lo = Two(0.f);
+      return;
+    }
+    const float2 less = Two(-1.f);
+    const float2 d = __fadd2_rn(x, Two(-top));
+    const float2 b = __ffma2_rn(x, less, d);                                                   // d - x
+    const float2 e = __fadd2_rn(__ffma2_rn(__ffma2_rn(b, less, d), less, x), __ffma2_rn(b, less, Two(-top)));  // what d lost
+    const float2 y = __fmul2_rn(d, Two(c));
+    float2 z = __ffma2_rn(d, Two(-c), y);  // y less what it should be
+    z = __ffma2_rn(d, Two(-c_low), z);
+    z = __ffma2_rn(e, Two(-c), z);
+    constexpr float kMagic = 12582912.f;  // 1.5 2^23
+    const float2 t = __ffma2_rn(y, Two(256.f), Two(kMagic));
+    const float2 n = __fadd2_rn(t, Two(-kMagic));
+    const float2 r = __ffma2_rn(z, less, __ffma2_rn(n, Two(-0.00390625f), y));
+    // (ln 2, its square over 2 and cube over 6; the first is off by 1.9e-9 as f32, which r makes 2^-38)
+    float2 q = __ffma2_rn(r, Two(0.055504109f), Two(0.24022651f));
+    q = __fmul2_rn(__ffma2_rn(r, q, Two(0.69314718f)), r);
+    const uint32_t tx = __float_as_uint(t.x), ty = __float_as_uint(t.y);
+    const float2 px = power[tx & 255], py = power[ty & 255];
+    const float2 scale = make_float2(__uint_as_float((tx << 15 & 0xFF800000u) + 0x3F800000u),
+                                     __uint_as_float((ty << 15 & 0xFF800000u) + 0x3F800000u));
+    hi = __fmul2_rn(make_float2(px.x, py.x), scale);
+    lo = __fmul2_rn(__ffma2_rn(make_float2(px.x, py.x), q, make_float2(px.y, py.y)), scale);
+    if (!(y.x >= -60.f)) hi.x = lo.x = 0.f;  // (NaN too)
+    if (!(y.y >= -60.f)) hi.y = lo.y = 0.f;
+  }
   __device__ __forceinline__ double operator()(float x) const {
-    const double y = (static_cast<double>(x) - top) * c;
-    if (!(y >= -60.0)) return x == INFINITY ? 1.0 : 0.0;  // (under 2^-45; infinities are each other's equals)
-    constexpr double kMagic = 6755399441055744.0 / 256.0;  // 1.5 2^52 in units of 1 / 256
-    const double t = y + kMagic;
-    const double r = y - (t - kMagic);
-    const int n = __double2loint(t);
-    double q = fma(r, 0.055504108664821580, 0.24022650695910072);
-    q = fma(r, q, 0.69314718055994531) * r;
-    const double p = power[n & 255];
-    const double w = fma(p, q, p);
-    return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
+    float2 hi, lo;
+    (*this)(Two(x), hi, lo);
+    return static_cast<double>(hi.x) + static_cast<double>(lo.x);
+  }
+  __device__ __forceinline__ u64 Fixed(float x) const { return ToFixed((*this)(x)); }
+  // times 2^44, to the nearest integer
+  static __device__ __forceinline__ u64 ToFixed(double w) {
+    return static_cast<u64>(__double_as_longlong(fma(w, kFix, 4503599627370496.0)) - 0x4330000000000000ll);
+  }
+  // How far x lies under the largest value, in units of 2^-23 of a factor 2 of
+  // weight; what is farther than 2^-127 counts as alike.  Larger values are never farther.
+  __device__ __forceinline__ uint32_t Distance(float x) const {
+    const float d = (top - x) * c;
+    return x == top ? 0u : (d < 127.f ? static_cast<uint32_t>(d * 8388608.f) : 0x3FFFFFFFu);
   }
 };
-__device__ __forceinline__ u64 Fixed(double w) {  // (w 2^44 to the nearest integer, which 2^52 + it holds)
-  return static_cast<u64>(__double_as_longlong(fma(w, kFix, 4503599627370496.0)) - 0x4330000000000000ll);
-}
+// A running sum of weights: f32 with what its additions lose.
+struct Sum {
+  float2 hi = make_float2(0.f, 0.f), lo = make_float2(0.f, 0.f);
+  __device__ __forceinline__ void Add(float2 h, float2 l) {
+    const float2 less = make_float2(-1.f, -1.f), s = __fadd2_rn(hi, h), b = __ffma2_rn(hi, less, s);
+    lo = __fadd2_rn(lo, __fadd2_rn(l, __fadd2_rn(__ffma2_rn(__ffma2_rn(b, less, s), less, hi), __ffma2_rn(b, less, h))));
+    hi = s;
+  }
+  __device__ __forceinline__ double Total() const {
+    return (static_cast<double>(hi.x) + static_cast<double>(hi.y)) + (static_cast<double>(lo.x) + static_cast<double>(lo.y));
+  }
+};
 
 __device__ __forceinline__ u64 WarpAdd(u64 v) {
 #pragma unroll
@@ -126,21 +183,27 @@ __device__ __forceinline__ u64 WarpScan(u64 v, int lane) {  // with the lane's o
   return v;
 }
 
-// Sorts n (a power of two from 2) keys, the largest first.
+// Sorts n (a power of two from 64) keys, the largest first.  Up to 128 one warp
+// does it without barriers for all.
 __device__ __forceinline__ void Sort(u64* x, int n) {
-  for (int k = 2; k <= n; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const u64 u = x[a], v = x[b];
-        if ((u < v) == ((a & k) == 0)) {
-          x[a] = v;
-          x[b] = u;
+  const bool small = n <= 128;
+  const int threads = small ? 32 : kThreads;
+  if (threadIdx.x < threads) {
+    for (int k = 2; k <= n; k <<= 1) {
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int i = threadIdx.x; i < n / 2; i += threads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const u64 u = x[a], v = x[b];
+          if ((u < v) == ((a & k) == 0)) {
+            x[a] = v;
+            x[b] = u;
+          }
         }
+        small ? __syncwarp() : __syncthreads();
       }
-      __syncthreads();
     }
   }
+  __syncthreads();
 }
 
 // `u` of a sum of weights: the target is exceeded by exactly one token's running sum.
@@ -159,11 +222,6 @@ template <typename F>
 __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, bool by_mass, float share, u64 need, uint32_t cut,
                                            int n, F value, uint32_t rank) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto distance = [&](float v) -> uint32_t {  // (what is farther than a weight of 2^-127 counts as alike)
-    const double d = (weigh.top - static_cast<double>(v)) * weigh.c;
-    return static_cast<double>(v) == weigh.top ? 0u
-                                               : (d < 127.0 ? static_cast<uint32_t>(__double2int_rz(d * 8388608.0)) : 0x3FFFFFFFu);
-  };
   u64 over = 0;          // counts or weights before the prefix's range
   uint32_t prefix = 0, at = 0;
   for (int digit = 0; digit < 7; ++digit) {
@@ -181,7 +239,7 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
       for (int i = tid; i < n; i += kThreads) {
         const float v = value(i);
         const uint32_t k = Key(v);
-        if (k >= cut && distance(v) == at) {
+        if (k >= cut && weigh.Distance(v) == at) {
           a = min(a, k);
           b = max(b, k);
         }
@@ -209,7 +267,7 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
       const float v = value(i);
       const uint32_t k = Key(v);
       if (k < cut) continue;
-      uint32_t code = distance(v);
+      uint32_t code = weigh.Distance(v);
       if (by_key) {
         if (code != at) continue;
         code = ~k;
@@ -217,7 +275,7 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
       if (digit != 0 && digit != 3 && code >> (shift + bits) != prefix) continue;
       const uint32_t bin = code >> shift & ((1u << bits) - 1);
       if (by_mass) {
-        const u64 w = Fixed(weigh(v));
+        const u64 w = weigh.Fixed(v);
         const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
         if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
         if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
@@ -276,7 +334,11 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = ClusterRank();
   const int row = blockIdx.x / kCluster;
-  if (tid < 256) sh.power[tid] = exp2(tid / 256.0);
+  if (tid < 256) {
+    const double x = exp2(tid / 256.0);
+    const float h = static_cast<float>(x);
+    sh.power[tid] = make_float2(h, static_cast<float>(x - static_cast<double>(h)));
+  }
   if (tid == 0) sh.n_mine = 0;
   dev::GridLaunchDependents();
   dev::GridWait();
@@ -335,7 +397,11 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
   const unsigned my_key = Key(best);
   sh.thread_top[tid] = my_key;
   {
-    const unsigned w = __reduce_max_sync(0xFFFFFFFFu, my_key);
+    unsigned w = my_key;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) w = max(w, __shfl_xor_sync(0xFFFFFFFFu, w, o));
+    if (lane % 8 == 0) sh.group_top[tid / 8] = w;
+    w = __reduce_max_sync(0xFFFFFFFFu, w);
     if (lane == 0) sh.wide[warp] = w;
   }
   __syncthreads();
@@ -386,20 +452,51 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     const float low = cut - (fabsf(most) + fabsf(temperature * logf(min_p))) * 9.5367431640625e-7f;
     if (low > -INFINITY && most < INFINITY) least_min = max(1u, Key(low));
   }
-  // the weight of a value, 0 where a filter drops it
-  auto kept = [&](float v, double& w) -> u64 {
-    const uint32_t k = Key(v);
-    if (k < least_min || k < cut) return 0;
-    w = weigh(v);
-    return min_p > 0.f && min_p <= 1.f && w < static_cast<double>(min_p) ? 0 : Fixed(w);
+  const bool by_min = min_p > 0.f && min_p <= 1.f;
+  // the weights of two values, 0 where a filter drops them
+  auto kept = [&](float2 v, float2& hi, float2& lo) {
+    weigh(v, hi, lo);
+    const uint32_t least = max(least_min, cut);
+    if (least == 1) return;  // (what is not finite has no weight)
+    if (Key(v.x) < least || (by_min && static_cast<double>(hi.x) + static_cast<double>(lo.x) < static_cast<double>(min_p))) {
+      hi.x = lo.x = 0.f;
+    }
+    if (Key(v.y) < least || (by_min && static_cast<double>(hi.y) + static_cast<double>(lo.y) < static_cast<double>(min_p))) {
+      hi.y = lo.y = 0.f;
+    }
   };
 
   if (by_k || by_p) {
-    // ---- a bound that at least `want` values reach: the want-th largest of the threads' values (its upper 22 bits)
+    // ---- a bound that at least `want` values reach: the want-th largest of the
+    // largest values of groups of the row (its upper 22 bits).  Of 512 groups of
+    // eight threads one warp finds it; where more are wanted, of all threads, together.
     const int want = by_k ? min(top_k, kMostK + 1) : kFirst;
-    bool listed = want <= kMostK;
+    const bool listed = want <= kMostK;
     uint32_t bound = 0;
-    if (listed) {
+    if (want <= kGroups / 4 * 3) {
+      if (warp == 0) {
+        unsigned key[kGroups / 32];
+#pragma unroll
+        for (int i = 0; i < kGroups / 32; i += 4) {
+          const int at = lane * (kGroups / 32) + i;
+          const uint4 w = *reinterpret_cast<const uint4*>(In(sh.group_top, at / (kGroups / kCluster)) + at % (kGroups / kCluster));
+          key[i] = w.x;
+          key[i + 1] = w.y;
+          key[i + 2] = w.z;
+          key[i + 3] = w.w;
+        }
+        for (int bit = 31; bit >= 10; --bit) {
+          const uint32_t try_ = bound | 1u << bit;
+          int c = 0;
+#pragma unroll
+          for (int i = 0; i < kGroups / 32; ++i) c += key[i] >= try_;
+          if (__reduce_add_sync(0xFFFFFFFFu, c) >= want) bound = try_;
+        }
+        if (lane == 0) sh.least = bound;
+      }
+      __syncthreads();
+      bound = sh.least;
+    } else if (listed) {
       unsigned key[kCluster];
 #pragma unroll
       for (uint32_t b = 0; b < kCluster; ++b) key[b] = In(sh.thread_top, b)[tid];
@@ -409,31 +506,52 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
 #pragma unroll
         for (int b = 0; b < kCluster; ++b) c += key[b] >= try_;
         c = __reduce_add_sync(0xFFFFFFFFu, c);
-        if (lane == 0) sh.wide[warp] = c;
+        unsigned* wide = sh.wide + (bit & 1) * kWarps;
+        if (lane == 0) wide[warp] = c;
         __syncthreads();
-        int all = lane < kWarps ? static_cast<int>(sh.wide[lane]) : 0;
-        all = __reduce_add_sync(0xFFFFFFFFu, all);
-        if (all >= want) bound = try_;
-        __syncthreads();
+        int all = lane < kWarps ? static_cast<int>(wide[lane]) : 0;
+        if (__reduce_add_sync(0xFFFFFFFFu, all) >= want) bound = try_;
       }
-      bound = max(bound, 1u);
     }
+    bound = max(bound, kLowest);
     // ---- what reaches it, and the sum of all weights where the list may not hold all that counts
-    u64 mass = 0;
-    for (int i0 = warp * 32; i0 < n; i0 += kThreads) {
-      const int i = i0 + lane;
-      const uint32_t k = i < n ? Key(kvd::ToFloat(vals[i])) : 0;
-      if (!by_k && k != 0) mass += Fixed(weigh(kvd::ToFloat(vals[i])));
-      const bool in = listed && k >= bound;
-      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, in);
-      if (mask != 0) {
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&sh.n_mine, __popc(mask));
-        at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(mask & ((1u << lane) - 1));
-        if (in && at < kList / 4) sh.mine[at] = static_cast<u64>(k) << 32 | ~static_cast<uint32_t>(begin + i);
+    const float bound_value = listed ? FromKey(bound) : INFINITY;
+    Sum sum;
+    constexpr int kAhead = 4;
+    for (int i0 = warp * 32 * kAhead; i0 < n; i0 += kThreads * kAhead) {
+      float v[kAhead];
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int i = i0 + e * 32 + lane;
+        v[e] = i < n ? kvd::ToFloat(vals[i]) : -INFINITY;
+        any |= v[e] >= bound_value;
+      }
+      if (!by_k) {
+#pragma unroll
+        for (int e = 0; e < kAhead; e += 2) {
+          float2 h, l;
+          weigh(make_float2(v[e], v[e + 1]), h, l);
+          sum.Add(h, l);
+        }
+      }
+      if (listed && __any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          const bool in = v[e] >= bound_value;
+          const uint32_t mask = __ballot_sync(0xFFFFFFFFu, in);
+          if (mask != 0) {
+            unsigned at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n_mine, __popc(mask));
+            at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(mask & ((1u << lane) - 1));
+            if (in && at < kList / 4) {
+              sh.mine[at] = static_cast<u64>(Key(v[e])) << 32 | ~static_cast<uint32_t>(begin + i0 + e * 32 + lane);
+            }
+          }
+        }
       }
     }
-    mass = WarpAdd(mass);
+    const u64 mass = WarpAdd(Weights::ToFixed(sum.Total()));
     if (lane == 0) sh.wsum[warp] = mass;
     __syncthreads();
     if (tid == 0) {
@@ -466,14 +584,14 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
         for (int i = m + tid; i < size; i += kThreads) sh.list[i] = 0;
         __syncthreads();
         Sort(sh.list, size);
-        const uint32_t least_k = by_k ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
+        const uint32_t least_k = by_k && top_k <= m ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
         // weights of the values from least_k on, and their running sums: four values a thread
         u64 w[4], own = 0;
         const int i = 4 * tid;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
-          w[e] = k >= least_k ? Fixed(weigh(FromKey(k))) : 0;
+          w[e] = k >= least_k && k != 0 ? weigh.Fixed(FromKey(k)) : 0;
           own += w[e];
         }
         u64 excl = WarpScan(own, lane);
@@ -505,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
           int last = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            double d = 0.0;
-            w[e] = i + e < m ? kept(FromKey(sh.list[i + e] >> 32), d) : 0;
+            const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
+            if (k < cut || k < least_min || (by_min && weigh(FromKey(k)) < static_cast<double>(min_p))) w[e] = 0;
             weight[i + e] = w[e];
             own += w[e];
             if (w[e] > 0) last = i + e + 1;
@@ -558,10 +676,28 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
 
   // ---- the kept weights: a run of the row for each warp
   const int run = (per + kThreads - 1) / kThreads, lo = min(warp * 32 * run, n), hi = min(lo + 32 * run, n);
-  double w = 0.0;
-  u64 mine = 0;
-  for (int i = lo + lane; i < hi; i += 32) mine += kept(kvd::ToFloat(vals[i]), w);
-  mine = WarpAdd(mine);
+  const float floor_ = fmaxf(cut > 1 ? FromKey(cut) : -INFINITY, least_min > 1 ? FromKey(least_min) : -INFINITY);
+  Sum sum;
+  constexpr int kAhead = 4;
+  for (int i0 = lo; i0 < hi; i0 += 32 * kAhead) {
+    float v[kAhead];
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int i = i0 + e * 32 + lane;
+      v[e] = i < hi ? kvd::ToFloat(vals[i]) : -INFINITY;
+      any |= v[e] >= floor_;
+    }
+    if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+      for (int e = 0; e < kAhead; e += 2) {
+        float2 h, l;
+        kept(make_float2(v[e], v[e + 1]), h, l);
+        sum.Add(h, l);
+      }
+    }
+  }
+  const u64 mine = WarpAdd(Weights::ToFixed(sum.Total()));
   if (lane == 0) sh.wsum[warp] = mine;
   __syncthreads();
   if (tid == 0) {
@@ -576,29 +712,56 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     if (b < rank) before += s;
     total += s;
   }
+  ClusterArrive();
   for (int k = 0; k < warp; ++k) before += sh.wsum[k];
   const u64 target = Target(p, row, total);
   if (before <= target && target - before < mine) {
-    // this warp has it: a run for each lane, then the values of that run
-    u64 own = 0;
+    // This warp has it: a run for each lane, then the values of that run.  (These
+    // sums round elsewhere than the warp's, by 2^-44: what is past the end goes to
+    // the last that is kept.)
+    Sum run_sum;
     const int a = min(lo + lane * run, hi), b = min(a + run, hi);
-    for (int i = a; i < b; ++i) own += kept(kvd::ToFloat(vals[i]), w);
-    const u64 excl = WarpScan(own, lane) - own + before;
-    const int who = __ffs(__ballot_sync(0xFFFFFFFFu, excl <= target && target - excl < own)) - 1;
-    const int a1 = __shfl_sync(0xFFFFFFFFu, a, who), b1 = __shfl_sync(0xFFFFFFFFu, b, who);
-    u64 so_far = __shfl_sync(0xFFFFFFFFu, excl, who);
-    for (int i0 = a1; i0 < b1; i0 += 32) {
-      const int i = i0 + lane;
-      const u64 v = i < b1 ? kept(kvd::ToFloat(vals[i]), w) : 0;
-      const u64 incl = so_far + WarpScan(v, lane);
-      if (incl - v <= target && target < incl) {
-        p.tok[row] = begin + i;
-        if (p.prob != nullptr) p.prob[row] = static_cast<float>(w * kFix / static_cast<double>(total));
+    for (int i0 = 0; i0 < run; i0 += kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) v[e] = a + i0 + e < b ? kvd::ToFloat(vals[a + i0 + e]) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < kAhead; e += 2) {
+        float2 h, l;
+        kept(make_float2(v[e], v[e + 1]), h, l);
+        run_sum.Add(h, l);
       }
-      so_far = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    }
+    const u64 own = Weights::ToFixed(run_sum.Total());
+    const u64 incl = before + WarpScan(own, lane);
+    const uint32_t over = __ballot_sync(0xFFFFFFFFu, own > 0 && target < incl), some = __ballot_sync(0xFFFFFFFFu, own > 0);
+    const int who = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
+    const int a1 = __shfl_sync(0xFFFFFFFFu, a, who), b1 = __shfl_sync(0xFFFFFFFFu, b, who);
+    u64 so_far = __shfl_sync(0xFFFFFFFFu, incl - own, who);
+    int last = -1;  // the lane's last kept value
+    bool found = false;
+    for (int i0 = a1; i0 < b1 && !found; i0 += 32) {
+      const int i = i0 + lane;
+      float2 h, l;
+      kept(make_float2(i < b1 ? kvd::ToFloat(vals[i]) : -INFINITY, -INFINITY), h, l);
+      const u64 w = Weights::ToFixed(static_cast<double>(h.x) + static_cast<double>(l.x));
+      const u64 to = so_far + WarpScan(w, lane);
+      if (w > 0) last = i;
+      const uint32_t here = __ballot_sync(0xFFFFFFFFu, w > 0 && target < to);
+      if (here != 0) {
+        last = __shfl_sync(0xFFFFFFFFu, i, __ffs(here) - 1);
+        found = true;
+      }
+      so_far = __shfl_sync(0xFFFFFFFFu, to, 31);
+    }
+    if (!found) last = __reduce_max_sync(0xFFFFFFFFu, last);
+    if (lane == 0) {
+      p.tok[row] = begin + last;
+      if (p.prob != nullptr) p.prob[row] = static_cast<float>(weigh(kvd::ToFloat(vals[last])) * kFix / static_cast<double>(total));
     }
   }
-  ClusterSync();  // no block ends while another reads its sums
+  __syncwarp();
+  ClusterWait();  // no block ends while another reads its sums
 }
 
 template <typename T>

@@ -170,6 +170,26 @@ def test_not_finite():
     assert tok[4] in (100, 3500) and prob[4] == 0.5 and tok[7] == 1234
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_fewer_values_than_are_wanted(act):
+    # a mask that leaves a few values, scattered or side by side, under a larger k and a share
+    x, u = logits(8, 40000, act, seed=9)
+    for r in range(8):
+        keep = torch.arange(40000, device="cuda") % (5000 + r) == r if r % 2 else torch.arange(40000, device="cuda") < 3 * r + 1
+        x[r, ~keep] = -math.inf if r < 4 else math.nan
+    for kw in (dict(k=100), dict(k=600), dict(k=2000, p=0.9), dict(p=0.7), dict(k=30, m=0.2)):
+        check(x, u, t=1.2, **kw)
+
+
+def test_values_in_order():
+    # the largest values side by side, in one block's part
+    x = torch.linspace(-20, 20, 100000, device="cuda").flip(0).expand(6, -1).contiguous()
+    x[3:] = x[3:].flip(1)
+    u = [0.1, 0.5, 0.9] * 2
+    for kw in (dict(k=50), dict(k=700), dict(p=0.9), dict(k=1200, p=0.5), dict(k=5000), dict()):
+        check(x, u, t=1.0, **kw)
+
+
 def test_temperatures_near_zero_and_huge():
     x, u = logits(6, 9000, seed=2)
     check(x, u, t=[1e-30, 1e-3, 1e-2, 100.0, 1e6, 1e30])
