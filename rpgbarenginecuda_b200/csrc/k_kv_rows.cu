@@ -38,12 +38,20 @@ struct Seen {
   int start, end;
   bool past;
 };
-__device__ __forceinline__ Seen SeenBy(const KvRowsParams& p, int row) {
+struct Bounds {
+  int start, end, prefix;  // as the caller gives them
+  __device__ __forceinline__ void Load(const KvRowsParams& p, int row) {
+    start = p.starts != nullptr ? p.starts[row] : 0;
+    end = p.ends[row];
+    prefix = p.prefix != nullptr ? p.prefix[row] : 0;
+  }
+};
+__device__ __forceinline__ Seen SeenBy(const KvRowsParams& p, const Bounds& b) {
   const int64_t cap = static_cast<int64_t>(p.table.max_pages) << p.kv.page_log2;
   Seen s;
-  s.start = p.starts != nullptr ? max(p.starts[row], 0) : 0;
-  int64_t end = max(p.ends[row], 0);
-  if (p.prefix != nullptr) end = min(end, static_cast<int64_t>(max(p.prefix[row], 0)));
+  s.start = max(b.start, 0);
+  int64_t end = max(b.end, 0);
+  if (p.prefix != nullptr) end = min(end, static_cast<int64_t>(max(b.prefix, 0)));
   s.past = end > cap && s.start < end;
   s.end = static_cast<int>(min(end, cap));
   if (s.start >= s.end) s.start = s.end = 0;
@@ -229,6 +237,7 @@ struct Slots {
   int list = 0;
   __device__ __forceinline__ void Seek(const KvRowsParams& p, const Split& sp, int slot) {
     int lo = 0, hi = p.n_lists - 1;
+#pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       SlotOf(p, sp, mid) <= slot ? lo = mid : hi = mid - 1;
@@ -237,6 +246,7 @@ struct Slots {
   }
   // Item of the slot (head and steps taken are the caller's); returns its steps, 0 where there is none.
   __device__ __forceinline__ int Get(const KvRowsParams& p, const Split& sp, int slot, Item& it) {
+#pragma unroll 1
     while (list + 1 < p.n_lists && SlotOf(p, sp, list + 1) <= slot) ++list;
     const int begin = RowBegin(p, list), end = RowEnd(p, list);
     const int64_t j = slot - (begin / sp.tokens + list), row0 = begin + j * sp.tokens;
@@ -278,6 +288,14 @@ __device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_gro
 template <int N>
 __device__ __forceinline__ void CopyWait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Bounded wait; one small loop (kernels.cuh's is unrolled, and there are many here).
+__device__ __forceinline__ bool Wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < 1u << 16; ++i) {
+    if (dev::MbarTryWait(bar, parity)) return true;
+  }
+  return false;
 }
 // 16 positions of 64 values of a head's page.
 __device__ __forceinline__ void LoadTile(void* dst, const CUtensorMap* map, int value, int at, int head, int page,
@@ -355,7 +373,7 @@ struct Reader {
   int n = 0;
   __device__ __forceinline__ bool Next(Bars& b, const Item* items, Item& it, int lane) {
     const int i = n % kItems;
-    if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&b.item_full[i], (n / kItems) & 1))) return false;
+    if (!__all_sync(0xFFFFFFFFu, Wait(&b.item_full[i], (n / kItems) & 1))) return false;
     it = items[i];
     __syncwarp();
     if (lane == 0) tc::MbarArrive(&b.item_empty[i]);
@@ -386,42 +404,29 @@ struct Join {
 };
 
 // 32 values of an output row.
-__device__ __forceinline__ void Put32(const KvRowsParams& p, bool wide, int64_t at, const float* y) {
+__device__ __forceinline__ void Put32(const KvRowsParams& p, int64_t at, const float* y) {
   if (p.type == ElemType::kF32) {
-    float* o = static_cast<float*>(p.out) + at;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + at);
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint32_t w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(y[i + e]);
-      if (wide) {
-        kvd::Store32(o + i, w);
-      } else {
-        reinterpret_cast<uint4*>(o + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(o + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      }
+    for (int i = 0; i < 8; ++i) {
+      o[i] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]),
+                        __float_as_uint(y[4 * i + 3]));
     }
   } else {
-    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+    uint32_t w[16];
+    if (p.type == ElemType::kF16) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 16) {
-      uint32_t w[8];
+      for (int i = 0; i < 16; ++i) w[i] = PackHalf(y[2 * i], y[2 * i + 1]);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (p.type == ElemType::kF16) {
-          w[e] = PackHalf(y[i + 2 * e], y[i + 2 * e + 1]);
-        } else {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(y[i + 2 * e], y[i + 2 * e + 1]);
-          w[e] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-      }
-      if (wide) {
-        kvd::Store32(o + i, w);
-      } else {
-        reinterpret_cast<uint4*>(o + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(o + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      for (int i = 0; i < 16; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 
@@ -491,6 +496,7 @@ struct RowState {
   Item it;
   int note0;  // steps before the item
   int row, qh;
+  Bounds bounds;
   Seen seen;
   float cs, slope;  // scores (in units of log2 where they are not capped) are products times cs
   int pos;
@@ -550,6 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     Slots<C> sl;
     Item it;
     if (slot_lo < slot_hi) sl.Seek(p, sp, slot_lo);
+#pragma unroll 1
     for (int i = slot_lo; i < slot_hi; ++i) {
       const int steps = sl.Get(p, sp, i, it);
       mine += steps > 0 ? steps + C::BORDER : 0;
@@ -567,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
   FenceAfterSync();
   const uint32_t tmem = s_tmem;
   long long before = incl - mine, per_head = 0;
+#pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += s_part[w];
     per_head += s_part[w];
@@ -597,9 +605,11 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       sl.Seek(p, sp, slot);
     }
     bool ok = true;
+#pragma unroll 1
     for (bool more = true; more && ok;) {
       Item it;
       it.steps = 0;
+      it.n_tok = 0;
       if (x < x1) {
         const int steps = sl.Get(p, sp, slot, it);
         const int weight = steps > 0 ? steps + C::BORDER : 0;
@@ -634,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         more = false;
       }
       const int i = n % kItems;
-      if (n >= kItems) ok = __all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.item_empty[i], (n / kItems - 1) & 1));
+      if (n >= kItems) ok = __all_sync(0xFFFFFFFFu, Wait(&bars.item_empty[i], (n / kItems - 1) & 1));
       if (!ok) break;
       if (lane == 0) {
         items[i] = it;
@@ -642,6 +652,15 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       }
       __syncwarp();
       ++n;
+      // its queries on their way into L2, an item or more before they are read
+      const int size = p.type == ElemType::kF32 ? 4 : 2;
+      const int heads = it.steps > 0 ? min(sp.per, sp.group - it.chunk * sp.per) : 0;
+      const int lines = (heads * D * size + 127) / 128;
+#pragma unroll 1
+      for (int k = lane; k < it.n_tok * lines; k += 32) {
+        const int64_t at = (it.row0 + k / lines) * p.q_stride + static_cast<int64_t>(it.head * sp.group + it.chunk * sp.per) * D;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.q) + at * size + k % lines * 128));
+      }
     }
     if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
   } else if (warp == kMmaWarp) {
@@ -654,19 +673,22 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
       int c = 0;  // steps so far
       bool ok = true;
+#pragma unroll 1
       while (ok) {
         const int i = n % kItems;
-        if (!dev::MbarWait(&bars.item_full[i], (n / kItems) & 1)) break;
+        if (!Wait(&bars.item_full[i], (n / kItems) & 1)) break;
         const int steps = items[i].steps, rows = items[i].n_tok * sp.per;
         MbarArrive(&bars.item_empty[i]);
         ++n;
         if (steps <= 0) break;
         const int tiles = rows > kTileRows ? 2 : 1;
+#pragma unroll 1
         for (int j = 0; j <= steps && ok; ++j) {
+#pragma unroll 1
           for (int t = 0; t < tiles && ok; ++t) {
             if (j > 0) {
               const int st = (c + j - 1) % C::STAGES, par = ((c + j - 1) / C::STAGES) & 1;
-              ok = (t > 0 || dev::MbarWait(&bars.v_full[st], par)) && dev::MbarWait(&bars.p_full[t], p_parity[t]);
+              ok = (t > 0 || Wait(&bars.v_full[st], par)) && Wait(&bars.p_full[t], p_parity[t]);
               if (!ok) break;
               p_parity[t] ^= 1;
               FenceAfterSync();
@@ -690,8 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             }
             if (j < steps) {
               const int st = (c + j) % C::STAGES, par = ((c + j) / C::STAGES) & 1;
-              ok = (j > 0 || dev::MbarWait(&bars.q_full[t], q_parity[t])) &&
-                   (t > 0 || dev::MbarWait(&bars.k_full[st], par));
+              ok = (j > 0 || Wait(&bars.q_full[t], q_parity[t])) &&
+                   (t > 0 || Wait(&bars.k_full[st], par));
               if (!ok) break;
               if (j == 0) q_parity[t] ^= 1;
               FenceAfterSync();
@@ -717,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         c += steps;
       }
       MmaCommit(&bars.fin);  // no product is under way when the block ends
-      dev::MbarWait(&bars.fin, 0);
+      Wait(&bars.fin, 0);
     }
     __syncwarp();
   } else {
@@ -734,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     auto finish = [&]() {
       const int step = ended >> 1, st = step % C::STAGES;
       const bool v = ended & 1;
-      if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(v ? &bars.v_empty[st] : &bars.k_empty[st], ((step / C::STAGES) & 1) ^ 1))) {
+      if (!__all_sync(0xFFFFFFFFu, Wait(v ? &bars.v_empty[st] : &bars.k_empty[st], ((step / C::STAGES) & 1) ^ 1))) {
         ok = false;
         return;
       }
@@ -772,6 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     };
     Reader rd;
     Item it;
+#pragma unroll 1
     while (ok && rd.Next(bars, items, it, lane)) {
       // lane g has to do with positions 16 g .. 16 g + 15 of a step: their page
       auto lookup = [&](int pos) {
@@ -780,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
                    : -1;
       };
       int next = lookup(it.base + it.step0 * KT + 16 * lane);
+#pragma unroll 1
       for (int j = 0; j < it.steps && ok; ++j) {
         const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
         const int page = next;
@@ -801,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           for (int v = 0; v < 2; ++v) {
             const int st = (begun >> 1) % C::STAGES;
             uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
-            if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
+            if (!__all_sync(0xFFFFFFFFu, Wait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
               ok = false;
               break;
             }
@@ -810,6 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             uint32_t rest = v ? groups & ~full : 0;
             if (rest != 0) {
               // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
+#pragma unroll 1
               while (rest != 0) {
                 const int q = __ffs(rest) - 1;
                 rest &= rest - 1;
@@ -887,8 +912,8 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       // copies that nobody waits for any more have landed before the block ends
       for (int n = max(0, begun / 2 - C::STAGES); n < begun / 2; ++n) {
         const int st = n % C::STAGES;
-        dev::MbarWait(&bars.k_full[st], (n / C::STAGES) & 1);
-        dev::MbarWait(&bars.v_full[st], (n / C::STAGES) & 1);
+        Wait(&bars.k_full[st], (n / C::STAGES) & 1);
+        Wait(&bars.v_full[st], (n / C::STAGES) & 1);
       }
     }
   }
@@ -898,8 +923,6 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     const int t = warp >> 2, in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128;
-    const int size = p.type == ElemType::kF32 ? 4 : 2;
-    const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.out_stride * size)) & 31) == 0;
     uint32_t s_parity = 0;
     int c = 0, note = 0;  // products with V begun for this tile; steps so far
     bool ok = true;
@@ -920,6 +943,13 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       w.cs = w.slope = 0.f;
       w.pos = 0;
       w.is_nan = false;
+      if (w.valid) {  // (on their way while the queries are read)
+        w.bounds.Load(p, w.row);
+        if (p.slopes != nullptr) {
+          w.slope = p.slopes[w.qh];
+          w.pos = p.pos[w.row];
+        }
+      }
       return true;
     };
     auto write_q = [&](RowState& w) {
@@ -932,23 +962,19 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           w.cs = p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
                                           : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile);
         }
-        w.seen = SeenBy(p, w.row);
+        w.seen = SeenBy(p, w.bounds);
         const Seen& s = w.seen;
         w.is_nan = s.past || (s.start < s.end && (s.start < w.it.lo || s.end > w.it.hi)) || !(w.cs == w.cs) ||
-                   (p.prefix != nullptr && p.prefix[w.row] > w.it.first_prefix);
+                   (p.prefix != nullptr && w.bounds.prefix > w.it.first_prefix);
         if (!(p.cap > 0.f)) w.cs = fmaxf(w.cs * kLog2e, 1e-37f);  // (a scale of 0: minus infinity times it is to stay)
-        if (p.slopes != nullptr) {
-          w.slope = p.slopes[w.qh];
-          w.pos = p.pos[w.row];
-        }
       }
       dev::FenceProxyAsync();
       __syncwarp();
       if (lane == 0) MbarArrive(&bars.q_full[t]);
     };
-    RowState now;
-    bool more = next_item(now);
-    if (more) write_q(now);
+    RowState now{};  // (an item of no steps, before the first)
+    bool more = true;
+#pragma unroll 1
     while (ok && more) {
       const Item& it = now.it;
       const int steps = it.steps, note0 = now.note0, row = now.row, qh = now.qh;
@@ -966,7 +992,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         for (int i = 0; i < D / 2; ++i) acc[i % (C::TWO ? D / 2 : 1)] = make_float2(0.f, 0.f);
       }
       auto ProductsDone = [&]() {  // those with V of the last step
-        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) return false;
+        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t], (c - 1) & 1))) return false;
         FenceAfterSync();
         return true;
       };
@@ -1171,8 +1197,9 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         FenceBeforeSync();
         return true;
       };
+#pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        if (!__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.s_full[t], s_parity))) {
+        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.s_full[t], s_parity))) {
           ok = false;
           break;
         }
@@ -1202,7 +1229,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       more = ok && next_item(then);
       if (!C::TWO && more) write_q(then);
       // ---- the end of the item, or of this block's piece of it
-      if (ok && !__all_sync(0xFFFFFFFFu, dev::MbarWait(&bars.pv_done[t], (c - 1) & 1))) ok = false;
+      if (ok && steps > 0 && !__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t], (c - 1) & 1))) ok = false;
       FenceAfterSync();
       const int64_t row_head = static_cast<int64_t>(row) * p.n_heads + qh;
       const int64_t out = row * p.out_stride + static_cast<int64_t>(qh) * D;
@@ -1212,7 +1239,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       if (active) {
         const Join jn = valid && whole ? Join(p, row_head, ref, l) : Join(p, 0, 0.f, 0.f);
         float check = 0.f;
-#pragma unroll
+#pragma unroll (C::TWO ? D / 32 : 1)
         for (int k = 0; k < D; k += 32) {
           uint32_t o[32];
           TmemLoad32(a_o + k, o);
@@ -1237,7 +1264,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
                 y[i + 3] += jn.g * w.w;
               }
             }
-            Put32(p, wide, out + k, y);
+            Put32(p, out + k, y);
           } else if (valid) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
@@ -1256,6 +1283,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           // infinities and NaN: such rows again, by the formula
           uint32_t again = __ballot_sync(0xFFFFFFFFu, valid && !nan_row && ok && !(check + l * 0.f == 0.f));
           const int from = it.base + it.step0 * KT, to = from + steps * KT;
+#pragma unroll 1
           while (again != 0) {
             const int w = __ffs(again) - 1;
             again &= again - 1;
