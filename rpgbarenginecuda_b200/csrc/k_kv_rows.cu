@@ -172,7 +172,8 @@ constexpr int kSoftRegs = 216, kOtherRegs = 72;
 static_assert(kThreads == 384 && kSoftRegs * 256 + kOtherRegs * 128 <= 168 * kThreads, "registers");
 constexpr int kMaxBlocks = 160;
 constexpr int kItems = 4;    // items described ahead
-constexpr int kNotes = 8;    // steps whose scales and bad pages are held
+constexpr int kNotes = 8;    // steps whose bad pages are held
+constexpr int kScales = 4;   // steps whose scales are held, as they come and as f32
 constexpr int kLeast = 2;    // steps that a block is started for
 constexpr int kHeadroom = 15, kSlack = 8;  // weights are at most 2^15, and 2^7 when their reference was set
 
@@ -194,9 +195,10 @@ struct Cfg {
   static constexpr int CPR = ROW / 16;
   static constexpr int PER = KT * CPR / (32 * kLoadWarps);  // 16-byte pieces of a thread
   static constexpr int RAW = QUANT ? KT * ROW : 0;
-  static constexpr int NOTE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
+  static constexpr int SCALE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
+  static constexpr int NOTE = 2 * SCALE;                     // the same as f32, [K or V][group][position]
   static constexpr int BORDER = TWO ? 5 : (QUANT ? 6 : 4);  // steps that the beginning and end of an item are worth
-  static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kNotes * NOTE;
+  static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kScales * (SCALE + NOTE);
   static_assert(SMEM <= 230 * 1024, "shared memory");
 };
 
@@ -512,6 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
   __shared__ Bars bars;
   __shared__ Item items[kItems];
   __shared__ uint32_t s_tmem, s_bad[kNotes];
+  __shared__ int2 s_seen[kLoadWarps][kScales];  // a warp's own notes of what a step's rows see
   __shared__ long long s_part[kThreads / 32], s_before;
   __shared__ int s_slot;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -519,7 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
   char* s_k = s_q + 2 * C::QTILE;
   char* s_v = s_k + C::STAGES * C::PLANE;
   char* s_raw = s_v + C::STAGES * C::PLANE;
-  char* s_note = s_raw + (C::LAG + 1) * C::RAW;
+  char* s_scale = s_raw + (C::LAG + 1) * C::RAW;
+  char* s_note = s_scale + kScales * C::SCALE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Split sp(p);
 
@@ -749,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     int begun = 0, ended = 0;  // copies: 2 n is K's of step n, 2 n + 1 V's
     bool ok = true;
     asm volatile("fence.proxy.async.global;" ::: "memory");  // (what kernels before this one stored is read by copies)
-    const uint32_t a_raw = dev::SmemAddr(s_raw), a_note = dev::SmemAddr(s_note);
+    const uint32_t a_raw = dev::SmemAddr(s_raw), a_scale = dev::SmemAddr(s_scale);
     const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
     constexpr int kRowStep = 32 * kLoadWarps / C::CPR;
     // The oldest copy of codes has arrived: spread them to f16, tell the products.
@@ -787,6 +791,18 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
         }
       }
+      if (!v) {
+        // the scales that this warp copied, group after group; 0 where no row sees the position
+        __syncwarp();
+        const int2 seen = s_seen[lw][step % kScales];
+        const __half* h = reinterpret_cast<const __half*>(s_scale + step % kScales * C::SCALE + lw * (C::SCALE / 2));
+        float* f = reinterpret_cast<float*>(s_note + step % kScales * C::NOTE + lw * (C::NOTE / 2));
+#pragma unroll 1
+        for (int i = lane; i < KT * C::NG; i += 32) {
+          const int pos = i / C::NG;
+          f[i % C::NG * KT + pos] = pos >= seen.x && pos < seen.y ? __half2float(h[i]) : 0.f;
+        }
+      }
       dev::FenceProxyAsync();
       __syncwarp();
       if (lane == 0) MbarArrive(v ? &bars.v_full[st] : &bars.k_full[st]);
@@ -814,6 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
         const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
         if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
+        if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % kScales] = make_int2(it.lo - pos0, it.hi - pos0);
         if (!C::QUANT) {
           // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
           const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
@@ -892,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
               if (lane < KT / 16 * kPer) {
                 const bool in = (have >> i) & 1;
                 const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
-                CopyAsync16(a_note + (begun >> 1) % kNotes * C::NOTE + lw * (C::NOTE / 2) + lane * 16, in ? src + o : src, in);
+                CopyAsync16(a_scale + (begun >> 1) % kScales * C::SCALE + lw * (C::SCALE / 2) + lane * 16, in ? src + o : src, in);
               }
             }
             CopyCommit();
@@ -997,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         return true;
       };
       // Softmax of a step's scores, weights into tensor memory.  EDGE: some row of the warp does not see all positions.
-      auto step = [&](auto edge, int j, int from, int to, int pos0, const char* scales) {
+      auto step = [&](auto edge, int j, int from, int to, int pos0, const float* scales) {
         constexpr bool EDGE = decltype(edge)::value;
         if (C::TWO && j > 0) {
           if (!ProductsDone()) return false;  // (they came before these scores)
@@ -1024,13 +1041,13 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             TmemLoad16(a_s + 64 + h, b);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-              const uint4 w = *reinterpret_cast<const uint4*>(scales + (h + i) * 4);
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 d = __half22float2(kvd::BitsHalf(ww[e]));
-                u[h + i + e] = __float_as_uint(__uint_as_float(u[h + i + e]) * d.x + __uint_as_float(b[i + e]) * d.y);
-              }
+              const float4 d0 = *reinterpret_cast<const float4*>(scales + h + i);
+              const float4 d1 = *reinterpret_cast<const float4*>(scales + KT + h + i);
+              float2 &x = s[(h + i) / 2], &y = s[(h + i) / 2 + 1];
+              const float2 bx = make_float2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]));
+              const float2 by = make_float2(__uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
+              x = __ffma2_rn(bx, make_float2(d1.x, d1.y), __fmul2_rn(x, make_float2(d0.x, d0.y)));
+              y = __ffma2_rn(by, make_float2(d1.z, d1.w), __fmul2_rn(y, make_float2(d0.z, d0.w)));
             }
           }
         } else {
@@ -1039,11 +1056,10 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           TmemLoadWait();
           if (C::QUANT) {
 #pragma unroll
-            for (int i = 0; i < KT / 2; i += 4) {
-              const uint4 w = *reinterpret_cast<const uint4*>(scales + i * 4);
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[i + e] = __fmul2_rn(s[i + e], __half22float2(kvd::BitsHalf(ww[e])));
+            for (int i = 0; i < KT; i += 4) {
+              const float4 d = *reinterpret_cast<const float4*>(scales + i);
+              s[i / 2] = __fmul2_rn(s[i / 2], make_float2(d.x, d.y));
+              s[i / 2 + 1] = __fmul2_rn(s[i / 2 + 1], make_float2(d.z, d.w));
             }
           }
         }
@@ -1066,29 +1082,24 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         }
         float2 top = s[0], top2 = s[1];
 #pragma unroll
-        for (int i = 2; i < KT / 2; i += 2) {
-          top.x = fmaxf(top.x, s[i].x);
-          top.y = fmaxf(top.y, s[i].y);
-          top2.x = fmaxf(top2.x, s[i + 1].x);
-          top2.y = fmaxf(top2.y, s[i + 1].y);
+        for (int i = 2; i + 3 < KT / 2; i += 4) {  // (three at a time is one instruction)
+          top.x = fmaxf(fmaxf(top.x, s[i].x), s[i + 1].x);
+          top.y = fmaxf(fmaxf(top.y, s[i].y), s[i + 1].y);
+          top2.x = fmaxf(fmaxf(top2.x, s[i + 2].x), s[i + 3].x);
+          top2.y = fmaxf(fmaxf(top2.y, s[i + 2].y), s[i + 3].y);
         }
+        static_assert(KT / 2 % 4 == 0, "two pairs are left");
+        top.x = fmaxf(fmaxf(top.x, s[KT / 2 - 2].x), s[KT / 2 - 1].x);
+        top.y = fmaxf(fmaxf(top.y, s[KT / 2 - 2].y), s[KT / 2 - 1].y);
         const float mx = fmaxf(fmaxf(top.x, top.y), fmaxf(top2.x, top2.y));
         const float to_log2 = bend.capped || bend.biased ? 1.f : cs;
         if (C::QUANT) {
-          // an exponent over the V scales that count
-          const char* vs = scales + C::NOTE / 2;
+          // an exponent over the step's V scales
+          const float* vs = scales + C::NG * KT;
           float most = 0.f;
-          if (EDGE) {
-            for (int i = from * C::NG; i < to * C::NG; ++i) {
-              most = fmaxf(most, fabsf(__half2float(reinterpret_cast<const __half*>(vs)[i])));
-            }
-          } else {
-            for (int i = lane; i < KT * C::NG / 2; i += 32) {
-              const float2 d = __half22float2(__habs2(reinterpret_cast<const __half2*>(vs)[i]));
-              most = fmaxf(most, fmaxf(d.x, d.y));
-            }
-            most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
-          }
+#pragma unroll
+          for (int i = 0; i < KT * C::NG / 32; ++i) most = fmaxf(most, fabsf(vs[32 * i + lane]));
+          most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
           nu = max(nu, static_cast<int>(__float_as_uint(most) >> 23) - 126);
         }
         m = fmaxf(m, mx * to_log2);
@@ -1155,32 +1166,23 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         l += sum.x + sum.y;
         if (C::QUANT) {
           // times the scales of each group's values
-          const char* vs = scales + C::NOTE / 2;
+          const float* vs = scales + C::NG * KT;
 #pragma unroll
           for (int gp = 0; gp < C::NG; ++gp) {
 #pragma unroll
             for (int h = 0; h < KT; h += 32) {
               uint32_t w[16], w2[16];
 #pragma unroll
-              for (int i = 0; i < 32; i += 8 / C::NG) {
-                const uint4 x = *reinterpret_cast<const uint4*>(vs + (h + i) * 2 * C::NG);
-                const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
+              for (int i = 0; i < 32; i += 4) {
+                const float4 d = *reinterpret_cast<const float4*>(vs + gp * KT + h + i);
 #pragma unroll
-                for (int e = 0; e < 4 / C::NG; ++e) {
-                  float2 d;
-                  if (C::NG == 2) {
-                    const float2 d0 = __half22float2(kvd::BitsHalf(xx[2 * e % 4])), d1 = __half22float2(kvd::BitsHalf(xx[(2 * e + 1) % 4]));
-                    d = gp == 0 ? make_float2(d0.x, d1.x) : make_float2(d0.y, d1.y);
-                  } else {
-                    d = __half22float2(kvd::BitsHalf(xx[e]));
-                  }
-                  const int k = h + i + 2 * e;
-                  float2 y = __fmul2_rn(s[k / 2], d);
+                for (int e = 0; e < 2; ++e) {
+                  const int k = h + i + 2 * e, at = i / 2 + e;
+                  float2 y = __fmul2_rn(s[k / 2], e == 0 ? make_float2(d.x, d.y) : make_float2(d.z, d.w));
                   if (EDGE) {  // (a scale that the row does not see may be NaN)
                     if (k < from || k >= to) y.x = 0.f;
                     if (k + 1 < from || k + 1 >= to) y.y = 0.f;
                   }
-                  const int at = (i + 2 * e) / 2;
                   w[at] = PackHalf(y.x, y.y);
                   if (C::TWO) {
                     const float2 f = __half22float2(kvd::BitsHalf(w[at]));
@@ -1213,7 +1215,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             // columns from .. to - 1 in units of 16
             if (bad & ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u)) nan_row = true;
           }
-          const char* scales = s_note + (note0 + j) % kNotes * C::NOTE;
+          const float* scales = reinterpret_cast<const float*>(s_note + (note0 + j) % kScales * C::NOTE);
           ok = __any_sync(0xFFFFFFFFu, valid && (from > 0 || to < KT)) ? step(std::true_type(), j, from, to, pos0, scales)
                                                                        : step(std::false_type(), j, from, to, pos0, scales);
           if (!ok) break;
