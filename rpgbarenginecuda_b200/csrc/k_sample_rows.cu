@@ -149,11 +149,11 @@ struct Weights {
   static __device__ __forceinline__ u64 ToFixed(double w) {
     return static_cast<u64>(__double_as_longlong(fma(w, kFix, 4503599627370496.0)) - 0x4330000000000000ll);
   }
-  // How far x lies under the largest value, in units of 2^-23 of a factor 2 of
-  // weight; what is farther than 2^-127 counts as alike.  Larger values are never farther.
+  // How far x lies under the largest value, in units of 2^-24 of a factor 2 of
+  // weight; what is farther than 2^-63 counts as alike.  Larger values are never farther.
   __device__ __forceinline__ uint32_t Distance(float x) const {
     const float d = (top - x) * c;
-    return x == top ? 0u : (d < 127.f ? static_cast<uint32_t>(d * 8388608.f) : 0x3FFFFFFFu);
+    return x == top ? 0u : (d < 63.f ? static_cast<uint32_t>(d * 16777216.f) : 0x3FFFFFFFu);
   }
 };
 // A running sum of weights: f32 with what its additions lose.
@@ -215,18 +215,57 @@ __device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 to
 // Among the row's values with keys from `cut` on: the key of the `need`-th
 // largest, or (by_mass) the largest key from which on the weights reach `share`
 // of their sum; `cut` where there is none.  First by the distance from the
-// largest value, in units of 2^-23 of a factor 2 of weight, ten bits at a time:
-// a row's values spread over many bins so.  Then, where distances round alike
-// and keys do not, by the keys.
+// largest value, in units of 2^-24 of a factor 2 of weight, ten bits at a time:
+// a row's values spread over many bins so, and the few in the bin that counts
+// are listed for what follows.  Then, where distances round alike and keys do
+// not, by the keys.
 template <typename F>
 __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, bool by_mass, float share, u64 need, uint32_t cut,
                                            int n, F value, uint32_t rank) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  u64 over = 0;          // counts or weights before the prefix's range
+  u64 over = 0;  // counts or weights before the prefix's range
   uint32_t prefix = 0, at = 0;
+  int listed = -1;  // values of this block that are listed in sh.mine; -1: all are looked through
+  constexpr int kAhead = 4;
+  // every value that counts, four of a thread at a time
+  auto each = [&](auto f) {
+    const int count = listed >= 0 ? listed : n;
+#pragma unroll 1
+    for (int i0 = tid; i0 < count; i0 += kThreads * kAhead) {
+      float v[kAhead];
+      int i[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        i[e] = i0 + e * kThreads;
+        v[e] = -INFINITY;
+        if (i[e] < count) {
+          if (listed >= 0) i[e] = static_cast<int>(sh.mine[i[e]]);
+          v[e] = value(i[e]);
+        }
+      }
+      f(v, i);
+    }
+  };
+#pragma unroll 1
   for (int digit = 0; digit < 7; ++digit) {
     const bool by_key = digit >= 3;  // three digits of the distance, then four of 8 bits of the key's complement
     const int bits = by_key ? 8 : kBinBits, shift = by_key ? 24 - 8 * (digit - 3) : 20 - 10 * digit;
+    if (digit == 1) {
+      // what is in the bin
+      if (tid == 0) sh.n_mine = 0;
+      __syncthreads();
+      each([&](const float (&v)[kAhead], const int (&i)[kAhead]) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          if (Key(v[e]) >= cut && weigh.Distance(v[e]) >> 20 == prefix) {
+            const unsigned to = atomicAdd(&sh.n_mine, 1u);
+            if (to < kList / 4) sh.mine[to] = static_cast<u64>(i[e]);
+          }
+        }
+      });
+      __syncthreads();
+      if (sh.n_mine <= kList / 4) listed = static_cast<int>(sh.n_mine);
+    }
     if (digit == 3) {
       at = prefix;
       prefix = 0;
@@ -236,14 +275,16 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
       }
       __syncthreads();
       uint32_t a = 0xFFFFFFFFu, b = 0;
-      for (int i = tid; i < n; i += kThreads) {
-        const float v = value(i);
-        const uint32_t k = Key(v);
-        if (k >= cut && weigh.Distance(v) == at) {
-          a = min(a, k);
-          b = max(b, k);
+      each([&](const float (&v)[kAhead], const int (&)[kAhead]) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          const uint32_t k = Key(v[e]);
+          if (k >= cut && weigh.Distance(v[e]) == at) {
+            a = min(a, k);
+            b = max(b, k);
+          }
         }
-      }
+      });
       a = __reduce_min_sync(0xFFFFFFFFu, a);
       b = __reduce_max_sync(0xFFFFFFFFu, b);
       if (lane == 0) {
@@ -263,36 +304,47 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
     for (int i = tid; i < kBins; i += kThreads) sh.bins.part[0][i] = sh.bins.part[1][i] = sh.bins.part[2][i] = 0;
     if (tid == 0) sh.found = -1;
     __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = value(i);
-      const uint32_t k = Key(v);
-      if (k < cut) continue;
-      uint32_t code = weigh.Distance(v);
-      if (by_key) {
-        if (code != at) continue;
-        code = ~k;
-      }
-      if (digit != 0 && digit != 3 && code >> (shift + bits) != prefix) continue;
-      const uint32_t bin = code >> shift & ((1u << bits) - 1);
+    each([&](const float (&v)[kAhead], const int (&)[kAhead]) {
+      float2 hi[kAhead / 2], lo[kAhead / 2];
       if (by_mass) {
-        const u64 w = weigh.Fixed(v);
-        const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
-        if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
-        if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
-        if ((low & 0x7FFFu) != 0) atomicAdd(&sh.bins.part[2][bin], low & 0x7FFFu);
-      } else {
-        atomicAdd(&sh.bins.part[2][bin], 1u);
+#pragma unroll
+        for (int e = 0; e < kAhead / 2; ++e) weigh(make_float2(v[2 * e], v[2 * e + 1]), hi[e], lo[e]);
       }
-    }
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const uint32_t k = Key(v[e]);
+        uint32_t code = weigh.Distance(v[e]);
+        const bool in = k >= cut && (!by_key || code == at);
+        if (by_key) code = ~k;
+        if (!in || (digit != 0 && digit != 3 && code >> (shift + bits) != prefix)) continue;
+        const uint32_t bin = code >> shift & ((1u << bits) - 1);
+        if (by_mass) {
+          const u64 w = Weights::ToFixed(static_cast<double>(e & 1 ? hi[e / 2].y : hi[e / 2].x) +
+                                         static_cast<double>(e & 1 ? lo[e / 2].y : lo[e / 2].x));
+          const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
+          if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
+          if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
+          if ((low & 0x7FFFu) != 0) atomicAdd(&sh.bins.part[2][bin], low & 0x7FFFu);
+        } else {
+          atomicAdd(&sh.bins.part[2][bin], 1u);
+        }
+      }
+    });
     ClusterSync();
-    if (tid < kBins / kCluster) {
+    {
+      // all blocks' sums of this block's bins, four threads to a bin
+      const int bin = rank * (kBins / kCluster) + tid / 4;
       u64 sum = 0;
-      const int bin = rank * (kBins / kCluster) + tid;
-      for (uint32_t c = 0; c < kCluster; ++c) {
-        sum += (static_cast<u64>(In(sh.bins.part[0], c)[bin]) << 30) + (static_cast<u64>(In(sh.bins.part[1], c)[bin]) << 15) +
-               In(sh.bins.part[2], c)[bin];
+#pragma unroll
+      for (int c = 0; c < kCluster / 4; ++c) {
+        const uint32_t b = tid % 4 * (kCluster / 4) + c;
+        sum += (static_cast<u64>(In(sh.bins.part[0], b)[bin]) << 30) + (static_cast<u64>(In(sh.bins.part[1], b)[bin]) << 15) +
+               In(sh.bins.part[2], b)[bin];
       }
-      sh.bins.all[tid] = sum;
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      static_assert(4 * kBins / kCluster == kThreads, "threads of a bin");
+      if (tid % 4 == 0) sh.bins.all[tid / 4] = sum;
     }
     ClusterSync();
     // the bin in which the sum from the front reaches what is needed: two bins a thread
