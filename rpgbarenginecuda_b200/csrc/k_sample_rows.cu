@@ -12,7 +12,8 @@
 // row in shared memory; what follows is the row's largest value, then
 //  * with top-k or top-p: the largest value of each of the cluster's 4096
 //    threads bounds the K-th largest from below, so the few values from that
-//    bound on are gathered in the first block, sorted, cut and drawn from there;
+//    bound on are gathered in the first block, sorted and cut, and drawn from
+//    there where few are left;
 //  * where that list does not hold what the filters leave (a flat row and a
 //    large top-p, very many equal values, a large k): the least x by selection,
 //    ten bits of its distance from the largest at a time, over counts (top-k) or
@@ -38,6 +39,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024, kBinBits = 10;
 constexpr int kGroups = 512;     // of eight threads
 constexpr int kList = 2048;      // values that the first block sorts
+constexpr int kFew = 128;        // kept values that the first block draws from itself
 constexpr int kMostK = 1280;     // the largest k that the list is tried for
 constexpr int kFirst = 384;      // the K of rows with top-p alone
 constexpr double kFix = 17592186044416.0;  // 2^44
@@ -79,13 +81,14 @@ struct Shared {
     unsigned thread_top[kThreads];
     struct {
       // sums of weights in three parts of 15 bits, which 2^15 terms (a block's share) do not overflow
-      unsigned part[3][kBins];
+      int part[3][kBins];
       u64 all[kBins / kCluster];  // of all blocks, this block's bins
     } bins;
     u64 list[kList];  // key and the complement of the index
   };
   u64 mine[kList / 4];  // what this block found for the list
-  u64 wsum[kWarps], sum, over;
+  u64 weight[kFew];
+  u64 wsum[kWarps], sum, over, listed;
   alignas(16) unsigned group_top[kGroups / kCluster];
   unsigned wide[2 * kWarps], top, n_mine;
   int first;
@@ -149,11 +152,21 @@ struct Weights {
   static __device__ __forceinline__ u64 ToFixed(double w) {
     return static_cast<u64>(__double_as_longlong(fma(w, kFix, 4503599627370496.0)) - 0x4330000000000000ll);
   }
-  // How far x lies under the largest value, in units of 2^-24 of a factor 2 of
-  // weight; what is farther than 2^-63 counts as alike.  Larger values are never farther.
+  // The same as a 2^30 + b 2^15 + c, b and c within 2^14 of 0, by f32 operations.
+  static __device__ __forceinline__ void ToParts(float hi, float lo, int& a, int& b, int& c) {
+    constexpr float kMagic = 12582912.f;
+    constexpr int kBits = 0x4B400000;
+    const float h = hi * 16384.f, t = h + kMagic;
+    a = __float_as_int(t) - kBits;
+    const float r = fmaf(lo, 536870912.f, (h - (t - kMagic)) * 32768.f), u = r + kMagic;
+    b = __float_as_int(u) - kBits;
+    c = __float_as_int(fmaf(r - (u - kMagic), 32768.f, kMagic)) - kBits;
+  }
+  // How far x lies under the largest value, in units of 2^-25 of a factor 2 of
+  // weight; what is farther than 2^-31 counts as alike.  Larger values are never farther.
   __device__ __forceinline__ uint32_t Distance(float x) const {
     const float d = (top - x) * c;
-    return x == top ? 0u : (d < 63.f ? static_cast<uint32_t>(d * 16777216.f) : 0x3FFFFFFFu);
+    return x == top ? 0u : (d < 31.f ? static_cast<uint32_t>(d * 33554432.f) : 0x3FFFFFFFu);
   }
 };
 // A running sum of weights: f32 with what its additions lose.
@@ -215,7 +228,7 @@ __device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 to
 // Among the row's values with keys from `cut` on: the key of the `need`-th
 // largest, or (by_mass) the largest key from which on the weights reach `share`
 // of their sum; `cut` where there is none.  First by the distance from the
-// largest value, in units of 2^-24 of a factor 2 of weight, ten bits at a time:
+// largest value, in units of 2^-25 of a factor 2 of weight, ten bits at a time:
 // a row's values spread over many bins so, and the few in the bin that counts
 // are listed for what follows.  Then, where distances round alike and keys do
 // not, by the keys.
@@ -252,7 +265,10 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
     const int bits = by_key ? 8 : kBinBits, shift = by_key ? 24 - 8 * (digit - 3) : 20 - 10 * digit;
     if (digit == 1) {
       // what is in the bin
-      if (tid == 0) sh.n_mine = 0;
+      if (tid == 0) {
+    sh.n_mine = 0;
+    sh.listed = 0;
+  }
       __syncthreads();
       each([&](const float (&v)[kAhead], const int (&i)[kAhead]) {
 #pragma unroll
@@ -319,14 +335,13 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
         if (!in || (digit != 0 && digit != 3 && code >> (shift + bits) != prefix)) continue;
         const uint32_t bin = code >> shift & ((1u << bits) - 1);
         if (by_mass) {
-          const u64 w = Weights::ToFixed(static_cast<double>(e & 1 ? hi[e / 2].y : hi[e / 2].x) +
-                                         static_cast<double>(e & 1 ? lo[e / 2].y : lo[e / 2].x));
-          const uint32_t high = static_cast<uint32_t>(w >> 30), low = static_cast<uint32_t>(w) & 0x3FFFFFFFu;
-          if (high != 0) atomicAdd(&sh.bins.part[0][bin], high);
-          if (low >> 15 != 0) atomicAdd(&sh.bins.part[1][bin], low >> 15);
-          if ((low & 0x7FFFu) != 0) atomicAdd(&sh.bins.part[2][bin], low & 0x7FFFu);
+          int x, y, z;
+          Weights::ToParts(e & 1 ? hi[e / 2].y : hi[e / 2].x, e & 1 ? lo[e / 2].y : lo[e / 2].x, x, y, z);
+          if (x != 0) atomicAdd(&sh.bins.part[0][bin], x);
+          if (y != 0) atomicAdd(&sh.bins.part[1][bin], y);
+          if (z != 0) atomicAdd(&sh.bins.part[2][bin], z);
         } else {
-          atomicAdd(&sh.bins.part[2][bin], 1u);
+          atomicAdd(&sh.bins.part[2][bin], 1);
         }
       }
     });
@@ -338,8 +353,8 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
 #pragma unroll
       for (int c = 0; c < kCluster / 4; ++c) {
         const uint32_t b = tid % 4 * (kCluster / 4) + c;
-        sum += (static_cast<u64>(In(sh.bins.part[0], b)[bin]) << 30) + (static_cast<u64>(In(sh.bins.part[1], b)[bin]) << 15) +
-               In(sh.bins.part[2], b)[bin];
+        sum += static_cast<u64>(In(sh.bins.part[0], b)[bin] * (1ll << 30) + In(sh.bins.part[1], b)[bin] * (1ll << 15) +
+                                In(sh.bins.part[2], b)[bin]);
       }
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
@@ -391,7 +406,10 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     const float h = static_cast<float>(x);
     sh.power[tid] = make_float2(h, static_cast<float>(x - static_cast<double>(h)));
   }
-  if (tid == 0) sh.n_mine = 0;
+  if (tid == 0) {
+    sh.n_mine = 0;
+    sh.listed = 0;
+  }
   dev::GridLaunchDependents();
   dev::GridWait();
   const int begin = min(static_cast<int>(rank) * per, p.vocab), n = min(per, p.vocab - begin);
@@ -569,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     // ---- what reaches it, and the sum of all weights where the list may not hold all that counts
     const float bound_value = listed ? FromKey(bound) : INFINITY;
     Sum sum;
+    u64 in_list = 0;  // weights of what is listed
     constexpr int kAhead = 4;
     for (int i0 = warp * 32 * kAhead; i0 < n; i0 += kThreads * kAhead) {
       float v[kAhead];
@@ -579,12 +598,12 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
         v[e] = i < n ? kvd::ToFloat(vals[i]) : -INFINITY;
         any |= v[e] >= bound_value;
       }
+      float2 h[kAhead / 2], l[kAhead / 2];
       if (!by_k) {
 #pragma unroll
-        for (int e = 0; e < kAhead; e += 2) {
-          float2 h, l;
-          weigh(make_float2(v[e], v[e + 1]), h, l);
-          sum.Add(h, l);
+        for (int e = 0; e < kAhead / 2; ++e) {
+          weigh(make_float2(v[2 * e], v[2 * e + 1]), h[e], l[e]);
+          sum.Add(h[e], l[e]);
         }
       }
       if (listed && __any_sync(0xFFFFFFFFu, any)) {
@@ -594,6 +613,10 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
           const uint32_t mask = __ballot_sync(0xFFFFFFFFu, in);
           if (mask != 0) {
             unsigned at = 0;
+            if (!by_k && in) {
+              in_list += Weights::ToFixed(static_cast<double>(e & 1 ? h[e / 2].y : h[e / 2].x) +
+                                          static_cast<double>(e & 1 ? l[e / 2].y : l[e / 2].x));
+            }
             if (lane == 0) at = atomicAdd(&sh.n_mine, __popc(mask));
             at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(mask & ((1u << lane) - 1));
             if (in && at < kList / 4) {
@@ -604,7 +627,11 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
       }
     }
     const u64 mass = WarpAdd(Weights::ToFixed(sum.Total()));
-    if (lane == 0) sh.wsum[warp] = mass;
+    in_list = WarpAdd(in_list);
+    if (lane == 0) {
+      sh.wsum[warp] = mass;
+      if (in_list != 0) atomicAdd(&sh.listed, in_list);
+    }
     __syncthreads();
     if (tid == 0) {
       u64 s = 0;
@@ -612,116 +639,114 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
       sh.sum = s;
     }
     ClusterSync();
-    if (rank == 0) {
-      // ---- the first block sorts the list, cuts it and draws
-      unsigned start[kCluster + 1];
-      bool fits = listed;
-      u64 total = 0;
-      start[0] = 0;
-      for (uint32_t b = 0; b < kCluster; ++b) {
-        const unsigned c = *In(&sh.n_mine, b);
-        fits = fits && c <= kList / 4;
-        start[b + 1] = start[b] + c;
-        total += *In(&sh.sum, b);
-      }
-      const int m = static_cast<int>(start[kCluster]);
-      fits = fits && m <= kList;
-      if (tid == 0) sh.found = 0;
-      if (fits) {
+    bool fits = listed;
+    u64 total = 0, there = 0;
+    int m = 0;
+    for (uint32_t b = 0; b < kCluster; ++b) {
+      const unsigned c = *In(&sh.n_mine, b);
+      fits = fits && c <= kList / 4;
+      m += static_cast<int>(c);
+      total += *In(&sh.sum, b);
+      there += *In(&sh.listed, b);
+    }
+    u64 need = by_p ? static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))) : 0;
+    fits = fits && m <= kList && (by_k || there >= need);
+    if (fits) {
+      if (rank == 0) {
+        // ---- the first block sorts the list and cuts it
         int size = 64;
         while (size < m) size <<= 1;
-        for (uint32_t b = 0; b < kCluster; ++b) {
-          for (int i = tid; i < static_cast<int>(start[b + 1] - start[b]); i += kThreads) sh.list[start[b] + i] = In(sh.mine, b)[i];
+        for (uint32_t b = 0, to = 0; b < kCluster; ++b) {
+          const unsigned c = *In(&sh.n_mine, b);
+          for (unsigned i = tid; i < c; i += kThreads) sh.list[to + i] = In(sh.mine, b)[i];
+          to += c;
         }
         for (int i = m + tid; i < size; i += kThreads) sh.list[i] = 0;
         __syncthreads();
         Sort(sh.list, size);
-        const uint32_t least_k = by_k && top_k <= m ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
-        // weights of the values from least_k on, and their running sums: four values a thread
+        uint32_t least = by_k && top_k <= m ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
+        // weights of the values from there on, and their running sums: four values a thread
         u64 w[4], own = 0;
+        int kept_here = 0;
         const int i = 4 * tid;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
-          w[e] = k >= least_k && k != 0 ? weigh.Fixed(FromKey(k)) : 0;
+          w[e] = 0;
+          if (k >= least && k != 0) {
+            w[e] = weigh.Fixed(FromKey(k));
+            ++kept_here;
+          }
           own += w[e];
         }
-        u64 excl = WarpScan(own, lane);
-        if (lane == 31) sh.wsum[warp] = excl;
-        __syncthreads();
-        u64 sum = 0;
-        for (int k = 0; k < kWarps; ++k) {
-          if (k < warp) excl += sh.wsum[k];
-          sum += sh.wsum[k];
-        }
-        excl -= own;
-        if (by_k) total = sum;
-        // the first value with which the sum reaches its share is the last of the kept
-        const u64 need = by_p ? static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))) : ~0ull;
-        if (tid == 0) sh.least = by_p ? 0 : least_k;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (excl < need && need <= excl + w[e]) sh.least = static_cast<uint32_t>(sh.list[i + e] >> 32);
-          excl += w[e];
-        }
-        __syncthreads();
-        // (0 where the list does not reach the share; with top-k it holds all that counts)
-        if (sh.least != 0) {
-          cut = sh.least;
-          // the kept, in the list's order, over the row, which no one reads any more
-          u64* weight = reinterpret_cast<u64*>(raw);
-          own = 0;
-          int last = 0;
+        if (by_p) {
+          u64 before = WarpScan(own, lane);
+          if (lane == 31) sh.wsum[warp] = before;
+          if (tid == 0) sh.least = 1;
+          __syncthreads();
+          u64 sum = 0;
+          for (int k = 0; k < kWarps; ++k) {
+            if (k < warp) before += sh.wsum[k];
+            sum += sh.wsum[k];
+          }
+          before -= own;
+          if (by_k) need = static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(sum)));
+          // the first value with which the sum reaches the share is the last of the kept
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
-            if (k < cut || k < least_min || (by_min && weigh(FromKey(k)) < static_cast<double>(min_p))) w[e] = 0;
-            weight[i + e] = w[e];
-            own += w[e];
-            if (w[e] > 0) last = i + e + 1;
-          }
-          own = WarpAdd(own);
-          last = __reduce_max_sync(0xFFFFFFFFu, last);
-          __syncthreads();
-          if (lane == 0) {
-            sh.wsum[warp] = own;
-            sh.wide[warp] = static_cast<unsigned>(last);
+            if (before < need && need <= before + w[e]) sh.least = static_cast<uint32_t>(sh.list[i + e] >> 32);
+            before += w[e];
           }
           __syncthreads();
-          total = 0;
-          int count = 0;
-          for (int k = 0; k < kWarps; ++k) {
-            total += sh.wsum[k];
-            count = max(count, static_cast<int>(sh.wide[k]));
+          least = max(least, sh.least);
+          kept_here = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kept_here += i + e < m && static_cast<uint32_t>(sh.list[i + e] >> 32) >= least;
+        }
+        kept_here = __reduce_add_sync(0xFFFFFFFFu, kept_here);
+        if (lane == 0) sh.wide[warp] = static_cast<unsigned>(kept_here);
+        __syncthreads();
+        int count = 0;
+        for (int k = 0; k < kWarps; ++k) count += static_cast<int>(sh.wide[k]);
+        if (count <= kFew && warp < kFew / 32) {
+          // ---- few: drawn here.  What comes before a token by its index is added up for each.
+          const uint32_t key = tid < count ? static_cast<uint32_t>(sh.list[tid] >> 32) : 0;
+          const double d = key != 0 ? weigh(FromKey(key)) : 0.0;
+          const u64 mine_w = key < least_min || (by_min && d < static_cast<double>(min_p)) ? 0 : Weights::ToFixed(d);
+          sh.weight[tid] = mine_w;
+          asm volatile("bar.sync 1, %0;" ::"n"(kFew) : "memory");
+          const uint32_t index = ~static_cast<uint32_t>(sh.list[tid]);
+          u64 all = 0, before = 0;
+          for (int j = 0; j < count; ++j) {
+            const u64 x = sh.weight[j];
+            all += x;
+            before += ~static_cast<uint32_t>(sh.list[j]) < index ? x : 0;
           }
-          const u64 target = Target(p, row, total);
-          // what comes before a token by its index
-          for (int k = tid; k < count; k += kThreads) {
-            const uint32_t index = ~static_cast<uint32_t>(sh.list[k]);
-            u64 before = 0;
-            for (int j = 0; j < count; ++j) before += ~static_cast<uint32_t>(sh.list[j]) < index ? weight[j] : 0;
-            if (before <= target && target - before < weight[k]) {
-              p.tok[row] = static_cast<int>(index);
-              if (p.prob != nullptr) {
-                p.prob[row] = static_cast<float>(weigh(FromKey(sh.list[k] >> 32)) * kFix / static_cast<double>(total));
-              }
-            }
+          const u64 target = Target(p, row, all);
+          if (tid < count && before <= target && target - before < mine_w) {
+            p.tok[row] = static_cast<int>(index);
+            if (p.prob != nullptr) p.prob[row] = static_cast<float>(d * kFix / static_cast<double>(all));
           }
-          if (tid == 0) sh.found = 1;
+        }
+        if (tid == 0) {
+          sh.found = count <= kFew;
+          sh.least = least;
         }
       }
-    }
-    ClusterSync();
-    const bool found = *In(&sh.found, 0) != 0;
-    ClusterSync();  // (it has been read: the first block may end, or go on to use its memory)
-    if (found) return;
-
-    // ---- the least key that the filters leave
-    for (int pass = 0; pass < 2; ++pass) {
-      if (pass == 0 ? by_k : by_p) {
-        cut = Select(sh, weigh, pass == 1, top_p, static_cast<u64>(top_k), cut, n, [&](int i) { return kvd::ToFloat(vals[i]); },
-                     rank);
+      ClusterSync();
+      const bool found = *In(&sh.found, 0) != 0;
+      cut = *In(&sh.least, 0);
+      if (found) {
+        ClusterSync();  // (it has been read: the first block may end)
+        return;
+      }
+    } else {
+      // ---- the least key that the filters leave
+      for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 0 ? by_k : by_p) {
+          cut = Select(sh, weigh, pass == 1, top_p, static_cast<u64>(top_k), cut, n, [&](int i) { return kvd::ToFloat(vals[i]); },
+                       rank);
+        }
       }
     }
   }
@@ -819,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
 template <typename T>
 void Launch(const SampleRowsParams& p, cudaStream_t s) {
   const int per = ((p.vocab + kCluster - 1) / kCluster + 15) / 16 * 16;
-  const size_t row = static_cast<size_t>(per) * sizeof(T), smem = row > 8 * kList ? row : 8 * kList;
+  const size_t smem = static_cast<size_t>(per) * sizeof(T);
   const void* fn = reinterpret_cast<const void*>(SampleRowsKernel<T>);
   RPGB_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
   LaunchKernelClusterArgs(fn, dim3(static_cast<unsigned>(p.n_rows) * kCluster), dim3(kThreads), smem, s, true, kCluster, p,
