@@ -2,13 +2,17 @@
 
 A Qwen3 GGUF's layers run on the operator entries: the quantised matrices
 (`Matrix.matvec`), and per layer `PagedKv.append` (per-head norms, rotation and
-the write of k and v in one pass) and `PagedKv.attend` (one new token of every
-conversation).  The conversations share one pool of pages per layer; a page is
-taken when a conversation grows into it.  A prompt goes through the same two
-calls, one row per token, with every row's own length.
+the write of k and v in one pass) and the attention: `PagedKv.attend_rows` where
+a conversation has several new tokens (prompts, appended turns), `PagedKv.attend`
+for one new token of every conversation, `PagedKv.attend_shared` where some of
+them begin alike.  `sample_rows` draws the next token of all.  The conversations
+share one pool of pages per layer; a page is taken when a conversation grows into
+it.  A conversation can branch off another: it shares the whole pages of what
+they have in common.
 
     python examples/paged_batch.py                       # a toy model, written on the spot
     python examples/paged_batch.py --gguf model.gguf --cache q8 --conversations 32
+    python examples/paged_batch.py --instructions 200 --temperature 0.7 --top-p 0.9   # one beginning for all
 """
 
 from __future__ import annotations
@@ -119,10 +123,15 @@ class PagedModel:
             self.layers.append(w)
         self.rope = rope
         self.free = list(range(n_pages))[::-1]
+        self.used = np.zeros(n_pages, np.int32)  # conversations that hold a page
         self.table = np.full((max_conversations, self.max_pages), -1, np.int32)
         self.lengths: dict[int, int] = {}
-        self.workspace = torch.zeros(rpg.attend_workspace(self.n_heads, self.n_kv, self.dim), dtype=torch.uint8,
-                                     device="cuda")
+        self.alike: dict[int, tuple[int, int]] = {}  # (group, positions) of conversations that begin alike
+        self.groups = 0
+        shape = self.n_heads, self.n_kv, self.dim
+        # zeroed once; the one for shared beginnings holds the one for single tokens, prompts have one of their own
+        self.workspace = torch.zeros(rpg.attend_shared_workspace(*shape, max_conversations), dtype=torch.uint8, device="cuda")
+        self.rows_workspace = torch.empty(rpg.attend_rows_workspace(*shape), dtype=torch.uint8, device="cuda")
         torch.cuda.synchronize()  # forward may come on another stream
 
     def open(self) -> int:
@@ -133,18 +142,50 @@ class PagedModel:
         self.lengths[c] = 0
         return c
 
+    def branch(self, c: int, n: int | None = None) -> int:
+        """A new conversation that begins with the first n positions of c (None: all of them).
+
+        Whole pages are shared; of the page that n ends in, the new conversation gets a copy."""
+        n = self.lengths[c] if n is None else n
+        if not 0 <= n <= self.lengths[c]:
+            raise ValueError(f"conversation {c} has {self.lengths[c]} positions, not {n}")
+        whole, rest = divmod(n, self.page)
+        if rest and not self.free:
+            raise RuntimeError(f"no page for position {whole * self.page} of a branch of conversation {c}")
+        d = self.open()
+        self.table[d, :whole] = self.table[c, :whole]
+        if rest:
+            self.table[d, whole] = self.free.pop()
+            for w in self.layers:
+                for t in w["pool"]:
+                    t[int(self.table[d, whole])].copy_(t[int(self.table[c, whole])])
+        for p in self.table[d, :whole + (rest > 0)]:
+            self.used[p] += 1
+        self.lengths[d] = n
+        group, common = self.alike.get(c, (0, -1))
+        if n > common:  # c leaves a group that shares less than this
+            self.groups += 1
+            group, common = self.groups, n
+            self.alike[c] = (group, n)
+        self.alike[d] = (group, n)
+        return d
+
     def close(self, c: int):
-        """Ends a conversation; its pages go back to the pool."""
-        self.free += [int(p) for p in self.table[c] if p >= 0]
+        """Ends a conversation; pages that no other one holds go back to the pool."""
+        for p in self.table[c][self.table[c] >= 0]:
+            self.used[p] -= 1
+            if self.used[p] == 0:
+                self.free.append(int(p))
         self.table[c] = -1
         del self.lengths[c]
+        self.alike.pop(c, None)
 
     def forward(self, tokens: list[tuple[int, int]]) -> torch.Tensor:
         """Appends (conversation, token id) rows, in order, and returns their logits [row][vocabulary].
 
         Runs on torch's current stream.  A call that raises leaves the conversations as they were."""
         stream = torch.cuda.current_stream().cuda_stream
-        seq, pos, lengths, places = [], [], dict(self.lengths), self.table.copy()
+        lengths, places, at = dict(self.lengths), self.table.copy(), []
         taken = 0
         for c, _ in tokens:
             p = lengths[c]
@@ -155,18 +196,42 @@ class PagedModel:
             if p % self.page == 0:
                 taken += 1
                 places[c, p // self.page] = self.free[-taken]
-            seq.append(c)
-            pos.append(p)
+            at.append(p)
             lengths[c] = p + 1
         n = len(tokens)
-        # every row has its own page list and length: a prompt's rows see what comes before them
-        table = torch.from_numpy(places[seq]).cuda()
-        pages = rpg.PageTable(table.data_ptr(), n, self.max_pages)
-        pos = torch.tensor(pos, dtype=torch.int32, device="cuda")
-        lens = pos + 1
+        # rows by conversation, conversations that begin alike side by side
+        key = [(self.alike.get(c, (0, 0))[0], c) for c, _ in tokens]
+        order = sorted(range(n), key=lambda r: key[r])
+        convs = [c for r, c in enumerate(key[i][1] for i in order) if r == 0 or c != key[order[r - 1]][1]]
+        seq = torch.tensor([convs.index(key[i][1]) for i in order], dtype=torch.int32, device="cuda")
+        pos = torch.tensor([at[i] for i in order], dtype=torch.int32, device="cuda")
+        ends = pos + 1
+        table = torch.from_numpy(places[convs]).cuda()
+        pages = rpg.PageTable(table.data_ptr(), len(convs), self.max_pages)
+
+        def ints(x):
+            return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+        bounds = groups = None
+        if n > len(convs):  # several new tokens of a conversation
+            counts = [sum(key[i][1] == c for i in order) for c in convs]
+            bounds = ints(np.concatenate([[0], np.cumsum(counts)]))
+        else:
+            first, prefix = [], []
+            for i, c in enumerate(convs):
+                group, common = self.alike.get(c, (0, 0))
+                if i and group and group == self.alike.get(convs[i - 1], (0, 0))[0]:
+                    prefix[-1] = min(prefix[-1], common)
+                else:
+                    first.append(i)
+                    prefix.append(common)
+            first.append(n)
+            if len(first) <= n:  # some begin alike
+                groups = ints(first)
+                common = ints(np.repeat(prefix, np.diff(first)))
         x = torch.empty(n, self.embd.cols, device="cuda")
-        for i, (_, token) in enumerate(tokens):
-            self.embd.dequant(token, 1, x[i].data_ptr(), stream)
+        for i, r in enumerate(order):
+            self.embd.dequant(tokens[r][1], 1, x[i].data_ptr(), stream)
 
         def product(m, y):
             out = torch.empty(n, m.rows, device="cuda")
@@ -182,17 +247,44 @@ class PagedModel:
             y = norm(x, w["attn_norm"])
             qkv = torch.cat([product(w[m], y) for m in ("attn_q", "attn_k", "attn_v")], 1)
             w["kv"].append(pages, w["rotary"], rpg.F32, qkv.data_ptr(), self.n_heads, pos.data_ptr(), n, q.data_ptr(),
-                           stream=stream)
-            w["kv"].attend(pages, rpg.F32, q.data_ptr(), self.n_heads, lens.data_ptr(), self.dim ** -0.5, att.data_ptr(),
-                           self.workspace.data_ptr(), self.workspace.numel(), stream=stream)
+                           seq_ptr=seq.data_ptr(), stream=stream)
+            if bounds is not None:
+                w["kv"].attend_rows(pages, rpg.F32, q.data_ptr(), self.n_heads, bounds.data_ptr(), n, ends.data_ptr(),
+                                    self.dim ** -0.5, att.data_ptr(), self.rows_workspace.data_ptr(),
+                                    self.rows_workspace.numel(), stream=stream)
+            elif groups is not None:
+                w["kv"].attend_shared(pages, rpg.F32, q.data_ptr(), self.n_heads, ends.data_ptr(), groups.data_ptr(),
+                                      len(first) - 1, common.data_ptr(), self.dim ** -0.5, att.data_ptr(),
+                                      self.workspace.data_ptr(), self.workspace.numel(), stream=stream)
+            else:
+                w["kv"].attend(pages, rpg.F32, q.data_ptr(), self.n_heads, ends.data_ptr(), self.dim ** -0.5,
+                               att.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(), stream=stream)
             x = x + product(w["attn_output"], att)
             y = norm(x, w["ffn_norm"])
             h = torch.nn.functional.silu(product(w["ffn_gate"], y)) * product(w["ffn_up"], y)
             x = x + product(w["ffn_down"], h)
         logits = product(self.head, norm(x, self.out_norm))
-        del self.free[len(self.free) - taken:]
+        if taken:
+            self.used[self.free[-taken:]] = 1
+            del self.free[-taken:]
         self.table, self.lengths = places, lengths
-        return logits
+        back = np.empty(n, np.int64)
+        back[order] = np.arange(n)
+        return logits[torch.from_numpy(back).cuda()]
+
+    def sample(self, logits: torch.Tensor, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0, generator: torch.Generator | None = None) -> list[int]:
+        """The next token of every row of logits; a temperature of 0 takes the largest."""
+        n = logits.shape[0]
+        options = torch.tensor([temperature, top_p, min_p], device="cuda")[:, None].expand(3, n).contiguous()
+        k = torch.full((n,), top_k, dtype=torch.int32, device="cuda")
+        u = torch.rand(n, generator=generator, device="cuda")
+        out = torch.empty(n, dtype=torch.int32, device="cuda")
+        rpg.sample_rows(logits.data_ptr(), rpg.F32, n, logits.shape[1], out.data_ptr(), u.data_ptr(),
+                        temperature_ptr=options[0].data_ptr(), top_k_ptr=k.data_ptr(), top_p_ptr=options[1].data_ptr(),
+                        min_p_ptr=options[2].data_ptr(), stride=logits.stride(0),
+                        stream=torch.cuda.current_stream().cuda_stream)
+        return out.tolist()
 
 
 def main(argv=None):
@@ -201,6 +293,11 @@ def main(argv=None):
     ap.add_argument("--cache", choices=sorted(CACHES), default="f16")
     ap.add_argument("--conversations", type=int, default=4)
     ap.add_argument("--steps", type=int, default=16)
+    ap.add_argument("--instructions", type=int, default=0, help="tokens that all conversations begin with")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest token")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
     if a.gguf is None:
         from dataclasses import replace
@@ -208,19 +305,31 @@ def main(argv=None):
         from rpgbarenginecuda_b200 import synthetic
 
         a.gguf = synthetic.cached_model(replace(synthetic.PRESETS["tiny"], weight_std=0.06), seed=1)
-    m = PagedModel(a.gguf, a.cache, n_pages=16 * a.conversations, max_conversations=a.conversations)
+    m = PagedModel(a.gguf, a.cache, n_pages=16 * a.conversations + a.instructions // 16 + 1,
+                   max_conversations=a.conversations + 1)
     rng = np.random.default_rng(0)
-    ids = [m.open() for _ in range(a.conversations)]
+    dice = torch.Generator(device="cuda").manual_seed(0)
+
+    def draw(logits):
+        return m.sample(logits, a.temperature, a.top_k, a.top_p, a.min_p, dice)
+
+    if a.instructions:
+        root = m.open()
+        m.forward([(root, int(t)) for t in rng.integers(0, m.embd.rows, a.instructions)])
+        ids = [m.branch(root) for _ in range(a.conversations)]
+        m.close(root)
+    else:
+        ids = [m.open() for _ in range(a.conversations)]
     last = {}
     for c in ids:  # prompts of different lengths
         prompt = rng.integers(0, m.embd.rows, 5 + 7 * (c % 5))
-        last[c] = int(m.forward([(c, int(t)) for t in prompt])[-1].argmax())
+        last[c] = draw(m.forward([(c, int(t)) for t in prompt])[-1:])[0]
     out = {c: [last[c]] for c in ids}
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     for _ in range(a.steps):
         logits = m.forward([(c, last[c]) for c in ids])
-        for c, t in zip(ids, logits.argmax(-1).tolist()):
+        for c, t in zip(ids, draw(logits)):
             last[c] = t
             out[c].append(t)
     torch.cuda.synchronize()
