@@ -330,9 +330,10 @@ typedef struct rpgb_kv_scores {
  * row's end of its neighbours gives NaN.  An empty range gives zeros, one past
  * the table NaN.  Rows whose k and v are to be seen are appended before.
  *
- * Sums are in f32.  q is held to 2^-22 of its head's largest value where it is
- * f32 and to 2^-11 of each value where it has 16 bits, and so are the softmax
- * weights.  NaN and infinities count as in rpgb_kv_attend.
+ * Sums are in f32.  f32 q is held to 2^-22 of its head's largest value, bf16 q to
+ * 2^-37 of it, f16 q as it is; the softmax weights to 2^-22 of themselves where q
+ * is f32 and to 2^-11 where it has 16 bits, never finer than 2^-31 and 2^-20 of
+ * the largest.  NaN and infinities count as in rpgb_kv_attend.
  * workspace_dev: rpgb_kv_attend_rows_workspace bytes (or more), 256-byte
  * aligned; it need not be zeroed, and calls that may overlap need one each. */
 RPGB_API int64_t rpgb_kv_attend_rows_workspace(int32_t n_heads, int32_t n_kv, int32_t head_dim);
@@ -346,7 +347,7 @@ RPGB_API int32_t rpgb_kv_attend_rows(const rpgb_kv_pages* kv, const rpgb_kv_tabl
  * the same world): what they share is read and multiplied once for all.
  * Conversations groups_dev[g] .. groups_dev[g + 1] - 1 (int32 [n_groups + 1], not
  * decreasing, within [0, n_seq]) hold the same k and v at positions [0,
- * prefix_dev[s]) (int32 [n_seq], one value per group), which are read through
+ * prefix_dev[s]) (int32 [n_seq], the same within a group), which are read through
  * the page list of the group's first conversation; the positions behind through
  * each conversation's own list.  The page lists may hold the same pages there
  * or copies, and prefix need not end a page.  A conversation whose prefix is
@@ -387,8 +388,8 @@ typedef struct rpgb_sample_rows_options {
 /* Draws one token per row of logits_dev (n_rows rows of vocab values of
  * `type`, `stride` elements apart, aligned as their type is) into
  * tok_out_dev[r]; prob_out_dev[r] (NULL: not wanted) receives the probability
- * it was drawn with.  Weights and their sums hold 2^-32 or better where they
- * decide a draw.  NaN and minus infinity are never drawn; rows that hold
+ * it was drawn with.  Weights are held to 2^-34, their sums to 2^-44 of the
+ * largest weight.  NaN and minus infinity are never drawn; rows that hold
  * nothing else give -1 and NaN; where there are plus infinities, they alone
  * are drawn, each alike.  Rows are independent of one another: a row's token
  * does not depend on the batch.  Allocates nothing, needs no workspace, returns

@@ -403,7 +403,7 @@ int32_t rpgb_sample_rows(int32_t type, const void* logits_dev, int64_t stride, i
     SampleRowsParams p;
     RPGB_CHECK(type == RPGB_F32 || type == RPGB_F16 || type == RPGB_BF16, "sample_rows: unknown element type %d", type);
     p.type = static_cast<ElemType>(type);
-    RPGB_CHECK(n_rows >= 0, "sample_rows: bad row count %d", n_rows);
+    RPGB_CHECK(n_rows >= 0 && n_rows <= kKvMaxRows, "sample_rows: bad row count %d", n_rows);
     RPGB_CHECK(vocab > 0 && vocab <= RPGB_SAMPLE_ROWS_MAX_VOCAB, "sample_rows: vocabulary of %d; 1 to %d are taken", vocab,
                RPGB_SAMPLE_ROWS_MAX_VOCAB);
     RPGB_CHECK(stride >= vocab, "sample_rows: stride %lld under the vocabulary's %d", static_cast<long long>(stride),

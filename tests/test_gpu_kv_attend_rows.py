@@ -227,6 +227,63 @@ def test_bad_pages_positions_past_the_table_and_bounds_that_decrease_give_nan():
     close(out[:-1], want[:-1], pool, "f16")
 
 
+def test_bounds_that_decrease_give_nan_and_lists_without_rows_nothing():
+    counts, ats = [50, 30], [10, 0]
+    pool, q, _, _, ends = problem("f16", 4, 2, 128, "f16", 16, counts, ats)
+    want = formula(pool, q, counts, ends)
+    odd = list(ends)
+    odd[49] = 30  # the last of the first conversation sees less than the others before it
+    out = attend_rows(pool, q, counts, odd, act="f16")
+    bad = torch.tensor([e > 30 for e in odd[:50]] + [False] * 30, device="cuda")
+    assert bool(out[bad].isnan().all())
+    good = ~bad
+    good[49] = False  # (it sees something else now)
+    close(out[good], want[good], pool, "f16")
+    out = attend_rows(pool, q, [0, 0], ends, act="f16")
+    assert bool((out == 7.0).all())
+
+
+def test_on_another_stream_behind_what_fills_its_inputs():
+    counts, ats = [90, 40], [10, 0]
+    pool, q, _, _, ends = problem("q8", 4, 2, 128, "f16", 16, counts, ats)
+    want = formula(pool, q, counts, ends)
+    side = torch.cuda.Stream()
+    late = torch.zeros_like(q)
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(rpg.attend_rows_workspace(4, 2, 128), dtype=torch.uint8, device="cuda")
+    rows, e = i32(row_bounds(counts)), i32(ends)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(4):
+            big = big @ big * 1e-3
+        late.copy_(q)
+        pool.kv.attend_rows(pool.pt, rpg.F16, late.data_ptr(), 4, rows.data_ptr(), q.shape[0], e.data_ptr(), 128 ** -0.5,
+                            out.data_ptr(), ws.data_ptr(), ws.numel(), stream=side.cuda_stream)
+        late.zero_()
+    torch.cuda.synchronize()
+    close(out, want, pool, "f16")
+
+
+def test_two_calls_at_once():
+    # each with a workspace of its own, on streams of their own
+    problems = [problem(kind, 8, 2, 128, act, 16, [300, 70], [400, 5], seed=i)
+                for i, (kind, act) in enumerate((("f16", "f16"), ("q8", "f32"), ("f16", "f32")))]
+    alone = [attend_rows(pool, q, [300, 70], ends, act="f32" if q.dtype == torch.float32 else "f16")
+             for pool, q, _, _, ends in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    outs = [torch.empty_like(q) for _, q, *_ in problems]
+    ws = [torch.empty(rpg.attend_rows_workspace(8, 2, 128), dtype=torch.uint8, device="cuda") for _ in problems]
+    args = [(i32([0, 300, 370]), i32(ends)) for *_, ends in problems]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (pool, q, *_), s, o, w, (r, e) in zip(problems, streams, outs, ws, args):
+            pool.kv.attend_rows(pool.pt, rpg.F32 if q.dtype == torch.float32 else rpg.F16, q.data_ptr(), 8, r.data_ptr(),
+                                370, e.data_ptr(), 128 ** -0.5, o.data_ptr(), w.data_ptr(), w.numel(), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, o) for a, o in zip(alone, outs))
+
+
 def nonfinite(pool, name, s, h, pos, dim, value):
     page, at = int(pool.table[s, pos // pool.page]), pos % pool.page
     pool.mem[name][page, h, at, dim] = value
@@ -459,6 +516,38 @@ def test_shared_bad_pages_lengths_and_prefixes_give_nan():
     out = attend_shared(pool, q, groups, prefix, lens, act="f16")
     assert bool(out[1].isnan().all())
     close(out[2:], want[2:], pool, "f16")
+
+
+def test_shared_prefixes_that_differ():
+    # shorter than the group's first: the rest is the conversation's own; longer: NaN
+    pool, q, groups, lens = shared_problem("f16", 4, 2, 128, "f16", 16, [4], [100], [40])
+    want = formula(pool, q, [1] * 4, lens)
+    lens_dev, g, per = i32(lens), i32([0, 4]), i32([100, 60, 0, 101])
+    ws = torch.zeros(rpg.attend_shared_workspace(4, 2, 128, 4), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    pool.kv.attend_shared(pool.pt, rpg.F16, q.data_ptr(), 4, lens_dev.data_ptr(), g.data_ptr(), 1, per.data_ptr(), 128 ** -0.5,
+                          out.data_ptr(), ws.data_ptr(), ws.numel())
+    torch.cuda.synchronize()
+    close(out[:3], want[:3], pool, "f16")
+    assert bool(out[3].isnan().all())
+
+
+def test_shared_in_a_graph_with_lengths_that_grow():
+    pool, q, groups, lens = shared_problem("q8", 8, 2, 128, "f32", 16, [20, 11], [150, 70], [30])
+    short = [n - 10 for n in lens]
+    n, g, per = i32(short), i32([0, 20, 31]), i32([150] * 20 + [70] * 11)
+    ws = torch.zeros(rpg.attend_shared_workspace(8, 2, 128, 31), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        pool.kv.attend_shared(pool.pt, rpg.F32, q.data_ptr(), 8, n.data_ptr(), g.data_ptr(), 2, per.data_ptr(), 128 ** -0.5,
+                              out.data_ptr(), ws.data_ptr(), ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+    for k in (0, 3, 10):
+        n.copy_(i32([x + k for x in short]))
+        graph.replay()
+        torch.cuda.synchronize()
+        close(out, formula(pool, q, [1] * 31, [x + k for x in short]), pool, "f32")
 
 
 def test_shared_infinities():

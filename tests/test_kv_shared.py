@@ -85,7 +85,7 @@ def test_workspace_sizes():
 
 
 @pytest.mark.parametrize("bad,why", [
-    (dict(dtype=5), "type"), (dict(n_rows=-1), "row count"), (dict(vocab=0), "vocabulary"), (dict(vocab=262145), "vocabulary"),
+    (dict(dtype=5), "type"), (dict(n_rows=-1), "row count"), (dict(n_rows=(1 << 24) + 1), "row count"), (dict(vocab=0), "vocabulary"), (dict(vocab=262145), "vocabulary"),
     (dict(stride=99), "stride"), (dict(u_ptr=0), "random"), (dict(u_ptr=FAKE + 2), "aligned"),
     (dict(top_k_ptr=FAKE + 1), "aligned"), (dict(logits_ptr=0), "NULL"), (dict(logits_ptr=FAKE + 2), "aligned"),
     (dict(tok_ptr=0), "NULL"), (dict(prob_ptr=FAKE + 2), "aligned"),
