@@ -202,8 +202,11 @@ __device__ __forceinline__ void Sort(u64* x, int n) {
   const bool small = n <= 128;
   const int threads = small ? 32 : kThreads;
   if (threadIdx.x < threads) {
+#pragma unroll 1
     for (int k = 2; k <= n; k <<= 1) {
+#pragma unroll 1
       for (int j = k >> 1; j > 0; j >>= 1) {
+#pragma unroll 1
         for (int i = threadIdx.x; i < n / 2; i += threads) {
           const int a = 2 * i - (i & (j - 1)), b = a + j;
           const u64 u = x[a], v = x[b];
@@ -219,6 +222,23 @@ __device__ __forceinline__ void Sort(u64* x, int n) {
   __syncthreads();
 }
 
+// What all blocks have found (m in all) into the first block's list, filled up
+// to a power of two, which it returns.
+__device__ __forceinline__ int Gather(Shared& sh, int m) {
+  int size = 64;
+  while (size < m) size <<= 1;
+  int to = 0;
+#pragma unroll 1
+  for (uint32_t b = 0; b < kCluster; ++b) {
+    const int c = static_cast<int>(*In(&sh.n_mine, b));
+    for (int i = threadIdx.x; i < c; i += kThreads) sh.list[to + i] = In(sh.mine, b)[i];
+    to += c;
+  }
+  for (int i = m + threadIdx.x; i < size; i += kThreads) sh.list[i] = 0;
+  __syncthreads();
+  return size;
+}
+
 // `u` of a sum of weights: the target is exceeded by exactly one token's running sum.
 __device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 total) {
   const double u = fmin(fmax(p.u != nullptr ? static_cast<double>(p.u[row]) : 0.0, 0.0), 1.0);
@@ -230,7 +250,7 @@ __device__ __forceinline__ u64 Target(const SampleRowsParams& p, int row, u64 to
 // of their sum; `cut` where there is none.  First by the distance from the
 // largest value, in units of 2^-25 of a factor 2 of weight, ten bits at a time:
 // a row's values spread over many bins so, and the few in the bin that counts
-// are listed for what follows.  Then, where distances round alike and keys do
+// are sorted in the first block, or listed for what follows.  Then, where distances round alike and keys do
 // not, by the keys.
 template <typename F>
 __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, bool by_mass, float share, u64 need, uint32_t cut,
@@ -252,7 +272,7 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
         i[e] = i0 + e * kThreads;
         v[e] = -INFINITY;
         if (i[e] < count) {
-          if (listed >= 0) i[e] = static_cast<int>(sh.mine[i[e]]);
+          if (listed >= 0) i[e] = static_cast<int>(~static_cast<uint32_t>(sh.mine[i[e]]));
           v[e] = value(i[e]);
         }
       }
@@ -275,11 +295,49 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
         for (int e = 0; e < kAhead; ++e) {
           if (Key(v[e]) >= cut && weigh.Distance(v[e]) >> 20 == prefix) {
             const unsigned to = atomicAdd(&sh.n_mine, 1u);
-            if (to < kList / 4) sh.mine[to] = static_cast<u64>(i[e]);
+            if (to < kList / 4) sh.mine[to] = static_cast<u64>(Key(v[e])) << 32 | ~static_cast<uint32_t>(i[e]);
           }
         }
       });
-      __syncthreads();
+      ClusterSync();
+      int m = 0;
+      bool fits = true;
+      for (uint32_t c = 0; c < kCluster; ++c) {
+        const unsigned x = *In(&sh.n_mine, c);
+        fits = fits && x <= kList / 4;
+        m += static_cast<int>(x);
+      }
+      if (fits && m <= kList) {
+        // few enough for the first block to sort
+        if (rank == 0) {
+          const int size = Gather(sh, m);
+          Sort(sh.list, size);
+          u64 w[4], own = 0;
+          const int i = 4 * tid;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t k = i + e < m ? static_cast<uint32_t>(sh.list[i + e] >> 32) : 0;
+            w[e] = k == 0 ? 0 : (by_mass ? weigh.Fixed(FromKey(k)) : 1);
+            own += w[e];
+          }
+          u64 before = WarpScan(own, lane);
+          if (lane == 31) sh.wsum[warp] = before;
+          // (sums of weights that round otherwise than the bins': the last of them then)
+          if (tid == 0) sh.least = static_cast<uint32_t>(sh.list[m - 1] >> 32);
+          __syncthreads();
+          before += over - own;
+          for (int k = 0; k < warp; ++k) before += sh.wsum[k];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (before < need && need <= before + w[e]) sh.least = static_cast<uint32_t>(sh.list[i + e] >> 32);
+            before += w[e];
+          }
+        }
+        ClusterSync();
+        const uint32_t least = *In(&sh.least, 0);
+        ClusterSync();  // (it has been read)
+        return least;
+      }
       if (sh.n_mine <= kList / 4) listed = static_cast<int>(sh.n_mine);
     }
     if (digit == 3) {
@@ -317,6 +375,7 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
       ClusterSync();
       if (a == b) return a;
     }
+#pragma unroll 1
     for (int i = tid; i < kBins; i += kThreads) sh.bins.part[0][i] = sh.bins.part[1][i] = sh.bins.part[2][i] = 0;
     if (tid == 0) sh.found = -1;
     __syncthreads();
@@ -393,8 +452,11 @@ __device__ __forceinline__ uint32_t Select(Shared& sh, const Weights& weigh, boo
   return ~prefix;
 }
 
+// Three blocks on an SM for 16-bit rows (40 registers a thread): 256 rows 121 us,
+// two blocks of 64 registers 132.  Of f32 rows of 151936 two fit: 64 rows 94 us
+// with 64 registers, 99 with 40.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRowsParams p, int per) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) SampleRowsKernel(const SampleRowsParams p, int per) {
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ Shared sh;
   T* vals = reinterpret_cast<T*>(raw);
@@ -427,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
     const int vecs = n / kVec;
     constexpr int kFlight = 4;
+#pragma unroll 1
     for (int i0 = tid; i0 < vecs; i0 += kThreads * kFlight) {
       uint4 w[kFlight];
 #pragma unroll
@@ -443,12 +506,14 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
         }
       }
     }
+#pragma unroll 1
     for (int i = vecs * kVec + tid; i < n; i += kThreads) {
       vals[i] = src[i];
       best = fmaxf(best, kvd::ToFloat(vals[i]));
     }
   } else {
     constexpr int kFlight = 8;
+#pragma unroll 1
     for (int i0 = tid; i0 < n; i0 += kThreads * kFlight) {
       T w[kFlight];
 #pragma unroll
@@ -489,6 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     // ---- nothing to draw, or the largest value's lowest index
     int at = INT_MAX;
     if (top != 0 && sh.top == top) {
+#pragma unroll 1
       for (int i = tid; i < n; i += kThreads) {
         if (Key(kvd::ToFloat(vals[i])) == top) {
           at = begin + i;
@@ -555,7 +621,9 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
           key[i + 2] = w.z;
           key[i + 3] = w.w;
         }
-        for (int bit = 31; bit >= 10; --bit) {
+#pragma unroll 1
+  #pragma unroll 1
+      for (int bit = 31; bit >= 10; --bit) {
           const uint32_t try_ = bound | 1u << bit;
           int c = 0;
 #pragma unroll
@@ -570,6 +638,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
       unsigned key[kCluster];
 #pragma unroll
       for (uint32_t b = 0; b < kCluster; ++b) key[b] = In(sh.thread_top, b)[tid];
+#pragma unroll 1
       for (int bit = 31; bit >= 10; --bit) {
         const uint32_t try_ = bound | 1u << bit;
         int c = 0;
@@ -589,6 +658,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     Sum sum;
     u64 in_list = 0;  // weights of what is listed
     constexpr int kAhead = 4;
+#pragma unroll 1
     for (int i0 = warp * 32 * kAhead; i0 < n; i0 += kThreads * kAhead) {
       float v[kAhead];
       bool any = false;
@@ -654,16 +724,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     if (fits) {
       if (rank == 0) {
         // ---- the first block sorts the list and cuts it
-        int size = 64;
-        while (size < m) size <<= 1;
-        for (uint32_t b = 0, to = 0; b < kCluster; ++b) {
-          const unsigned c = *In(&sh.n_mine, b);
-          for (unsigned i = tid; i < c; i += kThreads) sh.list[to + i] = In(sh.mine, b)[i];
-          to += c;
-        }
-        for (int i = m + tid; i < size; i += kThreads) sh.list[i] = 0;
-        __syncthreads();
-        Sort(sh.list, size);
+        Sort(sh.list, Gather(sh, m));
         uint32_t least = by_k && top_k <= m ? static_cast<uint32_t>(sh.list[top_k - 1] >> 32) : 1;
         // weights of the values from there on, and their running sums: four values a thread
         u64 w[4], own = 0;
@@ -717,6 +778,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
           asm volatile("bar.sync 1, %0;" ::"n"(kFew) : "memory");
           const uint32_t index = ~static_cast<uint32_t>(sh.list[tid]);
           u64 all = 0, before = 0;
+#pragma unroll 1
           for (int j = 0; j < count; ++j) {
             const u64 x = sh.weight[j];
             all += x;
@@ -742,6 +804,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
       }
     } else {
       // ---- the least key that the filters leave
+#pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         if (pass == 0 ? by_k : by_p) {
           cut = Select(sh, weigh, pass == 1, top_p, static_cast<u64>(top_k), cut, n, [&](int i) { return kvd::ToFloat(vals[i]); },
@@ -756,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
   const float floor_ = fmaxf(cut > 1 ? FromKey(cut) : -INFINITY, least_min > 1 ? FromKey(least_min) : -INFINITY);
   Sum sum;
   constexpr int kAhead = 4;
+#pragma unroll 1
   for (int i0 = lo; i0 < hi; i0 += 32 * kAhead) {
     float v[kAhead];
     bool any = false;
@@ -798,6 +862,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     // the last that is kept.)
     Sum run_sum;
     const int a = min(lo + lane * run, hi), b = min(a + run, hi);
+#pragma unroll 1
     for (int i0 = 0; i0 < run; i0 += kAhead) {
       float v[kAhead];
 #pragma unroll
@@ -817,6 +882,7 @@ __global__ void __launch_bounds__(kThreads, 2) SampleRowsKernel(const SampleRows
     u64 so_far = __shfl_sync(0xFFFFFFFFu, incl - own, who);
     int last = -1;  // the lane's last kept value
     bool found = false;
+#pragma unroll 1
     for (int i0 = a1; i0 < b1 && !found; i0 += 32) {
       const int i = i0 + lane;
       float2 h, l;
