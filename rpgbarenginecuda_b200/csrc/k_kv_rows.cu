@@ -164,12 +164,7 @@ __device__ __forceinline__ void PlainRow(const KvRowsParams& p, int table_row, i
 
 constexpr int kTileRows = 128;            // rows of a tile: the lanes of tensor memory
 constexpr int kItemRows = 2 * kTileRows;  // two tiles share the positions that pass through
-constexpr int kSoftWarps = 8, kLoadWarps = 2;
-constexpr int kMmaWarp = kSoftWarps, kDealWarp = kMmaWarp + 1, kLoadWarp0 = kDealWarp + 1;
-constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
-// Registers: 168 a thread at launch; the rows' warps take what the last four leave: 216 * 256 + 72 * 128 = 168 * 384.
-constexpr int kSoftRegs = 216, kOtherRegs = 72;
-static_assert(kThreads == 384 && kSoftRegs * 256 + kOtherRegs * 128 <= 168 * kThreads, "registers");
+constexpr int kLoadWarps = 2;
 constexpr int kMaxBlocks = 160;
 constexpr int kItems = 4;    // items described ahead
 constexpr int kNotes = 8;    // steps whose bad pages are held
@@ -184,8 +179,27 @@ struct Cfg {
   static constexpr bool QUANT = KIND != KvType::kF16;
   static constexpr bool TWO = TWO_;  // q and weights in two f16 terms (f32 activations)
   static constexpr int TERMS = TWO ? 2 : 1;
-  static constexpr int KT = QUANT || TWO ? 64 : 128;  // positions of a step
+  // Warps of the softmax: four to a tile and half.  Over codes with one term two
+  // threads share a row, half of the positions and half of the values each: what a
+  // thread does in turn, one after the other, is what bounds a step there (16 prompts
+  // of 1024 over 8 bits 367 -> 333 us, 6 of 1501 over 4 bits 205 -> 158; the few
+  // steps of 64 rows over a prefix of 4096 lose, 62 -> 67).  An f16 cache has 64
+  // scores a thread in this form, more than 104 registers hold (4 prompts of 4096
+  // 460 -> 689).  With two terms the row's result stays in registers, which takes
+  // all of one thread's.
+  static constexpr int HALVES = QUANT && !TWO ? 2 : 1;
+  static constexpr int SOFT = 8 * HALVES, MMA = SOFT, DEAL = SOFT + 1, LOAD = SOFT + 2, WARPS = LOAD + kLoadWarps;
+  static constexpr int THREADS = 32 * WARPS;
+  // Registers a thread at launch, and how the groups of four warps share them.
+  static constexpr int REGS = HALVES == 1 ? 168 : 96, SOFT_REGS = HALVES == 1 ? 216 : 104, OTHER_REGS = HALVES == 1 ? 72 : 64;
+  static_assert(32 * SOFT * SOFT_REGS + 128 * OTHER_REGS <= REGS * THREADS, "registers");
+  // Positions of a step.  128 where scores and weights of two tiles fit 256
+  // columns of tensor memory; codes take one product per 64-value group and two
+  // terms two, so 64 there (two terms over f16 at 128 spill: 135 -> 152 us for a
+  // prompt of 2811).
+  static constexpr int KT = QUANT || TWO ? 64 : 128;
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
+  static constexpr int COLS = KT / HALVES, DIMS = D / HALVES;  // positions and values of a thread
   static constexpr int BOX = D / 64;                  // 128-byte columns of a tile of f16
   static constexpr int QTERM = BOX * kTileRows * 128, QTILE = TERMS * QTERM;
   static constexpr int PLANE = BOX * KT * 128;
@@ -197,7 +211,11 @@ struct Cfg {
   static constexpr int RAW = QUANT ? KT * ROW : 0;
   static constexpr int SCALE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
   static constexpr int NOTE = 2 * SCALE;                     // the same as f32, [K or V][group][position]
-  static constexpr int BORDER = TWO ? 5 : (QUANT ? 6 : 4);  // steps that the beginning and end of an item are worth
+  // Steps that the beginning and end of an item (its queries, its result) count
+  // for when the work is dealt.  Codes, 16 prompts of 1024 with 1, 2, 3, 4 and 6:
+  // 341, 332, 335, 347, 359 us; f16, 4 of 4096 with 2, 4 and 6: 474, 460, 467; two
+  // terms, a prompt of 2811 with 3, 5 and 8: 143, 134, 135.
+  static constexpr int BORDER = TWO ? 5 : (QUANT ? 2 : 4);
   static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kScales * (SCALE + NOTE);
   static_assert(SMEM <= 230 * 1024, "shared memory");
 };
@@ -368,6 +386,7 @@ struct Bars {
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t s_full[2], p_full[2], q_full[2], pv_done[2];
   uint64_t item_full[kItems], item_empty[kItems], fin;
+  uint64_t pair[8];  // of the two warps that have the halves of 32 rows
 };
 
 // The ring of items, as a reader sees it.
@@ -389,6 +408,21 @@ __device__ __forceinline__ float* RecordOf(const KvRowsParams& p, int block, boo
   return reinterpret_cast<float*>(static_cast<char*>(p.workspace) + kJobBytes) +
          (2 * block + (begins ? 1 : 0)) * RecordFloats(C::D);
 }
+
+// The same for those that go on reading the item where it is, until they let go of it.
+struct Holder {
+  int n = 0;
+  __device__ __forceinline__ const Item* Next(Bars& b, const Item* items) {
+    const int i = n % kItems;
+    if (!__all_sync(0xFFFFFFFFu, Wait(&b.item_full[i], (n / kItems) & 1))) return nullptr;
+    ++n;
+    return items + i;
+  }
+  static __device__ __forceinline__ void Release(Bars& b, const Item* items, const Item* it, int lane) {
+    __syncwarp();
+    if (lane == 0) tc::MbarArrive(&b.item_empty[it - items]);
+  }
+};
 
 // How a row's result and what was found elsewhere add up.
 struct Join {
@@ -432,20 +466,30 @@ __device__ __forceinline__ void Put32(const KvRowsParams& p, int64_t at, const f
   }
 }
 
-// Queries of one row into the tile, the sign of the softmax scale in them:
-// f16 ones as they are, others times 2^-e (a largest value in [2^12, 2^13)) as
-// f16 terms.  Returns the factor from products to scores, NaN for a row that is
+// A thread's values of a query row into the tile, the sign of the softmax scale
+// in them: f16 ones as they are, others times 2^-e (the row's largest value in
+// [2^12, 2^13)) as f16 terms.  `most_of` makes the largest magnitude that of the
+// whole row.  Returns the factor from products to scores, NaN for a row that is
 // not finite.
-template <typename C, typename T>
-__device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char* tile, int row) {
+template <typename C, typename T, typename F>
+__device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, bool there, char* tile, int row, int chunk0,
+                                        F most_of) {
   constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, __half>::value;
-  kvd::Raw8<T> q[C::D / 8];  // all of the row on its way at once
+  constexpr int kChunks = C::DIMS / 8;
+  kvd::Raw8<T> q[kChunks];  // all on their way at once
 #pragma unroll
-  for (int c = 0; c < C::D / 8; ++c) q[c].Load(static_cast<const T*>(p.q) + at + 8 * c);
+  for (int c = 0; c < kChunks; ++c) {
+    if (there) {
+      q[c].Load(static_cast<const T*>(p.q) + at + 8 * (chunk0 + c));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kvd::Raw8<T>::N; ++i) q[c].w[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
   // the bits of the largest magnitude: those of infinity and NaN are above all others
   uint32_t most = 0;
 #pragma unroll
-  for (int c = 0; c < C::D / 8; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
     for (int i = 0; i < kvd::Raw8<T>::N; ++i) {
       for (const uint32_t w : {q[c].w[i].x, q[c].w[i].y, q[c].w[i].z, q[c].w[i].w}) {
@@ -454,6 +498,7 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
     }
   }
   if (!kF32) most = max(most & 0xFFFFu, most >> 16) << 16;
+  most = most_of(most);
   const bool finite = most < (kF16 ? 0x7C000000u : 0x7F800000u);
   const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0;
   float f0 = 1.f, f1 = 1.f;
@@ -464,7 +509,7 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
     f1 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
   }
 #pragma unroll
-  for (int c = 0; c < C::D / 8; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     uint32_t hi[4], lo[4];
     if (kF16) {
       const uint4 w = q[c].w[0];
@@ -486,7 +531,7 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
         hi[i] ^= sign;
       }
     }
-    char* dst = tile + (c >> 3) * (kTileRows * 128) + Swz(row, c & 7);
+    char* dst = tile + ((chunk0 + c) >> 3) * (kTileRows * 128) + Swz(row, (chunk0 + c) & 7);
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (C::TWO) *reinterpret_cast<uint4*>(dst + C::QTERM) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
@@ -495,7 +540,7 @@ __device__ __forceinline__ float WriteQ(const KvRowsParams& p, int64_t at, char*
 
 // A row of an item, as the thread that has it sees it.
 struct RowState {
-  Item it;
+  const Item* it;
   int note0;  // steps before the item
   int row, qh;
   Bounds bounds;
@@ -506,16 +551,17 @@ struct RowState {
 };
 
 template <typename C>
-__global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const KvRowsParams p,
-               uint32_t magic) {
+__global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constant__ CUtensorMap map_k,
+                                                            const __grid_constant__ CUtensorMap map_v,
+                                                            const KvRowsParams p, uint32_t magic) {
   using namespace tc;
   constexpr int D = C::D, KT = C::KT;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ Item items[kItems];
-  __shared__ uint32_t s_tmem, s_bad[kNotes];
+  __shared__ uint32_t s_tmem, s_bad[kNotes], s_pair[2][2][2 * kTileRows];
   __shared__ int2 s_seen[kLoadWarps][kScales];  // a warp's own notes of what a step's rows see
-  __shared__ long long s_part[kThreads / 32], s_before;
+  __shared__ long long s_part[C::THREADS / 32], s_before;
   __shared__ int s_slot;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* s_q = smem;
@@ -538,14 +584,15 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     for (int i = 0; i < 2; ++i) {
       dev::MbarInit(&bars.s_full[i], 1);
       dev::MbarInit(&bars.pv_done[i], 1);
-      dev::MbarInit(&bars.p_full[i], kSoftWarps / 2);
-      dev::MbarInit(&bars.q_full[i], kSoftWarps / 2);
+      dev::MbarInit(&bars.p_full[i], C::SOFT / 2);
+      dev::MbarInit(&bars.q_full[i], C::SOFT / 2);
     }
     for (int i = 0; i < kItems; ++i) {
       dev::MbarInit(&bars.item_full[i], 1);
-      dev::MbarInit(&bars.item_empty[i], kSoftWarps + kLoadWarps + 1);
+      dev::MbarInit(&bars.item_empty[i], C::SOFT + kLoadWarps + 1);
     }
     dev::MbarInit(&bars.fin, 1);
+    for (int i = 0; i < 8; ++i) dev::MbarInit(&bars.pair[i], 2);
     dev::MbarInitFence();
   }
   dev::GridLaunchDependents();
@@ -553,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
 
   // ---- this block's share of the steps: a run of slots per thread, their steps added up
   const int n_slots = p.n_rows / sp.tokens + p.n_lists;
-  const int run = (n_slots + kThreads - 1) / kThreads;
+  const int run = (n_slots + C::THREADS - 1) / C::THREADS;
   const int slot_lo = min(tid * run, n_slots), slot_hi = min(slot_lo + run, n_slots);
   long long mine = 0;
   {
@@ -579,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
   const uint32_t tmem = s_tmem;
   long long before = incl - mine, per_head = 0;
 #pragma unroll 1
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < C::THREADS / 32; ++w) {
     if (w < warp) before += s_part[w];
     per_head += s_part[w];
   }
@@ -594,368 +641,388 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
     s_before = before;
   }
   __syncthreads();
-  if (warp >= kSoftWarps) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kDealWarp) {
-    // ---- items of this block, in order
-    Job job{};
-    Slots<C> sl;
-    int n = 0, slot = 0, hc = 0;
-    long long x = x0, skip = 0;
-    if (x0 < x1) {
-      slot = s_slot;
-      skip = rem - s_before;  // steps of the run to leave out
-      hc = static_cast<int>(x0 / per_head);
-      sl.Seek(p, sp, slot);
-    }
-    bool ok = true;
-#pragma unroll 1
-    for (bool more = true; more && ok;) {
-      Item it;
-      it.steps = 0;
-      it.n_tok = 0;
-      if (x < x1) {
-        const int steps = sl.Get(p, sp, slot, it);
-        const int weight = steps > 0 ? steps + C::BORDER : 0;
-        if (steps <= skip) {  // nothing of it, or its border alone
-          x += weight > skip ? weight - skip : 0;
-          skip -= min(skip, static_cast<long long>(weight));
-          it.steps = -1;
-        } else {
-          it.step0 = static_cast<int>(skip);
-          it.steps = static_cast<int>(min(static_cast<long long>(steps) - skip, x1 - x));
-          it.head = hc / sp.chunks;
-          it.chunk = hc % sp.chunks;
-          it.begins = it.step0 == 0;
-          it.ends = it.step0 + it.steps == steps;
-          if (it.begins && !it.ends) {
-            job.row0 = it.row0;
-            job.n_tok = it.n_tok;
-            job.head = it.head;
-            job.chunk = it.chunk;
-            job.last = min(max(ShareOf(x + steps - 1, total, blocks), block), blocks - 1);
-          }
-          x += it.steps + (it.ends ? C::BORDER : 0);
-          skip = 0;
-        }
-        if (++slot == n_slots) {
-          slot = 0;
-          ++hc;
-          sl.list = 0;
-        }
-        if (it.steps < 0) continue;
-      } else {
-        more = false;
+  if (warp >= C::SOFT) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+    if (warp == C::DEAL) {
+      // ---- items of this block, in order
+      Job job{};
+      Slots<C> sl;
+      int n = 0, slot = 0, hc = 0;
+      long long x = x0, skip = 0;
+      if (x0 < x1) {
+        slot = s_slot;
+        skip = rem - s_before;  // steps of the run to leave out
+        hc = static_cast<int>(x0 / per_head);
+        sl.Seek(p, sp, slot);
       }
-      const int i = n % kItems;
-      if (n >= kItems) ok = __all_sync(0xFFFFFFFFu, Wait(&bars.item_empty[i], (n / kItems - 1) & 1));
-      if (!ok) break;
-      if (lane == 0) {
-        items[i] = it;
-        MbarArrive(&bars.item_full[i]);
-      }
-      __syncwarp();
-      ++n;
-      // its queries on their way into L2, an item or more before they are read
-      const int size = p.type == ElemType::kF32 ? 4 : 2;
-      const int heads = it.steps > 0 ? min(sp.per, sp.group - it.chunk * sp.per) : 0;
-      const int lines = (heads * D * size + 127) / 128;
-#pragma unroll 1
-      for (int k = lane; k < it.n_tok * lines; k += 32) {
-        const int64_t at = (it.row0 + k / lines) * p.q_stride + static_cast<int64_t>(it.head * sp.group + it.chunk * sp.per) * D;
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.q) + at * size + k % lines * 128));
-      }
-    }
-    if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
-  } else if (warp == kMmaWarp) {
-    // ---- products: per step and tile O += P V of the step before, then S = Q K^T
-    if (lane == 0) {
-      constexpr uint32_t id_s = InstrDesc(128, KT);
-      constexpr uint32_t id_o = InstrDesc(128, C::NG == 1 ? D : 64) | 1u << 16;  // (V: values contiguous)
-      const uint32_t a_q = dev::SmemAddr(s_q), a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v);
-      int n = 0;
-      uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
-      int c = 0;  // steps so far
       bool ok = true;
-#pragma unroll 1
-      while (ok) {
-        const int i = n % kItems;
-        if (!Wait(&bars.item_full[i], (n / kItems) & 1)) break;
-        const int steps = items[i].steps, rows = items[i].n_tok * sp.per;
-        MbarArrive(&bars.item_empty[i]);
-        ++n;
-        if (steps <= 0) break;
-        const int tiles = rows > kTileRows ? 2 : 1;
-#pragma unroll 1
-        for (int j = 0; j <= steps && ok; ++j) {
-#pragma unroll 1
-          for (int t = 0; t < tiles && ok; ++t) {
-            if (j > 0) {
-              const int st = (c + j - 1) % C::STAGES, par = ((c + j - 1) / C::STAGES) & 1;
-              ok = (t > 0 || Wait(&bars.v_full[st], par)) && Wait(&bars.p_full[t], p_parity[t]);
-              if (!ok) break;
-              p_parity[t] ^= 1;
-              FenceAfterSync();
-              const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128;
-              // with two terms every step's product starts anew (it is added up in registers)
-              const bool going_on = !C::TWO && j > 1;
-#pragma unroll
-              for (int g = 0; g < C::NG; ++g) {
-#pragma unroll
-                for (int term = C::TERMS - 1; term >= 0; --term) {
-                  const uint32_t v = Here(DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
-                  const uint32_t a = Here(w + (g * C::TERMS + term) * (KT / 2)), d = Here(o + 64 * g);
-#pragma unroll
-                  for (int k = 0; k < KT / 16; ++k) {
-                    MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
-                  }
-                }
-              }
-              MmaCommit(&bars.pv_done[t]);
-              if (t == tiles - 1) MmaCommit(&bars.v_empty[st]);
-            }
-            if (j < steps) {
-              const int st = (c + j) % C::STAGES, par = ((c + j) / C::STAGES) & 1;
-              ok = (j > 0 || Wait(&bars.q_full[t], q_parity[t])) &&
-                   (t > 0 || Wait(&bars.k_full[st], par));
-              if (!ok) break;
-              if (j == 0) q_parity[t] ^= 1;
-              FenceAfterSync();
-              // (second terms first: the sums that the tensor cores cut short are small then)
-#pragma unroll
-              for (int term = C::TERMS - 1; term >= 0; --term) {
-#pragma unroll
-                for (int box = 0; box < C::BOX; ++box) {
-                  const uint32_t d = Here(tmem + t * 128 + (C::NG == 2 ? 64 * box : 0));
-                  const uint32_t q = Here(DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
-                  const uint32_t kk = Here(DescRows(a_k + st * C::PLANE + box * (KT * 128)));
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
-                  }
-                }
-              }
-              MmaCommit(&bars.s_full[t]);
-              if (t == tiles - 1) MmaCommit(&bars.k_empty[st]);
-            }
-          }
-        }
-        c += steps;
-      }
-      MmaCommit(&bars.fin);  // no product is under way when the block ends
-      Wait(&bars.fin, 0);
-    }
-    __syncwarp();
-  } else {
-    // ---- copies
-    const int lt = tid - 32 * kLoadWarp0, lw = lt >> 5;
-    const int mask = (1 << p.kv.page_log2) - 1;
-    int begun = 0, ended = 0;  // copies: 2 n is K's of step n, 2 n + 1 V's
-    bool ok = true;
-    asm volatile("fence.proxy.async.global;" ::: "memory");  // (what kernels before this one stored is read by copies)
-    const uint32_t a_raw = dev::SmemAddr(s_raw), a_scale = dev::SmemAddr(s_scale);
-    const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
-    constexpr int kRowStep = 32 * kLoadWarps / C::CPR;
-    // The oldest copy of codes has arrived: spread them to f16, tell the products.
-    auto finish = [&]() {
-      const int step = ended >> 1, st = step % C::STAGES;
-      const bool v = ended & 1;
-      if (!__all_sync(0xFFFFFFFFu, Wait(v ? &bars.v_empty[st] : &bars.k_empty[st], ((step / C::STAGES) & 1) ^ 1))) {
-        ok = false;
-        return;
-      }
-      const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
-      char* dst = (v ? s_v : s_k) + st * C::PLANE;
-#pragma unroll 2
-      for (int i = 0; i < C::PER; ++i) {
-        const int r = r0 + i * kRowStep;
-        const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
-        constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          kvd::Codes16<C::KIND> code;
-          if (C::KIND == KvType::kQ8) {
-            code.w[0] = w.x;
-            code.w[1] = w.y;
-            code.w[C::KIND == KvType::kQ8 ? 2 : 0] = w.z;
-            code.w[C::KIND == KvType::kQ8 ? 3 : 0] = w.w;
+  #pragma unroll 1
+      for (bool more = true; more && ok;) {
+        Item it;
+        it.steps = 0;
+        it.n_tok = 0;
+        if (x < x1) {
+          const int steps = sl.Get(p, sp, slot, it);
+          const int weight = steps > 0 ? steps + C::BORDER : 0;
+          if (steps <= skip) {  // nothing of it, or its border alone
+            x += weight > skip ? weight - skip : 0;
+            skip -= min(skip, static_cast<long long>(weight));
+            it.steps = -1;
           } else {
-            code.w[0] = h == 0 ? w.x : w.z;
-            code.w[1] = h == 0 ? w.y : w.w;
-          }
-          uint32_t y[8];
-          code.Pairs(y, magic);
-          const int u = (c0 * kHalves + h) * 2;  // 8-value chunk of the row
-          char* d = dst + (u >> 3) * (KT * 128);
-          *reinterpret_cast<uint4*>(d + Swz(r, u & 7)) = make_uint4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
-        }
-      }
-      if (!v) {
-        // the scales that this warp copied, group after group; 0 where no row sees the position
-        __syncwarp();
-        const int2 seen = s_seen[lw][step % kScales];
-        const __half* h = reinterpret_cast<const __half*>(s_scale + step % kScales * C::SCALE + lw * (C::SCALE / 2));
-        float* f = reinterpret_cast<float*>(s_note + step % kScales * C::NOTE + lw * (C::NOTE / 2));
-#pragma unroll 1
-        for (int i = lane; i < KT * C::NG; i += 32) {
-          const int pos = i / C::NG;
-          f[i % C::NG * KT + pos] = pos >= seen.x && pos < seen.y ? __half2float(h[i]) : 0.f;
-        }
-      }
-      dev::FenceProxyAsync();
-      __syncwarp();
-      if (lane == 0) MbarArrive(v ? &bars.v_full[st] : &bars.k_full[st]);
-      ++ended;
-    };
-    Reader rd;
-    Item it;
-#pragma unroll 1
-    while (ok && rd.Next(bars, items, it, lane)) {
-      // lane g has to do with positions 16 g .. 16 g + 15 of a step: their page
-      auto lookup = [&](int pos) {
-        return lane < KT / 16 && pos + 16 > it.lo && pos < it.hi
-                   ? p.table.pages[it.table_row * p.table.stride + (pos >> p.kv.page_log2)]
-                   : -1;
-      };
-      int next = lookup(it.base + it.step0 * KT + 16 * lane);
-#pragma unroll 1
-      for (int j = 0; j < it.steps && ok; ++j) {
-        const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
-        const int page = next;
-        if (j + 1 < it.steps) next = lookup(at + KT);
-        const bool used = lane < KT / 16 && at + 16 > it.lo && at < it.hi;
-        const bool there = used && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
-        const uint32_t have = __ballot_sync(0xFFFFFFFFu, there);
-        const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
-        const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
-        if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
-        if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % kScales] = make_int2(it.lo - pos0, it.hi - pos0);
-        if (!C::QUANT) {
-          // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
-          const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
-          constexpr uint32_t kEvery = 0x55555555u & ((1u << KT / 16) - 1);  // groups of warp 0
-          const uint32_t groups = kEvery << lw;
-          const int g = lw + 2 * (lane / C::BOX), box = lane % C::BOX;
-          const int pg = __shfl_sync(0xFFFFFFFFu, page, g & 31), in = (pos0 + 16 * g) & mask;
-#pragma unroll 1
-          for (int v = 0; v < 2; ++v) {
-            const int st = (begun >> 1) % C::STAGES;
-            uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
-            if (!__all_sync(0xFFFFFFFFu, Wait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
-              ok = false;
-              break;
+            it.step0 = static_cast<int>(skip);
+            it.steps = static_cast<int>(min(static_cast<long long>(steps) - skip, x1 - x));
+            it.head = hc / sp.chunks;
+            it.chunk = hc % sp.chunks;
+            it.begins = it.step0 == 0;
+            it.ends = it.step0 + it.steps == steps;
+            if (it.begins && !it.ends) {
+              job.row0 = it.row0;
+              job.n_tok = it.n_tok;
+              job.head = it.head;
+              job.chunk = it.chunk;
+              job.last = min(max(ShareOf(x + steps - 1, total, blocks), block), blocks - 1);
             }
-            char* dst = (v ? s_v : s_k) + st * C::PLANE;
-            const uint32_t take = (v ? full : have) & groups;
-            uint32_t rest = v ? groups & ~full : 0;
-            if (rest != 0) {
-              // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
-#pragma unroll 1
-              while (rest != 0) {
-                const int q = __ffs(rest) - 1;
-                rest &= rest - 1;
-                const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
-#pragma unroll 1
-                for (int i = lane; i < 16 * C::CPR; i += 32) {
-                  const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
-                  const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
-                  CopyAsync16(dev::SmemAddr(dst + (c >> 3) * (KT * 128) + Swz(16 * q + r, c & 7)),
-                              seen ? src + r * p.kv.pos_stride + c * 16 : p.kv.v, seen);
+            x += it.steps + (it.ends ? C::BORDER : 0);
+            skip = 0;
+          }
+          if (++slot == n_slots) {
+            slot = 0;
+            ++hc;
+            sl.list = 0;
+          }
+          if (it.steps < 0) continue;
+        } else {
+          more = false;
+        }
+        const int i = n % kItems;
+        if (n >= kItems) ok = __all_sync(0xFFFFFFFFu, Wait(&bars.item_empty[i], (n / kItems - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          items[i] = it;
+          MbarArrive(&bars.item_full[i]);
+        }
+        __syncwarp();
+        ++n;
+        // its queries on their way into L2, an item or more before they are read
+        const int size = p.type == ElemType::kF32 ? 4 : 2;
+        const int heads = it.steps > 0 ? min(sp.per, sp.group - it.chunk * sp.per) : 0;
+        const int lines = (heads * D * size + 127) / 128;
+  #pragma unroll 1
+        for (int k = lane; k < it.n_tok * lines; k += 32) {
+          const int64_t at = (it.row0 + k / lines) * p.q_stride + static_cast<int64_t>(it.head * sp.group + it.chunk * sp.per) * D;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.q) + at * size + k % lines * 128));
+        }
+      }
+      if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
+    } else if (warp == C::MMA) {
+      // ---- products: per step and tile O += P V of the step before, then S = Q K^T
+      if (lane == 0) {
+        constexpr uint32_t id_s = InstrDesc(128, KT);
+        constexpr uint32_t id_o = InstrDesc(128, C::NG == 1 ? D : 64) | 1u << 16;  // (V: values contiguous)
+        const uint32_t a_q = dev::SmemAddr(s_q), a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v);
+        int n = 0;
+        uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
+        int c = 0;  // steps so far
+        bool ok = true;
+  #pragma unroll 1
+        while (ok) {
+          const int i = n % kItems;
+          if (!Wait(&bars.item_full[i], (n / kItems) & 1)) break;
+          const int steps = items[i].steps, rows = items[i].n_tok * sp.per;
+          MbarArrive(&bars.item_empty[i]);
+          ++n;
+          if (steps <= 0) break;
+          const int tiles = rows > kTileRows ? 2 : 1;
+  #pragma unroll 1
+          for (int j = 0; j <= steps && ok; ++j) {
+  #pragma unroll 1
+            for (int t = 0; t < tiles && ok; ++t) {
+              if (j > 0) {
+                const int st = (c + j - 1) % C::STAGES, par = ((c + j - 1) / C::STAGES) & 1;
+                ok = (t > 0 || Wait(&bars.v_full[st], par)) && Wait(&bars.p_full[t], p_parity[t]);
+                if (!ok) break;
+                p_parity[t] ^= 1;
+                FenceAfterSync();
+                const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128;
+                // with two terms every step's product starts anew (it is added up in registers)
+                const bool going_on = !C::TWO && j > 1;
+  #pragma unroll
+                for (int g = 0; g < C::NG; ++g) {
+  #pragma unroll
+                  for (int term = C::TERMS - 1; term >= 0; --term) {
+                    const uint32_t v = Here(DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
+                    const uint32_t a = Here(w + (g * C::TERMS + term) * (KT / 2)), d = Here(o + 64 * g);
+  #pragma unroll
+                    for (int k = 0; k < KT / 16; ++k) {
+                      MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
+                    }
+                  }
+                }
+                MmaCommit(&bars.pv_done[t]);
+                if (t == tiles - 1) MmaCommit(&bars.v_empty[st]);
+              }
+              if (j < steps) {
+                const int st = (c + j) % C::STAGES, par = ((c + j) / C::STAGES) & 1;
+                ok = (j > 0 || Wait(&bars.q_full[t], q_parity[t])) &&
+                     (t > 0 || Wait(&bars.k_full[st], par));
+                if (!ok) break;
+                if (j == 0) q_parity[t] ^= 1;
+                FenceAfterSync();
+                // (second terms first: the sums that the tensor cores cut short are small then)
+  #pragma unroll
+                for (int term = C::TERMS - 1; term >= 0; --term) {
+  #pragma unroll
+                  for (int box = 0; box < C::BOX; ++box) {
+                    const uint32_t d = Here(tmem + t * 128 + (C::NG == 2 ? 64 * box : 0));
+                    const uint32_t q = Here(DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
+                    const uint32_t kk = Here(DescRows(a_k + st * C::PLANE + box * (KT * 128)));
+  #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                      MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
+                    }
+                  }
+                }
+                MmaCommit(&bars.s_full[t]);
+                if (t == tiles - 1) MmaCommit(&bars.k_empty[st]);
+              }
+            }
+          }
+          c += steps;
+        }
+        MmaCommit(&bars.fin);  // no product is under way when the block ends
+        Wait(&bars.fin, 0);
+      }
+      __syncwarp();
+    } else {
+      // ---- copies
+      const int lt = tid - 32 * C::LOAD, lw = lt >> 5;
+      const int mask = (1 << p.kv.page_log2) - 1;
+      int begun = 0, ended = 0;  // copies: 2 n is K's of step n, 2 n + 1 V's
+      bool ok = true;
+      asm volatile("fence.proxy.async.global;" ::: "memory");  // (what kernels before this one stored is read by copies)
+      const uint32_t a_raw = dev::SmemAddr(s_raw), a_scale = dev::SmemAddr(s_scale);
+      const int c0 = lt % C::CPR, r0 = lt / C::CPR;  // piece and first row of this thread
+      constexpr int kRowStep = 32 * kLoadWarps / C::CPR;
+      // The oldest copy of codes has arrived: spread them to f16, tell the products.
+      auto finish = [&]() {
+        const int step = ended >> 1, st = step % C::STAGES;
+        const bool v = ended & 1;
+        if (!__all_sync(0xFFFFFFFFu, Wait(v ? &bars.v_empty[st] : &bars.k_empty[st], ((step / C::STAGES) & 1) ^ 1))) {
+          ok = false;
+          return;
+        }
+        const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
+        char* dst = (v ? s_v : s_k) + st * C::PLANE;
+  #pragma unroll 2
+        for (int i = 0; i < C::PER; ++i) {
+          const int r = r0 + i * kRowStep;
+          const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
+          constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
+  #pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            kvd::Codes16<C::KIND> code;
+            if (C::KIND == KvType::kQ8) {
+              code.w[0] = w.x;
+              code.w[1] = w.y;
+              code.w[C::KIND == KvType::kQ8 ? 2 : 0] = w.z;
+              code.w[C::KIND == KvType::kQ8 ? 3 : 0] = w.w;
+            } else {
+              code.w[0] = h == 0 ? w.x : w.z;
+              code.w[1] = h == 0 ? w.y : w.w;
+            }
+            uint32_t y[8];
+            code.Pairs(y, magic);
+            const int u = (c0 * kHalves + h) * 2;  // 8-value chunk of the row
+            char* d = dst + (u >> 3) * (KT * 128);
+            *reinterpret_cast<uint4*>(d + Swz(r, u & 7)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(d + Swz(r, (u & 7) + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+        }
+        if (!v) {
+          // the scales that this warp copied, group after group; 0 where no row sees the position
+          __syncwarp();
+          const int2 seen = s_seen[lw][step % kScales];
+          const __half* h = reinterpret_cast<const __half*>(s_scale + step % kScales * C::SCALE + lw * (C::SCALE / 2));
+          float* f = reinterpret_cast<float*>(s_note + step % kScales * C::NOTE + lw * (C::NOTE / 2));
+  #pragma unroll 1
+          for (int i = lane; i < KT * C::NG; i += 32) {
+            const int pos = i / C::NG;
+            f[i % C::NG * KT + pos] = pos >= seen.x && pos < seen.y ? __half2float(h[i]) : 0.f;
+          }
+        }
+        dev::FenceProxyAsync();
+        __syncwarp();
+        if (lane == 0) MbarArrive(v ? &bars.v_full[st] : &bars.k_full[st]);
+        ++ended;
+      };
+      Reader rd;
+      Item it;
+  #pragma unroll 1
+      while (ok && rd.Next(bars, items, it, lane)) {
+        // lane g has to do with positions 16 g .. 16 g + 15 of a step: their page
+        auto lookup = [&](int pos) {
+          return lane < KT / 16 && pos + 16 > it.lo && pos < it.hi
+                     ? p.table.pages[it.table_row * p.table.stride + (pos >> p.kv.page_log2)]
+                     : -1;
+        };
+        int next = lookup(it.base + it.step0 * KT + 16 * lane);
+  #pragma unroll 1
+        for (int j = 0; j < it.steps && ok; ++j) {
+          const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
+          const int page = next;
+          if (j + 1 < it.steps) next = lookup(at + KT);
+          const bool used = lane < KT / 16 && at + 16 > it.lo && at < it.hi;
+          const bool there = used && static_cast<unsigned>(page) < static_cast<unsigned>(p.kv.n_pages);
+          const uint32_t have = __ballot_sync(0xFFFFFFFFu, there);
+          const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
+          const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
+          if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
+          if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % kScales] = make_int2(it.lo - pos0, it.hi - pos0);
+          if (!C::QUANT) {
+            // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
+            const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
+            constexpr uint32_t kEvery = 0x55555555u & ((1u << KT / 16) - 1);  // groups of warp 0
+            const uint32_t groups = kEvery << lw;
+            const int g = lw + 2 * (lane / C::BOX), box = lane % C::BOX;
+            const int pg = __shfl_sync(0xFFFFFFFFu, page, g & 31), in = (pos0 + 16 * g) & mask;
+  #pragma unroll 1
+            for (int v = 0; v < 2; ++v) {
+              const int st = (begun >> 1) % C::STAGES;
+              uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
+              if (!__all_sync(0xFFFFFFFFu, Wait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
+                ok = false;
+                break;
+              }
+              char* dst = (v ? s_v : s_k) + st * C::PLANE;
+              const uint32_t take = (v ? full : have) & groups;
+              uint32_t rest = v ? groups & ~full : 0;
+              if (rest != 0) {
+                // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
+  #pragma unroll 1
+                while (rest != 0) {
+                  const int q = __ffs(rest) - 1;
+                  rest &= rest - 1;
+                  const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
+  #pragma unroll 1
+                  for (int i = lane; i < 16 * C::CPR; i += 32) {
+                    const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
+                    const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
+                    CopyAsync16(dev::SmemAddr(dst + (c >> 3) * (KT * 128) + Swz(16 * q + r, c & 7)),
+                                seen ? src + r * p.kv.pos_stride + c * 16 : p.kv.v, seen);
+                  }
+                }
+                CopyCommit();
+                CopyWait<0>();
+                dev::FenceProxyAsync();
+              }
+              __syncwarp();
+              if (lane == 0) dev::MbarExpectTx(whole, __popc(take) * (C::BOX * 2048));  // (an arrival too)
+              __syncwarp();
+              if (lane < KT / 32 * C::BOX && ((take >> g) & 1)) {
+                LoadTile(dst + box * (KT * 128) + g * 2048, v ? &map_v : &map_k, 64 * box, in, it.head, pg, whole);
+              }
+              ++begun;
+            }
+            ended = begun;
+          } else {
+  #pragma unroll 1
+            for (int v = 0; v < 2 && ok; ++v) {
+              const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
+              const uint32_t dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
+              // 16 positions at a time: rows r0 + k * kRowStep of them are this thread's
+  #pragma unroll 1
+              for (int g = 0; g < KT / 16; ++g) {
+                const char* src = plane + __shfl_sync(0xFFFFFFFFu, off, g);
+                const bool have_g = (have >> g) & 1;
+                const int first = pos0 + 16 * g;
+                auto copy = [&](uint32_t to, int r) {
+                  const bool in = have_g && first + r >= it.lo && first + r < it.hi;
+                  CopyAsync16(to, in ? src + r * p.kv.pos_stride : plane, in);
+                };
+                if (kRowStep > 16) {  // (a thread has rows of every other sixteen)
+                  constexpr int kSkip = kRowStep > 16 ? kRowStep / 16 : 1;
+                  if ((r0 >> 4) == g % kSkip) copy(dst + g / kSkip * (32 * kLoadWarps * 16), r0 & 15);
+                } else {
+  #pragma unroll
+                  for (int k = 0; k < 16 / kRowStep; ++k) copy(dst + g * (16 * C::ROW) + k * (kRowStep * C::ROW), r0 + k * kRowStep);
+                }
+              }
+              if (v == 0) {
+                // scales of K and V: 16 positions are dense, 2 NG 16-byte pieces
+                constexpr int kPer = 2 * C::NG;
+                const int i = lane / kPer % (KT / 16);
+                const int64_t so = there ? kvd::ScaleOffset(p.kv, page, it.head, at & mask) : 0;
+                const int64_t o = __shfl_sync(0xFFFFFFFFu, so, i) + lane % kPer * 16;
+                if (lane < KT / 16 * kPer) {
+                  const bool in = (have >> i) & 1;
+                  const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
+                  CopyAsync16(a_scale + (begun >> 1) % kScales * C::SCALE + lw * (C::SCALE / 2) + lane * 16, in ? src + o : src, in);
                 }
               }
               CopyCommit();
-              CopyWait<0>();
-              dev::FenceProxyAsync();
-            }
-            __syncwarp();
-            if (lane == 0) dev::MbarExpectTx(whole, __popc(take) * (C::BOX * 2048));  // (an arrival too)
-            __syncwarp();
-            if (lane < KT / 32 * C::BOX && ((take >> g) & 1)) {
-              LoadTile(dst + box * (KT * 128) + g * 2048, v ? &map_v : &map_k, 64 * box, in, it.head, pg, whole);
-            }
-            ++begun;
-          }
-          ended = begun;
-        } else {
-#pragma unroll 1
-          for (int v = 0; v < 2 && ok; ++v) {
-            const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
-            const uint32_t dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
-            // 16 positions at a time: rows r0 + k * kRowStep of them are this thread's
-#pragma unroll 1
-            for (int g = 0; g < KT / 16; ++g) {
-              const char* src = plane + __shfl_sync(0xFFFFFFFFu, off, g);
-              const bool have_g = (have >> g) & 1;
-              const int first = pos0 + 16 * g;
-              auto copy = [&](uint32_t to, int r) {
-                const bool in = have_g && first + r >= it.lo && first + r < it.hi;
-                CopyAsync16(to, in ? src + r * p.kv.pos_stride : plane, in);
-              };
-              if (kRowStep > 16) {  // (a thread has rows of every other sixteen)
-                constexpr int kSkip = kRowStep > 16 ? kRowStep / 16 : 1;
-                if ((r0 >> 4) == g % kSkip) copy(dst + g / kSkip * (32 * kLoadWarps * 16), r0 & 15);
-              } else {
-#pragma unroll
-                for (int k = 0; k < 16 / kRowStep; ++k) copy(dst + g * (16 * C::ROW) + k * (kRowStep * C::ROW), r0 + k * kRowStep);
+              ++begun;
+              if (begun - ended > C::LAG) {
+                CopyWait<C::LAG>();
+                finish();
               }
-            }
-            if (v == 0) {
-              // scales of K and V: 16 positions are dense, 2 NG 16-byte pieces
-              constexpr int kPer = 2 * C::NG;
-              const int i = lane / kPer % (KT / 16);
-              const int64_t so = there ? kvd::ScaleOffset(p.kv, page, it.head, at & mask) : 0;
-              const int64_t o = __shfl_sync(0xFFFFFFFFu, so, i) + lane % kPer * 16;
-              if (lane < KT / 16 * kPer) {
-                const bool in = (have >> i) & 1;
-                const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
-                CopyAsync16(a_scale + (begun >> 1) % kScales * C::SCALE + lw * (C::SCALE / 2) + lane * 16, in ? src + o : src, in);
-              }
-            }
-            CopyCommit();
-            ++begun;
-            if (begun - ended > C::LAG) {
-              CopyWait<C::LAG>();
-              finish();
             }
           }
         }
       }
-    }
-    if (C::QUANT) {
-      CopyWait<0>();
-      while (ok && ended < begun) finish();
-    } else if (begun > 0) {
-      // copies that nobody waits for any more have landed before the block ends
-      for (int n = max(0, begun / 2 - C::STAGES); n < begun / 2; ++n) {
-        const int st = n % C::STAGES;
-        Wait(&bars.k_full[st], (n / C::STAGES) & 1);
-        Wait(&bars.v_full[st], (n / C::STAGES) & 1);
+      if (C::QUANT) {
+        CopyWait<0>();
+        while (ok && ended < begun) finish();
+      } else if (begun > 0) {
+        // copies that nobody waits for any more have landed before the block ends
+        for (int n = max(0, begun / 2 - C::STAGES); n < begun / 2; ++n) {
+          const int st = n % C::STAGES;
+          Wait(&bars.k_full[st], (n / C::STAGES) & 1);
+          Wait(&bars.v_full[st], (n / C::STAGES) & 1);
+        }
       }
     }
-  }
   } else {
-    // ---- softmax: a thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-    const int t = warp >> 2, in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
+    // ---- softmax: a thread per row, or two
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFT_REGS));
+    const int t = warp / (4 * C::HALVES), half = C::HALVES == 2 ? (warp >> 2) & 1 : 0;
+    const int in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
+    const int col0 = half * C::COLS, dim0 = half * C::DIMS;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128;
-    uint32_t s_parity = 0;
+    const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128 + dim0;
+    uint32_t s_parity = 0, pair_parity = 0;
     int c = 0, note = 0;  // products with V begun for this tile; steps so far
     bool ok = true;
-    Reader rd;
+    // What the thread with the row's other half has in its place.
+    auto other = [&](uint32_t v) -> uint32_t {
+      uint32_t* place = s_pair[pair_parity][t];
+      place[half * kTileRows + in_tile] = v;
+      FenceBeforeSync();  // (what either has read of tensor memory, the other may write over)
+      __syncwarp();
+      uint64_t* bar = &bars.pair[t * 4 + (warp & 3)];
+      if (lane == 0) MbarArrive(bar);
+      if (!__all_sync(0xFFFFFFFFu, Wait(bar, pair_parity))) ok = false;
+      FenceAfterSync();
+      pair_parity ^= 1;
+      return place[(half ^ 1) * kTileRows + in_tile];
+    };
+    Holder rd;
+    const Item* first_item = items;
     // The next item that this tile has rows of, and what the thread has to know of its row.
     auto next_item = [&](RowState& w) {
-      do {
-        if (!rd.Next(bars, items, w.it, lane)) return false;
+      for (;;) {
+        w.it = rd.Next(bars, items);
+        if (w.it == nullptr) return false;
         w.note0 = note;
-        note += w.it.steps;
-      } while (t == 1 && w.it.n_tok * sp.per <= kTileRows);
-      const int tok = r / sp.per, g = r - tok * sp.per + w.it.chunk * sp.per;
-      w.valid = tok < w.it.n_tok && g < sp.group;
+        note += w.it->steps;
+        if (w.it->steps <= 0) return false;
+        if (t == 0 || w.it->n_tok * sp.per > kTileRows) break;
+        Holder::Release(bars, first_item, w.it, lane);
+      }
+      const int tok = r / sp.per, g = r - tok * sp.per + w.it->chunk * sp.per;
+      w.valid = tok < w.it->n_tok && g < sp.group;
       w.active = __any_sync(0xFFFFFFFFu, w.valid);
-      w.row = w.it.row0 + tok;
-      w.qh = w.it.head * sp.group + g;
+      w.row = w.it->row0 + tok;
+      w.qh = w.it->head * sp.group + g;
       w.seen = Seen{0, 0, false};
       w.cs = w.slope = 0.f;
       w.pos = 0;
@@ -970,31 +1037,33 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       return true;
     };
     auto write_q = [&](RowState& w) {
-      if (w.valid) {
+      if (w.active) {
         const int64_t q_at = w.row * p.q_stride + static_cast<int64_t>(w.qh) * D;
         char* tile = s_q + t * C::QTILE;
+        auto most_of = [&](uint32_t most) { return C::HALVES == 2 ? max(most, other(most)) : most; };
         if (C::TWO) {
-          w.cs = WriteQ<C, float>(p, q_at, tile, in_tile);
+          w.cs = WriteQ<C, float>(p, q_at, w.valid, tile, in_tile, dim0 / 8, most_of);
         } else {
-          w.cs = p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, tile, in_tile)
-                                          : WriteQ<C, __nv_bfloat16>(p, q_at, tile, in_tile);
+          w.cs = p.type == ElemType::kF16 ? WriteQ<C, __half>(p, q_at, w.valid, tile, in_tile, dim0 / 8, most_of)
+                                          : WriteQ<C, __nv_bfloat16>(p, q_at, w.valid, tile, in_tile, dim0 / 8, most_of);
         }
+      }
+      if (w.valid) {
         w.seen = SeenBy(p, w.bounds);
         const Seen& s = w.seen;
-        w.is_nan = s.past || (s.start < s.end && (s.start < w.it.lo || s.end > w.it.hi)) || !(w.cs == w.cs) ||
-                   (p.prefix != nullptr && w.bounds.prefix > w.it.first_prefix);
+        w.is_nan = s.past || (s.start < s.end && (s.start < w.it->lo || s.end > w.it->hi)) || !(w.cs == w.cs) ||
+                   (p.prefix != nullptr && w.bounds.prefix > w.it->first_prefix);
         if (!(p.cap > 0.f)) w.cs = fmaxf(w.cs * kLog2e, 1e-37f);  // (a scale of 0: minus infinity times it is to stay)
       }
       dev::FenceProxyAsync();
       __syncwarp();
       if (lane == 0) MbarArrive(&bars.q_full[t]);
     };
-    RowState now{};  // (an item of no steps, before the first)
+    RowState now{};  // (nothing, before the first item)
     bool more = true;
 #pragma unroll 1
     while (ok && more) {
-      const Item& it = now.it;
-      const int steps = it.steps, note0 = now.note0, row = now.row, qh = now.qh;
+      const int steps = now.it != nullptr ? now.it->steps : 0, note0 = now.note0, row = now.row, qh = now.qh;
       const Seen seen = now.seen;
       const float cs = now.cs, slope = now.slope;
       const int pos = now.pos;
@@ -1030,19 +1099,19 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             }
           }
         }
-        float2 s[KT / 2];
+        float2 s[C::COLS / 2];
         uint32_t* u = reinterpret_cast<uint32_t*>(s);
         if (C::NG == 2) {
           // the parts of the two groups, each times its scale
 #pragma unroll
-          for (int h = 0; h < KT; h += 16) {
+          for (int h = 0; h < C::COLS; h += 16) {
             uint32_t b[16];
-            TmemLoad16(a_s + h, *reinterpret_cast<uint32_t(*)[16]>(u + h));
-            TmemLoad16(a_s + 64 + h, b);
+            TmemLoad16(a_s + col0 + h, *reinterpret_cast<uint32_t(*)[16]>(u + h));
+            TmemLoad16(a_s + 64 + col0 + h, b);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-              const float4 d0 = *reinterpret_cast<const float4*>(scales + h + i);
-              const float4 d1 = *reinterpret_cast<const float4*>(scales + KT + h + i);
+              const float4 d0 = *reinterpret_cast<const float4*>(scales + col0 + h + i);
+              const float4 d1 = *reinterpret_cast<const float4*>(scales + KT + col0 + h + i);
               float2 &x = s[(h + i) / 2], &y = s[(h + i) / 2 + 1];
               const float2 bx = make_float2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]));
               const float2 by = make_float2(__uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
@@ -1052,12 +1121,12 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
           }
         } else {
 #pragma unroll
-          for (int h = 0; h < KT; h += 32) TmemLoad32(a_s + h, u + h);
+          for (int h = 0; h < C::COLS; h += 32) TmemLoad32(a_s + col0 + h, u + h);
           TmemLoadWait();
           if (C::QUANT) {
 #pragma unroll
-            for (int i = 0; i < KT; i += 4) {
-              const float4 d = *reinterpret_cast<const float4*>(scales + i);
+            for (int i = 0; i < C::COLS; i += 4) {
+              const float4 d = *reinterpret_cast<const float4*>(scales + col0 + i);
               s[i / 2] = __fmul2_rn(s[i / 2], make_float2(d.x, d.y));
               s[i / 2 + 1] = __fmul2_rn(s[i / 2 + 1], make_float2(d.z, d.w));
             }
@@ -1065,33 +1134,37 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         }
         if (bend.capped) {
 #pragma unroll
-          for (int i = 0; i < KT; ++i) u[i] = __float_as_uint(bend.Capped(__uint_as_float(u[i]) * cs));
+          for (int i = 0; i < C::COLS; ++i) u[i] = __float_as_uint(bend.Capped(__uint_as_float(u[i]) * cs));
         }
         if (bend.biased) {
-          const float first = static_cast<float>(pos - pos0), f = bend.capped ? 1.f : cs;
+          const float first = static_cast<float>(pos - pos0 - col0), f = bend.capped ? 1.f : cs;
 #pragma unroll
-          for (int i = 0; i < KT; ++i) {
+          for (int i = 0; i < C::COLS; ++i) {
             u[i] = __float_as_uint(__uint_as_float(u[i]) * f - bend.slope * fabsf(first - static_cast<float>(i)));
           }
         }
         if (EDGE) {
 #pragma unroll
-          for (int i = 0; i < KT; ++i) {
+          for (int i = 0; i < C::COLS; ++i) {
             if (i < from || i >= to) u[i] = __float_as_uint(-INFINITY);
           }
         }
         float2 top = s[0], top2 = s[1];
 #pragma unroll
-        for (int i = 2; i + 3 < KT / 2; i += 4) {  // (three at a time is one instruction)
+        for (int i = 2; i + 3 < C::COLS / 2; i += 4) {  // (three at a time is one instruction)
           top.x = fmaxf(fmaxf(top.x, s[i].x), s[i + 1].x);
           top.y = fmaxf(fmaxf(top.y, s[i].y), s[i + 1].y);
           top2.x = fmaxf(fmaxf(top2.x, s[i + 2].x), s[i + 3].x);
           top2.y = fmaxf(fmaxf(top2.y, s[i + 2].y), s[i + 3].y);
         }
-        static_assert(KT / 2 % 4 == 0, "two pairs are left");
-        top.x = fmaxf(fmaxf(top.x, s[KT / 2 - 2].x), s[KT / 2 - 1].x);
-        top.y = fmaxf(fmaxf(top.y, s[KT / 2 - 2].y), s[KT / 2 - 1].y);
-        const float mx = fmaxf(fmaxf(top.x, top.y), fmaxf(top2.x, top2.y));
+        static_assert(C::COLS / 2 % 4 == 0, "two pairs are left");
+        top.x = fmaxf(fmaxf(top.x, s[C::COLS / 2 - 2].x), s[C::COLS / 2 - 1].x);
+        top.y = fmaxf(fmaxf(top.y, s[C::COLS / 2 - 2].y), s[C::COLS / 2 - 1].y);
+        float mx = fmaxf(fmaxf(top.x, top.y), fmaxf(top2.x, top2.y));
+        if (C::HALVES == 2) {
+          mx = fmaxf(mx, __uint_as_float(other(__float_as_uint(mx))));
+          if (!ok) return false;
+        }
         const float to_log2 = bend.capped || bend.biased ? 1.f : cs;
         if (C::QUANT) {
           // an exponent over the step's V scales
@@ -1124,7 +1197,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         if (rescale && !C::TWO && j > 0) {
           if (!ProductsDone()) return false;
 #pragma unroll 1
-          for (int k = 0; k < D; k += 32) {
+          for (int k = 0; k < C::DIMS; k += 32) {
             uint32_t o[32];
             TmemLoad32(a_o + k, o);
             TmemLoadWait();
@@ -1137,7 +1210,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         const float2 f2 = make_float2(to_log2, to_log2), less2 = make_float2(less, less);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int h = 0; h < KT; h += 32) {
+        for (int h = 0; h < C::COLS; h += 32) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1152,7 +1225,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             }
           }
           if (!C::QUANT) {
-            TmemStore16(a_s + h / 2, w);
+            TmemStore16(a_s + (col0 + h) / 2, w);
             if (C::TWO) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -1170,11 +1243,11 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
 #pragma unroll
           for (int gp = 0; gp < C::NG; ++gp) {
 #pragma unroll
-            for (int h = 0; h < KT; h += 32) {
+            for (int h = 0; h < C::COLS; h += 32) {
               uint32_t w[16], w2[16];
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                const float4 d = *reinterpret_cast<const float4*>(vs + gp * KT + h + i);
+                const float4 d = *reinterpret_cast<const float4*>(vs + gp * KT + col0 + h + i);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int k = h + i + 2 * e, at = i / 2 + e;
@@ -1190,7 +1263,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
                   }
                 }
               }
-              TmemStore16(a_s + gp * C::TERMS * 32 + h / 2, w);
+              TmemStore16(a_s + gp * C::TERMS * 32 + (col0 + h) / 2, w);
               if (C::TWO) TmemStore16(a_s + (gp * C::TERMS + 1) * 32 + h / 2, w2);
             }
           }
@@ -1208,7 +1281,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         s_parity ^= 1;
         FenceAfterSync();
         if (active) {
-          const int pos0 = it.base + (it.step0 + j) * KT;
+          const int pos0 = now.it->base + (now.it->step0 + j) * KT;
           const int from = min(max(seen.start - pos0, 0), KT), to = min(max(seen.end - pos0, 0), KT);  // columns seen
           const uint32_t bad = s_bad[(note0 + j) % kNotes];
           if (bad != 0 && from < to) {
@@ -1216,9 +1289,12 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             if (bad & ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u)) nan_row = true;
           }
           const float* scales = reinterpret_cast<const float*>(s_note + (note0 + j) % kScales * C::NOTE);
-          ok = __any_sync(0xFFFFFFFFu, valid && (from > 0 || to < KT)) ? step(std::true_type(), j, from, to, pos0, scales)
-                                                                       : step(std::false_type(), j, from, to, pos0, scales);
-          if (!ok) break;
+          const bool edge = __any_sync(0xFFFFFFFFu, valid && (from > 0 || to < KT));
+          if (!(edge ? step(std::true_type(), j, from - col0, to - col0, pos0, scales)
+                     : step(std::false_type(), j, from - col0, to - col0, pos0, scales))) {
+            ok = false;
+            break;
+          }
         }
         __syncwarp();
         if (lane == 0) MbarArrive(&bars.p_full[t]);
@@ -1227,7 +1303,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       // The next item's queries go into the place of this one's (whose products
       // with K are done) before this one's result is taken, so that the tensor
       // cores have work meanwhile.  (With two terms the registers do not hold both.)
-      RowState then;
+      RowState then{};
       more = ok && next_item(then);
       if (!C::TWO && more) write_q(then);
       // ---- the end of the item, or of this block's piece of it
@@ -1235,14 +1311,15 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
       FenceAfterSync();
       const int64_t row_head = static_cast<int64_t>(row) * p.n_heads + qh;
       const int64_t out = row * p.out_stride + static_cast<int64_t>(qh) * D;
-      const bool whole = it.begins && it.ends;
-      float* rec = RecordOf<C>(p, block, it.begins);
       if (nan_row || !ok) l = kvd::Nan();  // (a wait that gave up is not to pass for a result)
       if (active) {
+        const bool whole = now.it->begins && now.it->ends;
+        float* rec = RecordOf<C>(p, block, now.it->begins);
+        if (C::HALVES == 2) l += __uint_as_float(other(__float_as_uint(l)));
         const Join jn = valid && whole ? Join(p, row_head, ref, l) : Join(p, 0, 0.f, 0.f);
         float check = 0.f;
 #pragma unroll (C::TWO ? D / 32 : 1)
-        for (int k = 0; k < D; k += 32) {
+        for (int k = 0; k < C::DIMS; k += 32) {
           uint32_t o[32];
           TmemLoad32(a_o + k, o);
           TmemLoadWait();
@@ -1259,32 +1336,34 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             if (p.own != nullptr) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(p.own + row_head * D + k + i);
+                const float4 w = *reinterpret_cast<const float4*>(p.own + row_head * D + dim0 + k + i);
                 y[i] += jn.g * w.x;
                 y[i + 1] += jn.g * w.y;
                 y[i + 2] += jn.g * w.z;
                 y[i + 3] += jn.g * w.w;
               }
             }
-            Put32(p, out + k, y);
+            Put32(p, out + dim0 + k, y);
           } else if (valid) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               uint32_t w[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(y[i + e]);
-              kvd::Store32(rec + r * D + k + i, w);
+              kvd::Store32(rec + r * D + dim0 + k + i, w);
             }
           }
         }
-        if (valid && !whole) {
+        if (valid && !whole && half == 0) {
           rec[kItemRows * D + r] = ref;
           rec[kItemRows * (D + 1) + r] = l;
         }
         if (!C::QUANT) {
           // infinities and NaN: such rows again, by the formula
-          uint32_t again = __ballot_sync(0xFFFFFFFFu, valid && !nan_row && ok && !(check + l * 0.f == 0.f));
-          const int from = it.base + it.step0 * KT, to = from + steps * KT;
+          uint32_t bad = valid && !nan_row && ok && !(check + l * 0.f == 0.f);
+          if (C::HALVES == 2) bad |= other(bad);  // (and the other half's values are written)
+          uint32_t again = __ballot_sync(0xFFFFFFFFu, bad != 0 && half == 0 && ok);
+          const int from = now.it->base + now.it->step0 * KT, to = from + steps * KT;
 #pragma unroll 1
           while (again != 0) {
             const int w = __ffs(again) - 1;
@@ -1292,7 +1371,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
             const int start = __shfl_sync(0xFFFFFFFFu, seen.start, w), end = __shfl_sync(0xFFFFFFFFu, seen.end, w);
             constexpr int N = D / 32;
             float acc[N], pm, pl;
-            PlainRow<D, C::KIND>(p, it.table_row, it.head, __shfl_sync(0xFFFFFFFFu, row * p.q_stride + static_cast<int64_t>(qh) * D, w),
+            PlainRow<D, C::KIND>(p, now.it->table_row, now.it->head, __shfl_sync(0xFFFFFFFFu, row * p.q_stride + static_cast<int64_t>(qh) * D, w),
                                  __shfl_sync(0xFFFFFFFFu, slope, w), __shfl_sync(0xFFFFFFFFu, pos, w), max(start, from),
                                  min(end, to), acc, pm, pl);
             const int rr = __shfl_sync(0xFFFFFFFFu, r, w);
@@ -1317,6 +1396,7 @@ __global__ void __launch_bounds__(kThreads, 1) RowsKernel(const __grid_constant_
         }
       }
       FenceBeforeSync();  // (what was read of tensor memory, before the next item's products)
+      if (now.it != nullptr) Holder::Release(bars, first_item, now.it, lane);
       if (C::TWO && more) write_q(then);
       now = then;
     }
@@ -1439,6 +1519,9 @@ int Grid() {
   if (grid == 0) {
     int sms = 0;
     RPGB_CUDA(cudaFuncSetAttribute(RowsKernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    cudaFuncAttributes attr;
+    RPGB_CUDA(cudaFuncGetAttributes(&attr, RowsKernel<C>));
+    RPGB_CHECK(attr.numRegs == C::REGS, "kv: the rows kernel has %d registers a thread, not %d", attr.numRegs, C::REGS);
     RPGB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     grid = sms < kMaxBlocks ? sms : kMaxBlocks;
     grids[dev].store(grid, std::memory_order_release);
@@ -1454,7 +1537,7 @@ void Launch(const KvRowsParams& p, cudaStream_t s) {
     map_k = PlaneMap(p.kv, p.kv.k);
     map_v = PlaneMap(p.kv, p.kv.v);
   }
-  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(kThreads), C::SMEM, s, true, map_k, map_v,
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(C::THREADS), C::SMEM, s, true, map_k, map_v,
                    p, kvd::kMagic);
   LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, kJoinBlocks), dim3(256), 0, s, true, p);
 }
