@@ -168,7 +168,6 @@ constexpr int kLoadWarps = 2;
 constexpr int kMaxBlocks = 160;
 constexpr int kItems = 4;    // items described ahead
 constexpr int kNotes = 8;    // steps whose bad pages are held
-constexpr int kScales = 4;   // steps whose scales are held, as they come and as f32
 constexpr int kLeast = 2;    // steps that a block is started for
 constexpr int kHeadroom = 15, kSlack = 8;  // weights are at most 2^15, and 2^7 when their reference was set
 
@@ -193,17 +192,17 @@ struct Cfg {
   // Registers a thread at launch, and how the groups of four warps share them.
   static constexpr int REGS = HALVES == 1 ? 168 : 96, SOFT_REGS = HALVES == 1 ? 216 : 104, OTHER_REGS = HALVES == 1 ? 72 : 64;
   static_assert(32 * SOFT * SOFT_REGS + 128 * OTHER_REGS <= REGS * THREADS, "registers");
-  // Positions of a step.  128 where scores and weights of two tiles fit 256
-  // columns of tensor memory; codes take one product per 64-value group and two
-  // terms two, so 64 there (two terms over f16 at 128 spill: 135 -> 152 us for a
-  // prompt of 2811).
-  static constexpr int KT = QUANT || TWO ? 64 : 128;
+  static constexpr int KT = 64;  // positions of a step
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int COLS = KT / HALVES, DIMS = D / HALVES;  // positions and values of a thread
   static constexpr int BOX = D / 64;                  // 128-byte columns of a tile of f16
   static constexpr int QTERM = BOX * kTileRows * 128, QTILE = TERMS * QTERM;
   static constexpr int PLANE = BOX * KT * 128;
-  static constexpr int STAGES = QUANT && !TWO ? 3 : 2;
+  // Buffers for a tile's scores: 128 columns of tensor memory are there, and a step
+  // takes 64 for each group of values that has its own scale.
+  static constexpr int BUFS = NG == 1 ? 2 : 1;
+  static constexpr int STAGES = QUANT ? (TWO && D == 128 ? 2 : 3) : (TWO ? 3 : 4);
+  static constexpr int SCALES = BUFS == 2 ? 8 : 4;  // steps whose scales are held, as they come and as f32
   static constexpr int LAG = QUANT && !TWO ? 4 : 2;  // copies of codes begun before the oldest is waited for
   static constexpr int ROW = KIND == KvType::kF16 ? 2 * D : (KIND == KvType::kQ8 ? D : D / 2);
   static constexpr int CPR = ROW / 16;
@@ -215,9 +214,9 @@ struct Cfg {
   // for when the work is dealt.  Codes, 16 prompts of 1024 with 1, 2, 3, 4 and 6:
   // 341, 332, 335, 347, 359 us; f16, 4 of 4096 with 2, 4 and 6: 474, 460, 467; two
   // terms, a prompt of 2811 with 3, 5 and 8: 143, 134, 135.
-  static constexpr int BORDER = TWO ? 5 : (QUANT ? 2 : 4);
-  static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + kScales * (SCALE + NOTE);
-  static_assert(SMEM <= 230 * 1024, "shared memory");
+  static constexpr int BORDER = TWO ? 5 : (QUANT ? 2 : 8);
+  static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + SCALES * (SCALE + NOTE);
+  static_assert(SMEM <= 226 * 1024, "shared memory");
 };
 
 struct Item {
@@ -358,19 +357,31 @@ constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t DescRows(uint32_t a) { return a >> 4 | 1u << 16; }
 // V: the sum runs over rows, and the next 64 values are `box` bytes on.
 __device__ __forceinline__ uint32_t DescV(uint32_t a, int box) { return a >> 4 | static_cast<uint32_t>(box >> 4) << 16; }
+// Products are issued by one elected lane of a warp that stays together: their
+// operands are in uniform registers then.  In a branch of one lane each of them
+// waits for its operands to be moved there (4 prompts of 4096 over f16 561 -> 433 us,
+// 16 of 1024 over 8 bits 330 -> 307).
 __device__ __forceinline__ void MmaSs(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
       "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(kDescHigh)
       : "memory");
 }
 // A in tensor memory.
 __device__ __forceinline__ void MmaTs(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
       "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void Commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(dev::SmemAddr(bar))
       : "memory");
 }
 // A value that is worked out here and not kept over loops (32 of them would be spilled).
@@ -383,8 +394,8 @@ __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return kvd::H
 // ------------------------------------------------------------------ kernel
 
 struct Bars {
-  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
-  uint64_t s_full[2], p_full[2], q_full[2], pv_done[2];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2];  // [tile][buffer], [tile]
   uint64_t item_full[kItems], item_empty[kItems], fin;
   uint64_t pair[8];  // of the two warps that have the halves of 32 rows
 };
@@ -560,7 +571,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
   __shared__ Bars bars;
   __shared__ Item items[kItems];
   __shared__ uint32_t s_tmem, s_bad[kNotes], s_pair[2][2][2 * kTileRows];
-  __shared__ int2 s_seen[kLoadWarps][kScales];  // a warp's own notes of what a step's rows see
+  __shared__ int2 s_seen[kLoadWarps][C::SCALES];  // a warp's own notes of what a step's rows see
   __shared__ long long s_part[C::THREADS / 32], s_before;
   __shared__ int s_slot;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -569,8 +580,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
   char* s_v = s_k + C::STAGES * C::PLANE;
   char* s_raw = s_v + C::STAGES * C::PLANE;
   char* s_scale = s_raw + (C::LAG + 1) * C::RAW;
-  char* s_note = s_scale + kScales * C::SCALE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  char* s_note = s_scale + C::SCALES * C::SCALE;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
   const Split sp(p);
 
   if (warp == 0) TmemAlloc(&s_tmem, 512u);
@@ -582,9 +593,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       dev::MbarInit(&bars.v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      dev::MbarInit(&bars.s_full[i], 1);
-      dev::MbarInit(&bars.pv_done[i], 1);
-      dev::MbarInit(&bars.p_full[i], C::SOFT / 2);
+      for (int b = 0; b < 2; ++b) {
+        dev::MbarInit(&bars.s_full[i][b], 1);
+        dev::MbarInit(&bars.pv_done[i][b], 1);
+        dev::MbarInit(&bars.p_full[i][b], C::SOFT / 2);
+      }
       dev::MbarInit(&bars.q_full[i], C::SOFT / 2);
     }
     for (int i = 0; i < kItems; ++i) {
@@ -623,7 +636,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
   FenceBeforeSync();
   __syncthreads();
   FenceAfterSync();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, s_tmem, 0);
   long long before = incl - mine, per_head = 0;
 #pragma unroll 1
   for (int w = 0; w < C::THREADS / 32; ++w) {
@@ -656,7 +669,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         sl.Seek(p, sp, slot);
       }
       bool ok = true;
-  #pragma unroll 1
+#pragma unroll 1
       for (bool more = true; more && ok;) {
         Item it;
         it.steps = 0;
@@ -707,7 +720,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         const int size = p.type == ElemType::kF32 ? 4 : 2;
         const int heads = it.steps > 0 ? min(sp.per, sp.group - it.chunk * sp.per) : 0;
         const int lines = (heads * D * size + 127) / 128;
-  #pragma unroll 1
+#pragma unroll 1
         for (int k = lane; k < it.n_tok * lines; k += 32) {
           const int64_t at = (it.row0 + k / lines) * p.q_stride + static_cast<int64_t>(it.head * sp.group + it.chunk * sp.per) * D;
           asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.q) + at * size + k % lines * 128));
@@ -715,81 +728,91 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       }
       if (lane == 0) static_cast<Job*>(p.workspace)[block] = job;
     } else if (warp == C::MMA) {
-      // ---- products: per step and tile O += P V of the step before, then S = Q K^T
-      if (lane == 0) {
+      // ---- products: per step and tile S = Q K^T, and O += P V of the step before.
+      // With two buffers the scores come first, so that they are there when the
+      // softmax is done with those before; their buffer had the weights of two
+      // steps ago, whose product is issued.
+      {
         constexpr uint32_t id_s = InstrDesc(128, KT);
         constexpr uint32_t id_o = InstrDesc(128, C::NG == 1 ? D : 64) | 1u << 16;  // (V: values contiguous)
         const uint32_t a_q = dev::SmemAddr(s_q), a_k = dev::SmemAddr(s_k), a_v = dev::SmemAddr(s_v);
         int n = 0;
-        uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
-        int c = 0;  // steps so far
+        uint32_t q_parity = 0;
+        int c = 0, ct0 = 0, ct1 = 0;  // steps so far, and those of each tile
         bool ok = true;
-  #pragma unroll 1
+#pragma unroll 1
         while (ok) {
           const int i = n % kItems;
-          if (!Wait(&bars.item_full[i], (n / kItems) & 1)) break;
-          const int steps = items[i].steps, rows = items[i].n_tok * sp.per;
-          MbarArrive(&bars.item_empty[i]);
+          if (!__all_sync(0xFFFFFFFFu, Wait(&bars.item_full[i], (n / kItems) & 1))) break;
+          const int steps = __shfl_sync(0xFFFFFFFFu, items[i].steps, 0);
+          const int rows = __shfl_sync(0xFFFFFFFFu, items[i].n_tok * sp.per, 0);
+          if (lane == 0) MbarArrive(&bars.item_empty[i]);
+          __syncwarp();
           ++n;
           if (steps <= 0) break;
           const int tiles = rows > kTileRows ? 2 : 1;
-  #pragma unroll 1
+#pragma unroll 1
           for (int j = 0; j <= steps && ok; ++j) {
-  #pragma unroll 1
+#pragma unroll 1
             for (int t = 0; t < tiles && ok; ++t) {
-              if (j > 0) {
-                const int st = (c + j - 1) % C::STAGES, par = ((c + j - 1) / C::STAGES) & 1;
-                ok = (t > 0 || Wait(&bars.v_full[st], par)) && Wait(&bars.p_full[t], p_parity[t]);
-                if (!ok) break;
-                p_parity[t] ^= 1;
+              auto pv = [&]() {
+                const int n = c + j - 1, st = n % C::STAGES, nt = (t == 0 ? ct0 : ct1) + j - 1, buf = nt % C::BUFS;
+                ok = __all_sync(0xFFFFFFFFu, (t > 0 || Wait(&bars.v_full[st], (n / C::STAGES) & 1)) &&
+                                                 Wait(&bars.p_full[t][buf], (nt / C::BUFS) & 1));
+                if (!ok) return;
                 FenceAfterSync();
-                const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128;
+                const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128 + buf * 64;
                 // with two terms every step's product starts anew (it is added up in registers)
                 const bool going_on = !C::TWO && j > 1;
-  #pragma unroll
+#pragma unroll
                 for (int g = 0; g < C::NG; ++g) {
-  #pragma unroll
+#pragma unroll
                   for (int term = C::TERMS - 1; term >= 0; --term) {
-                    const uint32_t v = Here(DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
-                    const uint32_t a = Here(w + (g * C::TERMS + term) * (KT / 2)), d = Here(o + 64 * g);
-  #pragma unroll
+                    const uint32_t v = (DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
+                    const uint32_t a = (w + (g * C::TERMS + term) * (KT / 2)), d = (o + 64 * g);
+#pragma unroll
                     for (int k = 0; k < KT / 16; ++k) {
                       MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
                     }
                   }
                 }
-                MmaCommit(&bars.pv_done[t]);
-                if (t == tiles - 1) MmaCommit(&bars.v_empty[st]);
-              }
-              if (j < steps) {
-                const int st = (c + j) % C::STAGES, par = ((c + j) / C::STAGES) & 1;
-                ok = (j > 0 || Wait(&bars.q_full[t], q_parity[t])) &&
-                     (t > 0 || Wait(&bars.k_full[st], par));
-                if (!ok) break;
-                if (j == 0) q_parity[t] ^= 1;
+                Commit(&bars.pv_done[t][buf]);
+                if (t == tiles - 1) Commit(&bars.v_empty[st]);
+              };
+              auto qk = [&]() {
+                const int n = c + j, st = n % C::STAGES, buf = ((t == 0 ? ct0 : ct1) + j) % C::BUFS;
+                ok = __all_sync(0xFFFFFFFFu, (j > 0 || Wait(&bars.q_full[t], q_parity >> t & 1)) &&
+                                                 (t > 0 || Wait(&bars.k_full[st], (n / C::STAGES) & 1)));
+                if (!ok) return;
+                if (j == 0) q_parity ^= 1u << t;
                 FenceAfterSync();
                 // (second terms first: the sums that the tensor cores cut short are small then)
-  #pragma unroll
+#pragma unroll
                 for (int term = C::TERMS - 1; term >= 0; --term) {
-  #pragma unroll
+#pragma unroll
                   for (int box = 0; box < C::BOX; ++box) {
-                    const uint32_t d = Here(tmem + t * 128 + (C::NG == 2 ? 64 * box : 0));
-                    const uint32_t q = Here(DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
-                    const uint32_t kk = Here(DescRows(a_k + st * C::PLANE + box * (KT * 128)));
-  #pragma unroll
+                    const uint32_t d = (tmem + t * 128 + (C::NG == 2 ? 64 * box : 64 * buf));
+                    const uint32_t q = (DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
+                    const uint32_t kk = (DescRows(a_k + st * C::PLANE + box * (KT * 128)));
+#pragma unroll
                     for (int k = 0; k < 4; ++k) {
                       MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
                     }
                   }
                 }
-                MmaCommit(&bars.s_full[t]);
-                if (t == tiles - 1) MmaCommit(&bars.k_empty[st]);
-              }
+                Commit(&bars.s_full[t][buf]);
+                if (t == tiles - 1) Commit(&bars.k_empty[st]);
+              };
+              if (C::BUFS == 2 && j < steps) qk();
+              if (ok && j > 0) pv();
+              if (C::BUFS == 1 && ok && j < steps) qk();
             }
           }
           c += steps;
+          ct0 += steps;
+          if (tiles == 2) ct1 += steps;
         }
-        MmaCommit(&bars.fin);  // no product is under way when the block ends
+        Commit(&bars.fin);  // no product is under way when the block ends
         Wait(&bars.fin, 0);
       }
       __syncwarp();
@@ -813,12 +836,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         }
         const char* raw = s_raw + ended % (C::LAG + 1) * C::RAW + lt * 16;
         char* dst = (v ? s_v : s_k) + st * C::PLANE;
-  #pragma unroll 2
+#pragma unroll 2
         for (int i = 0; i < C::PER; ++i) {
           const int r = r0 + i * kRowStep;
           const uint4 w = *reinterpret_cast<const uint4*>(raw + i * (32 * kLoadWarps * 16));
           constexpr int kHalves = C::KIND == KvType::kQ8 ? 1 : 2;  // runs of 16 values
-  #pragma unroll
+#pragma unroll
           for (int h = 0; h < kHalves; ++h) {
             kvd::Codes16<C::KIND> code;
             if (C::KIND == KvType::kQ8) {
@@ -841,10 +864,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         if (!v) {
           // the scales that this warp copied, group after group; 0 where no row sees the position
           __syncwarp();
-          const int2 seen = s_seen[lw][step % kScales];
-          const __half* h = reinterpret_cast<const __half*>(s_scale + step % kScales * C::SCALE + lw * (C::SCALE / 2));
-          float* f = reinterpret_cast<float*>(s_note + step % kScales * C::NOTE + lw * (C::NOTE / 2));
-  #pragma unroll 1
+          const int2 seen = s_seen[lw][step % C::SCALES];
+          const __half* h = reinterpret_cast<const __half*>(s_scale + step % C::SCALES * C::SCALE + lw * (C::SCALE / 2));
+          float* f = reinterpret_cast<float*>(s_note + step % C::SCALES * C::NOTE + lw * (C::NOTE / 2));
+#pragma unroll 1
           for (int i = lane; i < KT * C::NG; i += 32) {
             const int pos = i / C::NG;
             f[i % C::NG * KT + pos] = pos >= seen.x && pos < seen.y ? __half2float(h[i]) : 0.f;
@@ -857,7 +880,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       };
       Reader rd;
       Item it;
-  #pragma unroll 1
+#pragma unroll 1
       while (ok && rd.Next(bars, items, it, lane)) {
         // lane g has to do with positions 16 g .. 16 g + 15 of a step: their page
         auto lookup = [&](int pos) {
@@ -866,7 +889,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
                      : -1;
         };
         int next = lookup(it.base + it.step0 * KT + 16 * lane);
-  #pragma unroll 1
+#pragma unroll 1
         for (int j = 0; j < it.steps && ok; ++j) {
           const int pos0 = it.base + (it.step0 + j) * KT, at = pos0 + 16 * lane;
           const int page = next;
@@ -877,7 +900,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
           const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
           const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
           if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
-          if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % kScales] = make_int2(it.lo - pos0, it.hi - pos0);
+          if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % C::SCALES] = make_int2(it.lo - pos0, it.hi - pos0);
           if (!C::QUANT) {
             // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
             const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
@@ -885,7 +908,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
             const uint32_t groups = kEvery << lw;
             const int g = lw + 2 * (lane / C::BOX), box = lane % C::BOX;
             const int pg = __shfl_sync(0xFFFFFFFFu, page, g & 31), in = (pos0 + 16 * g) & mask;
-  #pragma unroll 1
+#pragma unroll 1
             for (int v = 0; v < 2; ++v) {
               const int st = (begun >> 1) % C::STAGES;
               uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
@@ -898,12 +921,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
               uint32_t rest = v ? groups & ~full : 0;
               if (rest != 0) {
                 // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
-  #pragma unroll 1
+#pragma unroll 1
                 while (rest != 0) {
                   const int q = __ffs(rest) - 1;
                   rest &= rest - 1;
                   const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
-  #pragma unroll 1
+#pragma unroll 1
                   for (int i = lane; i < 16 * C::CPR; i += 32) {
                     const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
                     const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
@@ -925,12 +948,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
             }
             ended = begun;
           } else {
-  #pragma unroll 1
+#pragma unroll 1
             for (int v = 0; v < 2 && ok; ++v) {
               const char* plane = (v ? p.kv.v : p.kv.k) + c0 * 16;
               const uint32_t dst = a_raw + begun % (C::LAG + 1) * C::RAW + lt * 16;
               // 16 positions at a time: rows r0 + k * kRowStep of them are this thread's
-  #pragma unroll 1
+#pragma unroll 1
               for (int g = 0; g < KT / 16; ++g) {
                 const char* src = plane + __shfl_sync(0xFFFFFFFFu, off, g);
                 const bool have_g = (have >> g) & 1;
@@ -943,7 +966,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
                   constexpr int kSkip = kRowStep > 16 ? kRowStep / 16 : 1;
                   if ((r0 >> 4) == g % kSkip) copy(dst + g / kSkip * (32 * kLoadWarps * 16), r0 & 15);
                 } else {
-  #pragma unroll
+#pragma unroll
                   for (int k = 0; k < 16 / kRowStep; ++k) copy(dst + g * (16 * C::ROW) + k * (kRowStep * C::ROW), r0 + k * kRowStep);
                 }
               }
@@ -956,7 +979,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
                 if (lane < KT / 16 * kPer) {
                   const bool in = (have >> i) & 1;
                   const char* src = lw == 0 ? p.kv.k_scale : p.kv.v_scale;
-                  CopyAsync16(a_scale + (begun >> 1) % kScales * C::SCALE + lw * (C::SCALE / 2) + lane * 16, in ? src + o : src, in);
+                  CopyAsync16(a_scale + (begun >> 1) % C::SCALES * C::SCALE + lw * (C::SCALE / 2) + lane * 16, in ? src + o : src, in);
                 }
               }
               CopyCommit();
@@ -988,9 +1011,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
     const int in_tile = (warp & 3) * 32 + lane, r = t * kTileRows + in_tile;
     const int col0 = half * C::COLS, dim0 = half * C::DIMS;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t a_s = lanes + t * 128, a_o = lanes + 256 + t * 128 + dim0;
-    uint32_t s_parity = 0, pair_parity = 0;
-    int c = 0, note = 0;  // products with V begun for this tile; steps so far
+    const uint32_t a_t = lanes + t * 128, a_o = lanes + 256 + t * 128 + dim0;
+    uint32_t pair_parity = 0;
+    int c = 0, note = 0;  // steps so far, of this tile and all
     bool ok = true;
     // What the thread with the row's other half has in its place.
     auto other = [&](uint32_t v) -> uint32_t {
@@ -1078,13 +1101,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         for (int i = 0; i < D / 2; ++i) acc[i % (C::TWO ? D / 2 : 1)] = make_float2(0.f, 0.f);
       }
       auto ProductsDone = [&]() {  // those with V of the last step
-        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t], (c - 1) & 1))) return false;
+        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t][(c - 1) % C::BUFS], ((c - 1) / C::BUFS) & 1))) return false;
         FenceAfterSync();
         return true;
       };
       // Softmax of a step's scores, weights into tensor memory.  EDGE: some row of the warp does not see all positions.
       auto step = [&](auto edge, int j, int from, int to, int pos0, const float* scales) {
         constexpr bool EDGE = decltype(edge)::value;
+        const uint32_t a_s = a_t + c % C::BUFS * 64;
         if (C::TWO && j > 0) {
           if (!ProductsDone()) return false;  // (they came before these scores)
 #pragma unroll
@@ -1274,11 +1298,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       };
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.s_full[t], s_parity))) {
+        if (!__all_sync(0xFFFFFFFFu, Wait(&bars.s_full[t][c % C::BUFS], (c / C::BUFS) & 1))) {
           ok = false;
           break;
         }
-        s_parity ^= 1;
         FenceAfterSync();
         if (active) {
           const int pos0 = now.it->base + (now.it->step0 + j) * KT;
@@ -1288,7 +1311,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
             // columns from .. to - 1 in units of 16
             if (bad & ((2u << ((to - 1) >> 4)) - 1u) & ~((1u << (from >> 4)) - 1u)) nan_row = true;
           }
-          const float* scales = reinterpret_cast<const float*>(s_note + (note0 + j) % kScales * C::NOTE);
+          const float* scales = reinterpret_cast<const float*>(s_note + (note0 + j) % C::SCALES * C::NOTE);
           const bool edge = __any_sync(0xFFFFFFFFu, valid && (from > 0 || to < KT));
           if (!(edge ? step(std::true_type(), j, from - col0, to - col0, pos0, scales)
                      : step(std::false_type(), j, from - col0, to - col0, pos0, scales))) {
@@ -1297,7 +1320,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
           }
         }
         __syncwarp();
-        if (lane == 0) MbarArrive(&bars.p_full[t]);
+        if (lane == 0) MbarArrive(&bars.p_full[t][c % C::BUFS]);
         ++c;
       }
       // The next item's queries go into the place of this one's (whose products
@@ -1307,7 +1330,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       more = ok && next_item(then);
       if (!C::TWO && more) write_q(then);
       // ---- the end of the item, or of this block's piece of it
-      if (ok && steps > 0 && !__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t], (c - 1) & 1))) ok = false;
+      if (ok && steps > 0 && !__all_sync(0xFFFFFFFFu, Wait(&bars.pv_done[t][(c - 1) % C::BUFS], ((c - 1) / C::BUFS) & 1))) ok = false;
       FenceAfterSync();
       const int64_t row_head = static_cast<int64_t>(row) * p.n_heads + qh;
       const int64_t out = row * p.out_stride + static_cast<int64_t>(qh) * D;
