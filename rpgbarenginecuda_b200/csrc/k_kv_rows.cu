@@ -1,5 +1,48 @@
 // k_kv_rows.cu -- attention of several rows that read one page list: new tokens
 // of a conversation, or the conversations of a group over what they share.
+//
+// Row r, query head h: o = sum_j w_j V_j / sum_j w_j, w_j = 2^(s_j - ref), over the
+// positions j that the row sees, s_j = bend(scale q . K_j) log2(e), ref a bound that
+// follows the largest score (it moves when a weight would pass 2^15, by as much as
+// brings it to 2^7; the result so far is scaled then).  Sums and results are f32.
+// Where a call also has attention over other positions (own, own_lse) the two are
+// added with the weights 2^lse.
+//
+// Rows times the heads of a KV head are the rows of two 128-row tiles, so every
+// position is read once for up to 256 rows, and both products are tcgen05 ones:
+// S = Q K^T from shared memory, O += P V with P in tensor memory (in the columns
+// that had S).  An item is such a pair of tiles and the positions that any of its
+// rows sees, in steps of 64.  All items' steps are dealt to one block an SM in equal
+// shares, whatever the lists' lengths; what begins or ends inside a block's share
+// leaves its result, reference and sum as a record, and RowsJoinKernel adds the
+// records of an item up in block order (no atomics: calls repeat bit by bit).
+//
+// Operands of the products are f16.  f16 queries go in as they are, bf16 and f32
+// ones times a power of two a row; an f32 row is two f16 terms, hi + lo, which leave
+// 2^-22 of it, as are its weights: errors of 6e-7 of the largest value (2^-11 with
+// one term).  Codes are exact in f16; K's scale
+// multiplies the scores and V's the weights, per 64-value group.  Rows where
+// infinities or NaN of an f16 cache reach the result are worked out again one by
+// one (PlainRow): a product with a tile's other columns would spread them.
+//
+// Warps: 8 or 16 have the softmax, one issues the products, one deals items, two
+// copy (f16 pages by TMA; codes by cp.async, spread to f16 on the way from one
+// place in shared memory to another).  Registers are shared out between them
+// by setmaxnreg.
+//
+// What bounds it: 4 prompts of 4096 over f16, 32 heads of 8 KV heads, bf16: 423 us,
+// 730 TFLOP/s of the pairs that are seen.  A step of a tile takes its softmax warps
+// some 1400 cycles (exponentials 700 of them, 16 a cycle an SM; reading the scores
+// 250, the largest 230, storing weights 80), the two tiles of a block run side by
+// side on the same four schedulers, and an item's beginning and end add 400 a step
+// at 9 steps an item; the tensor cores are at 40 %.  Over codes it is the spreading
+// (16 prompts of 1024 over 8 bits 308 us) and, with few steps a block, what a launch
+// costs: the pair of kernels 4 us, the plan 1.6, the roles' first instructions 3.
+//
+// Tried and not kept, 4 prompts of 4096 at the time: a part of the exponentials as
+// polynomials, weights in two halves so that their product begins earlier, results
+// through shared memory for whole lines (each slower); mixed f32 + f16 additions for
+// the sum (423 -> 422).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -180,19 +223,22 @@ struct Cfg {
   static constexpr int TERMS = TWO ? 2 : 1;
   // Warps of the softmax: four to a tile and half.  Over codes with one term two
   // threads share a row, half of the positions and half of the values each: what a
-  // thread does in turn, one after the other, is what bounds a step there (16 prompts
-  // of 1024 over 8 bits 367 -> 333 us, 6 of 1501 over 4 bits 205 -> 158; the few
-  // steps of 64 rows over a prefix of 4096 lose, 62 -> 67).  An f16 cache has 64
-  // scores a thread in this form, more than 104 registers hold (4 prompts of 4096
-  // 460 -> 689).  With two terms the row's result stays in registers, which takes
-  // all of one thread's.
+  // thread does in turn is what bounds a step there (16 prompts
+  // of 1024 over 8 bits 324 -> 308 us, 6 of 1501 over 4 bits 171 -> 145; 64 rows over
+  // a prefix of 4096, few steps a block, lose, 60 -> 65).  An f16 cache
+  // keeps a thread per row (4 prompts of 4096 423 us; 473 with two, whose exchange of
+  // the row's largest score costs more than the shorter turn gives).  With two terms
+  // the row's result stays in registers, which takes all of one thread's.
   static constexpr int HALVES = QUANT && !TWO ? 2 : 1;
   static constexpr int SOFT = 8 * HALVES, MMA = SOFT, DEAL = SOFT + 1, LOAD = SOFT + 2, WARPS = LOAD + kLoadWarps;
   static constexpr int THREADS = 32 * WARPS;
   // Registers a thread at launch, and how the groups of four warps share them.
   static constexpr int REGS = HALVES == 1 ? 168 : 96, SOFT_REGS = HALVES == 1 ? 216 : 104, OTHER_REGS = HALVES == 1 ? 72 : 64;
   static_assert(32 * SOFT * SOFT_REGS + 128 * OTHER_REGS <= REGS * THREADS, "registers");
-  static constexpr int KT = 64;  // positions of a step
+  // Positions of a step.  With 128 a tile's scores take all of its 128 columns of
+  // tensor memory and the softmax waits for every product (4 prompts of 4096 over
+  // f16 460 us, 423 with 64 and two buffers).
+  static constexpr int KT = 64;
   static constexpr int NG = QUANT ? D / kKvGroup : 1;
   static constexpr int COLS = KT / HALVES, DIMS = D / HALVES;  // positions and values of a thread
   static constexpr int BOX = D / 64;                  // 128-byte columns of a tile of f16
@@ -212,7 +258,7 @@ struct Cfg {
   static constexpr int NOTE = 2 * SCALE;                     // the same as f32, [K or V][group][position]
   // Steps that the beginning and end of an item (its queries, its result) count
   // for when the work is dealt.  Codes, 16 prompts of 1024 with 1, 2, 3, 4 and 6:
-  // 341, 332, 335, 347, 359 us; f16, 4 of 4096 with 2, 4 and 6: 474, 460, 467; two
+  // 341, 332, 335, 347, 359 us; f16, 4 of 4096 with 4, 8 and 12: 430, 418, 431; two
   // terms, a prompt of 2811 with 3, 5 and 8: 143, 134, 135.
   static constexpr int BORDER = TWO ? 5 : (QUANT ? 2 : 8);
   static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + SCALES * (SCALE + NOTE);
@@ -284,7 +330,8 @@ struct Slots {
       it.hi = static_cast<int>(min(static_cast<int64_t>(max(p.ends[it.row0 + it.n_tok - 1], 0)), cap));
     }
     if (it.lo >= it.hi) it.lo = it.hi = 0;
-    it.base = it.lo & ~15;
+    // (an f16 cache's steps begin where pages of as many positions do)
+    it.base = it.lo & ~(!C::QUANT && 1 << p.kv.page_log2 >= C::KT ? C::KT - 1 : 15);
     return max(1, (it.hi - it.base + C::KT - 1) / C::KT);
   }
 };
@@ -316,13 +363,13 @@ __device__ __forceinline__ bool Wait(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
-// 16 positions of 64 values of a head's page.
-__device__ __forceinline__ void LoadTile(void* dst, const CUtensorMap* map, int value, int at, int head, int page,
+// Positions at .. of a head's page, from its `box`th 64 values on: as many as the map's boxes have.
+__device__ __forceinline__ void LoadTile(void* dst, const CUtensorMap* map, int at, int box, int head, int page,
                                          uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dev::SmemAddr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(value), "r"(at), "r"(head), "r"(page), "r"(dev::SmemAddr(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::
+          "r"(dev::SmemAddr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(at), "r"(box), "r"(head), "r"(page), "r"(dev::SmemAddr(bar))
       : "memory");
 }
 __device__ __forceinline__ void TmemLoad32(uint32_t a, uint32_t* r) {
@@ -383,11 +430,6 @@ __device__ __forceinline__ void Commit(uint64_t* bar) {
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\t"
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(dev::SmemAddr(bar))
       : "memory");
-}
-// A value that is worked out here and not kept over loops (32 of them would be spilled).
-__device__ __forceinline__ uint32_t Here(uint32_t x) {
-  asm volatile("" : "+r"(x));
-  return x;
 }
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return kvd::HalfBits(__floats2half2_rn(lo, hi)); }
 
@@ -561,9 +603,13 @@ struct RowState {
   bool valid, active, is_nan;  // active: some row of the warp is valid
 };
 
+// An f16 cache's planes, in boxes of 16 positions and 64 values and, where pages hold them, of whole steps.
+struct Maps {
+  CUtensorMap k, v, step_k, step_v;
+};
+
 template <typename C>
-__global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constant__ CUtensorMap map_k,
-                                                            const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constant__ Maps maps,
                                                             const KvRowsParams p, uint32_t magic) {
   using namespace tc;
   constexpr int D = C::D, KT = C::KT;
@@ -587,8 +633,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
   if (warp == 0) TmemAlloc(&s_tmem, 512u);
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) {
-      dev::MbarInit(&bars.k_full[i], kLoadWarps);
-      dev::MbarInit(&bars.v_full[i], kLoadWarps);
+      dev::MbarInit(&bars.k_full[i], C::QUANT ? kLoadWarps : 1);
+      dev::MbarInit(&bars.v_full[i], C::QUANT ? kLoadWarps : 1);
       dev::MbarInit(&bars.k_empty[i], 1);
       dev::MbarInit(&bars.v_empty[i], 1);
     }
@@ -753,59 +799,68 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
           const int tiles = rows > kTileRows ? 2 : 1;
 #pragma unroll 1
           for (int j = 0; j <= steps && ok; ++j) {
-#pragma unroll 1
-            for (int t = 0; t < tiles && ok; ++t) {
-              auto pv = [&]() {
-                const int n = c + j - 1, st = n % C::STAGES, nt = (t == 0 ? ct0 : ct1) + j - 1, buf = nt % C::BUFS;
-                ok = __all_sync(0xFFFFFFFFu, (t > 0 || Wait(&bars.v_full[st], (n / C::STAGES) & 1)) &&
-                                                 Wait(&bars.p_full[t][buf], (nt / C::BUFS) & 1));
-                if (!ok) return;
-                FenceAfterSync();
-                const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128 + buf * 64;
-                // with two terms every step's product starts anew (it is added up in registers)
-                const bool going_on = !C::TWO && j > 1;
+            auto pv = [&](int t) {
+              const int n = c + j - 1, st = n % C::STAGES, nt = (t == 0 ? ct0 : ct1) + j - 1, buf = nt % C::BUFS;
+              ok = __all_sync(0xFFFFFFFFu, (t > 0 || Wait(&bars.v_full[st], (n / C::STAGES) & 1)) &&
+                                               Wait(&bars.p_full[t][buf], (nt / C::BUFS) & 1));
+              if (!ok) return;
+              FenceAfterSync();
+              const uint32_t o = tmem + 256 + t * 128, w = tmem + t * 128 + buf * 64;
+              // with two terms every step's product starts anew (it is added up in registers)
+              const bool going_on = !C::TWO && j > 1;
 #pragma unroll
-                for (int g = 0; g < C::NG; ++g) {
-#pragma unroll
-                  for (int term = C::TERMS - 1; term >= 0; --term) {
-                    const uint32_t v = (DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128));
-                    const uint32_t a = (w + (g * C::TERMS + term) * (KT / 2)), d = (o + 64 * g);
-#pragma unroll
-                    for (int k = 0; k < KT / 16; ++k) {
-                      MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
-                    }
-                  }
-                }
-                Commit(&bars.pv_done[t][buf]);
-                if (t == tiles - 1) Commit(&bars.v_empty[st]);
-              };
-              auto qk = [&]() {
-                const int n = c + j, st = n % C::STAGES, buf = ((t == 0 ? ct0 : ct1) + j) % C::BUFS;
-                ok = __all_sync(0xFFFFFFFFu, (j > 0 || Wait(&bars.q_full[t], q_parity >> t & 1)) &&
-                                                 (t > 0 || Wait(&bars.k_full[st], (n / C::STAGES) & 1)));
-                if (!ok) return;
-                if (j == 0) q_parity ^= 1u << t;
-                FenceAfterSync();
-                // (second terms first: the sums that the tensor cores cut short are small then)
+              for (int g = 0; g < C::NG; ++g) {
 #pragma unroll
                 for (int term = C::TERMS - 1; term >= 0; --term) {
+                  const uint32_t v = DescV(a_v + st * C::PLANE + g * (KT * 128), KT * 128);
+                  const uint32_t a = w + (g * C::TERMS + term) * (KT / 2), d = o + 64 * g;
 #pragma unroll
-                  for (int box = 0; box < C::BOX; ++box) {
-                    const uint32_t d = (tmem + t * 128 + (C::NG == 2 ? 64 * box : 64 * buf));
-                    const uint32_t q = (DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128)));
-                    const uint32_t kk = (DescRows(a_k + st * C::PLANE + box * (KT * 128)));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                      MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
-                    }
+                  for (int k = 0; k < KT / 16; ++k) {
+                    MmaTs(d, a + 8 * k, v + k * (2048 >> 4), id_o, k > 0 || term < C::TERMS - 1 || going_on);
                   }
                 }
-                Commit(&bars.s_full[t][buf]);
-                if (t == tiles - 1) Commit(&bars.k_empty[st]);
-              };
-              if (C::BUFS == 2 && j < steps) qk();
-              if (ok && j > 0) pv();
-              if (C::BUFS == 1 && ok && j < steps) qk();
+              }
+              Commit(&bars.pv_done[t][buf]);
+              if (t == tiles - 1) Commit(&bars.v_empty[st]);
+            };
+            auto qk = [&](int t) {
+              const int n = c + j, st = n % C::STAGES, buf = ((t == 0 ? ct0 : ct1) + j) % C::BUFS;
+              ok = __all_sync(0xFFFFFFFFu, (j > 0 || Wait(&bars.q_full[t], q_parity >> t & 1)) &&
+                                               (t > 0 || Wait(&bars.k_full[st], (n / C::STAGES) & 1)));
+              if (!ok) return;
+              if (j == 0) q_parity ^= 1u << t;
+              FenceAfterSync();
+              // (second terms first: the sums that the tensor cores cut short are small then)
+#pragma unroll
+              for (int term = C::TERMS - 1; term >= 0; --term) {
+#pragma unroll
+                for (int box = 0; box < C::BOX; ++box) {
+                  const uint32_t d = tmem + t * 128 + (C::NG == 2 ? 64 * box : 64 * buf);
+                  const uint32_t q = DescRows(a_q + t * C::QTILE + term * C::QTERM + box * (kTileRows * 128));
+                  const uint32_t kk = DescRows(a_k + st * C::PLANE + box * (KT * 128));
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    MmaSs(d, q + 2 * k, kk + 2 * k, id_s, k > 0 || term < C::TERMS - 1 || (C::NG == 1 && box > 0));
+                  }
+                }
+              }
+              Commit(&bars.s_full[t][buf]);
+              if (t == tiles - 1) Commit(&bars.k_empty[st]);
+            };
+            // With two terms both tiles' scores come first (a prompt of 2811 128 us, not
+            // 131); with one, a tile's products together (4 of 4096 418 us, not 441).
+            if constexpr (C::BUFS == 2 && C::TWO) {
+#pragma unroll 1
+              for (int t = 0; t < tiles && ok && j < steps; ++t) qk(t);
+#pragma unroll 1
+              for (int t = 0; t < tiles && ok && j > 0; ++t) pv(t);
+            } else {
+#pragma unroll 1
+              for (int t = 0; t < tiles && ok; ++t) {
+                if (C::BUFS == 2 && j < steps) qk(t);
+                if (ok && j > 0) pv(t);
+                if (C::BUFS == 1 && ok && j < steps) qk(t);
+              }
             }
           }
           c += steps;
@@ -820,7 +875,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
       // ---- copies
       const int lt = tid - 32 * C::LOAD, lw = lt >> 5;
       const int mask = (1 << p.kv.page_log2) - 1;
-      int begun = 0, ended = 0;  // copies: 2 n is K's of step n, 2 n + 1 V's
+      int begun = 0, ended = 0;  // copies: of codes 2 n is K's of step n and 2 n + 1 V's, of f16 n is step n's
       bool ok = true;
       asm volatile("fence.proxy.async.global;" ::: "memory");  // (what kernels before this one stored is read by copies)
       const uint32_t a_raw = dev::SmemAddr(s_raw), a_scale = dev::SmemAddr(s_scale);
@@ -899,54 +954,54 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
           const uint32_t have = __ballot_sync(0xFFFFFFFFu, there);
           const uint32_t bad = __ballot_sync(0xFFFFFFFFu, used && !there);
           const int64_t off = there ? kvd::CodeOffset(p.kv, page, it.head, at & mask) : 0;
-          if (lt == 0) s_bad[(begun >> 1) % kNotes] = bad;
+          if (lt == 0) s_bad[(C::QUANT ? begun >> 1 : begun) % kNotes] = bad;
           if (C::QUANT && lane == 0) s_seen[lw][(begun >> 1) % C::SCALES] = make_int2(it.lo - pos0, it.hi - pos0);
           if (!C::QUANT) {
-            // Tiles of 16 positions and 64 values by TMA: a lane's is (g, box), every second g for this warp.
+            // By TMA: whole steps where a page holds them, or else 16 positions and 64
+            // values at a time.  One warp has K, the other V.  (A lane takes some 100
+            // cycles for each copy: 128 conversations over 4 prefixes of 16384 in pages
+            // of 64 122 us with 16 copies a step, 112 with two.)
             const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
-            constexpr uint32_t kEvery = 0x55555555u & ((1u << KT / 16) - 1);  // groups of warp 0
-            const uint32_t groups = kEvery << lw;
-            const int g = lw + 2 * (lane / C::BOX), box = lane % C::BOX;
+            constexpr uint32_t kAll = (1u << KT / 16) - 1;
+            const bool v = lw != 0;
+            const int st = begun % C::STAGES, g = lane / C::BOX, box = lane % C::BOX;
             const int pg = __shfl_sync(0xFFFFFFFFu, page, g & 31), in = (pos0 + 16 * g) & mask;
-#pragma unroll 1
-            for (int v = 0; v < 2; ++v) {
-              const int st = (begun >> 1) % C::STAGES;
-              uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
-              if (!__all_sync(0xFFFFFFFFu, Wait(empty, (((begun >> 1) / C::STAGES) & 1) ^ 1))) {
-                ok = false;
-                break;
-              }
-              char* dst = (v ? s_v : s_k) + st * C::PLANE;
-              const uint32_t take = (v ? full : have) & groups;
-              uint32_t rest = v ? groups & ~full : 0;
-              if (rest != 0) {
-                // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
-#pragma unroll 1
-                while (rest != 0) {
-                  const int q = __ffs(rest) - 1;
-                  rest &= rest - 1;
-                  const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
-#pragma unroll 1
-                  for (int i = lane; i < 16 * C::CPR; i += 32) {
-                    const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
-                    const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
-                    CopyAsync16(dev::SmemAddr(dst + (c >> 3) * (KT * 128) + Swz(16 * q + r, c & 7)),
-                                seen ? src + r * p.kv.pos_stride + c * 16 : p.kv.v, seen);
-                  }
-                }
-                CopyCommit();
-                CopyWait<0>();
-                dev::FenceProxyAsync();
-              }
-              __syncwarp();
-              if (lane == 0) dev::MbarExpectTx(whole, __popc(take) * (C::BOX * 2048));  // (an arrival too)
-              __syncwarp();
-              if (lane < KT / 32 * C::BOX && ((take >> g) & 1)) {
-                LoadTile(dst + box * (KT * 128) + g * 2048, v ? &map_v : &map_k, 64 * box, in, it.head, pg, whole);
-              }
-              ++begun;
+            uint64_t *empty = v ? &bars.v_empty[st] : &bars.k_empty[st], *whole = v ? &bars.v_full[st] : &bars.k_full[st];
+            if (!__all_sync(0xFFFFFFFFu, Wait(empty, ((begun / C::STAGES) & 1) ^ 1))) {
+              ok = false;
+              break;
             }
-            ended = begun;
+            char* dst = (v ? s_v : s_k) + st * C::PLANE;
+            const uint32_t take = v ? full : have;
+            uint32_t rest = v ? kAll & ~full : 0;
+            if (rest != 0) {
+              // V of positions that no row sees may hold anything, and zero times NaN is NaN: zeros instead
+#pragma unroll 1
+              while (rest != 0) {
+                const int q = __ffs(rest) - 1;
+                rest &= rest - 1;
+                const char* src = p.kv.v + __shfl_sync(0xFFFFFFFFu, off, q);
+#pragma unroll 1
+                for (int i = lane; i < 16 * C::CPR; i += 32) {
+                  const int r = i / C::CPR, c = i % C::CPR, pos = pos0 + 16 * q + r;
+                  const bool seen = ((have >> q) & 1) && pos >= it.lo && pos < it.hi;
+                  CopyAsync16(dev::SmemAddr(dst + (c >> 3) * (KT * 128) + Swz(16 * q + r, c & 7)),
+                              seen ? src + r * p.kv.pos_stride + c * 16 : p.kv.v, seen);
+                }
+              }
+              CopyCommit();
+              CopyWait<0>();
+              dev::FenceProxyAsync();
+            }
+            __syncwarp();
+            if (lane == 0) dev::MbarExpectTx(whole, __popc(take) * (C::BOX * 2048));  // (an arrival too)
+            __syncwarp();
+            if (take == kAll && (1 << p.kv.page_log2) >= KT && (pos0 & (KT - 1)) == 0) {
+              if (lane == 0) LoadTile(dst, v ? &maps.step_v : &maps.step_k, pos0 & mask, 0, it.head, pg, whole);
+            } else if (lane < KT / 16 * C::BOX && ((take >> g) & 1)) {
+              LoadTile(dst + box * (KT * 128) + g * 2048, v ? &maps.v : &maps.k, in, box, it.head, pg, whole);
+            }
+            ++begun;
           } else {
 #pragma unroll 1
             for (int v = 0; v < 2 && ok; ++v) {
@@ -997,10 +1052,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
         while (ok && ended < begun) finish();
       } else if (begun > 0) {
         // copies that nobody waits for any more have landed before the block ends
-        for (int n = max(0, begun / 2 - C::STAGES); n < begun / 2; ++n) {
+        for (int n = max(0, begun - C::STAGES); n < begun; ++n) {
           const int st = n % C::STAGES;
-          Wait(&bars.k_full[st], (n / C::STAGES) & 1);
-          Wait(&bars.v_full[st], (n / C::STAGES) & 1);
+          Wait(lw != 0 ? &bars.v_full[st] : &bars.k_full[st], (n / C::STAGES) & 1);
         }
       }
     }
@@ -1517,15 +1571,17 @@ PFN_cuTensorMapEncodeTiled_v12000 Encode() {
   return fn;
 }
 
-// A plane of an f16 cache, [page][head][position][value] by its strides.
-CUtensorMap PlaneMap(const KvPages& kv, char* plane) {
+// A plane of an f16 cache, [page][head][64 values][position][value] by its strides, in boxes of some positions and 64 values
+// `columns` times.
+CUtensorMap PlaneMap(const KvPages& kv, char* plane, int positions, int columns) {
   CUtensorMap m;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), cuuint64_t{1} << kv.page_log2,
+  const cuuint64_t dims[5] = {64, cuuint64_t{1} << kv.page_log2, static_cast<cuuint64_t>(kv.head_dim / 64),
                               static_cast<cuuint64_t>(kv.n_kv), static_cast<cuuint64_t>(kv.n_pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv.pos_stride), static_cast<cuuint64_t>(kv.head_stride),
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(kv.pos_stride), 128, static_cast<cuuint64_t>(kv.head_stride),
                                  static_cast<cuuint64_t>(kv.page_stride)};
-  const cuuint32_t box[4] = {64, 16, 1, 1}, steps[4] = {1, 1, 1, 1};
-  const CUresult r = Encode()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, plane, dims, strides, box, steps,
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(positions), static_cast<cuuint32_t>(columns), 1, 1};
+  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+  const CUresult r = Encode()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, plane, dims, strides, box, steps,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RPGB_CHECK(r == CUDA_SUCCESS, "kv: tensor map encoding failed (%d)", static_cast<int>(r));
@@ -1555,13 +1611,17 @@ int Grid() {
 template <typename C>
 void Launch(const KvRowsParams& p, cudaStream_t s) {
   const int grid = Grid<C>();
-  CUtensorMap map_k{}, map_v{};
+  Maps maps{};
   if (!C::QUANT) {
-    map_k = PlaneMap(p.kv, p.kv.k);
-    map_v = PlaneMap(p.kv, p.kv.v);
+    maps.k = PlaneMap(p.kv, p.kv.k, 16, 1);
+    maps.v = PlaneMap(p.kv, p.kv.v, 16, 1);
+    if (1 << p.kv.page_log2 >= C::KT) {
+      maps.step_k = PlaneMap(p.kv, p.kv.k, C::KT, C::BOX);
+      maps.step_v = PlaneMap(p.kv, p.kv.v, C::KT, C::BOX);
+    }
   }
-  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(C::THREADS), C::SMEM, s, true, map_k, map_v,
-                   p, kvd::kMagic);
+  LaunchKernelArgs(reinterpret_cast<const void*>(RowsKernel<C>), dim3(grid), dim3(C::THREADS), C::SMEM, s, true, maps, p,
+                   kvd::kMagic);
   LaunchKernelArgs(reinterpret_cast<const void*>(RowsJoinKernel<C>), dim3(grid, kJoinBlocks), dim3(256), 0, s, true, p);
 }
 
