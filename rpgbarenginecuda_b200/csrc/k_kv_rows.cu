@@ -847,8 +847,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
               Commit(&bars.s_full[t][buf]);
               if (t == tiles - 1) Commit(&bars.k_empty[st]);
             };
-            // With two terms both tiles' scores come first (a prompt of 2811 128 us, not
-            // 131); with one, a tile's products together (4 of 4096 418 us, not 441).
+            // With two terms both tiles' scores come first (a prompt of 40 24.9 us, not
+            // 25.6); with one, a tile's products together (4 of 4096 430 us, not 440).
             if constexpr (C::BUFS == 2 && C::TWO) {
 #pragma unroll 1
               for (int t = 0; t < tiles && ok && j < steps; ++t) qk(t);
@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) RowsKernel(const __grid_constan
             // By TMA: whole steps where a page holds them, or else 16 positions and 64
             // values at a time.  One warp has K, the other V.  (A lane takes some 100
             // cycles for each copy: 128 conversations over 4 prefixes of 16384 in pages
-            // of 64 122 us with 16 copies a step, 112 with two.)
+            // of 64 122 us with 16 copies a step, 117 with two.)
             const uint32_t full = __ballot_sync(0xFFFFFFFFu, there && at >= it.lo && at + 16 <= it.hi);
             constexpr uint32_t kAll = (1u << KT / 16) - 1;
             const bool v = lw != 0;

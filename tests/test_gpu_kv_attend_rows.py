@@ -166,6 +166,28 @@ def test_pages_and_strides(page, order, kind):
     assert bool((out[:, q.shape[1]:] == 7.0).all())
 
 
+@pytest.mark.parametrize("page", [32, 64, 256])
+@pytest.mark.parametrize("mask,span", [("causal", 0), ("window", 100), ("documents", 90), ("prefix", 700)])
+@pytest.mark.parametrize("heads,dim,act", [(4, 128, "f16"), (8, 64, "bf16"), (4, 128, "f32"), (2, 64, "f32")])
+def test_pages_that_hold_a_whole_step(page, mask, span, heads, dim, act):
+    # one tile of rows and two, in turn; ranges that begin and end inside a step
+    counts, ats = [70, 300, 1, 129, 64, 5], [500, 0, 640, 63, 64, 129]
+    pool, q, _, starts, ends = problem("f16", heads, 2, dim, act, page, counts, ats, mask, span)
+    out = attend_rows(pool, q, counts, ends, starts, act=act)
+    close(out, formula(pool, q, counts, ends, starts), pool, act)
+
+
+@pytest.mark.parametrize("kind,act", [("f16", "f32"), ("f16", "f16"), ("q8", "f32"), ("q8", "bf16"), ("q4", "f16")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_that_rise_step_after_step(kind, act, dim):
+    # by 32 to 128 over 64 positions, so that the largest one so far is left behind at every step
+    counts, ats = [200, 33], [400, 900]
+    pool, q, pos, starts, ends = problem(kind, 4, 2, dim, act, 64, counts, ats)
+    kw = dict(slopes=[0.5, 1.0, 2.0, 0.7], pos=pos)
+    out = attend_rows(pool, q, counts, ends, starts, act=act, **kw)
+    close(out, formula(pool, q, counts, ends, starts, **kw), pool, act)
+
+
 @pytest.mark.parametrize("heads,n_kv", [(1, 1), (5, 1), (40, 1), (96, 3), (300, 1)])
 @pytest.mark.parametrize("act", ["f16", "f32"])
 def test_many_queries_of_a_kv_head(heads, n_kv, act):
