@@ -30,8 +30,8 @@
 // place in shared memory to another).  Registers are shared out between them
 // by setmaxnreg.
 //
-// What bounds it: 4 prompts of 4096 over f16, 32 heads of 8 KV heads, bf16: 423 us,
-// 730 TFLOP/s of the pairs that are seen.  A step of a tile takes its softmax warps
+// What bounds it: 4 prompts of 4096 over f16, 32 heads of 8 KV heads, bf16: 427 us,
+// 720 TFLOP/s of the pairs that are seen.  A step of a tile takes its softmax warps
 // some 1400 cycles (exponentials 700 of them, 16 a cycle an SM; reading the scores
 // 250, the largest 230, storing weights 80), the two tiles of a block run side by
 // side on the same four schedulers, and an item's beginning and end add 400 a step
