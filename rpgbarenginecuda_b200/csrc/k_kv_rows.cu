@@ -35,9 +35,12 @@
 // some 1400 cycles (exponentials 700 of them, 16 a cycle an SM; reading the scores
 // 250, the largest 230, storing weights 80), the two tiles of a block run side by
 // side on the same four schedulers, and an item's beginning and end add 400 a step
-// at 9 steps an item; the tensor cores are at 40 %.  Over codes it is the spreading
-// (16 prompts of 1024 over 8 bits 308 us) and, with few steps a block, what a launch
-// costs: the pair of kernels 4 us, the plan 1.6, the roles' first instructions 3.
+// at 18 steps an item; the tensor cores are at 40 %.  Over codes of 128 values a
+// tile's products and its softmax take turns (one buffer of scores: two groups with
+// scales of their own fill the columns), 16 prompts of 1024 over 8 bits 308 us; four
+// copying warps and a thread per row gave 298 there and 171 in place of 145 for 6
+// prompts of 1501 over 4 bits.  With few steps a block it is what a launch costs: the
+// pair of kernels 4 us, the plan 1.6, the roles' first instructions 3.
 //
 // Tried and not kept, 4 prompts of 4096 at the time: a part of the exponentials as
 // polynomials, weights in two halves so that their product begins earlier, results
