@@ -64,9 +64,9 @@ __device__ __forceinline__ T* In(T* p, uint32_t rank) {
   return reinterpret_cast<T*>(r);
 }
 
-// Floats in order as integers; NaN and minus infinity (never drawn) as 0.
+// Floats in order as integers, the two zeros the same; NaN and minus infinity (never drawn) as 0.
 __device__ __forceinline__ uint32_t Key(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
   return x > -INFINITY ? k : 0u;
 }
@@ -622,8 +622,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) SampleRowsKe
           key[i + 3] = w.w;
         }
 #pragma unroll 1
-  #pragma unroll 1
-      for (int bit = 31; bit >= 10; --bit) {
+        for (int bit = 31; bit >= 10; --bit) {
           const uint32_t try_ = bound | 1u << bit;
           int c = 0;
 #pragma unroll

@@ -144,6 +144,23 @@ def test_equal_values():
     check(torch.full((4, 7000), 1.0, device="cuda").bfloat16(), [0.0, 0.3, 0.7, 0.999])
 
 
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [9, 5000])
+def test_zeros_of_both_signs_are_equal(act, vocab):
+    x = torch.full((12, vocab), -1.0, device="cuda")
+    x[:, 2], x[:, 4], x[:, vocab - 2] = -0.0, 0.0, -0.0
+    u = np.linspace(0.02, 0.98, 12)
+    for rows in (x, x - 1.0 * (torch.arange(vocab, device="cuda") == 4), x.index_fill(1, torch.tensor([6], device="cuda"), 1.5)):
+        rows = rows.to(TYPES[act][1])
+        check(rows, u, t=0.0)
+        check(rows, u, t=1.0)
+        check(rows, u, t=1.0, k=2)
+        check(rows, u, t=1.0, k=3)
+        check(rows, u, t=1.0, p=0.0005)
+        check(rows, u, t=0.2, p=0.5, k=4)
+        check(rows, u, t=1.0, m=1.0)
+
+
 def test_extremes_of_the_random_number():
     x, _ = logits(4, 3000, seed=5)
     check(x, [0.0, 2.0 ** -30, 1.0 - 2.0 ** -24, 0.5], t=1.0)
