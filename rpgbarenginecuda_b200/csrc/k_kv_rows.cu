@@ -260,10 +260,10 @@ struct Cfg {
   static constexpr int SCALE = QUANT ? 2 * KT * NG * 2 : 0;  // scales of a step: K, then V
   static constexpr int NOTE = 2 * SCALE;                     // the same as f32, [K or V][group][position]
   // Steps that the beginning and end of an item (its queries, its result) count
-  // for when the work is dealt.  Codes, 16 prompts of 1024 with 1, 2, 3, 4 and 6:
-  // 341, 332, 335, 347, 359 us; f16, 4 of 4096 with 4, 8 and 12: 430, 418, 431; two
-  // terms, a prompt of 2811 with 3, 5 and 8: 143, 134, 135.
-  static constexpr int BORDER = TWO ? 5 : (QUANT ? 2 : 8);
+  // for when the work is dealt.  Codes, 16 prompts of 1024 with 1, 2, 3 and 4: 318,
+  // 307, 309, 318 us; f16, 4 of 4096 with 4, 8 and 12: 430, 418, 431; two terms, a
+  // prompt of 2811 with 3, 5, 7 and 10: 138, 129, 122, 125.
+  static constexpr int BORDER = TWO ? 7 : (QUANT ? 2 : 8);
   static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * PLANE + (LAG + 1) * RAW + SCALES * (SCALE + NOTE);
   static_assert(SMEM <= 226 * 1024, "shared memory");
 };
